@@ -281,6 +281,74 @@ int rwkv6_layer_norm_bwd(const void* x, const void* gamma, int gamma_dtype, cons
                          int param_dtype, void* workspace, int64_t N, int64_t C, void* stream);
 
 /* ------------------------------------------------------------------------
+ * A block's output into the residual stream, and the LayerNorm that the next block reads
+ * (rwkv6_layer_specs.py:543-548; the channel mix's gate, :533-536), N rows of C channels, C a
+ * multiple of 8 up to 8192 (else RWKV6_ERR_UNSUPPORTED):
+ *   f = (branch + branch_bias) * sigmoid(gate), s = x + scale * f, y = LayerNorm(s) * gamma + beta
+ * x, s: [N,C] in x_dtype; branch, gate, y: [N,C] bf16; branch_bias [C] in bias_dtype and gate nullable;
+ * gamma, beta: [C] in param_dtype; mean, rstd: [N] f32 for the backward (both NULL without one).  The
+ * statistics and y are those of s before it is rounded to x_dtype.
+ *   bwd: ds [N,C] in x_dtype (nullable: zero), dy [N,C] bf16 -> dx in x_dtype, d_branch, d_gate bf16
+ *        (d_gate NULL exactly when gate is), dgamma, dbeta in param_dtype and d_branch_bias in bias_dtype
+ *        (all NULL: not wanted, no workspace; d_branch_bias NULL also when branch_bias is).  d_branch may
+ *        be NULL where it equals dx: x_dtype bf16, scale 1, neither gate nor branch_bias.
+ * ---------------------------------------------------------------------- */
+int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias,
+                            int bias_dtype, const void* gate, float scale, const void* gamma,
+                            const void* beta, int param_dtype, float eps, void* s, void* y,
+                            float* mean, float* rstd, int64_t N, int64_t C, void* stream);
+size_t rwkv6_residual_norm_bwd_workspace_bytes(int64_t N, int64_t C);
+int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias,
+                            int bias_dtype, const void* gate, float scale, const void* gamma,
+                            int gamma_dtype, const float* mean, const float* rstd, const void* ds,
+                            const void* dy, void* dx, void* d_branch, void* d_gate, void* dgamma,
+                            void* dbeta, int param_dtype, void* d_branch_bias, void* workspace,
+                            int64_t N, int64_t C, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Cross entropy a row over V classes (the loss a token of pretrain_rwkv6.py:144-179) and its gradient.
+ *   logits: N rows of V in dtype, `ld` elements apart, aligned to an element; target: [N] int64
+ *   loss: [N] f32 = log sum_j exp(l_j) - l_target; stats: [N,2] f32 for the backward (8-byte aligned)
+ *   d_logits: [N,V] in dtype = d_loss[n] (softmax(l) - onehot(target)), d_loss [N] f32
+ * A target equal to ignore_index gives loss 0 and a gradient of zeros, whatever the row's logits; one
+ * outside 0 .. V - 1 gives NaN for both.
+ * ---------------------------------------------------------------------- */
+int rwkv6_cross_entropy_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target,
+                            int64_t ignore_index, float* loss, float* stats, int64_t N, int64_t V,
+                            void* stream);
+int rwkv6_cross_entropy_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target,
+                            int64_t ignore_index, const float* stats, const float* d_loss,
+                            void* d_logits, int64_t N, int64_t V, void* stream);
+
+/* ------------------------------------------------------------------------
+ * AdamW over `count` tensors at once (the optimizer step of example_config.yaml:199-221), in place.
+ * Arrays of `count` are host arrays; tensors are dense, bf16 or f32 (dtype codes a tensor), aligned to
+ * an element.
+ *   grad_norm_sums  partials (grad_norm_partials doubles) = sums of the gradients' squares, by blocks
+ *   grad_norm       norm[0] = sqrt(sum partials)
+ *   adamw_step      t = step[0] += 1; with partials (nullable: no clipping) the gradients count times
+ *                   min(1, max_norm / (norm + 1e-6)) and norm[0] (nullable) is written; lr from
+ *                   lr_dev[0] where that is not NULL;
+ *                   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ *                   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ * exp_avg, exp_avg_sq: f32; or, with exp_avg_scale and exp_avg_sq_scale (ceil(n / 256) floats a tensor),
+ * float8 e4m3 codes of m and of sqrt(v) in blocks of 256 elements, value = code * scale.  workspace: 16
+ * bytes.  No output may overlap another tensor of the call (a tensor listed twice:
+ * RWKV6_ERR_INVALID_ARG).
+ * ---------------------------------------------------------------------- */
+int64_t rwkv6_grad_norm_partials(const int64_t* numel, int64_t count);
+int rwkv6_grad_norm_sums(const void* const* grad, const int* grad_dtype, const int64_t* numel,
+                         int64_t count, double* partials, void* stream);
+int rwkv6_grad_norm(const double* partials, int64_t P, float* norm, void* stream);
+int rwkv6_adamw_step(void* const* param, const int* param_dtype, const void* const* grad,
+                     const int* grad_dtype, void* const* exp_avg, void* const* exp_avg_sq,
+                     float* const* exp_avg_scale, float* const* exp_avg_sq_scale,
+                     const int64_t* numel, int64_t count, float* step, double lr,
+                     const float* lr_dev, double beta1, double beta2, double eps,
+                     double weight_decay, const double* partials, int64_t P, float max_norm,
+                     float* norm, void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------
  * Forward without a workspace argument.  No counterpart in the reference: for callers that
  * cannot allocate device memory (code under HIP graph capture, tight serving loops, harnesses
  * that forbid hipMalloc).  Same arguments and results as rwkv6_wkv_fwd minus `workspace`:

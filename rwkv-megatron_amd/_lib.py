@@ -25,6 +25,7 @@ _fp = ctypes.c_void_p          # float* passed as an address
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/rwkv6_amd.h
 SIGNATURES = {
@@ -77,6 +78,17 @@ SIGNATURES = {
     "rwkv6_linear_f32": (_int, [_vp, _fp, _vp, _vp] + [_i64] * 3 + [_vp]),
     "rwkv6_layer_norm_fwd": (_int, [_vp] * 3 + [_int, _f32, _vp, _fp, _fp, _fp] + [_i64] * 2 + [_vp]),
     "rwkv6_layer_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64] * 2),
+    "rwkv6_residual_norm_fwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _vp, _vp, _int, _f32, _vp, _vp, _fp, _fp]
+                                + [_i64] * 2 + [_vp]),
+    "rwkv6_residual_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64] * 2),
+    "rwkv6_residual_norm_bwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _vp, _int, _fp, _fp] + [_vp] * 7
+                                + [_int, _vp, _vp] + [_i64] * 2 + [_vp]),
+    "rwkv6_cross_entropy_fwd": (_int, [_vp, _int, _i64, _vp, _i64, _fp, _fp] + [_i64] * 2 + [_vp]),
+    "rwkv6_cross_entropy_bwd": (_int, [_vp, _int, _i64, _vp, _i64, _fp, _fp, _vp] + [_i64] * 2 + [_vp]),
+    "rwkv6_grad_norm_partials": (_i64, [_vp, _i64]),
+    "rwkv6_grad_norm_sums": (_int, [_vp, _vp, _vp, _i64, _vp, _vp]),
+    "rwkv6_grad_norm": (_int, [_vp, _i64, _fp, _vp]),
+    "rwkv6_adamw_step": (_int, [_vp] * 9 + [_i64, _fp, _f64, _fp] + [_f64] * 4 + [_vp, _i64, _f32, _fp, _vp, _vp]),
     "rwkv6_layer_norm_bwd": (_int, [_vp, _vp, _int, _fp, _fp] + [_vp] * 4 + [_int, _vp] + [_i64] * 2 + [_vp]),
 }
 

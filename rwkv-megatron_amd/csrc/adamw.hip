@@ -1,0 +1,460 @@
+// An AdamW step over many tensors at once for MI355X (gfx950), states in 32 or 8 bits, clipped by the
+// norm of all gradients.
+//
+// Reference: the optimizer step after the backward (/root/reference/example_config.yaml:199-221: AdamW
+// with weight decay and a gradient clip; Megatron's training loop runs it, pretrain_rwkv6.py:281-286).
+//   norm = sqrt(sum g^2) over all tensors (64-bit sums),  c = min(1, max_norm / (norm + 1e-6))
+//   g' = c g;  m' = b1 m + (1 - b1) g';  v' = b2 v + (1 - b2) g'^2;  t = step + 1
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+// Everything is elementwise in 32 bits with one rounding of p at the end; p' takes the unrounded m' and
+// v' also where the states are kept in 8 bits.
+//
+// States in 8 bits: a block of 256 consecutive elements of a tensor holds float8 (e4m3) codes and one
+// fp32 scale, the block's largest magnitude over 448; m as code * scale and v by its root, v = (code *
+// scale)^2, which doubles the range in the exponent (a code reaches from 448 to 2^-9: 2^-36 of the
+// block's largest v).  Values that are not finite do not enter the scale and become NaN codes, so that
+// they spoil no other element of the block; a block below 2^-118 stores zeros.
+//
+// The tensors' addresses travel in the kernels' arguments, AW_T tensors a launch: nothing is copied to
+// the device or kept between calls, and a captured call replays with the addresses it was made with.
+// The step count and the norm stay on the device, for the same reason.
+//
+// Bound by memory: bytes a parameter 22 (bf16 p and g, fp32 states), 28 (all fp32), 10 and 16 with
+// 8-bit states, and once more the gradient where it is clipped.
+#include "common.h"
+#include "../../include/rwkv6_amd.h"
+
+#include <algorithm>
+#include <vector>
+
+#define AW_THR 256
+#define AW_STEP (8 * AW_THR)    // elements a block takes at once
+#define AW_T 60                 // tensors a launch: the arguments stay below 4 KB
+#define AW_BLK 256              // elements under one 8-bit scale: 32 lanes of 8
+#define AW_F8_MAX 448.f
+#define AW_TINY 0x1p-118f
+
+namespace {
+
+struct NormTable {
+    const void* g[AW_T];
+    int64_t n[AW_T];
+    int first[AW_T];            // first block of the tensor in this launch
+    int dt[AW_T];
+    int count, base;            // base: blocks of the launches before
+};
+struct StepTable {
+    void* p[AW_T];
+    const void* g[AW_T];
+    void *m[AW_T], *v[AW_T];
+    float *ms[AW_T], *vs[AW_T];
+    int64_t n[AW_T];
+    int first[AW_T];
+    int dt[AW_T];               // the parameter's type, and the gradient's 8 bits up
+    int count;
+};
+static_assert(sizeof(StepTable) <= 4000 && sizeof(NormTable) <= 4000, "kernel arguments");
+// The tables hold no element below 4 bytes.  A uniform index into them becomes scalar loads, whose address
+// is a sum of which the hardware drops the two low bits of every term; with byte arrays beside the pointers
+// the compiler (ROCm 7.2) shares the byte address between them and forms 8 k as k + 7 k.
+
+// The launch's tensor that holds block b: the last one whose first block is not after it.
+__device__ __forceinline__ int aw_find(const int* first, int count, int b) {
+    const int lane = threadIdx.x & 63;
+    const bool at = lane < count && first[lane < count ? lane : 0] <= b;
+    return __popcll(__ballot(at)) - 1;
+}
+
+// Eight elements from i of a tensor of n: as vectors where they are all there and aligned (`vec`), else
+// one by one, zeros past the end.
+__device__ __forceinline__ void aw_load8(const void* p, int dt, int64_t i, int64_t n, bool vec, float* f) {
+    if (vec && i + 8 <= n) {
+        if (dt == RWKV6_BF16) {
+            load8(reinterpret_cast<const uint16_t*>(p) + i, f);
+        } else {
+            const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+            const float4 a = q[0], b = q[1];
+            f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+            f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            f[j] = 0.f;
+            if (i + j < n)
+                f[j] = dt == RWKV6_BF16 ? bf2f(reinterpret_cast<const uint16_t*>(p)[i + j])
+                                        : reinterpret_cast<const float*>(p)[i + j];
+        }
+    }
+}
+__device__ __forceinline__ void aw_store8(void* p, int dt, int64_t i, int64_t n, bool vec, const float* f) {
+    if (vec && i + 8 <= n) {
+        if (dt == RWKV6_BF16) {
+            store8(reinterpret_cast<uint16_t*>(p) + i, f);
+        } else {
+            float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i);
+            q[0] = make_float4(f[0], f[1], f[2], f[3]);
+            q[1] = make_float4(f[4], f[5], f[6], f[7]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < n) {
+                if (dt == RWKV6_BF16) reinterpret_cast<uint16_t*>(p)[i + j] = f2bf(f[j]);
+                else reinterpret_cast<float*>(p)[i + j] = f[j];
+            }
+    }
+}
+__device__ __forceinline__ bool aw_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Eight float8 codes.
+__device__ __forceinline__ uint2 aw_codes_load(const void* p, int64_t i, int64_t n, bool vec) {
+    const uint8_t* b = reinterpret_cast<const uint8_t*>(p) + i;
+    if (vec && i + 8 <= n) return *reinterpret_cast<const uint2*>(b);
+    uint2 q = make_uint2(0u, 0u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (i + j < n) (j < 4 ? q.x : q.y) |= (unsigned)b[j] << (8 * (j & 3));
+    return q;
+}
+__device__ __forceinline__ void aw_codes_store(void* p, int64_t i, int64_t n, bool vec, uint2 q) {
+    uint8_t* b = reinterpret_cast<uint8_t*>(p) + i;
+    if (vec && i + 8 <= n) {
+        *reinterpret_cast<uint2*>(b) = q;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (i + j < n) b[j] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+}
+__device__ __forceinline__ void aw_decode(uint2 q, float s, float* f) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, true);
+    const f32x2 c = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, true);
+    f[0] = a[0] * s; f[1] = a[1] * s; f[2] = b[0] * s; f[3] = b[1] * s;
+    f[4] = c[0] * s; f[5] = c[1] * s; f[6] = d[0] * s; f[7] = d[1] * s;
+}
+__device__ __forceinline__ uint2 aw_encode(const float* f, float inv) {
+    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, f[1] * inv, 0, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv, f[3] * inv, lo, true);
+    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv, f[5] * inv, 0, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv, f[7] * inv, hi, true);
+    return make_uint2((unsigned)lo, (unsigned)hi);
+}
+// Largest finite magnitude of the 8 values of each of 32 lanes.
+__device__ __forceinline__ float aw_top(const float* f) {
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(f[j]);
+        t = fmaxf(t, a < INFINITY ? a : 0.f);
+    }
+    t = fmaxf(t, lane_xor1(t));
+    t = fmaxf(t, lane_xor2(t));
+    t = fmaxf(t, dpp_mov<0x141>(t));              // the other quad of 8 lanes
+    t = fmaxf(t, dpp_mov<0x140>(t));              // the other 8 of 16
+    return fmaxf(t, lane_xor_swz<16>(t));
+}
+struct Coef {
+    float clip, keep, lr, rbc2;                   // c, 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+};
+
+}  // namespace
+
+// Sum of squares of the blocks' elements, `per` of a tensor each: part[base + block].
+__global__ void __launch_bounds__(AW_THR)
+rwkv6_grad_square_sums_kernel(const NormTable tab, int64_t per, double* __restrict__ part) {
+    __shared__ double red[AW_THR / 64];
+    const int k = aw_find(tab.first, tab.count, blockIdx.x);
+    const int64_t n = tab.n[k], i0 = (int64_t)((int)blockIdx.x - tab.first[k]) * per, i1 = min(n, i0 + per);
+    const void* g = tab.g[k];
+    const int dt = tab.dt[k];
+    const bool vec = aw_al16(g);
+    double acc = 0.;
+    for (int64_t i = i0 + 8 * threadIdx.x; i < i1; i += AW_STEP) {
+        float f[8];
+        aw_load8(g, dt, i, i1, vec, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc = fma((double)f[j], (double)f[j], acc);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) acc += __shfl_xor(acc, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) part[tab.base + blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
+}
+
+// One block: the norm from the partial sums (none: c = 1), the step counted, the coefficients.
+__global__ void __launch_bounds__(1024)
+rwkv6_adamw_coef_kernel(const double* __restrict__ part, int P, float max_norm, float* __restrict__ norm_out,
+                        float* __restrict__ step, const float* __restrict__ lr_dev, double lr, double log_b1,
+                        double log_b2, double wd, Coef* __restrict__ coef) {
+    __shared__ double red[16];
+    double acc = 0.;
+    for (int i = threadIdx.x; i < P; i += 1024) acc += part[i];
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) acc += __shfl_xor(acc, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    if (threadIdx.x) return;
+    acc = 0.;
+    for (int w = 0; w < 16; ++w) acc += red[w];
+    const float norm = (float)sqrt(acc), r = max_norm / (norm + 1e-6f);
+    if (norm_out) norm_out[0] = norm;
+    if (!coef) return;
+    const float t = step[0] + 1.f;
+    step[0] = t;
+    if (lr_dev) lr = (double)lr_dev[0];
+    // a NaN norm stays one: the whole update is NaN, as clipped gradients would be
+    coef[0] = Coef{part && !(r > 1.f) ? r : 1.f, (float)(1. - lr * wd), (float)(lr / -expm1((double)t * log_b1)),
+                   (float)(1. / sqrt(-expm1((double)t * log_b2)))};
+}
+
+// Block b: `per` elements of a tensor, 8 a thread and step.  32 lanes hold the 256 elements of one scale.
+template <bool F8>
+__global__ void __launch_bounds__(AW_THR)
+rwkv6_adamw_step_kernel(const StepTable tab, const Coef* __restrict__ coef, int64_t per, float b1, float ob1, float b2,
+                        float ob2, float eps) {
+    const int k = aw_find(tab.first, tab.count, blockIdx.x);
+    const Coef c = coef[0];
+    const int64_t n = tab.n[k], i0 = (int64_t)((int)blockIdx.x - tab.first[k]) * per, i1 = min(n, i0 + per);
+    void *p = tab.p[k], *m = tab.m[k], *v = tab.v[k];
+    const void* g = tab.g[k];
+    const int pt = tab.dt[k] & 0xff, gt = tab.dt[k] >> 8;
+    const bool vec = aw_al16(p) && aw_al16(g) && aw_al16(m) && aw_al16(v);
+    // all lanes of a scale's 32 step together, up to the end of its block
+    for (int64_t i = i0 + 8 * threadIdx.x; (i & ~(int64_t)(AW_BLK - 1)) < i1; i += AW_STEP) {
+        float pf[8], gf[8], mf[8], vf[8];
+        aw_load8(p, pt, i, n, vec, pf);
+        aw_load8(g, gt, i, n, vec, gf);
+        float* ms = nullptr;
+        float* vs = nullptr;
+        if constexpr (F8) {
+            ms = tab.ms[k] + i / AW_BLK;
+            vs = tab.vs[k] + i / AW_BLK;
+            aw_decode(aw_codes_load(m, i, n, vec), ms[0], mf);
+            aw_decode(aw_codes_load(v, i, n, vec), vs[0], vf);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) vf[j] *= vf[j];
+        } else {
+            aw_load8(m, RWKV6_F32, i, n, vec, mf);
+            aw_load8(v, RWKV6_F32, i, n, vec, vf);
+        }
+        float root[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // each product and sum rounded, so that a state's value, and the code it falls on, is the
+            // formula's in 32 bits and not one of its contractions
+#pragma clang fp contract(off)
+            const float gc = gf[j] * c.clip;
+            mf[j] = mf[j] * b1 + gc * ob1;
+            vf[j] = vf[j] * b2 + (gc * gc) * ob2;
+            root[j] = sqrtf(vf[j]);
+            pf[j] = pf[j] * c.keep - c.lr * (mf[j] * __builtin_amdgcn_rcpf(root[j] * c.rbc2 + eps));
+        }
+        aw_store8(p, pt, i, n, vec, pf);
+        if constexpr (F8) {
+            float tm = aw_top(mf), tv = aw_top(root);
+            tm = tm < AW_TINY ? 0.f : tm;
+            tv = tv < AW_TINY ? 0.f : tv;
+            aw_codes_store(m, i, n, vec, aw_encode(mf, tm > 0.f ? AW_F8_MAX / tm : 0.f));
+            aw_codes_store(v, i, n, vec, aw_encode(root, tv > 0.f ? AW_F8_MAX / tv : 0.f));
+            if ((threadIdx.x & 31) == 0) {
+                ms[0] = tm / AW_F8_MAX;
+                vs[0] = tv / AW_F8_MAX;
+            }
+        } else {
+            aw_store8(m, RWKV6_F32, i, n, vec, mf);
+            aw_store8(v, RWKV6_F32, i, n, vec, vf);
+        }
+    }
+}
+
+namespace {
+// Elements a block takes: 2048 blocks over all tensors (8 a CU), in steps of AW_STEP.
+int64_t aw_per(const int64_t* numel, int64_t count, int64_t most) {
+    int64_t total = 0;
+    for (int64_t k = 0; k < count; ++k) total += numel[k];
+    int64_t per = (total / 2048 + AW_STEP - 1) / AW_STEP * AW_STEP;
+    if (per < AW_STEP) per = AW_STEP;
+    return most && per > most ? most : per;
+}
+int64_t aw_blocks(int64_t n, int64_t per) { return (n + per - 1) / per; }
+bool aw_dt(int dt) { return dt == RWKV6_F32 || dt == RWKV6_BF16; }
+int aw_sizes(const int64_t* numel, int64_t count) {
+    if (count < 0 || (count && !numel)) return RWKV6_ERR_INVALID_ARG;
+    if (count > (1 << 20)) return RWKV6_ERR_UNSUPPORTED;
+    int64_t total = 0;
+    for (int64_t k = 0; k < count; ++k) {
+        if (numel[k] < 0) return RWKV6_ERR_INVALID_ARG;
+        if (numel[k] > ((int64_t)1 << 40)) return RWKV6_ERR_UNSUPPORTED;
+        total += numel[k];
+    }
+    return total > ((int64_t)1 << 40) ? RWKV6_ERR_UNSUPPORTED : RWKV6_OK;
+}
+int64_t aw_partials(const int64_t* numel, int64_t count) {
+    const int64_t per = aw_per(numel, count, 0);
+    int64_t P = 0;
+    for (int64_t k = 0; k < count; ++k) P += aw_blocks(numel[k], per);
+    return P;
+}
+bool aw_misaligned(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
+
+// Whether an output of the step overlaps another or an input, over all tensors: a parameter listed
+// twice would be updated by two blocks at once.
+struct Range {
+    uintptr_t from, to;
+    bool out;
+};
+void aw_add(std::vector<Range>& r, const void* p, size_t bytes, bool out) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    if (p && bytes) r.push_back({a, a + bytes, out});
+}
+bool aw_overlap(std::vector<Range>& r) {
+    std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+    uintptr_t outs = 0, any = 0;                  // where the ones before end
+    for (const Range& x : r) {
+        if (x.from < (x.out ? any : outs)) return true;
+        if (x.out) outs = std::max(outs, x.to);
+        any = std::max(any, x.to);
+    }
+    return false;
+}
+}  // namespace
+
+extern "C" {
+
+int64_t rwkv6_grad_norm_partials(const int64_t* numel, int64_t count) {
+    return aw_sizes(numel, count) ? 0 : aw_partials(numel, count);
+}
+
+int rwkv6_grad_norm_sums(const void* const* grad, const int* grad_dtype, const int64_t* numel, int64_t count,
+                         double* partials, void* stream) {
+    const int st = aw_sizes(numel, count);
+    if (st) return st;
+    if (count && (!grad || !grad_dtype)) return RWKV6_ERR_INVALID_ARG;
+    const int64_t per = aw_per(numel, count, 0);
+    const Span out = {partials, (size_t)aw_partials(numel, count) * 8};
+    for (int64_t k = 0; k < count; ++k) {
+        if (!aw_dt(grad_dtype[k]) || (numel[k] && (!grad[k] || !partials))) return RWKV6_ERR_INVALID_ARG;
+        if (aw_misaligned(grad[k], param_bytes(grad_dtype[k]))) return RWKV6_ERR_ALIGNMENT;
+        if (spans_overlap(out, {grad[k], (size_t)numel[k] * param_bytes(grad_dtype[k])}))
+            return RWKV6_ERR_INVALID_ARG;
+    }
+    if (aw_misaligned(partials, 8)) return RWKV6_ERR_ALIGNMENT;
+    NormTable tab;
+    int blocks = 0, base = 0;
+    tab.count = 0;
+    auto launch = [&] {
+        if (!blocks) return;
+        tab.base = base;
+        hipLaunchKernelGGL(rwkv6_grad_square_sums_kernel, dim3((unsigned)blocks), dim3(AW_THR), 0,
+                           reinterpret_cast<hipStream_t>(stream), tab, per, partials);
+        base += blocks;
+        blocks = tab.count = 0;
+    };
+    for (int64_t k = 0; k < count; ++k) {
+        if (numel[k] == 0) continue;
+        if (tab.count == AW_T) launch();
+        const int i = tab.count++;
+        tab.g[i] = grad[k];
+        tab.n[i] = numel[k];
+        tab.dt[i] = grad_dtype[k];
+        tab.first[i] = blocks;
+        blocks += (int)aw_blocks(numel[k], per);
+    }
+    launch();
+    return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+}
+
+int rwkv6_grad_norm(const double* partials, int64_t P, float* norm, void* stream) {
+    if (P < 0 || (P && !partials) || !norm) return RWKV6_ERR_INVALID_ARG;
+    if (P > 0x7fffffff) return RWKV6_ERR_UNSUPPORTED;
+    if (aw_misaligned(partials, 8) || aw_misaligned(norm, 4)) return RWKV6_ERR_ALIGNMENT;
+    if (any_alias({{norm, 4}}, {{partials, (size_t)P * 8}})) return RWKV6_ERR_INVALID_ARG;
+    hipLaunchKernelGGL(rwkv6_adamw_coef_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), partials,
+                       (int)P, 0.f, norm, nullptr, nullptr, 0., 0., 0., 0., nullptr);
+    return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+}
+
+int rwkv6_adamw_step(void* const* param, const int* param_dtype, const void* const* grad, const int* grad_dtype,
+                     void* const* exp_avg, void* const* exp_avg_sq, float* const* exp_avg_scale,
+                     float* const* exp_avg_sq_scale, const int64_t* numel, int64_t count, float* step, double lr,
+                     const float* lr_dev, double beta1, double beta2, double eps, double weight_decay, const double* partials,
+                     int64_t P, float max_norm, float* norm, void* workspace, void* stream) {
+    const int st = aw_sizes(numel, count);
+    if (st) return st;
+    const bool f8 = exp_avg_scale != nullptr;
+    if (!step || !workspace || P < 0 || (P && !partials)) return RWKV6_ERR_INVALID_ARG;
+    if (P > 0x7fffffff) return RWKV6_ERR_UNSUPPORTED;
+    if (!(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1.)) return RWKV6_ERR_INVALID_ARG;
+    if (count && (!param || !param_dtype || !grad || !grad_dtype || !exp_avg || !exp_avg_sq)) return RWKV6_ERR_INVALID_ARG;
+    if (f8 != (exp_avg_sq_scale != nullptr)) return RWKV6_ERR_INVALID_ARG;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15u) || aw_misaligned(partials, 8) || aw_misaligned(step, 4) ||
+        aw_misaligned(lr_dev, 4) || aw_misaligned(norm, 4))
+        return RWKV6_ERR_ALIGNMENT;
+    try {
+        std::vector<Range> ranges;
+        ranges.reserve((size_t)count * 6 + 5);
+        aw_add(ranges, workspace, sizeof(Coef), true);
+        aw_add(ranges, step, 4, true);
+        aw_add(ranges, norm, 4, true);
+        aw_add(ranges, lr_dev, 4, false);
+        aw_add(ranges, partials, (size_t)P * 8, false);
+        for (int64_t k = 0; k < count; ++k) {
+            if (!aw_dt(param_dtype[k]) || !aw_dt(grad_dtype[k])) return RWKV6_ERR_INVALID_ARG;
+            if (numel[k] == 0) continue;
+            if (!param[k] || !grad[k] || !exp_avg[k] || !exp_avg_sq[k] || (f8 && (!exp_avg_scale[k] || !exp_avg_sq_scale[k])))
+                return RWKV6_ERR_INVALID_ARG;
+            const size_t n = (size_t)numel[k], ps = param_bytes(param_dtype[k]), gs = param_bytes(grad_dtype[k]), ss = f8 ? 1 : 4;
+            if (aw_misaligned(param[k], ps) || aw_misaligned(grad[k], gs) || aw_misaligned(exp_avg[k], ss) ||
+                aw_misaligned(exp_avg_sq[k], ss) || (f8 && (aw_misaligned(exp_avg_scale[k], 4) || aw_misaligned(exp_avg_sq_scale[k], 4))))
+                return RWKV6_ERR_ALIGNMENT;
+            aw_add(ranges, param[k], n * ps, true);
+            aw_add(ranges, grad[k], n * gs, false);
+            aw_add(ranges, exp_avg[k], n * ss, true);
+            aw_add(ranges, exp_avg_sq[k], n * ss, true);
+            if (f8) {
+                aw_add(ranges, exp_avg_scale[k], (n + AW_BLK - 1) / AW_BLK * 4, true);
+                aw_add(ranges, exp_avg_sq_scale[k], (n + AW_BLK - 1) / AW_BLK * 4, true);
+            }
+        }
+        if (aw_overlap(ranges)) return RWKV6_ERR_INVALID_ARG;
+    } catch (...) {                               // no host memory for the check
+        return RWKV6_ERR_LAUNCH;
+    }
+    Coef* coef = (Coef*)workspace;
+    hipLaunchKernelGGL(rwkv6_adamw_coef_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), partials,
+                       partials ? (int)P : 0, max_norm, norm, step, lr_dev, lr, log(beta1), log(beta2), weight_decay, coef);
+    const int64_t per = aw_per(numel, count, 8 * AW_STEP);
+    StepTable tab;
+    int64_t blocks = 0;
+    tab.count = 0;
+    auto launch = [&] {
+        if (!blocks) return;
+        hipLaunchKernelGGL(f8 ? rwkv6_adamw_step_kernel<true> : rwkv6_adamw_step_kernel<false>, dim3((unsigned)blocks),
+                           dim3(AW_THR), 0, reinterpret_cast<hipStream_t>(stream), tab, (const Coef*)coef, per, (float)beta1,
+                           (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps);
+        blocks = tab.count = 0;
+    };
+    for (int64_t k = 0; k < count; ++k) {
+        if (numel[k] == 0) continue;
+        const int64_t need = aw_blocks(numel[k], per);
+        // a launch has fewer than 2^32 threads
+        if (tab.count == AW_T || blocks + need >= ((int64_t)1 << 24)) launch();
+        const int i = tab.count++;
+        tab.p[i] = param[k];
+        tab.g[i] = grad[k];
+        tab.m[i] = exp_avg[k];
+        tab.v[i] = exp_avg_sq[k];
+        tab.ms[i] = f8 ? exp_avg_scale[k] : nullptr;
+        tab.vs[i] = f8 ? exp_avg_sq_scale[k] : nullptr;
+        tab.n[i] = numel[k];
+        tab.dt[i] = param_dtype[k] | grad_dtype[k] << 8;
+        tab.first[i] = (int)blocks;
+        blocks += need;
+    }
+    launch();
+    return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+}
+
+}  // extern "C"

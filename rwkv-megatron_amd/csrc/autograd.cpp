@@ -428,6 +428,283 @@ py::object layer_norm(const Tensor& x, const OptTensor& gamma, const OptTensor& 
 }
 
 // ---------------------------------------------------------------------------------------
+// A block's output into the stream, and the next LayerNorm
+// ---------------------------------------------------------------------------------------
+struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
+    struct Args {
+        Tensor x, branch, gate;
+        Param cbias;
+        int xt;
+        int64_t N, C;
+    };
+    static Args args(const Tensor& x, const Tensor& branch, const Tensor& gate, const Tensor& cbias) {
+        const int64_t C = x.size(-1);
+        return {dense(x), dense(branch), gate.defined() ? dense(gate) : gate, cbias.defined() ? param(cbias) : Param{cbias, 0},
+                x.scalar_type() == at::kFloat ? RWKV6_F32 : RWKV6_BF16, C ? x.numel() / C : 0, C};
+    }
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& branch, const Tensor& gamma,
+                                 const Tensor& beta, const OptTensor& gate, const OptTensor& cbias, double eps,
+                                 double scale, bool grad) {
+        const Tensor gt = gate.value_or(Tensor()), cb = cbias.value_or(Tensor());
+        const Args a = args(x, branch, gt, cb);
+        Param ga = param(gamma), be = param(beta);
+        if (ga.dt != be.dt) ga = {to_f32(gamma), RWKV6_F32}, be = {to_f32(beta), RWKV6_F32};
+        const Tensor s = at::empty_like(a.x), y = at::empty_like(a.branch);
+        const Tensor mean = grad ? empty({a.N}, at::kFloat, x) : Tensor(), rstd = grad ? at::empty_like(mean) : Tensor();
+        check(rwkv6_residual_norm_fwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
+                                      ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), fptr(mean), fptr(rstd), a.N,
+                                      a.C, stream_of(x)),
+              "rwkv6_residual_norm_fwd");
+        if (grad) {
+            ctx->set_materialize_grads(false);
+            ctx->save_for_backward({x, branch, gt, cb, gamma, beta, mean, rstd});
+            put(ctx, {bits(scale)});
+        }
+        return {s, y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const auto sv = ctx->get_saved_variables();
+        const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2], &cbias = sv[3], &gamma = sv[4], &beta = sv[5];
+        const double scale = unbits(meta(ctx)[0]);
+        // an output no loss uses has no gradient
+        const Tensor dy = g[1].defined() ? to_bf16(g[1]) : at::zeros(branch.sizes(), branch.options());
+        if (at::GradMode::is_enabled()) return differentiable(sv, g[0], g[1].defined() ? g[1] : dy, scale);
+        const Args a = args(x, branch, gate, cbias);
+        const Tensor ds = g[0].defined() ? dense(cast(g[0], x.scalar_type())) : Tensor();
+        const Param ga = param(gamma);
+        const bool gated = gate.defined(), biased = cbias.defined();
+        bool sums = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
+        if (biased) sums = sums || ctx->needs_input_grad(gated ? 5 : 4);
+        const bool same = a.xt == RWKV6_BF16 && scale == 1. && !gated && !biased;      // d_branch is dx
+        const Tensor dx = at::empty_like(a.x), db = same ? Tensor() : at::empty_like(a.branch);
+        const Tensor dg = gated ? at::empty_like(a.gate) : Tensor();
+        const int dt = grad_code(gamma) == grad_code(beta) ? grad_code(gamma) : RWKV6_F32;
+        const Tensor dga = sums ? empty({a.C}, param_type(dt), x) : Tensor(), dbe = sums ? at::empty_like(dga) : Tensor();
+        const Tensor dcb = sums && biased ? empty({a.C}, a.cbias.t.scalar_type(), x) : Tensor();
+        const Tensor ws = sums ? bytes(rwkv6_residual_norm_bwd_workspace_bytes(a.N, a.C), x) : Tensor();
+        check(rwkv6_residual_norm_bwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
+                                      ptr(ga.t), ga.dt, fptr(sv[6]), fptr(sv[7]), ptr(ds), ptr(dy), ptr(dx), ptr(db), ptr(dg),
+                                      ptr(dga), ptr(dbe), dt, ptr(dcb), ptr(ws), a.N, a.C, stream_of(x)),
+              "rwkv6_residual_norm_bwd");
+        return {dx, same ? dx : db, sums ? cast(dga, gamma.scalar_type()) : dga, sums ? cast(dbe, beta.scalar_type()) : dbe, dg,
+                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor(), Tensor()};
+    }
+    // A backward that is differentiated itself: the same formulas in torch's operators.
+    static variable_list differentiable(const variable_list& sv, const Tensor& ds, const Tensor& dy, double scale) {
+        const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2], &cbias = sv[3], &gamma = sv[4], &beta = sv[5];
+        const Tensor f = cbias.defined() ? branch.to(at::kFloat) + cbias.to(at::kFloat) : branch.to(at::kFloat);
+        const Tensor sg = gate.defined() ? at::sigmoid(gate.to(at::kFloat)) : Tensor();
+        const Tensor s = x.to(at::kFloat) + (gate.defined() ? f * sg : f) * scale;
+        std::vector<int64_t> st(x.sizes().begin(), x.sizes().end());
+        st.back() = 1;
+        auto [dS, dga, dbe] = at::native_layer_norm_backward(dy.to(at::kFloat), s, {x.size(-1)}, sv[6].view(st), sv[7].view(st),
+                                                             gamma.to(at::kFloat), beta.to(at::kFloat), {true, true, true});
+        if (ds.defined()) dS = dS + ds.to(at::kFloat);
+        const Tensor df = dS * scale, db = gate.defined() ? df * sg : df;
+        const Tensor dg = gate.defined() ? (df * f * sg * (1 - sg)).to(gate.scalar_type()) : Tensor();
+        const Tensor dcb = cbias.defined() ? db.reshape({-1, x.size(-1)}).sum(0).to(cbias.scalar_type()) : Tensor();
+        return {dS.to(x.scalar_type()), db.to(branch.scalar_type()), dga.to(gamma.scalar_type()), dbe.to(beta.scalar_type()),
+                dg, dcb, Tensor(), Tensor(), Tensor()};
+    }
+};
+// None when the kernels do not take the call (only_plain: nor one that a mode or transform wants to see);
+// the callers check and raise, or run torch's operators.
+py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta, double eps,
+                         const OptTensor& gate, const OptTensor& cbias, double scale, bool only_plain) {
+    if (!x.is_cuda() || x.dim() < 1 || x.size(-1) < 1 || x.layout() != at::kStrided ||
+        (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat))
+        return py::none();
+    const int64_t C = x.size(-1);
+    if (rwkv6_residual_norm_bwd_workspace_bytes(x.numel() / C, C) == 0) return py::none();
+    for (const Tensor* t : {&branch, gate ? &*gate : &branch})
+        if (t->device() != x.device() || t->scalar_type() != at::kBFloat16 || t->sizes() != x.sizes() || t->layout() != at::kStrided)
+            return py::none();
+    for (const Tensor* t : {&gamma, &beta, cbias ? &*cbias : &gamma})
+        if (t->device() != x.device() || t->sizes() != at::IntArrayRef({C}) ||
+            (t->scalar_type() != at::kBFloat16 && t->scalar_type() != at::kFloat && t->scalar_type() != at::kHalf))
+            return py::none();
+    if (only_plain && !plain({&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})) return py::none();
+    no_transforms();
+    const bool grad = recorded({&x, &branch, &gamma, &beta, gate ? &*gate : &x}, cbias);
+    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, grad); });
+    return py::make_tuple(o[0], o[1]);
+}
+
+// ---------------------------------------------------------------------------------------
+// cross entropy over the last dimension
+// ---------------------------------------------------------------------------------------
+struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
+    // logits as rows, `ld` elements apart: as they lie where that is possible
+    static std::pair<Tensor, int64_t> rows(const Tensor& logits) {
+        const int64_t V = logits.size(-1);
+        Tensor l = logits.reshape({-1, V});
+        if ((V > 1 && l.stride(1) != 1) || (l.size(0) > 1 && l.stride(0) < V)) l = l.contiguous();
+        return {l, l.size(0) > 1 ? l.stride(0) : V};
+    }
+    static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, int64_t ignore) {
+        const auto [l, ld] = rows(logits);
+        const Tensor t = targets.to(at::kLong).contiguous();
+        const Tensor loss = empty(targets.sizes(), at::kFloat, logits), stats = empty({t.numel(), 2}, at::kFloat, logits);
+        check(rwkv6_cross_entropy_fwd(ptr(l), l.scalar_type() == at::kFloat ? RWKV6_F32 : RWKV6_BF16, ld,
+                                      static_cast<const int64_t*>(ptr(t)), ignore, fptr(loss), fptr(stats), t.numel(), l.size(1),
+                                      stream_of(logits)),
+              "rwkv6_cross_entropy_fwd");
+        ctx->save_for_backward({logits, t, stats});
+        put(ctx, {ignore});
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor &logits = s[0], &t = s[1];
+        const int64_t ignore = meta(ctx)[0], V = logits.size(-1);
+        if (at::GradMode::is_enabled()) {
+            // a backward that is differentiated itself: the formula in torch's operators
+            const Tensor at_t = t.clamp(0, V - 1).unsqueeze(-1), bad = ((t < 0) | (t >= V)) & (t != ignore);
+            const Tensor p = at::softmax(logits.to(at::kFloat), -1);
+            const Tensor d = (p - at::zeros_like(p).scatter(-1, at_t, 1)) * g[0].to(at::kFloat).unsqueeze(-1);
+            return {d.masked_fill((t == ignore).unsqueeze(-1), 0).masked_fill(bad.unsqueeze(-1), NAN).to(logits.scalar_type()), Tensor(), Tensor()};
+        }
+        const auto [l, ld] = rows(logits);
+        const Tensor dl = to_f32(g[0]), d = empty({l.size(0), V}, l.scalar_type(), l);
+        check(rwkv6_cross_entropy_bwd(ptr(l), l.scalar_type() == at::kFloat ? RWKV6_F32 : RWKV6_BF16, ld,
+                                      static_cast<const int64_t*>(ptr(t)), ignore, fptr(s[2]), fptr(dl), ptr(d), l.size(0), V,
+                                      stream_of(logits)),
+              "rwkv6_cross_entropy_bwd");
+        return {d.view(logits.sizes()), Tensor(), Tensor()};
+    }
+};
+Tensor cross_entropy(const Tensor& logits, const Tensor& targets, int64_t ignore) {
+    no_transforms();
+    return unlocked([&] { return CrossEntropy::apply(logits, targets, ignore); });
+}
+
+// ---------------------------------------------------------------------------------------
+// AdamW over many tensors
+// ---------------------------------------------------------------------------------------
+int float_code(const Tensor& t, const char* what) {
+    if (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kFloat)
+        C10_THROW_ERROR(TypeError, std::string(what) + " must be bfloat16 or float32");
+    return t.scalar_type() == at::kBFloat16 ? RWKV6_BF16 : RWKV6_F32;
+}
+void need(bool ok, const std::string& msg) {
+    if (!ok) C10_THROW_ERROR(ValueError, msg);
+}
+// whether the elements of two tensors of the same sizes lie in the same order
+bool same_order(const Tensor& a, const Tensor& b) {
+    for (int64_t d = 0; d < a.dim(); ++d)
+        if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+    return true;
+}
+
+struct Grads {
+    std::vector<Tensor> t;
+    std::vector<const void*> p;
+    std::vector<int> dt;
+    std::vector<int64_t> n;
+};
+// The squares' partial sums over all gradients (rwkv6_grad_norm_sums), on their device.
+Tensor grad_norm_sums(const std::vector<Tensor>& grads) {
+    Grads g;
+    for (const Tensor& t : grads) {
+        need(t.is_cuda() && t.layout() == at::kStrided && t.device() == grads[0].device(), "gradients must be dense, on one GPU");
+        g.t.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
+        g.p.push_back(ptr(g.t.back()));
+        g.dt.push_back(float_code(t, "gradients"));
+        g.n.push_back(t.numel());
+    }
+    need(!grads.empty(), "no gradients");
+    const int64_t n = (int64_t)g.n.size();
+    const Tensor part = empty({rwkv6_grad_norm_partials(g.n.data(), n)}, at::kDouble, grads[0]);
+    unlocked([&] {
+        check(rwkv6_grad_norm_sums(g.p.data(), g.dt.data(), g.n.data(), n, static_cast<double*>(ptr(part)), stream_of(part)),
+              "rwkv6_grad_norm_sums");
+    });
+    return part;
+}
+Tensor grad_norm(const Tensor& partials) {
+    const Tensor norm = empty({}, at::kFloat, partials);
+    check(rwkv6_grad_norm(static_cast<const double*>(ptr(partials)), partials.numel(), fptr(norm), stream_of(partials)),
+          "rwkv6_grad_norm");
+    return norm;
+}
+
+// One step over the lists, in place; returns the norm (0-dim) when there are partial sums, else None.
+py::object adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m,
+                      const std::vector<Tensor>& v, const std::vector<Tensor>& ms, const std::vector<Tensor>& vs,
+                      const Tensor& step, double lr, const OptTensor& lr_dev, double b1, double b2, double eps, double wd,
+                      double max_norm, const OptTensor& partials) {
+    const size_t n = params.size();
+    const bool f8 = !ms.empty() || !vs.empty();
+    need(n > 0, "no parameters");
+    need(grads.size() == n && m.size() == n && v.size() == n && (!f8 || (ms.size() == n && vs.size() == n)), "lists of different lengths");
+    need(step.is_cuda() && step.scalar_type() == at::kFloat && step.numel() == 1, "step must be one float32 number on the GPU");
+    std::vector<Tensor> kept;
+    std::vector<void*> pp(n), pm(n), pv(n);
+    std::vector<const void*> pg(n);
+    std::vector<float*> psm(n), psv(n);
+    std::vector<int> pt(n), gt(n);
+    std::vector<int64_t> num(n);
+    const auto dev = params[0].device();
+    need(step.device() == dev, "step must lie on the parameters' device");
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor &p = params[i], *g = &grads[i];
+        need(p.is_cuda() && p.device() == dev, "parameters must live on one GPU");
+        need(p.layout() == at::kStrided && p.is_non_overlapping_and_dense(), "a parameter's elements must be dense in memory");
+        need(g->device() == dev && g->layout() == at::kStrided && g->sizes() == p.sizes(), "a gradient does not match its parameter");
+        pt[i] = float_code(p, "parameters");
+        gt[i] = float_code(*g, "gradients");
+        if (!g->is_non_overlapping_and_dense() || !same_order(p, *g)) {
+            kept.push_back(at::empty_like(p, p.options().dtype(g->scalar_type()), at::MemoryFormat::Preserve));
+            kept.back().copy_(*g);
+            g = &kept.back();
+        }
+        pg[i] = ptr(*g);
+        for (const Tensor* t : {&m[i], &v[i]}) {
+            need(t->device() == dev && t->layout() == at::kStrided && t->sizes() == p.sizes() && t->is_non_overlapping_and_dense() && same_order(p, *t),
+                 "a state does not match its parameter");
+            if (t->scalar_type() != (f8 ? at::kFloat8_e4m3fn : at::kFloat))
+                C10_THROW_ERROR(TypeError, f8 ? "states with scales must be float8_e4m3fn" : "states without scales must be float32");
+        }
+        if (f8)
+            for (const Tensor* t : {&ms[i], &vs[i]})
+                need(t->device() == dev && t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == (p.numel() + 255) / 256,
+                     "scales must be float32, one for 256 elements");
+        pp[i] = ptr(p);
+        pm[i] = ptr(m[i]);
+        pv[i] = ptr(v[i]);
+        if (f8) {
+            psm[i] = fptr(ms[i]);
+            psv[i] = fptr(vs[i]);
+        }
+        num[i] = p.numel();
+    }
+    float* lrp = nullptr;
+    if (lr_dev) {
+        need(lr_dev->device() == dev && lr_dev->scalar_type() == at::kFloat && lr_dev->numel() == 1, "a learning rate tensor must be one float32 number on the parameters' device");
+        lrp = fptr(*lr_dev);
+    }
+    const bool clip = partials.has_value();
+    if (clip) need(partials->device() == dev && partials->scalar_type() == at::kDouble && partials->is_contiguous(), "partial sums must be float64 on the parameters' device");
+    const Tensor work = empty({4}, at::kFloat, step), norm = clip ? empty({}, at::kFloat, step) : Tensor();
+    unlocked([&] {
+        check(rwkv6_adamw_step(pp.data(), pt.data(), pg.data(), gt.data(), pm.data(), pv.data(), f8 ? psm.data() : nullptr,
+                               f8 ? psv.data() : nullptr, num.data(), (int64_t)n, fptr(step), lr, lrp, b1, b2, eps, wd,
+                               clip ? static_cast<const double*>(ptr(*partials)) : nullptr, clip ? partials->numel() : 0,
+                               (float)max_norm, fptr(norm), fptr(work), stream_of(step)),
+              "rwkv6_adamw_step");
+    });
+    // the tensors changed: a backward that still needs one of them as it was says so
+    auto bump = [](const Tensor& t) {
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    bump(step);
+    for (const auto* list : {&params, &m, &v, &ms, &vs})
+        for (const Tensor& t : *list) bump(t);
+    if (!clip) return py::none();
+    return py::cast(norm);
+}
+
+// ---------------------------------------------------------------------------------------
 // channel mix
 // ---------------------------------------------------------------------------------------
 struct CmixLerp : torch::autograd::Function<CmixLerp> {
@@ -615,6 +892,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("decay_lora", torch::wrap_pybind_function(decay_lora));
     m.def("group_norm_gate", torch::wrap_pybind_function(group_norm_gate));
     m.def("layer_norm", torch::wrap_pybind_function(layer_norm));
+    m.def("residual_norm", torch::wrap_pybind_function(residual_norm));
+    m.def("cross_entropy", torch::wrap_pybind_function(cross_entropy));
+    m.def("grad_norm_sums", torch::wrap_pybind_function(grad_norm_sums));
+    m.def("grad_norm", torch::wrap_pybind_function(grad_norm));
+    m.def("adamw_step", torch::wrap_pybind_function(adamw_step));
     m.def("cmix_lerp", torch::wrap_pybind_function(cmix_lerp));
     m.def("relu_sq", torch::wrap_pybind_function(relu_sq));
     m.def("sigmoid_gate", torch::wrap_pybind_function(sigmoid_gate));

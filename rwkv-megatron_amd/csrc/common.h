@@ -194,6 +194,14 @@ __device__ __forceinline__ float sum8lanes(float v) {
     return v;
 }
 
+// Sum over the wave; all lanes get the same bits.
+__device__ __forceinline__ float wave_sum(float v) {
+    v = sum8lanes(v);
+    v += dpp_mov<0x140>(v);                       // row_mirror: the other 8 lanes of the row
+    const RowSums r = row_sums(v);
+    return r.lo + r.hi;
+}
+
 // Host side: a device buffer as (address, bytes).  Entry points reject calls where an output
 // overlaps an input or another output: several kernels re-load a clamped last piece after
 // other threads have stored theirs, and the walks read chunk c + 1 before storing chunk c, so

@@ -23,12 +23,6 @@
 
 namespace {
 
-__device__ __forceinline__ float ln_wave_sum(float v) {
-    v = sum8lanes(v);
-    v += dpp_mov<0x140>(v);                       // row_mirror: the other 8 lanes of the row
-    const RowSums r = row_sums(v);
-    return r.lo + r.hi;
-}
 // The lane's pieces of a row: channels 8 (lane + 64 i).., zeros past the end.
 template <int NV>
 __device__ __forceinline__ void ln_load(const uint16_t* row, int C, int lane, uint4* q) {
@@ -74,7 +68,7 @@ rwkv6_layer_norm_fwd_kernel(const uint16_t* __restrict__ x, const void* __restri
 #pragma unroll
         for (int j = 0; j < 8; ++j) s += v[j];
     }
-    const float inv = 1.f / (float)C, mean = ln_wave_sum(s) * inv;
+    const float inv = 1.f / (float)C, mean = wave_sum(s) * inv;
     float var = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -84,7 +78,7 @@ rwkv6_layer_norm_fwd_kernel(const uint16_t* __restrict__ x, const void* __restri
 #pragma unroll
             for (int j = 0; j < 8; ++j) var += (v[j] - mean) * (v[j] - mean);
     }
-    const float rstd = rsqrtf(ln_wave_sum(var) * inv + eps);
+    const float rstd = rsqrtf(wave_sum(var) * inv + eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = 8 * (lane + 64 * i);
@@ -162,8 +156,8 @@ rwkv6_layer_norm_bwd_kernel(const uint16_t* __restrict__ x, const void* __restri
                 s2 += g[j] * ga[j] * xh[j];
             }
         }
-        s1 = ln_wave_sum(s1) * inv;
-        s2 = ln_wave_sum(s2) * inv;
+        s1 = wave_sum(s1) * inv;
+        s2 = wave_sum(s2) * inv;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = 8 * (lane + 64 * i);

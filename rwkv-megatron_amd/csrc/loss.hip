@@ -1,0 +1,226 @@
+// Cross entropy of token rows over the vocabulary and its gradient, for MI355X (gfx950).
+//
+// Reference: the language model's loss a token, which the training driver averages over the unmasked
+// tokens (/root/reference/pretrain_rwkv6.py:144-179; the output head's logits, rwkv6_model.py:28-184).
+//   loss = log z + (m - l_t),  m = max_j l_j,  z = sum_j exp(l_j - m)     (0 for an ignored target)
+//   d_l_j = d_loss (exp(l_j - m) / z - [j = t])                            (0 for an ignored target)
+// The forward reads the logits once, each thread with a running maximum and sum that are joined at the
+// end, and keeps m and z of a row: (m, 1/z) instead of log z + m keeps the gradient's exponent free of
+// the rounding of a number of size 10.  Bound by the reads (forward) and reads and writes (backward).
+#include "common.h"
+#include "../../include/rwkv6_amd.h"
+
+#define CE_GRID (1 << 16)
+
+namespace {
+
+template <bool F32> struct CeVec { static constexpr int E = F32 ? 4 : 8; };     // elements of 16 bytes
+
+template <bool F32>
+__device__ __forceinline__ void ce_unpack(uint4 q, float* f) {
+    if constexpr (F32) {
+        f[0] = __uint_as_float(q.x); f[1] = __uint_as_float(q.y);
+        f[2] = __uint_as_float(q.z); f[3] = __uint_as_float(q.w);
+    } else {
+        unpack8(q, f);
+    }
+}
+template <bool F32>
+__device__ __forceinline__ float ce_load(const char* row, int64_t j) {
+    if constexpr (F32) return reinterpret_cast<const float*>(row)[j];
+    else return bf2f(reinterpret_cast<const uint16_t*>(row)[j]);
+}
+// elements before the row's first 16-byte boundary (rows lie at multiples of the element's size)
+template <bool F32>
+__device__ __forceinline__ int ce_lead(const void* row, int64_t V) {
+    const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15u) / (F32 ? 4 : 2), E = CeVec<F32>::E;
+    const int lead = off ? E - off : 0;
+    return lead < V ? lead : (int)V;
+}
+
+// (m, z) of a set of logits: z = sum exp(l - m).  An empty set, or one of -inf alone, is (-inf, 0).
+struct Soft {
+    float m, z;
+};
+__device__ __forceinline__ float ce_ref(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ Soft join(Soft a, Soft b) {
+    const float m = fmaxf(a.m, b.m), r = ce_ref(m);
+    return {m, a.z * ex2((a.m - r) * RW_L2E) + b.z * ex2((b.m - r) * RW_L2E)};
+}
+template <int K> __device__ __forceinline__ void ce_take(Soft& s, const float* v) {
+    float m = s.m;
+#pragma unroll
+    for (int k = 0; k < K; ++k) m = fmaxf(m, v[k]);
+    const float r = ce_ref(m);
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) t += ex2((v[k] - r) * RW_L2E);
+    s.z = s.z * ex2((s.m - r) * RW_L2E) + t;
+    s.m = m;
+}
+}  // namespace
+
+// One block a row (striding over the rows), CE_U pieces of 16 bytes a thread in flight.
+#define CE_U 4
+template <bool F32, int THR>
+__global__ void __launch_bounds__(THR)
+rwkv6_cross_entropy_fwd_kernel(const void* __restrict__ logits, int64_t ld, const int64_t* __restrict__ target,
+                               int64_t ignore, float* __restrict__ loss, float2* __restrict__ stats, int64_t N,
+                               int64_t V) {
+    constexpr int E = CeVec<F32>::E, ES = F32 ? 4 : 2;
+    __shared__ Soft part[THR / 64];
+    for (int64_t n = blockIdx.x; n < N; n += gridDim.x) {
+        const int64_t t = target[n];
+        const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
+        if (ignored || bad) {                             // uniform over the block
+            if (threadIdx.x == 0) {
+                loss[n] = ignored ? 0.f : NAN;
+                stats[n] = make_float2(0.f, 1.f);
+            }
+            continue;
+        }
+        const char* row = reinterpret_cast<const char*>(logits) + n * ld * ES;
+        const int lead = ce_lead<F32>(row, V);
+        const int64_t pieces = (V - lead) / E, tail = lead + pieces * E;
+        const uint4* body = reinterpret_cast<const uint4*>(row + (int64_t)lead * ES);
+        Soft s = {-INFINITY, 0.f};
+        int64_t i = threadIdx.x;
+        for (; i + (CE_U - 1) * THR < pieces; i += CE_U * THR) {
+            float v[CE_U * E];
+#pragma unroll
+            for (int u = 0; u < CE_U; ++u) ce_unpack<F32>(body[i + u * THR], v + u * E);
+            ce_take<CE_U * E>(s, v);
+        }
+        for (; i < pieces; i += THR) {
+            float v[E];
+            ce_unpack<F32>(body[i], v);
+            ce_take<E>(s, v);
+        }
+        // fewer than 8 elements at either end
+        if ((int)threadIdx.x < lead) {
+            const float v = ce_load<F32>(row, threadIdx.x);
+            ce_take<1>(s, &v);
+        }
+        if ((int64_t)threadIdx.x < V - tail) {
+            const float v = ce_load<F32>(row, tail + threadIdx.x);
+            ce_take<1>(s, &v);
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) s = join(s, Soft{__shfl_xor(s.m, o), __shfl_xor(s.z, o)});
+        __syncthreads();                                  // the row before has been read from `part`
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < THR / 64; ++w) s = join(s, part[w]);
+            loss[n] = logf(s.z) + (s.m - ce_load<F32>(row, t));
+            stats[n] = make_float2(s.m, s.z);
+        }
+    }
+}
+
+// Block (row, segment): the row's elements cut into gridDim.y runs of pieces.
+template <bool F32>
+__global__ void __launch_bounds__(256)
+rwkv6_cross_entropy_bwd_kernel(const void* __restrict__ logits, int64_t ld, const int64_t* __restrict__ target,
+                               int64_t ignore, const float2* __restrict__ stats, const float* __restrict__ d_loss,
+                               void* __restrict__ d_logits, int64_t N, int64_t V) {
+    constexpr int E = CeVec<F32>::E, ES = F32 ? 4 : 2;
+    for (int64_t n = blockIdx.x; n < N; n += gridDim.x) {
+        const int64_t t = target[n];
+        const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
+        const char* row = reinterpret_cast<const char*>(logits) + n * ld * ES;
+        char* out = reinterpret_cast<char*>(d_logits) + n * V * ES;
+        const float2 st = stats[n];
+        // an ignored row's zeros and a bad one's NaN do not depend on its logits
+        const float w = bad ? NAN : ignored ? 0.f : d_loss[n], q = w / st.y, m = st.x;
+        auto grad = [&](float l, int64_t j) {
+            if (ignored || bad) return w;
+            const float p = q * ex2((l - m) * RW_L2E);
+            return j == t ? p - w : p;
+        };
+        auto store = [&](int64_t j, float g) {
+            if constexpr (F32) reinterpret_cast<float*>(out)[j] = g;
+            else reinterpret_cast<uint16_t*>(out)[j] = f2bf(g);
+        };
+        const int lead = ce_lead<F32>(out, V);
+        const int64_t pieces = (V - lead) / E, tail = lead + pieces * E;
+        const bool vec = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+        const int64_t per = (pieces + gridDim.y - 1) / gridDim.y, i0 = per * blockIdx.y;
+        const int64_t i1 = i0 + per < pieces ? i0 + per : pieces;
+        for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
+            const int64_t j = lead + i * E;
+            float v[E];
+            if (vec) {
+                ce_unpack<F32>(*reinterpret_cast<const uint4*>(row + j * ES), v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < E; ++k) v[k] = ce_load<F32>(row, j + k);
+            }
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[k] = grad(v[k], j + k);
+            if constexpr (F32) *reinterpret_cast<float4*>(out + j * ES) = make_float4(v[0], v[1], v[2], v[3]);
+            else store8(reinterpret_cast<uint16_t*>(out) + j, v);
+        }
+        if (blockIdx.y == 0) {
+            if ((int)threadIdx.x < lead) store(threadIdx.x, grad(ce_load<F32>(row, threadIdx.x), threadIdx.x));
+            if ((int64_t)threadIdx.x < V - tail)
+                store(tail + threadIdx.x, grad(ce_load<F32>(row, tail + threadIdx.x), tail + threadIdx.x));
+        }
+    }
+}
+
+namespace {
+int ce_check(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t N, int64_t V) {
+    if (N < 0 || V < 1 || ld < V) return RWKV6_ERR_INVALID_ARG;
+    if (dtype != RWKV6_F32 && dtype != RWKV6_BF16) return RWKV6_ERR_INVALID_ARG;
+    if (V > ((int64_t)1 << 30) || ld > ((int64_t)1 << 40) || N > ((int64_t)1 << 50) / ld) return RWKV6_ERR_UNSUPPORTED;
+    if (N > 0 && (!logits || !target)) return RWKV6_ERR_INVALID_ARG;
+    // rows may start at any element
+    if (reinterpret_cast<uintptr_t>(logits) % param_bytes(dtype)) return RWKV6_ERR_ALIGNMENT;
+    return RWKV6_OK;
+}
+// bytes from the first logit to the last
+size_t ce_span(int64_t ld, int64_t N, int64_t V, int dtype) { return (size_t)((N - 1) * ld + V) * param_bytes(dtype); }
+}  // namespace
+
+extern "C" {
+
+int rwkv6_cross_entropy_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t ignore_index,
+                            float* loss, float* stats, int64_t N, int64_t V, void* stream) {
+    const int st = ce_check(logits, dtype, ld, target, N, V);
+    if (st || N == 0) return st;
+    if (!loss || !stats) return RWKV6_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(stats) & 7u) return RWKV6_ERR_ALIGNMENT;
+    if (any_alias({{loss, (size_t)N * 4}, {stats, (size_t)N * 8}},
+                  {{logits, ce_span(ld, N, V, dtype)}, {target, (size_t)N * 8}}))
+        return RWKV6_ERR_INVALID_ARG;
+    const bool f32 = dtype == RWKV6_F32, few = N < 1024;
+    auto k = f32 ? (few ? rwkv6_cross_entropy_fwd_kernel<true, 1024> : rwkv6_cross_entropy_fwd_kernel<true, 256>)
+                 : (few ? rwkv6_cross_entropy_fwd_kernel<false, 1024> : rwkv6_cross_entropy_fwd_kernel<false, 256>);
+    hipLaunchKernelGGL(k, dim3((unsigned)(N < CE_GRID ? N : CE_GRID)), dim3(few ? 1024 : 256), 0,
+                       reinterpret_cast<hipStream_t>(stream), logits, ld, target, ignore_index, loss, (float2*)stats, N, V);
+    return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+}
+
+int rwkv6_cross_entropy_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t ignore_index,
+                            const float* stats, const float* d_loss, void* d_logits, int64_t N, int64_t V,
+                            void* stream) {
+    const int st = ce_check(logits, dtype, ld, target, N, V);
+    if (st || N == 0) return st;
+    if (!stats || !d_loss || !d_logits) return RWKV6_ERR_INVALID_ARG;
+    if ((reinterpret_cast<uintptr_t>(stats) & 7u) || reinterpret_cast<uintptr_t>(d_logits) % param_bytes(dtype))
+        return RWKV6_ERR_ALIGNMENT;
+    if (any_alias({{d_logits, (size_t)(N * V) * param_bytes(dtype)}},
+                  {{logits, ce_span(ld, N, V, dtype)}, {target, (size_t)N * 8}, {stats, (size_t)N * 8}, {d_loss, (size_t)N * 4}}))
+        return RWKV6_ERR_INVALID_ARG;
+    // a row is cut until the blocks fill the device, each keeping a step of its 256 threads
+    int seg = 1;
+    while (seg < 64 && N * seg < 2048 && V >= (int64_t)seg * 2 * 256 * 8) seg *= 2;
+    auto k = dtype == RWKV6_F32 ? rwkv6_cross_entropy_bwd_kernel<true> : rwkv6_cross_entropy_bwd_kernel<false>;
+    hipLaunchKernelGGL(k, dim3((unsigned)(N < CE_GRID ? N : CE_GRID), (unsigned)seg), dim3(256), 0,
+                       reinterpret_cast<hipStream_t>(stream), logits, ld, target, ignore_index, (const float2*)stats, d_loss,
+                       d_logits, N, V);
+    return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -1,0 +1,250 @@
+"""AdamW over many tensors at once, with states in 32 or in 8 bits and clipping by the gradients' norm.
+
+The reference trains with AdamW, decoupled weight decay and a gradient clip
+(/root/reference/example_config.yaml:199-221; Megatron's training loop, pretrain_rwkv6.py:281-286).
+
+    norm = sqrt(sum of all gradients' squares)        c = min(1, max_norm / (norm + 1e-6))
+    g = c g;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  t = step + 1
+    p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+* ``AdamW`` is the optimizer (a torch.optim.Optimizer); ``adamw_step`` the same step on lists of
+  tensors; ``grad_norm`` the norm alone.
+* Parameters are bf16 or fp32; the arithmetic and the moments are fp32, p is rounded once.  A bf16
+  parameter has no wider copy: where that matters keep the parameters in fp32, as the modules here
+  take them.
+* 8-bit states: float8 (e4m3) codes and one fp32 scale for every 256 consecutive elements; the second
+  moment by its root, which doubles the range that a code covers.  A code rounds a value by 2^-4 of it
+  at most, and an element whose magnitude relative to its block's largest changes by less than that
+  in a step keeps its code: the second moments of a block rise and fall with the largest.
+* A step is a handful of launches whatever the number of tensors, nothing is copied to or read from
+  the device, and the step count lives there: a captured step (HIP graph) counts on replay.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+BLOCK = 256                    # elements under one scale of an 8-bit state
+
+
+def grad_norm(grads):
+    """The 2-norm of all elements of `grads` (bf16 or fp32 tensors on one GPU), a 0-dim fp32 tensor; the sum
+    of squares in 64 bits, in a fixed order."""
+    grads = _tensors("grads", grads)
+    native = _lib.native()
+    return native.grad_norm(native.grad_norm_sums(grads))
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               max_norm=None, scales=None):
+    """One AdamW step over lists of tensors, in place.
+
+    params, grads: bf16 or fp32, dense in memory; exp_avgs, exp_avg_sqs: fp32 of the parameters' shapes,
+    or with scales = (exp_avg_scales, exp_avg_sq_scales) float8_e4m3fn codes, the scales fp32
+    [ceil(numel / 256)] a tensor (exp_avg_sqs then stands for the roots: v = (code * scale)^2).  step: one
+    fp32 number on the GPU, the steps done before; it is counted up.  lr is a number or a one-element fp32
+    tensor on the GPU.  With max_norm the gradients count times min(1, max_norm / (norm + 1e-6)), without
+    being changed, and the norm over all of them is returned (0-dim fp32), else None."""
+    params, grads = _tensors("params", params), _tensors("grads", grads)
+    m, v = _tensors("exp_avgs", exp_avgs), _tensors("exp_avg_sqs", exp_avg_sqs)
+    ms, vs = ([], []) if scales is None else (_tensors("scales", scales[0]), _tensors("scales", scales[1]))
+    if scales is not None and not len(ms) == len(vs) == len(params):
+        raise ValueError("lists of different lengths")
+    _check_hyper(lr, betas, eps, weight_decay, max_norm)
+    native = _lib.native()
+    sums = None if max_norm is None else native.grad_norm_sums(grads)
+    return _step(native, params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, max_norm, sums)
+
+
+def _step(native, params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, max_norm, sums):
+    tensor = isinstance(lr, torch.Tensor)
+    return native.adamw_step(params, grads, m, v, ms, vs, step, 0.0 if tensor else float(lr), lr if tensor else None,
+                             betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, sums)
+
+
+def _tensors(name, ts):
+    ts = list(ts)
+    if not ts or not all(isinstance(t, torch.Tensor) for t in ts):
+        raise TypeError(f"{name} must be tensors, one at least")
+    return ts
+
+
+def _check_hyper(lr, betas, eps, weight_decay, max_norm):
+    if not isinstance(lr, torch.Tensor) and not lr >= 0:
+        raise ValueError(f"invalid learning rate {lr}")
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+        raise ValueError(f"betas must lie in [0, 1), got {betas}")
+    if not eps >= 0 or not weight_decay >= 0:
+        raise ValueError(f"eps and weight_decay must not be negative, got {eps} and {weight_decay}")
+    if max_norm is not None and not max_norm > 0:
+        raise ValueError(f"max_norm must be positive, got {max_norm}")
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay over bf16 or fp32 parameters on one GPU.
+
+    state_bits=8 keeps the moments in 8 bits (module docstring) for tensors of min_8bit_numel elements and
+    more; smaller ones (norms, biases, mixing coefficients) keep 32 bits.  max_norm clips by the norm of
+    all gradients of the step, in all groups (`grad_norm` holds it afterwards, a 0-dim tensor); the
+    gradients themselves stay as they are.  lr may be a one-element fp32 tensor on the GPU, which a
+    captured step reads on replay.
+
+    State of a parameter: ``step`` (one tensor for all parameters that have made the same steps),
+    ``exp_avg`` and ``exp_avg_sq`` (fp32), or in 8 bits ``exp_avg``, ``exp_avg_scale``, ``exp_avg_sq_root`` and
+    ``exp_avg_sq_scale``.  A state dict of torch.optim.AdamW loads; states are converted to the kind
+    that this optimizer keeps for the parameter."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32,
+                 max_norm=None, min_8bit_numel=4096):
+        _check_hyper(lr, betas, eps, weight_decay, max_norm)
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        self.state_bits, self.max_norm, self.min_8bit_numel = state_bits, max_norm, min_8bit_numel
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        try:
+            _check_hyper(g["lr"], g["betas"], g["eps"], g["weight_decay"], None)
+            for p in g["params"]:
+                if p.dtype not in (torch.bfloat16, torch.float32):
+                    raise TypeError(f"parameters must be bfloat16 or float32, got {p.dtype}")
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def _eight(self, p):
+        return self.state_bits == 8 and p.numel() >= self.min_8bit_numel
+
+    def _new_state(self, p):
+        like = dict(memory_format=torch.preserve_format)
+        if not self._eight(p):
+            return {"exp_avg": torch.zeros_like(p, dtype=torch.float32, **like),
+                    "exp_avg_sq": torch.zeros_like(p, dtype=torch.float32, **like)}
+        scale = lambda: torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
+        code = lambda: torch.zeros_like(p, dtype=torch.uint8, **like).view(torch.float8_e4m3fn)
+        return {"exp_avg": code(), "exp_avg_scale": scale(), "exp_avg_sq_root": code(), "exp_avg_sq_scale": scale()}
+
+    def _lists(self, group):
+        """The group's parameters with gradients in lists that one call updates: those of one kind of state
+        that have made the same steps, and so share the tensor that counts them."""
+        lists, sharing, new = {}, {}, {}
+        for p in group["params"]:
+            if p.grad is not None:
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                if p.device.type != "cuda":
+                    raise ValueError("parameters must live on the GPU")
+                if not self.state[p]:
+                    key = (p.device, self._eight(p))
+                    if key not in new:
+                        new[key] = torch.zeros((), dtype=torch.float32, device=p.device)
+                    self.state[p].update(step=new[key], **self._new_state(p))
+            if self.state.get(p):
+                key = id(self.state[p]["step"])
+                sharing[key] = sharing.get(key, 0) + 1
+                if p.grad is not None:
+                    lists.setdefault(key, []).append(p)
+        for key, ps in lists.items():
+            if len(ps) < sharing[key]:             # the others make no step: these go on with a count of their own
+                step = self.state[ps[0]]["step"].clone()
+                for p in ps:
+                    self.state[p]["step"] = step
+        return list(lists.values())
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step; returns the closure's loss, if there is one."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = [(group, ps) for group in self.param_groups for ps in self._lists(group)]
+        if not work:
+            return loss
+        native, sums = _lib.native(), None
+        if self.max_norm is not None:
+            _check_hyper(0.0, (0, 0), 0, 0, self.max_norm)
+            sums = native.grad_norm_sums([p.grad for _, ps in work for p in ps])
+        for group, ps in work:
+            states = [self.state[p] for p in ps]
+            eight = "exp_avg_scale" in states[0]
+            take = lambda name: [s[name] for s in states]
+            norm = _step(native, ps, [p.grad for p in ps], take("exp_avg"),
+                         take("exp_avg_sq_root" if eight else "exp_avg_sq"), take("exp_avg_scale") if eight else [],
+                         take("exp_avg_sq_scale") if eight else [], states[0]["step"], group["lr"], group["betas"],
+                         group["eps"], group["weight_decay"], self.max_norm, sums)
+        self.grad_norm = norm
+        return loss
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """Loads a state dict of this class or of torch.optim.AdamW; states keep their own types (torch's
+        loading would cast them to the parameters')."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        ps = [p for g in self.param_groups for p in g["params"]]
+        saved = {p: state_dict["state"][i] for i, p in zip(ids, ps) if i in state_dict["state"]}
+        self.state.clear()
+        for group in self.param_groups:
+            steps = {}                             # one tensor for equal counts, as a run would have made them
+            for p in group["params"]:
+                if not saved.get(p):
+                    continue
+                state, old = self._new_state(p), saved[p]
+                key = (float(old["step"]), p.device, "exp_avg_scale" in state)
+                if key not in steps:
+                    steps[key] = torch.full((), key[0], dtype=torch.float32, device=p.device)
+                if ("exp_avg_scale" in state and "exp_avg_scale" in old
+                        and state["exp_avg"].stride() == old["exp_avg"].stride()):
+                    for name, t in state.items():
+                        t.copy_(old[name])
+                else:
+                    m, v = _moments(old)
+                    if "exp_avg_scale" in state:
+                        _encode(state["exp_avg"], state["exp_avg_scale"], m.to(p.device))
+                        _encode(state["exp_avg_sq_root"], state["exp_avg_sq_scale"], v.to(p.device).sqrt())
+                    else:
+                        state["exp_avg"].copy_(m)
+                        state["exp_avg_sq"].copy_(v)
+                self.state[p] = dict(step=steps[key], **state)
+
+    def moments(self, p):
+        """The fp32 values that a parameter's states stand for: (exp_avg, exp_avg_sq)."""
+        return _moments(self.state[p])
+
+
+def _flat(t):
+    """The elements of a dense tensor in the order they lie in memory."""
+    return t.as_strided((t.numel(),), (1,))
+
+
+def _decode(code, scale):
+    out = torch.empty_like(code, dtype=torch.float32)
+    s = scale.repeat_interleave(BLOCK)[:code.numel()]
+    _flat(out).copy_(_flat(code).float() * s)
+    return out
+
+
+def _encode(code, scale, value):
+    """value into code (of the same strides as the parameter) and scale, as the kernel rounds."""
+    v = torch.empty_like(code, dtype=torch.float32).copy_(value)
+    n = code.numel()
+    b = torch.zeros(scale.numel() * BLOCK, dtype=torch.float32, device=code.device)
+    b[:n] = _flat(v)
+    b = b.view(-1, BLOCK)
+    top = torch.where(b.isfinite(), b, 0).abs().amax(-1)
+    top = torch.where(top < 2.0 ** -118, 0.0, top)
+    inv = torch.where(top > 0, 448.0 / top, 0.0)
+    _flat(code).copy_((b * inv[:, None]).to(torch.float8_e4m3fn).view(-1)[:n])
+    scale.copy_(top / 448.0)
+
+
+def _moments(state):
+    if "exp_avg_scale" in state:
+        return (_decode(state["exp_avg"], state["exp_avg_scale"]),
+                _decode(state["exp_avg_sq_root"], state["exp_avg_sq_scale"]).square())
+    return state["exp_avg"].float(), state["exp_avg_sq"].float()

@@ -1,0 +1,201 @@
+"""loss.cross_entropy: values and gradients against float64 and differences, rows at every alignment,
+targets that are ignored or out of range, infinities."""
+import importlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ce():
+    return importlib.import_module("rwkv-megatron_amd").loss.cross_entropy
+
+
+def _inputs(shape, V, dtype, seed=0, ignored=0.2):
+    g = torch.Generator().manual_seed(seed + V)
+    l = (torch.randn(*shape, V, generator=g) * 3).to(dtype).to(DEV).requires_grad_(True)
+    t = torch.randint(0, V, shape, generator=g)
+    t = torch.where(torch.rand(shape, generator=g) < ignored, -100, t).to(DEV)
+    return l, t, torch.randn(shape, generator=g).to(DEV)
+
+
+def _exact(l, t, w):
+    d = l.detach().double().requires_grad_(True)
+    live = (t != -100).double()
+    losses = (torch.logsumexp(d, -1) - d.gather(-1, t.clamp(min=0).unsqueeze(-1))[..., 0]) * live
+    return losses.detach(), torch.autograd.grad(losses, d, w.double())[0]
+
+
+# Bounds: a loss is the log of a sum (relative error below 2^-18: at most 2^7 additions a thread of 32-bit
+# exponentials, each off by 2^-20) and a difference of numbers up to 16 (2^-19); a gradient is w times a
+# quotient of such a sum, and one rounding of its type.
+def _check(l, t, w, losses, d):
+    want, dwant = _exact(l, t, w)
+    assert losses.dtype == F32 and losses.shape == t.shape and d.dtype == l.dtype and d.shape == l.shape
+    assert bool(((losses.double() - want).abs() <= 2.0 ** -17 + 2.0 ** -22 * want.abs()).all())
+    p = torch.softmax(l.detach().double(), -1)
+    half = torch.finfo(d.dtype).eps / 2 * 1.01
+    bound = half * dwant.abs() + w.double().abs().unsqueeze(-1) * (2.0 ** -17 * p + 2.0 ** -22)
+    assert bool(((d.double() - dwant).abs() <= bound).all()), float(((d.double() - dwant).abs() - bound).max())
+    assert not bool(losses[t == -100].any()) and not bool(d[t == -100].any())
+
+
+# A vocabulary of one, below a piece of 16 bytes, at a thread's and a block's steps and one past them, odd
+# (every row starts at another alignment); one row, few rows (1024 threads each), many.
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("shape,V", [((1,), 1), ((5,), 3), ((2, 3), 8), ((17,), 77), ((1,), 2048), ((3,), 2049), ((9,), 8191),
+                                     ((2,), 32768), ((7,), 65536), ((3,), 50001), ((1025,), 333), ((1030,), 4104)])
+def test_matches_float64(ce, shape, V, dtype):
+    l, t, w = _inputs(shape, V, dtype)
+    losses = ce(l, t)
+    d = torch.autograd.grad(losses, l, w)[0]
+    again = ce(l, t)
+    assert torch.equal(losses, again) and torch.equal(d, torch.autograd.grad(again, l, w)[0])
+    _check(l, t, w, losses.detach(), d)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("form", ["padded", "odd_start", "transposed", "expanded", "int32"])
+def test_rows_as_they_lie(ce, form, dtype):
+    l, t, w = _inputs((6, 5), 129, dtype)
+    losses = ce(l, t)
+    base = losses.detach(), torch.autograd.grad(losses, l, w)[0]
+    if form == "int32":
+        assert torch.equal(ce(l, t.int()), base[0])
+        return
+    if form == "expanded":
+        row = l.detach()[:1, :1].clone().requires_grad_(True)
+        losses = ce(row.expand(6, 5, 129), t)
+        full = row.detach().expand(6, 5, 129).contiguous().requires_grad_(True)
+        a, b = torch.autograd.grad(losses, row, w)[0], torch.autograd.grad(ce(full, t), full, w)[0]
+        want = b.double().sum((0, 1), keepdim=True)
+        # torch adds the 30 gradients and rounds once
+        assert bool(((a.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * b.double().abs().sum((0, 1))).all())
+        return
+    big = torch.randn(6, 5, 136, device=DEV).to(dtype)
+    if form == "padded":
+        u = big[..., :129]
+    elif form == "odd_start":
+        u = big[..., 3:132]
+    else:
+        u = torch.empty(5, 6, 129, device=DEV, dtype=dtype).transpose(0, 1)
+    u.copy_(l.detach())
+    u = u.detach().requires_grad_(True)
+    losses = ce(u, t)
+    d = torch.autograd.grad(losses, u, w)[0]
+    _check(u, t, w, losses.detach(), d)
+    # the elements meet other threads where a row starts elsewhere: values agree to the bounds, not the bits
+    assert float((losses.detach() - base[0]).abs().max()) <= 2.0 ** -16
+
+
+def test_gradient_against_differences(ce):
+    l, t, w = _inputs((12,), 300, F32)
+    grad = torch.autograd.grad(ce(l, t), l, w)[0].double()
+    move = 0.05 * grad / grad.norm()
+    hi, lo = (l.detach() + move).float(), (l.detach() - move).float()
+    value = lambda v: float((ce(v, t).double() * w.double()).sum())
+    want = float((grad * (hi.double() - lo.double())).sum())
+    # losses of size 10 in 32 bits: 12 roundings of 2^-20 over a difference of about 0.1 |grad|; the third
+    # derivative: 0.05^2 / 6 of it
+    assert abs(value(hi) - value(lo) - want) <= 2.0 ** -9 * abs(want)
+
+
+def test_edges_of_logits_and_targets(ce):
+    inf, nan = float("inf"), float("nan")
+    l, _, _ = _inputs((8,), 40, F32)
+    t = torch.tensor([3, 3, 3, 3, -100, 40, -1, 3], device=DEV)
+    with torch.no_grad():
+        l[0, 10:] = -inf                       # a masked vocabulary
+        l[1, 3] = -inf                         # the target itself masked
+        l[2] = torch.finfo(F32).min            # all at the lowest number
+        l[3, 7] = nan
+        l[4] = nan                             # an ignored row may hold anything
+        l[7] = -inf
+    losses = ce(l, t)
+    d = torch.autograd.grad(losses, l, torch.ones(8, device=DEV))[0]
+    want = torch.logsumexp(l[0, :10].double(), -1) - l[0, 3].double()
+    assert abs(float(losses[0] - want)) <= 2.0 ** -17 and not bool(d[0, 10:].any())
+    assert float(losses[1]) == inf and float(d[1, 3]) == -1
+    assert abs(float(losses[2]) - float(torch.log(torch.tensor(40.0)))) <= 2.0 ** -18
+    assert float(losses[4]) == 0 and not bool(d[4].any())
+    for row in (3, 5, 6, 7):
+        assert bool(losses[row].isnan()) and bool(d[row].isnan().any())
+    assert bool(ce(l[:1], torch.tensor([40], device=DEV), ignore_index=40).eq(0).all())
+
+
+def test_a_long_vocabulary_and_offsets_past_32_bits(ce):
+    """Rows further than 2^31 elements into the tensor, of a vocabulary of a million."""
+    V, N = 1 << 20, 2100
+    l = torch.empty(N, V, device=DEV, dtype=BF)
+    l.zero_()
+    t = torch.full((N,), -100, device=DEV)
+    g = torch.Generator().manual_seed(1)
+    rows = [0, 2047, 2049, 2099]
+    for r in rows:
+        l[r] = torch.randn(V, generator=g).to(BF).to(DEV)
+        t[r] = V - 1 - r
+    l.requires_grad_(True)
+    losses = ce(l, t)
+    w = torch.ones(N, device=DEV)
+    d = torch.autograd.grad(losses, l, w)[0]
+    for r in rows:
+        # 2^20 terms over 256 threads: 2^9 additions of pieces in 32 bits, 2^-15
+        x = l.detach()[r].double()
+        assert abs(float(losses[r].double() - (torch.logsumexp(x, -1) - x[V - 1 - r]))) <= 2.0 ** -14
+        want = torch.softmax(x, -1)
+        want[V - 1 - r] -= 1
+        assert bool(((d[r].double() - want).abs() <= 2.0 ** -8 * 1.02 * want.abs() + 2.0 ** -40).all())
+    assert not bool(d[1].any()) and not bool(d[2098].any())
+
+
+def test_empty_no_grad_second_derivative_and_hooks(ce):
+    l, t, w = _inputs((5,), 33, F32)
+    assert ce(l[:0], t[:0]).shape == (0,)
+    e = l.detach()[:0].requires_grad_(True)
+    assert torch.autograd.grad(ce(e, t[:0]), e, w[:0])[0].shape == (0, 33)
+    with torch.no_grad():
+        assert not ce(l, t).requires_grad
+    g1 = torch.autograd.grad(ce(l, t), l, w, create_graph=True)[0]
+    got = torch.autograd.grad(g1.square().sum(), l)[0]
+    d = l.detach().double().requires_grad_(True)
+    live = (t != -100).double()
+    f = (torch.logsumexp(d, -1) - d.gather(-1, t.clamp(min=0)[:, None])[:, 0]) * live
+    h = torch.autograd.grad(torch.autograd.grad(f, d, w.double(), create_graph=True)[0].square().sum(), d)[0]
+    # products of three 32-bit quantities of size 1
+    assert float((got.double() - h).abs().max()) <= 2.0 ** -18
+    base = torch.autograd.grad(ce(l, t), l, w)[0]
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), lambda v: v.to(DEV)):
+        out = ce(l, t)
+    assert torch.equal(torch.autograd.grad(out, l, w)[0], base)
+    out = ce(l, t)
+    with torch.no_grad():
+        l.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, l, w)
+
+
+def test_a_gradient_that_is_expanded_or_of_another_type(ce):
+    l, t, w = _inputs((64,), 100, BF)
+    a = torch.autograd.grad(ce(l, t).sum(), l)[0]
+    b = torch.autograd.grad(ce(l, t), l, torch.ones(64, device=DEV))[0]
+    assert torch.equal(a, b)
+
+
+def test_refusals(ce):
+    l, t, _ = _inputs((4,), 10, F32)
+    with pytest.raises(TypeError):
+        ce(l.half(), t)
+    with pytest.raises(TypeError):
+        ce(l, t.float())
+    with pytest.raises(ValueError):
+        ce(l, t[:3])
+    with pytest.raises(ValueError):
+        ce(l.cpu(), t.cpu())
+    with pytest.raises(ValueError):
+        ce(l[:, :0], t)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: ce(v, t[0]))(l)
