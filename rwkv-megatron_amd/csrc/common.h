@@ -202,6 +202,16 @@ __device__ __forceinline__ float wave_sum(float v) {
     return r.lo + r.hi;
 }
 
+// Largest value of the wave, in all lanes (NaN is passed over).
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, lane_xor1(v));
+    v = fmaxf(v, lane_xor2(v));
+    v = fmaxf(v, dpp_mov<0x141>(v));
+    v = fmaxf(v, dpp_mov<0x140>(v));
+    v = fmaxf(v, lane_xor_swz<16>(v));
+    return fmaxf(v, lane_xor32(v));
+}
+
 // Host side: a device buffer as (address, bytes).  Entry points reject calls where an output
 // overlaps an input or another output: several kernels re-load a clamped last piece after
 // other threads have stored theirs, and the walks read chunk c + 1 before storing chunk c, so

@@ -26,16 +26,16 @@ __device__ __forceinline__ void ce_unpack(uint4 q, float* f) {
     }
 }
 template <bool F32>
-__device__ __forceinline__ float ce_load(const char* row, int64_t j) {
+__device__ __forceinline__ float ce_load(const char* row, int j) {
     if constexpr (F32) return reinterpret_cast<const float*>(row)[j];
     else return bf2f(reinterpret_cast<const uint16_t*>(row)[j]);
 }
 // elements before the row's first 16-byte boundary (rows lie at multiples of the element's size)
 template <bool F32>
-__device__ __forceinline__ int ce_lead(const void* row, int64_t V) {
+__device__ __forceinline__ int ce_lead(const void* row, int V) {
     const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15u) / (F32 ? 4 : 2), E = CeVec<F32>::E;
     const int lead = off ? E - off : 0;
-    return lead < V ? lead : (int)V;
+    return lead < V ? lead : V;
 }
 
 // (m, z) of a set of logits: z = sum exp(l - m).  An empty set, or one of -inf alone, is (-inf, 0).
@@ -60,20 +60,24 @@ template <int K> __device__ __forceinline__ void ce_take(Soft& s, const float* v
 }
 }  // namespace
 
-// One block a row (striding over the rows), CE_U pieces of 16 bytes a thread in flight.
+// THR threads a row: a block, or a wave of the block's four (striding over the rows); CE_U pieces of 16
+// bytes a thread in flight.
 #define CE_U 4
+#define CE_BLOCK(THR) ((THR) < 256 ? 256 : (THR))
 template <bool F32, int THR>
-__global__ void __launch_bounds__(THR)
+__global__ void __launch_bounds__(CE_BLOCK(THR))
 rwkv6_cross_entropy_fwd_kernel(const void* __restrict__ logits, int64_t ld, const int64_t* __restrict__ target,
                                int64_t ignore, float* __restrict__ loss, float2* __restrict__ stats, int64_t N,
-                               int64_t V) {
-    constexpr int E = CeVec<F32>::E, ES = F32 ? 4 : 2;
+                               int V) {
+    constexpr int E = CeVec<F32>::E, ES = F32 ? 4 : 2, ROWS = CE_BLOCK(THR) / THR;
     __shared__ Soft part[THR / 64];
-    for (int64_t n = blockIdx.x; n < N; n += gridDim.x) {
+    const int tid = threadIdx.x % THR;
+    for (int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / THR; n < N; n += (int64_t)gridDim.x * ROWS) {
         const int64_t t = target[n];
         const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
-        if (ignored || bad) {                             // uniform over the block
-            if (threadIdx.x == 0) {
+        // the same for all threads of the row; a short row is read all the same, its loads do not wait then
+        if (THR > 64 && (ignored || bad)) {
+            if (tid == 0) {
                 loss[n] = ignored ? 0.f : NAN;
                 stats[n] = make_float2(0.f, 1.f);
             }
@@ -81,10 +85,10 @@ rwkv6_cross_entropy_fwd_kernel(const void* __restrict__ logits, int64_t ld, cons
         }
         const char* row = reinterpret_cast<const char*>(logits) + n * ld * ES;
         const int lead = ce_lead<F32>(row, V);
-        const int64_t pieces = (V - lead) / E, tail = lead + pieces * E;
+        const int pieces = (V - lead) / E, tail = lead + pieces * E;
         const uint4* body = reinterpret_cast<const uint4*>(row + (int64_t)lead * ES);
         Soft s = {-INFINITY, 0.f};
-        int64_t i = threadIdx.x;
+        int i = tid;
         for (; i + (CE_U - 1) * THR < pieces; i += CE_U * THR) {
             float v[CE_U * E];
 #pragma unroll
@@ -97,74 +101,101 @@ rwkv6_cross_entropy_fwd_kernel(const void* __restrict__ logits, int64_t ld, cons
             ce_take<E>(s, v);
         }
         // fewer than 8 elements at either end
-        if ((int)threadIdx.x < lead) {
-            const float v = ce_load<F32>(row, threadIdx.x);
+        if (tid < lead) {
+            const float v = ce_load<F32>(row, tid);
             ce_take<1>(s, &v);
         }
-        if ((int64_t)threadIdx.x < V - tail) {
-            const float v = ce_load<F32>(row, tail + threadIdx.x);
+        if (tid < V - tail) {
+            const float v = ce_load<F32>(row, tail + tid);
             ce_take<1>(s, &v);
         }
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) s = join(s, Soft{__shfl_xor(s.m, o), __shfl_xor(s.z, o)});
-        __syncthreads();                                  // the row before has been read from `part`
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < THR / 64; ++w) s = join(s, part[w]);
-            loss[n] = logf(s.z) + (s.m - ce_load<F32>(row, t));
+        // the wave's maximum first, then every lane's sum scaled to it once
+        const float m = wave_max(s.m);
+        s.z = wave_sum(s.z * ex2((s.m - ce_ref(m)) * RW_L2E));
+        s.m = m;
+        if constexpr (THR > 64) {
+            __syncthreads();                              // the row before has been read from `part`
+            if ((tid & 63) == 0) part[tid >> 6] = s;
+            __syncthreads();
+        }
+        if (tid == 0) {
+            if constexpr (THR > 64)
+                for (int w = 1; w < THR / 64; ++w) s = join(s, part[w]);
+            loss[n] = ignored ? 0.f : bad ? NAN : logf(s.z) + (s.m - ce_load<F32>(row, (int)t));
             stats[n] = make_float2(s.m, s.z);
         }
     }
 }
 
-// Block (row, segment): the row's elements cut into gridDim.y runs of pieces.
-template <bool F32>
-__global__ void __launch_bounds__(256)
+// THR threads a row as above; gridDim.y segments of a row's pieces.
+template <bool F32, int THR>
+__global__ void __launch_bounds__(CE_BLOCK(THR))
 rwkv6_cross_entropy_bwd_kernel(const void* __restrict__ logits, int64_t ld, const int64_t* __restrict__ target,
                                int64_t ignore, const float2* __restrict__ stats, const float* __restrict__ d_loss,
-                               void* __restrict__ d_logits, int64_t N, int64_t V) {
-    constexpr int E = CeVec<F32>::E, ES = F32 ? 4 : 2;
-    for (int64_t n = blockIdx.x; n < N; n += gridDim.x) {
+                               void* __restrict__ d_logits, int64_t N, int V) {
+    constexpr int E = CeVec<F32>::E, ES = F32 ? 4 : 2, ROWS = CE_BLOCK(THR) / THR;
+    const int tid = threadIdx.x % THR;
+    for (int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / THR; n < N; n += (int64_t)gridDim.x * ROWS) {
         const int64_t t = target[n];
         const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
         const char* row = reinterpret_cast<const char*>(logits) + n * ld * ES;
         char* out = reinterpret_cast<char*>(d_logits) + n * V * ES;
         const float2 st = stats[n];
+        const float dl = d_loss[n];
         // an ignored row's zeros and a bad one's NaN do not depend on its logits
-        const float w = bad ? NAN : ignored ? 0.f : d_loss[n], q = w / st.y, m = st.x;
-        auto grad = [&](float l, int64_t j) {
-            if (ignored || bad) return w;
+        const bool fixed = ignored || bad;
+        const float w = bad ? NAN : ignored ? 0.f : dl, q = w / st.y, m = st.x;
+        const int hit = fixed ? -1 : (int)t;
+        auto grad = [&](float l, int j) {
             const float p = q * ex2((l - m) * RW_L2E);
-            return j == t ? p - w : p;
+            return fixed ? w : j == hit ? p - w : p;
         };
-        auto store = [&](int64_t j, float g) {
+        auto put = [&](int j, const float* v) {
+            if constexpr (F32) *reinterpret_cast<float4*>(out + (int64_t)j * ES) = make_float4(v[0], v[1], v[2], v[3]);
+            else store8(reinterpret_cast<uint16_t*>(out) + j, v);
+        };
+        auto put1 = [&](int j) {
+            const float g = grad(ce_load<F32>(row, j), j);
             if constexpr (F32) reinterpret_cast<float*>(out)[j] = g;
             else reinterpret_cast<uint16_t*>(out)[j] = f2bf(g);
         };
         const int lead = ce_lead<F32>(out, V);
-        const int64_t pieces = (V - lead) / E, tail = lead + pieces * E;
+        const int pieces = (V - lead) / E, tail = lead + pieces * E;
         const bool vec = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-        const int64_t per = (pieces + gridDim.y - 1) / gridDim.y, i0 = per * blockIdx.y;
-        const int64_t i1 = i0 + per < pieces ? i0 + per : pieces;
-        for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
-            const int64_t j = lead + i * E;
+        const int per = (pieces + (int)gridDim.y - 1) / (int)gridDim.y, i0 = min(per * (int)blockIdx.y, pieces);
+        const int i1 = min(i0 + per, pieces);
+        int i = i0 + tid;
+        for (; vec && i + (CE_U - 1) * THR < i1; i += CE_U * THR) {
+            uint4 raw[CE_U];
+#pragma unroll
+            for (int u = 0; u < CE_U; ++u) raw[u] = *reinterpret_cast<const uint4*>(row + (int64_t)(lead + (i + u * THR) * E) * ES);
+#pragma unroll
+            for (int u = 0; u < CE_U; ++u) {
+                const int j = lead + (i + u * THR) * E;
+                float v[E];
+                ce_unpack<F32>(raw[u], v);
+#pragma unroll
+                for (int k = 0; k < E; ++k) v[k] = grad(v[k], j + k);
+                put(j, v);
+            }
+        }
+        for (; i < i1; i += THR) {
+            const int j = lead + i * E;
             float v[E];
             if (vec) {
-                ce_unpack<F32>(*reinterpret_cast<const uint4*>(row + j * ES), v);
+                ce_unpack<F32>(*reinterpret_cast<const uint4*>(row + (int64_t)j * ES), v);
             } else {
 #pragma unroll
                 for (int k = 0; k < E; ++k) v[k] = ce_load<F32>(row, j + k);
             }
 #pragma unroll
             for (int k = 0; k < E; ++k) v[k] = grad(v[k], j + k);
-            if constexpr (F32) *reinterpret_cast<float4*>(out + j * ES) = make_float4(v[0], v[1], v[2], v[3]);
-            else store8(reinterpret_cast<uint16_t*>(out) + j, v);
+            put(j, v);
         }
+        // fewer than 8 elements at either end
         if (blockIdx.y == 0) {
-            if ((int)threadIdx.x < lead) store(threadIdx.x, grad(ce_load<F32>(row, threadIdx.x), threadIdx.x));
-            if ((int64_t)threadIdx.x < V - tail)
-                store(tail + threadIdx.x, grad(ce_load<F32>(row, tail + threadIdx.x), tail + threadIdx.x));
+            if (tid < lead) put1(tid);
+            if (tid < V - tail) put1(tail + tid);
         }
     }
 }
@@ -194,11 +225,21 @@ int rwkv6_cross_entropy_fwd(const void* logits, int dtype, int64_t ld, const int
     if (any_alias({{loss, (size_t)N * 4}, {stats, (size_t)N * 8}},
                   {{logits, ce_span(ld, N, V, dtype)}, {target, (size_t)N * 8}}))
         return RWKV6_ERR_INVALID_ARG;
-    const bool f32 = dtype == RWKV6_F32, few = N < 1024;
-    auto k = f32 ? (few ? rwkv6_cross_entropy_fwd_kernel<true, 1024> : rwkv6_cross_entropy_fwd_kernel<true, 256>)
-                 : (few ? rwkv6_cross_entropy_fwd_kernel<false, 1024> : rwkv6_cross_entropy_fwd_kernel<false, 256>);
-    hipLaunchKernelGGL(k, dim3((unsigned)(N < CE_GRID ? N : CE_GRID)), dim3(few ? 1024 : 256), 0,
-                       reinterpret_cast<hipStream_t>(stream), logits, ld, target, ignore_index, loss, (float2*)stats, N, V);
+    const bool f32 = dtype == RWKV6_F32;
+    // A wave for a short row, whose cost is the joining of the threads' sums, more for a long one; one row
+    // of 1024 threads at a time streams best where the rows fill the device several times over.  Forward, us,
+    // with 64, 256, 512, 1024 threads: 65536 x 376 25, 74, 163, 338; 16384 x 4104 27, 36, 58, 103; 16384 x
+    // 8192 51, 44, 72, 116; 8192 x 32000 94, 93, 90, 116; 4096 x 65536 94, 96, 93, 87; 1024 x 65536 -, 41, 38,
+    // 40.
+    const int64_t pieces = V * (int64_t)param_bytes(dtype) / 16;
+    const int thr = pieces < 1024 ? 64 : pieces < 4096 ? 256 : N < 2048 ? 512 : 1024;
+#define CE_PICK(F) (thr == 64 ? rwkv6_cross_entropy_fwd_kernel<F, 64> : thr == 256 ? rwkv6_cross_entropy_fwd_kernel<F, 256> \
+                    : thr == 512 ? rwkv6_cross_entropy_fwd_kernel<F, 512> : rwkv6_cross_entropy_fwd_kernel<F, 1024>)
+    auto k = f32 ? CE_PICK(true) : CE_PICK(false);
+#undef CE_PICK
+    const int64_t blocks = thr == 64 ? (N + 3) / 4 : N;
+    hipLaunchKernelGGL(k, dim3((unsigned)(blocks < CE_GRID ? blocks : CE_GRID)), dim3(CE_BLOCK(thr)), 0,
+                       reinterpret_cast<hipStream_t>(stream), logits, ld, target, ignore_index, loss, (float2*)stats, N, (int)V);
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
 
@@ -213,13 +254,17 @@ int rwkv6_cross_entropy_bwd(const void* logits, int dtype, int64_t ld, const int
     if (any_alias({{d_logits, (size_t)(N * V) * param_bytes(dtype)}},
                   {{logits, ce_span(ld, N, V, dtype)}, {target, (size_t)N * 8}, {stats, (size_t)N * 8}, {d_loss, (size_t)N * 4}}))
         return RWKV6_ERR_INVALID_ARG;
-    // a row is cut until the blocks fill the device, each keeping a step of its 256 threads
+    // a wave for a short row; a long one is cut until the blocks fill the device, each keeping a step of its
+    // 256 threads
+    const bool f32 = dtype == RWKV6_F32, wave = V * (int64_t)param_bytes(dtype) / 16 < 1024;
     int seg = 1;
-    while (seg < 64 && N * seg < 2048 && V >= (int64_t)seg * 2 * 256 * 8) seg *= 2;
-    auto k = dtype == RWKV6_F32 ? rwkv6_cross_entropy_bwd_kernel<true> : rwkv6_cross_entropy_bwd_kernel<false>;
-    hipLaunchKernelGGL(k, dim3((unsigned)(N < CE_GRID ? N : CE_GRID), (unsigned)seg), dim3(256), 0,
+    while (!wave && seg < 64 && N * seg < 2048 && V >= (int64_t)seg * 2 * 256 * 8) seg *= 2;
+    auto k = f32 ? (wave ? rwkv6_cross_entropy_bwd_kernel<true, 64> : rwkv6_cross_entropy_bwd_kernel<true, 256>)
+                 : (wave ? rwkv6_cross_entropy_bwd_kernel<false, 64> : rwkv6_cross_entropy_bwd_kernel<false, 256>);
+    const int64_t blocks = wave ? (N + 3) / 4 : N;
+    hipLaunchKernelGGL(k, dim3((unsigned)(blocks < CE_GRID ? blocks : CE_GRID), (unsigned)seg), dim3(256), 0,
                        reinterpret_cast<hipStream_t>(stream), logits, ld, target, ignore_index, (const float2*)stats, d_loss,
-                       d_logits, N, V);
+                       d_logits, N, (int)V);
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
 
