@@ -17,8 +17,8 @@
 #define RN_PIECE 512      // channels of a wave: 8 a lane
 #define RN_MAX_C 8192
 #define RN_MAX_WAVES 8
-#define RN_FWD_BLOCKS 2048
-#define RN_PART 1024      // row ranges of the backward at most
+#define RN_FWD_BLOCKS (1 << 20)
+#define RN_PART 512      // row ranges of the backward at most
 
 namespace {
 
@@ -32,12 +32,21 @@ __device__ __forceinline__ void raw_f32(const WRaw<F32>& r, float* f) {
         unpack8(r.q[0], f);
     }
 }
+// Eight channels of an output; `nt`: past the caches (see rn_stream).
 template <bool F32>
-__device__ __forceinline__ void store8_as(void* p, int64_t off, const float* f) {
+__device__ __forceinline__ void store8_as(void* p, int64_t off, const float* f, bool nt = false) {
     if constexpr (F32) {
-        float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + off);
-        q[0] = make_float4(f[0], f[1], f[2], f[3]);
-        q[1] = make_float4(f[4], f[5], f[6], f[7]);
+        f32x4* q = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + off);
+        const f32x4 a = {f[0], f[1], f[2], f[3]}, b = {f[4], f[5], f[6], f[7]};
+        if (nt) {
+            __builtin_nontemporal_store(a, q);
+            __builtin_nontemporal_store(b, q + 1);
+        } else {
+            q[0] = a;
+            q[1] = b;
+        }
+    } else if (nt) {
+        store8_nt(reinterpret_cast<uint16_t*>(p) + off, f);
     } else {
         store8(reinterpret_cast<uint16_t*>(p) + off, f);
     }
@@ -73,7 +82,7 @@ __global__ void __launch_bounds__(64 * RN_MAX_WAVES)
 rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const void* __restrict__ beta, int pdt,
                                float eps, void* __restrict__ s, uint16_t* __restrict__ y,
                                float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t N, int C, int W,
-                               int RB) {
+                               int RB, bool nt) {
     __shared__ float red[2][RN_MAX_WAVES];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, gr = wv / W, w = wv - gr * W;
     const float inv = 1.f / (float)C;
@@ -131,10 +140,10 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (c[i] >= C) continue;
-            store8_as<XF>(s, row + c[i], v[i]);
+            store8_as<XF>(s, row + c[i], v[i], nt);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] - mean) * rstd * ga[i][j] + be[i][j];
-            store8(y + row + c[i], v[i]);
+            store8_as<false>(y, row + c[i], v[i], nt);
         }
         if (mean_out && lane == 0 && w == 0) {
             mean_out[n] = mean;
@@ -143,20 +152,19 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
     }
 }
 
-// Block p: rows [p rpb, (p + 1) rpb), RB at a time; part[p][CB ? 3 : 2][C] = its sums of dgamma, dbeta
+// Block p of P: rows [p N / P, (p + 1) N / P), RB at a time; part[p][CB ? 3 : 2][C] = its sums of dgamma, dbeta
 // and d_branch_bias (part null: none).  ds null: zero.  db null: d_branch equals dx, not stored twice.
 template <int NV, bool XF, bool GATE, bool CB>
 __global__ void __launch_bounds__(64 * RN_MAX_WAVES)
 rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt, const float* __restrict__ mean_in,
                                const float* __restrict__ rstd_in, const void* __restrict__ ds,
                                const uint16_t* __restrict__ dy, void* __restrict__ dx, uint16_t* __restrict__ db,
-                               uint16_t* __restrict__ dg, float* __restrict__ part, int64_t N, int C, int W, int RB,
-                               int64_t rpb) {
+                               uint16_t* __restrict__ dg, float* __restrict__ part, int64_t N, int C, int W, int RB, bool nt) {
     extern __shared__ __attribute__((aligned(16))) float rn_acc[];            // [CB ? 3 : 2][C]
     __shared__ float2 red[2][RN_MAX_WAVES];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, gr = wv / W, w = wv - gr * W;
     const float inv = 1.f / (float)C;
-    const int64_t n0 = (int64_t)blockIdx.x * rpb, n1 = min(N, n0 + rpb);
+    const int64_t n0 = N * blockIdx.x / gridDim.x, n1 = N * (blockIdx.x + 1) / gridDim.x;
     int c[NV];
     float ga[NV][8], cb[CB ? NV : 1][8], ag[NV][8], ab[NV][8], ac[CB ? NV : 1][8];
 #pragma unroll
@@ -224,7 +232,7 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
             if (c[i] >= C) continue;
 #pragma unroll
             for (int j = 0; j < 8; ++j) dS[i][j] += rstd * (g[i][j] - s1 - xh[i][j] * s2);
-            store8_as<XF>(dx, row + c[i], dS[i]);
+            store8_as<XF>(dx, row + c[i], dS[i], nt);
             if (!db) continue;
             float o[8];
 #pragma unroll
@@ -233,11 +241,11 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
                 o[j] = GATE ? dS[i][j] * sg[i][j] : dS[i][j];
                 if constexpr (CB) ac[i][j] += o[j];
             }
-            store8(db + row + c[i], o);
+            store8_as<false>(db, row + c[i], o, nt);
             if constexpr (GATE) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = o[j] * f[i][j] * (1.f - sg[i][j]);
-                store8(dg + row + c[i], o);
+                store8_as<false>(dg, row + c[i], o, nt);
             }
         }
     }
@@ -315,12 +323,16 @@ inline RnShape rn_shape(int64_t C) {
     const int NV = C > RN_PIECE * RN_MAX_WAVES ? 2 : 1, W = (int)((C + RN_PIECE * NV - 1) / (RN_PIECE * NV));
     return {NV, W, W >= 4 ? 1 : 4 / W};
 }
-// Row ranges of the backward: two steps of a block at least and RN_PART of them at most.
-inline int64_t rn_rows(int64_t N, int RB) {
-    const int64_t r = (N + RN_PART - 1) / RN_PART, step = 2 * RB;
-    return (r + step - 1) / step * step;
+// Whether the outputs are stored past the caches: where the call's tensors do not fit the 256 MB of the last
+// one anyway.  Kept in it, they push out what the call still reads: 16384 x 2048 bf16, us, cached and
+// streamed: backward 72 and 62, gated forward 64 and 55.  (A training step of the 1.6B shape, whose next
+// kernels read some of them again, takes the same time with either.)
+inline bool rn_stream(int64_t N, int64_t C) { return N * C >= (int64_t)1 << 24; }
+// Row ranges of the backward: RN_PART of them, two a CU, where that leaves each two steps of a block.
+inline int64_t rn_parts(int64_t N, int RB) {
+    const int64_t p = (N + 2 * RB - 1) / (2 * RB);
+    return p < 1 ? 1 : p < RN_PART ? p : RN_PART;
 }
-inline int64_t rn_parts(int64_t N, int RB) { return N > 0 ? (N + rn_rows(N, RB) - 1) / rn_rows(N, RB) : 1; }
 }  // namespace
 
 extern "C" {
@@ -351,7 +363,7 @@ int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, cons
     hipLaunchKernelGGL(k, dim3((unsigned)(blocks < RN_FWD_BLOCKS ? blocks : RN_FWD_BLOCKS)), dim3(64 * h.W * h.RB), 0,
                        reinterpret_cast<hipStream_t>(stream),
                        RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale}, gamma, beta,
-                       param_dtype, eps, s, (uint16_t*)y, mean, rstd, N, (int)C, h.W, h.RB);
+                       param_dtype, eps, s, (uint16_t*)y, mean, rstd, N, (int)C, h.W, h.RB, rn_stream(N, C));
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
 
@@ -398,7 +410,7 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
         hipLaunchKernelGGL(k, dim3((unsigned)parts), dim3(64 * h.W * h.RB), sums && h.RB > 1 ? (size_t)M * 4 : 0, stm,
                            RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale}, gamma,
                            gamma_dtype, mean, rstd, ds, (const uint16_t*)dy, dx, (uint16_t*)d_branch, (uint16_t*)d_gate, part,
-                           N, (int)C, h.W, h.RB, rn_rows(N, h.RB));
+                           N, (int)C, h.W, h.RB, rn_stream(N, C));
     }
     if (sums)
         hipLaunchKernelGGL(rwkv6_residual_norm_sums_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, stm, part,

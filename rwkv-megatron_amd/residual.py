@@ -32,11 +32,15 @@ def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, sca
 
     Gradients for x, branch, gate, weight, bias and branch_bias; sums over the rows run in a fixed
     order.  A backward that is differentiated again runs through torch's operators."""
-    gate_ = () if gate is None else (("gate", gate),)
-    acts = (("x", x), ("branch", branch), *gate_)
-    for name, t in acts:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
+    out = _lib.native().residual_norm(x, branch, weight, bias, eps, gate, branch_bias, scale, False)
+    return _refuse(x, branch, weight, bias, gate, branch_bias) if out is None else out
+
+
+def _refuse(x, branch, weight, bias, gate, branch_bias):
+    """Raises for a call that the kernels do not take, and says why."""
+    for name, t in (("x", x), ("branch", branch), ("gate", gate)):
+        if t is None:
+            continue
         if t.device.type != "cuda":
             raise ValueError(f"{name} must live on the GPU")
         if t.shape != x.shape:
@@ -49,15 +53,12 @@ def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, sca
     if C % 8 or C > MAX_CHANNELS:
         raise NotImplementedError(f"C must be a multiple of 8 up to {MAX_CHANNELS}, got {C}")
     for name, t in (("weight", weight), ("bias", bias), ("branch_bias", branch_bias)):
-        if t is None and name == "branch_bias":
+        if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or t.dtype not in (torch.bfloat16, torch.float32, torch.float16):
+        if t.dtype not in (torch.bfloat16, torch.float32, torch.float16):
             raise TypeError(f"{name} must be a bfloat16, float32 or float16 tensor")
         if tuple(t.shape) != (C,):
             raise ValueError(f"{name} must be [C] = {(C,)}, got {tuple(t.shape)}")
     if len({t.device for t in (x, branch, gate, weight, bias, branch_bias) if t is not None}) != 1:
         raise ValueError("all tensors must be on the same device")
-    out = _lib.native().residual_norm(x, branch, weight, bias, float(eps), gate, branch_bias, float(scale), False)
-    if out is None:
-        raise NotImplementedError("residual_norm takes dense (strided) tensors of at most 2^40 elements")
-    return out
+    raise NotImplementedError("residual_norm takes dense (strided) tensors of at most 2^40 elements")

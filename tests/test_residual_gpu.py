@@ -73,11 +73,11 @@ def test_matches_float64(rn, shape, C, stream, param, gate, cbias, scale):
     near = lambda v, w, slack: bool(((v.double() - w).abs() <= half(v) * w.abs() + slack).all())
     assert near(s.detach(), S.detach(), 2.0 ** -22 * parts)
     exh = 2.0 ** -17 * float(top * r.detach().max())                        # of xh
-    assert near(y.detach(), Y.detach(), exh * float(d["weight"].abs().max()) + 2.0 ** -22 * float(d["bias"].abs().max()))
+    assert near(y.detach(), Y.detach(), exh * float(d["weight"].detach().abs().max()) + 2.0 ** -22 * float(d["bias"].detach().abs().max()))
     g = float((dy.double() * d["weight"]).detach().abs().max())
     xm = float(xh.detach().abs().max())
     eds = 2.0 ** -17 * (float(ds.abs().max()) + float(r.detach().max()) * g * (1 + xm)) + float(r.detach().max()) * g * 4 * exh
-    fm = float((d["branch"].abs() + (d["branch_bias"].abs() if cbias else 0)).max())
+    fm = float((d["branch"].abs() + (d["branch_bias"].abs() if cbias else 0)).detach().max())
     rows = tuple(range(len(shape)))
     slack = {"x": eds, "branch": abs(scale) * eds, "gate": abs(scale) * fm * eds,
              "weight": 2.0 ** -17 * (dy.double().abs() * xh.detach().abs()).sum(rows) + exh * dy.double().abs().sum(rows),
