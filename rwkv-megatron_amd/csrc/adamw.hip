@@ -29,6 +29,8 @@
 
 #define AW_THR 256
 #define AW_STEP (8 * AW_THR)    // elements a block takes at once
+#define AW_PARTS 8192           // blocks of the norm's sums, at about
+#define AW_AHEAD 4              // steps of the norm's loads in flight
 #define AW_T 60                 // tensors a launch: the arguments stay below 4 KB
 #define AW_BLK 256              // elements under one 8-bit scale: 32 lanes of 8
 #define AW_F8_MAX 448.f
@@ -169,13 +171,25 @@ rwkv6_grad_square_sums_kernel(const NormTable tab, int64_t per, double* __restri
     const void* g = tab.g[k];
     const int dt = tab.dt[k];
     const bool vec = aw_al16(g);
-    double acc = 0.;
-    for (int64_t i = i0 + 8 * threadIdx.x; i < i1; i += AW_STEP) {
+    double sum[2] = {0., 0.};
+    int64_t i = i0 + 8 * threadIdx.x;
+    // whole steps, AW_AHEAD of them in flight
+    for (; vec && i + 8 + (AW_AHEAD - 1) * AW_STEP <= i1; i += AW_AHEAD * AW_STEP) {
+        float f[AW_AHEAD][8];
+#pragma unroll
+        for (int u = 0; u < AW_AHEAD; ++u) aw_load8(g, dt, i + u * AW_STEP, n, true, f[u]);
+#pragma unroll
+        for (int u = 0; u < AW_AHEAD; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j & 1] = fma((double)f[u][j], (double)f[u][j], sum[j & 1]);
+    }
+    for (; i < i1; i += AW_STEP) {
         float f[8];
         aw_load8(g, dt, i, i1, vec, f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc = fma((double)f[j], (double)f[j], acc);
+        for (int j = 0; j < 8; ++j) sum[j & 1] = fma((double)f[j], (double)f[j], sum[j & 1]);
     }
+    double acc = sum[0] + sum[1];
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) acc += __shfl_xor(acc, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
@@ -259,8 +273,8 @@ rwkv6_adamw_step_kernel(const StepTable tab, const Coef* __restrict__ coef, int6
             aw_codes_store(m, i, n, vec, aw_encode(mf, tm > 0.f ? AW_F8_MAX / tm : 0.f));
             aw_codes_store(v, i, n, vec, aw_encode(root, tv > 0.f ? AW_F8_MAX / tv : 0.f));
             if ((threadIdx.x & 31) == 0) {
-                ms[0] = tm / AW_F8_MAX;
-                vs[0] = tv / AW_F8_MAX;
+                ms[0] = tm * (1.f / AW_F8_MAX);
+                vs[0] = tv * (1.f / AW_F8_MAX);
             }
         } else {
             aw_store8(m, RWKV6_F32, i, n, vec, mf);
@@ -270,11 +284,11 @@ rwkv6_adamw_step_kernel(const StepTable tab, const Coef* __restrict__ coef, int6
 }
 
 namespace {
-// Elements a block takes: 2048 blocks over all tensors (8 a CU), in steps of AW_STEP.
-int64_t aw_per(const int64_t* numel, int64_t count, int64_t most) {
+// Elements a block takes: `blocks` blocks over all tensors, in steps of AW_STEP.
+int64_t aw_per(const int64_t* numel, int64_t count, int64_t blocks, int64_t most) {
     int64_t total = 0;
     for (int64_t k = 0; k < count; ++k) total += numel[k];
-    int64_t per = (total / 2048 + AW_STEP - 1) / AW_STEP * AW_STEP;
+    int64_t per = (total / blocks + AW_STEP - 1) / AW_STEP * AW_STEP;
     if (per < AW_STEP) per = AW_STEP;
     return most && per > most ? most : per;
 }
@@ -292,7 +306,7 @@ int aw_sizes(const int64_t* numel, int64_t count) {
     return total > ((int64_t)1 << 40) ? RWKV6_ERR_UNSUPPORTED : RWKV6_OK;
 }
 int64_t aw_partials(const int64_t* numel, int64_t count) {
-    const int64_t per = aw_per(numel, count, 0);
+    const int64_t per = aw_per(numel, count, AW_PARTS, 0);
     int64_t P = 0;
     for (int64_t k = 0; k < count; ++k) P += aw_blocks(numel[k], per);
     return P;
@@ -332,7 +346,7 @@ int rwkv6_grad_norm_sums(const void* const* grad, const int* grad_dtype, const i
     const int st = aw_sizes(numel, count);
     if (st) return st;
     if (count && (!grad || !grad_dtype)) return RWKV6_ERR_INVALID_ARG;
-    const int64_t per = aw_per(numel, count, 0);
+    const int64_t per = aw_per(numel, count, AW_PARTS, 0);
     const Span out = {partials, (size_t)aw_partials(numel, count) * 8};
     for (int64_t k = 0; k < count; ++k) {
         if (!aw_dt(grad_dtype[k]) || (numel[k] && (!grad[k] || !partials))) return RWKV6_ERR_INVALID_ARG;
@@ -425,7 +439,7 @@ int rwkv6_adamw_step(void* const* param, const int* param_dtype, const void* con
     Coef* coef = (Coef*)workspace;
     hipLaunchKernelGGL(rwkv6_adamw_coef_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), partials,
                        partials ? (int)P : 0, max_norm, norm, step, lr_dev, lr, log(beta1), log(beta2), weight_decay, coef);
-    const int64_t per = aw_per(numel, count, 8 * AW_STEP);
+    const int64_t per = aw_per(numel, count, 2048, 8 * AW_STEP);
     StepTable tab;
     int64_t blocks = 0;
     tab.count = 0;

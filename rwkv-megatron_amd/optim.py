@@ -64,8 +64,8 @@ def _step(native, params, grads, m, v, ms, vs, step, lr, betas, eps, weight_deca
 
 
 def _tensors(name, ts):
-    ts = list(ts)
-    if not ts or not all(isinstance(t, torch.Tensor) for t in ts):
+    ts = list(ts)                               # the tensors themselves are looked at where they are read
+    if not ts:
         raise TypeError(f"{name} must be tensors, one at least")
     return ts
 

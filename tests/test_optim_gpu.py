@@ -164,7 +164,7 @@ def test_optimizer_follows_torch(opt):
         a.step()
         b.step()
     for p, q in zip(ps, qs):
-        assert float((p.double() - q).abs().max()) <= 4 * (2.0 ** -17 * HYPER["lr"] + 2.0 ** -22 * float(q.abs().max()))
+        assert float((p.double() - q).detach().abs().max()) <= 4 * (2.0 ** -17 * HYPER["lr"] + 2.0 ** -22 * float(q.detach().abs().max()))
     assert a.grad_norm.shape == ()
 
 
