@@ -146,7 +146,6 @@ def config1_bench(pkg, gpu_steps, with_cpu):
     package's model (fp32 parameters, bf16 activations).  CPU: the reference's forward restated
     in torch fp32 with the C oracle's WKV (oracle/lm.py), 1 warm-up and the median of 3."""
     import torch
-    import torch.nn.functional as F
 
     M = pkg.modules
     cfg = M.TransformerConfig(hidden_size=512, num_attention_heads=8, ffn_hidden_size=1792,
@@ -159,11 +158,10 @@ def config1_bench(pkg, gpu_steps, with_cpu):
     targets = torch.cat([tokens[:, 1:], torch.zeros(B, 1, dtype=tokens.dtype)], 1)
     mask = torch.ones(B, T)
     mask[:, -1] = 0
-    tok_d, tgt_d, mask_d = tokens.cuda(), targets.cuda().reshape(-1), mask.cuda().reshape(-1)
+    tok_d, tgt_d, mask_d = tokens.cuda(), targets.cuda(), mask.cuda()
 
     def gpu_step():
-        logits = model(tok_d)
-        losses = F.cross_entropy(logits.float().transpose(0, 1).reshape(-1, V), tgt_d, reduction="none")
+        losses = model(tok_d, tgt_d)
         loss = (losses * mask_d).sum() / mask_d.sum()
         loss.backward()
         model.zero_grad(set_to_none=True)
@@ -184,8 +182,7 @@ def config1_bench(pkg, gpu_steps, with_cpu):
     # (~270 small kernels), which the graph's single submission removes.  Gradients land in
     # the graph's own .grad tensors, overwritten by every replay.
     def fwd_bwd():
-        logits = model(tok_d)
-        losses = F.cross_entropy(logits.float().transpose(0, 1).reshape(-1, V), tgt_d, reduction="none")
+        losses = model(tok_d, tgt_d)
         loss = (losses * mask_d).sum() / mask_d.sum()
         loss.backward()
         return loss
@@ -420,18 +417,16 @@ def train_step_bench(pkg, steps, warmup):
     torch.manual_seed(0)
     model = M.RWKV6Model(cfg, V, device="cuda:0")
     n_params = sum(p.numel() for p in model.parameters())
-    opt = torch.optim.AdamW(model.parameters(), lr=2.5e-4, betas=(0.9, 0.995), eps=1e-8,
-                            weight_decay=0.1, fused=True)
+    opt = pkg.optim.AdamW(model.parameters(), lr=2.5e-4, betas=(0.9, 0.995), eps=1e-8,
+                          weight_decay=0.1, max_norm=1.0)
     g = torch.Generator(device="cuda:0").manual_seed(1)
     tokens = torch.randint(0, V, (B, T + 1), device="cuda:0", generator=g)
     inp, tgt = tokens[:, :-1], tokens[:, 1:]
 
     def step():
-        logits = model(inp)                                      # [T, B, V]
-        loss = torch.nn.functional.cross_entropy(logits.float().view(-1, V), tgt.t().reshape(-1))
+        loss = model(inp, tgt).mean()                            # of the loss a token, [B, T]
         loss.backward()
-        torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0)
-        opt.step()
+        opt.step()                                               # clips by the norm, max_norm above
         opt.zero_grad(set_to_none=True)
         return loss
 

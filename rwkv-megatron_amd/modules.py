@@ -17,6 +17,10 @@ way (Megatron's module prefix aside).  The hot path runs on the HIP kernels:
     relu^2, sigmoid(gate) * out          -> channelmix.relu_sq / sigmoid_gate (HIP)
     up / gate / down projections         -> torch.matmul
 
+  between the blocks (RWKV6Layer, RWKV6Model)
+    residual add (+ bias, + the channel mix's gate) and the next LayerNorm -> residual.residual_norm's kernels (HIP)
+  loss (RWKV6Model with labels)          -> loss.cross_entropy         (HIP)
+
 Construction from Megatron's own TransformerConfig.  The layer spec (:539-550) builds
 ``RWKV6TimeMix(config, layer_number)`` and ``RWKV6ChannelMix(config)``; the config then carries
 Megatron's fields plus the two bottleneck sizes pretrain_rwkv6.py:61-69 adds.  Every field
@@ -48,7 +52,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import _lib, channelmix, timemix
+from . import _lib, channelmix, loss, timemix
 from .wkv import chunk_rwkv6, wkv6_seqfirst
 
 
@@ -307,10 +311,39 @@ class RWKV6ChannelMix(nn.Module):
 
     def forward(self, hidden_states):
         """:512-536 with the shift + lerps, relu^2 and sigmoid gate on HIP kernels."""
+        return channelmix.sigmoid_gate(*self.ungated(hidden_states)), None
+
+    def ungated(self, hidden_states):
+        """(out, gate_pre): the output before the sigmoid gate of :533-536, and the gate's input."""
         mixed_up, mixed_gate = channelmix.cmix_lerp(hidden_states, self.mix_coeffs)
         h = channelmix.relu_sq(self.linear_up(mixed_up)[0])
         out = self.linear_down(h)[0]
-        return channelmix.sigmoid_gate(out, self.linear_gate(mixed_gate)[0]), None
+        return out, self.linear_gate(mixed_gate)[0]
+
+
+def _add_norm(norm, x, branch, bias=None, gate=None):
+    """(s, LayerNorm(s)) for s = x + (branch + bias) sigmoid(gate): in one kernel (residual.residual_norm,
+    which rounds s and the norm once each) where it takes the call, else by the operators it stands
+    for.  A norm that is not this package's own class, or that has hooks, is called as a module."""
+    if _plain_module(norm, LayerNorm) and norm.weight is not None and norm.bias is not None and x.is_cuda:
+        out = _lib.native().residual_norm(x, branch, norm.weight, norm.bias, norm.eps, gate, bias, 1.0, True)
+        if out is not None:
+            return out
+    if bias is not None:
+        branch = branch + bias
+    x = x + (branch if gate is None else channelmix.sigmoid_gate(branch, gate))
+    return x, norm(x)
+
+
+def _plain_module(m, cls):
+    """Whether calling m is calling cls.forward: no subclass, no hooks (a profiler's, a sharding
+    wrapper's), no forward of its own, no compiler that traces the call."""
+    hooks = torch.nn.modules.module
+    return (type(m) is cls and "forward" not in m.__dict__
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                     or hooks._global_forward_hooks or hooks._global_forward_pre_hooks
+                     or hooks._global_backward_hooks or hooks._global_backward_pre_hooks)
+            and not torch.compiler.is_compiling())
 
 
 class RWKV6Layer(nn.Module):
@@ -328,10 +361,22 @@ class RWKV6Layer(nn.Module):
         self.mlp = RWKV6ChannelMix(config, layer_number, device)
 
     def forward(self, x):
-        a, a_bias = self.self_attention(self.input_layernorm(x), None)
-        x = x + a if a_bias is None else x + (a + a_bias)    # bias-dropout-add, dropout 0
-        m, _ = self.mlp(self.pre_mlp_layernorm(x))
+        x, h = self._time_mix(x, self.input_layernorm(x))
+        m, _ = self.mlp(h)
         return x + m
+
+    def _time_mix(self, x, h):
+        """The stream after the time mix of h = input_layernorm(x), and its norm for the channel mix
+        (bias-dropout-add, dropout 0)."""
+        a, a_bias = self.self_attention(h, None)
+        return _add_norm(self.pre_mlp_layernorm, x, a, a_bias)
+
+    def chained(self, x, h, next_norm):
+        """forward from h = input_layernorm(x), with the norm that follows this layer: (forward(x),
+        next_norm(forward(x))), the channel mix's gate, the residual and that norm in one kernel."""
+        x, h = self._time_mix(x, h)
+        out, gate = self.mlp.ungated(h)
+        return _add_norm(next_norm, x, out, gate=gate)
 
 
 def get_rwkv6_layer_spec():
@@ -358,12 +403,22 @@ class RWKV6Model(nn.Module):
         self.output_layer = OutputLayer(C, vocab_size, bias=False, device=device, dtype=dt)
         nn.init.normal_(self.output_layer.weight, 0.0, config.init_method_std)
 
-    def forward(self, tokens):
-        """tokens [B,T] -> logits [T,B,V] (sequence-first inside, as Megatron)."""
+    def forward(self, tokens, labels=None):
+        """tokens [B,T] -> logits [T,B,V] (sequence-first inside, as Megatron); with labels [B,T] the
+        loss a token, [B,T] fp32, as Megatron's GPTModel returns it (loss.cross_entropy: 0 for a label
+        of -100, which the training driver's mask leaves out, pretrain_rwkv6.py:144-160)."""
         x = self.pre_norm(self.embedding(tokens.t()).to(torch.bfloat16))
-        for layer in self.layers:
-            x = layer(x)
-        return self.output_layer(self.final_layernorm(x))
+        if x.is_cuda and len(self.layers) and all(_plain_module(m, RWKV6Layer) and _plain_module(m.mlp, RWKV6ChannelMix)
+                                                  for m in self.layers):
+            h = self.layers[0].input_layernorm(x)
+            for layer, nxt in zip(self.layers, [*self.layers[1:], None]):
+                x, h = layer.chained(x, h, self.final_layernorm if nxt is None else nxt.input_layernorm)
+        else:
+            for layer in self.layers:
+                x = layer(x)
+            h = self.final_layernorm(x)
+        logits = self.output_layer(h)
+        return logits if labels is None else loss.cross_entropy(logits, labels.t()).t()
 
     @torch.no_grad()
     def from_rwkv_lm(self, sd):

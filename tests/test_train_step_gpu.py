@@ -1,0 +1,188 @@
+"""The operators of a training step together: the model's stream through residual_norm, its loss through
+cross_entropy, gradients and AdamW with clipping; eager, captured, and beside the paths that a module with
+hooks takes."""
+import importlib
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF = torch.bfloat16
+V, B, T = 1001, 2, 70
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    return importlib.import_module("rwkv-megatron_amd")
+
+
+def _model(pkg, layers=3, bias=False):
+    cfg = pkg.modules.TransformerConfig(hidden_size=128, num_attention_heads=2, ffn_hidden_size=448, num_layers=layers,
+                                        params_dtype=torch.float32, add_bias_linear=bias, rwkv_lm_decay_init=True)
+    torch.manual_seed(0)
+    model = pkg.modules.RWKV6Model(cfg, V, device=DEV)
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if "bottleneck" in n and "weight" in n:
+                p.normal_(0, 0.1)
+            if n.endswith("linear_proj.bias"):
+                p.normal_(0, 0.5)
+    return model
+
+
+def _batch():
+    g = torch.Generator().manual_seed(1)
+    tokens, labels = torch.randint(0, V, (B, T), generator=g), torch.randint(0, V, (B, T), generator=g)
+    labels[0, :5] = -100
+    return tokens.to(DEV), labels.to(DEV)
+
+
+def _grads(model, loss):
+    return dict(zip([n for n, _ in model.named_parameters()], torch.autograd.grad(loss, list(model.parameters()))))
+
+
+def test_labels_give_the_loss_a_token(pkg):
+    model, (tokens, labels) = _model(pkg), _batch()
+    losses = model(tokens, labels)
+    logits = model(tokens)
+    assert losses.shape == (B, T) and losses.dtype == torch.float32 and logits.shape == (T, B, V)
+    assert torch.equal(losses, pkg.loss.cross_entropy(logits, labels.t()).t())
+    want = F.cross_entropy(logits.double().permute(1, 2, 0), labels, reduction="none")
+    # a log of a sum of 1001 exponentials in 32 bits, and a difference of numbers up to 16
+    assert float((losses.detach().double() - want.detach()).abs().max()) <= 2.0 ** -17
+
+
+# A layer with a hook is called as a module, and the stream's roundings are then the unfused operators': a
+# bf16 rounding (2^-8) more at two places a layer, of parts no larger than the stream.  Three layers and
+# the head: 2^-8 * sqrt(6) of the stream's norm on average, 2^-5 with the depth's amplification.
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("where", ["layers.1", "layers.1.pre_mlp_layernorm", "layers.2.mlp", "final_layernorm"])
+def test_hooks_are_called_and_the_paths_agree(pkg, where, bias):
+    model, (tokens, _) = _model(pkg, bias=bias), _batch()
+    logits = model(tokens).detach()
+    calls = []
+    model.get_submodule(where).register_forward_hook(lambda m, i, o: calls.append(m))
+    again = model(tokens).detach()
+    assert len(calls) == 1
+    assert float((again.double() - logits.double()).norm()) <= 2.0 ** -5 * float(logits.double().norm())
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_norms_with_hooks_run_the_operators_one_by_one(pkg, bias):
+    """Where every norm has a hook the model is the plain composition of its modules, bit for bit."""
+    model, (tokens, labels) = _model(pkg, bias=bias), _batch()
+    for layer in model.layers:
+        layer.register_forward_hook(lambda m, i, o: None)
+        for n in (layer.input_layernorm, layer.pre_mlp_layernorm):
+            n.register_forward_hook(lambda m, i, o: None)
+    x = model.pre_norm(model.embedding(tokens.t()).to(BF))
+    for layer in model.layers:
+        a, a_bias = layer.self_attention(layer.input_layernorm(x), None)
+        x = x + a if a_bias is None else x + (a + a_bias)
+        x = x + layer.mlp(layer.pre_mlp_layernorm(x))[0]
+    want = pkg.loss.cross_entropy(model.output_layer(model.final_layernorm(x)), labels.t()).t()
+    got = model(tokens, labels)
+    assert torch.equal(got, want)
+    for (n, u), v in zip(_grads(model, got.mean()).items(), _grads(model, want.mean()).values()):
+        assert torch.equal(u, v), n
+
+
+def test_layer_alone_and_other_norms(pkg):
+    """A layer called by itself, and one whose norm is another class: the same numbers to the roundings above."""
+    M = pkg.modules
+    model = _model(pkg)
+    layer = model.layers[1]
+    x = torch.randn(T, B, 128, generator=torch.Generator().manual_seed(3)).to(BF).to(DEV)
+    h = layer.input_layernorm(x)
+    s, y = layer.chained(x, h, model.final_layernorm)
+    alone = layer(x)
+    assert s.dtype == y.dtype == BF
+    assert float((s.double() - alone.double()).detach().norm()) <= 2.0 ** -7 * float(alone.detach().double().norm())
+
+    class Norm(M.LayerNorm):
+        pass
+
+    other = Norm(128, eps=layer.pre_mlp_layernorm.eps, device=DEV)
+    other.load_state_dict(layer.pre_mlp_layernorm.state_dict())
+    layer.pre_mlp_layernorm = other
+    assert float((layer(x).double() - alone.double()).detach().norm()) <= 2.0 ** -6 * float(alone.detach().double().norm())
+    assert layer(x[:, :, :].contiguous()).shape == x.shape
+
+
+def _train(pkg, model, steps, bits=32):
+    tokens, labels = _batch()
+    opt = pkg.optim.AdamW(model.parameters(), lr=1e-3, betas=(0.9, 0.995), weight_decay=0.1, max_norm=1.0, state_bits=bits,
+                          min_8bit_numel=1000)
+    mask = (labels != -100).float()
+
+    def step():
+        loss = (model(tokens, labels) * mask).sum() / mask.sum()
+        loss.backward()
+        opt.step()
+        return loss
+
+    out = []
+    for _ in range(steps):
+        out.append(step().detach().clone())
+        opt.zero_grad(set_to_none=True)
+    return opt, step, out
+
+
+# The gradients of one step, given to torch's optimizer in float64 with torch's clipping: the step of
+# AdamW is the only difference, 2^-17 of its length and a rounding of the parameter.
+def test_a_step_beside_torch(pkg):
+    model, (tokens, labels) = _model(pkg), _batch()
+    opt = pkg.optim.AdamW(model.parameters(), lr=1e-3, weight_decay=0.1, max_norm=0.5)
+    qs = [torch.nn.Parameter(p.detach().double()) for p in model.parameters()]
+    ref = torch.optim.AdamW(qs, lr=1e-3, weight_decay=0.1)
+    for k in range(3):
+        model(tokens, labels).mean().backward()
+        for p, q in zip(model.parameters(), qs):
+            q.grad = p.grad.double()
+        norm = torch.nn.utils.clip_grad_norm_(qs, 0.5)
+        opt.step()
+        ref.step()
+        opt.zero_grad()
+        assert abs(float(opt.grad_norm) - float(norm)) <= 2.0 ** -22 * float(norm)
+        for p, q in zip(model.parameters(), qs):
+            assert float((p.detach().double() - q).detach().abs().max()) <= (k + 1) * (2.0 ** -17 * 1e-3 + 2.0 ** -22 * float(q.detach().abs().max()))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_captured_training_step(pkg, bits):
+    """Forward, backward and optimizer captured once and replayed, eager work in between: the same losses and
+    parameters as eager steps, bit for bit."""
+    eager = _model(pkg)
+    opt_e, step_e, _ = _train(pkg, eager, 2, bits)
+    model = _model(pkg)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt, step, _ = _train(pkg, model, 2, bits)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(eager.parameters(), model.parameters()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    for rep in range(3):
+        graph.replay()
+        torch.randn(512, 512, device=DEV).sum().item()
+        torch.cuda.synchronize()
+        want = step_e()
+        opt_e.zero_grad(set_to_none=True)
+        assert torch.equal(loss, want), rep
+        assert all(torch.equal(p, q) for p, q in zip(eager.parameters(), model.parameters())), rep
+        # the captured gradients are written over by the next replay: none may be added to
+    assert float(opt.state[next(iter(model.parameters()))]["step"]) == 5
+
+
+def test_without_gradients_and_a_prompt_of_one_token(pkg):
+    model, (tokens, _) = _model(pkg), _batch()
+    with torch.no_grad():
+        full = model(tokens)
+        assert not full.requires_grad
+        one = model(tokens[:, :1])
+    # the first token does not depend on the later ones; kernels of few tokens sum in other orders
+    assert float((one.double() - full[:1].double()).norm()) <= 2.0 ** -5 * float(full[:1].double().norm())
