@@ -203,24 +203,36 @@ rwkv6_adamw_coef_kernel(const double* __restrict__ part, int P, float max_norm, 
                         float* __restrict__ step, const float* __restrict__ lr_dev, double lr, double log_b1,
                         double log_b2, double wd, Coef* __restrict__ coef) {
     __shared__ double red[16];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const bool first = wv == 0 && coef;
+    // 1 - b^t for b1 in the even lanes and b2 in the odd ones, while the sums come in
+    const float t = first ? step[0] + 1.f : 1.f;
+    const double bc = first ? -expm1((double)t * (lane & 1 ? log_b2 : log_b1)) : 1.;
+    if (first && lr_dev) lr = (double)lr_dev[0];
     double acc = 0.;
-    for (int i = threadIdx.x; i < P; i += 1024) acc += part[i];
+    for (int i = threadIdx.x; i < P; i += 4 * 1024) {
+        double v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = part[min(i + k * 1024, P - 1)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc += i + k * 1024 < P ? v[k] : 0.;
+    }
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) acc += __shfl_xor(acc, o);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+    if (lane == 0) red[wv] = acc;
     __syncthreads();
-    if (threadIdx.x) return;
-    acc = 0.;
-    for (int w = 0; w < 16; ++w) acc += red[w];
+    if (wv) return;
+    acc = lane < 16 ? red[lane] : 0.;
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) acc += __shfl_xor(acc, o);
+    const double bc2 = __shfl_xor(bc, 1);
+    if (lane) return;
     const float norm = (float)sqrt(acc), r = max_norm / (norm + 1e-6f);
     if (norm_out) norm_out[0] = norm;
     if (!coef) return;
-    const float t = step[0] + 1.f;
     step[0] = t;
-    if (lr_dev) lr = (double)lr_dev[0];
     // a NaN norm stays one: the whole update is NaN, as clipped gradients would be
-    coef[0] = Coef{part && !(r > 1.f) ? r : 1.f, (float)(1. - lr * wd), (float)(lr / -expm1((double)t * log_b1)),
-                   (float)(1. / sqrt(-expm1((double)t * log_b2)))};
+    coef[0] = Coef{part && !(r > 1.f) ? r : 1.f, (float)(1. - lr * wd), (float)(lr / bc), (float)(1. / sqrt(bc2))};
 }
 
 // Block b: `per` elements of a tensor, 8 a thread and step.  32 lanes hold the 256 elements of one scale.

@@ -450,14 +450,15 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         Param ga = param(gamma), be = param(beta);
         if (ga.dt != be.dt) ga = {to_f32(gamma), RWKV6_F32}, be = {to_f32(beta), RWKV6_F32};
         const Tensor s = at::empty_like(a.x), y = at::empty_like(a.branch);
-        const Tensor mean = grad ? empty({a.N}, at::kFloat, x) : Tensor(), rstd = grad ? at::empty_like(mean) : Tensor();
+        const Tensor stats = grad ? empty({2, a.N}, at::kFloat, x) : Tensor();           // mean, rstd
+        float* const mean = fptr(stats);
         check(rwkv6_residual_norm_fwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
-                                      ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), fptr(mean), fptr(rstd), a.N,
-                                      a.C, stream_of(x)),
+                                      ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), mean, mean ? mean + a.N : nullptr,
+                                      a.N, a.C, stream_of(x)),
               "rwkv6_residual_norm_fwd");
         if (grad) {
             ctx->set_materialize_grads(false);
-            ctx->save_for_backward({x, branch, gt, cb, gamma, beta, mean, rstd});
+            ctx->save_for_backward({x, branch, gt, cb, gamma, beta, stats});
             put(ctx, {bits(scale)});
         }
         return {s, y};
@@ -483,7 +484,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor dcb = sums && biased ? empty({a.C}, a.cbias.t.scalar_type(), x) : Tensor();
         const Tensor ws = sums ? bytes(rwkv6_residual_norm_bwd_workspace_bytes(a.N, a.C), x) : Tensor();
         check(rwkv6_residual_norm_bwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
-                                      ptr(ga.t), ga.dt, fptr(sv[6]), fptr(sv[7]), ptr(ds), ptr(dy), ptr(dx), ptr(db), ptr(dg),
+                                      ptr(ga.t), ga.dt, fptr(sv[6]), a.N ? fptr(sv[6]) + a.N : nullptr, ptr(ds), ptr(dy), ptr(dx), ptr(db), ptr(dg),
                                       ptr(dga), ptr(dbe), dt, ptr(dcb), ptr(ws), a.N, a.C, stream_of(x)),
               "rwkv6_residual_norm_bwd");
         return {dx, same ? dx : db, sums ? cast(dga, gamma.scalar_type()) : dga, sums ? cast(dbe, beta.scalar_type()) : dbe, dg,
@@ -497,7 +498,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor s = x.to(at::kFloat) + (gate.defined() ? f * sg : f) * scale;
         std::vector<int64_t> st(x.sizes().begin(), x.sizes().end());
         st.back() = 1;
-        auto [dS, dga, dbe] = at::native_layer_norm_backward(dy.to(at::kFloat), s, {x.size(-1)}, sv[6].view(st), sv[7].view(st),
+        auto [dS, dga, dbe] = at::native_layer_norm_backward(dy.to(at::kFloat), s, {x.size(-1)}, sv[6][0].view(st), sv[6][1].view(st),
                                                              gamma.to(at::kFloat), beta.to(at::kFloat), {true, true, true});
         if (ds.defined()) dS = dS + ds.to(at::kFloat);
         const Tensor df = dS * scale, db = gate.defined() ? df * sg : df;

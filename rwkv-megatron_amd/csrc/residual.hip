@@ -143,7 +143,7 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
             store8_as<XF>(s, row + c[i], v[i], nt);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] - mean) * rstd * ga[i][j] + be[i][j];
-            store8_as<false>(y, row + c[i], v[i], nt);
+            store8(y + row + c[i], v[i]);
         }
         if (mean_out && lane == 0 && w == 0) {
             mean_out[n] = mean;
@@ -323,10 +323,11 @@ inline RnShape rn_shape(int64_t C) {
     const int NV = C > RN_PIECE * RN_MAX_WAVES ? 2 : 1, W = (int)((C + RN_PIECE * NV - 1) / (RN_PIECE * NV));
     return {NV, W, W >= 4 ? 1 : 4 / W};
 }
-// Whether the outputs are stored past the caches: where the call's tensors do not fit the 256 MB of the last
-// one anyway.  Kept in it, they push out what the call still reads: 16384 x 2048 bf16, us, cached and
-// streamed: backward 72 and 62, gated forward 64 and 55.  (A training step of the 1.6B shape, whose next
-// kernels read some of them again, takes the same time with either.)
+// Whether the outputs but y (which the next kernel reads) are stored past the caches: where the call's
+// tensors do not fit the 256 MB of the last one anyway.  Kept in it, they push out what the call still
+// reads: 16384 x 2048 bf16, us, cached and streamed: backward 72 and 60, gated 103 and 92, gated forward
+// 64 and 56; y streamed too 58.  (A training step of the 1.6B shape, whose next kernels read some of them
+// again, takes the same time with either.)
 inline bool rn_stream(int64_t N, int64_t C) { return N * C >= (int64_t)1 << 24; }
 // Row ranges of the backward: RN_PART of them, two a CU, where that leaves each two steps of a block.
 inline int64_t rn_parts(int64_t N, int RB) {

@@ -58,7 +58,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
 
 
 def _step(native, params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, max_norm, sums):
-    tensor = isinstance(lr, torch.Tensor)
+    tensor = isinstance(lr, torch.Tensor) and lr.is_cuda
     return native.adamw_step(params, grads, m, v, ms, vs, step, 0.0 if tensor else float(lr), lr if tensor else None,
                              betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, sums)
 
@@ -103,6 +103,10 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_norm, self.min_8bit_numel = state_bits, max_norm, min_8bit_numel
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def __getstate__(self):                        # torch's own holds the state and the groups alone
+        own = dict(state_bits=self.state_bits, max_norm=self.max_norm, min_8bit_numel=self.min_8bit_numel, grad_norm=None)
+        return {**super().__getstate__(), **own}
 
     def add_param_group(self, group):
         super().add_param_group(group)

@@ -109,16 +109,21 @@ def test_grad_norm(opt):
 
 
 @pytest.mark.parametrize("eight", [False, True])
-def test_views_off_the_16_byte_grid(opt, eight):
+@pytest.mark.parametrize("off", [0, 1])
+def test_views_off_the_16_byte_grid_and_their_neighbours(opt, eight, off):
     t = _lists([4099], BF, BF, eight)
     u = copy.deepcopy(t)
+    wides = []
     for n in ("p", "g", "m", "v"):
         x = u[n][0]
-        wide = torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)
-        wide[1:].copy_(x)
-        u[n][0] = wide[1:]
+        wide = torch.full((x.numel() + 16,), 3, dtype=torch.float32, device=DEV).to(x.dtype)
+        wide[off:off + 4099].copy_(x)
+        u[n][0] = wide[off:off + 4099]
+        wides.append(wide)
     _call(opt, t, max_norm=0.1)
     _call(opt, u, max_norm=0.1)
+    for wide in wides:
+        assert bool((wide[:off].float() == 3).all()) and bool((wide[off + 4099:].float() == 3).all())
     for n in ("p", "m", "v"):
         assert torch.equal(t[n][0].view(torch.uint8), u[n][0].contiguous().view(torch.uint8))
 
@@ -186,7 +191,7 @@ def test_8_bit_states_of_the_large_tensors_alone(opt):
     for p, q in zip(ps, ref):
         # m and the root of v each off by 2^-4 at most a step: a step by a factor within (1 +- 2^-4)^2 / (1 -+ 2^-4)
         # of the first moments' |terms|; three steps of at most lr / (1 - b1) each
-        assert float((p - q).abs().max()) <= 3 * HYPER["lr"] * 3
+        assert float((p - q).detach().abs().max()) <= 3 * HYPER["lr"] * 3
         m, v = o.moments(p)
         m2, v2 = r.moments(q)
         assert float((m - m2).norm() / m2.norm()) <= 3 * 2.0 ** -4 and float((v.sqrt() - v2.sqrt()).norm() / v2.sqrt().norm()) <= 3 * 2.0 ** -4
@@ -206,7 +211,7 @@ def test_parameters_without_a_gradient_make_no_step(opt):
     assert [float(a.state[p]["step"]) for p in ps] == [3, 3, 3, 3] == [float(b.state[q]["step"]) for q in qs]
     for p, q in zip(ps, qs):
         # both in 32 bits: a few roundings a step
-        assert float((p - q).abs().max()) <= 5 * (2.0 ** -16 * HYPER["lr"] + 2.0 ** -22)
+        assert float((p - q).detach().abs().max()) <= 5 * (2.0 ** -16 * HYPER["lr"] + 2.0 ** -22)
     ps2 = _params(F32)
     o = opt.AdamW(ps2, **HYPER)
     o.step()
@@ -317,7 +322,7 @@ def test_learning_rate_on_the_device_and_captured_steps(opt):
         torch.cuda.synchronize()
         # the learning rate is 32 bits there and 64 here
         for p, q in zip(ps, qs):
-            assert float((p - q).abs().max()) <= k * 2.0 ** -20 * HYPER["lr"] * 8
+            assert float((p - q).detach().abs().max()) <= k * 2.0 ** -20 * HYPER["lr"] * 8
         assert torch.equal(a.grad_norm, b.grad_norm)
     assert all(float(a.state[p]["step"]) == 4 for p in ps)
 
@@ -339,6 +344,40 @@ def test_updates_are_seen_by_autograd_and_other_streams(opt):
         r.step()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_copy_of_the_optimizer_goes_on_by_itself(opt, bits):
+    ps = _params(F32)
+    a = opt.AdamW(ps, **HYPER, state_bits=bits, max_norm=0.3, min_8bit_numel=100)
+    _grads(ps, 0)
+    a.step()
+    b = copy.deepcopy(a)
+    qs = [q for g in b.param_groups for q in g["params"]]
+    assert (b.state_bits, b.max_norm, b.min_8bit_numel) == (bits, 0.3, 100) and qs[0] is not ps[0]
+    for k in (1, 2):
+        _grads(ps, k)
+        _grads(qs, k)
+        a.step()
+        if k == 1:
+            assert float(b.state[qs[0]]["step"]) == 1
+        b.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and float(b.state[qs[3]]["step"]) == 3
+
+
+def test_a_scheduler_and_a_learning_rate_on_the_cpu(opt):
+    ps, qs = _params(F32), _params(F32)
+    a = opt.AdamW(ps, **{**HYPER, "lr": torch.tensor(1e-2)})
+    b = opt.AdamW(qs, **HYPER)
+    for o in (a, b):
+        s = torch.optim.lr_scheduler.LambdaLR(o, lambda k: 0.5 ** k)
+        group = [p for g in o.param_groups for p in g["params"]]
+        for k in range(3):
+            _grads(group, k)
+            o.step()
+            s.step()
+    # 0.01 in 32 bits and in 64
+    assert all(float((p - q).detach().abs().max()) <= 3 * 2.0 ** -18 * 1e-2 + 2.0 ** -24 for p, q in zip(ps, qs))
 
 
 def test_refusals(opt):
