@@ -33,6 +33,7 @@
 #define AW_AHEAD 4              // steps of the norm's loads in flight
 #define AW_T 60                 // tensors a launch: the arguments stay below 4 KB
 #define AW_BLK 256              // elements under one 8-bit scale: 32 lanes of 8
+#define AW_MAX ((int64_t)1 << 37)   // elements a call: a launch stays below 2^32 threads
 #define AW_F8_MAX 448.f
 #define AW_TINY 0x1p-118f
 
@@ -312,10 +313,10 @@ int aw_sizes(const int64_t* numel, int64_t count) {
     int64_t total = 0;
     for (int64_t k = 0; k < count; ++k) {
         if (numel[k] < 0) return RWKV6_ERR_INVALID_ARG;
-        if (numel[k] > ((int64_t)1 << 40)) return RWKV6_ERR_UNSUPPORTED;
+        if (numel[k] > AW_MAX) return RWKV6_ERR_UNSUPPORTED;
         total += numel[k];
     }
-    return total > ((int64_t)1 << 40) ? RWKV6_ERR_UNSUPPORTED : RWKV6_OK;
+    return total > AW_MAX ? RWKV6_ERR_UNSUPPORTED : RWKV6_OK;
 }
 int64_t aw_partials(const int64_t* numel, int64_t count) {
     const int64_t per = aw_per(numel, count, AW_PARTS, 0);
@@ -394,7 +395,7 @@ int rwkv6_grad_norm_sums(const void* const* grad, const int* grad_dtype, const i
 
 int rwkv6_grad_norm(const double* partials, int64_t P, float* norm, void* stream) {
     if (P < 0 || (P && !partials) || !norm) return RWKV6_ERR_INVALID_ARG;
-    if (P > 0x7fffffff) return RWKV6_ERR_UNSUPPORTED;
+    if (P > (1 << 30)) return RWKV6_ERR_UNSUPPORTED;
     if (aw_misaligned(partials, 8) || aw_misaligned(norm, 4)) return RWKV6_ERR_ALIGNMENT;
     if (any_alias({{norm, 4}}, {{partials, (size_t)P * 8}})) return RWKV6_ERR_INVALID_ARG;
     hipLaunchKernelGGL(rwkv6_adamw_coef_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), partials,
@@ -411,7 +412,7 @@ int rwkv6_adamw_step(void* const* param, const int* param_dtype, const void* con
     if (st) return st;
     const bool f8 = exp_avg_scale != nullptr;
     if (!step || !workspace || P < 0 || (P && !partials)) return RWKV6_ERR_INVALID_ARG;
-    if (P > 0x7fffffff) return RWKV6_ERR_UNSUPPORTED;
+    if (P > (1 << 30)) return RWKV6_ERR_UNSUPPORTED;
     if (!(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1.)) return RWKV6_ERR_INVALID_ARG;
     if (count && (!param || !param_dtype || !grad || !grad_dtype || !exp_avg || !exp_avg_sq)) return RWKV6_ERR_INVALID_ARG;
     if (f8 != (exp_avg_sq_scale != nullptr)) return RWKV6_ERR_INVALID_ARG;
@@ -465,8 +466,7 @@ int rwkv6_adamw_step(void* const* param, const int* param_dtype, const void* con
     for (int64_t k = 0; k < count; ++k) {
         if (numel[k] == 0) continue;
         const int64_t need = aw_blocks(numel[k], per);
-        // a launch has fewer than 2^32 threads
-        if (tab.count == AW_T || blocks + need >= ((int64_t)1 << 24)) launch();
+        if (tab.count == AW_T) launch();
         const int i = tab.count++;
         tab.p[i] = param[k];
         tab.g[i] = grad[k];

@@ -20,6 +20,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
+#include <array>
 #include <cstring>
 #include <optional>
 #include <vector>
@@ -442,25 +443,29 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         return {dense(x), dense(branch), gate.defined() ? dense(gate) : gate, cbias.defined() ? param(cbias) : Param{cbias, 0},
                 x.scalar_type() == at::kFloat ? RWKV6_F32 : RWKV6_BF16, C ? x.numel() / C : 0, C};
     }
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& branch, const Tensor& gamma,
-                                 const Tensor& beta, const OptTensor& gate, const OptTensor& cbias, double eps,
-                                 double scale, bool grad) {
-        const Tensor gt = gate.value_or(Tensor()), cb = cbias.value_or(Tensor());
-        const Args a = args(x, branch, gt, cb);
+    // (s, y), and the rows' mean and rstd ([2, N]) where a backward will want them
+    static std::array<Tensor, 3> run(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta,
+                                     const Tensor& gate, const Tensor& cbias, double eps, double scale, bool grad) {
+        const Args a = args(x, branch, gate, cbias);
         Param ga = param(gamma), be = param(beta);
         if (ga.dt != be.dt) ga = {to_f32(gamma), RWKV6_F32}, be = {to_f32(beta), RWKV6_F32};
         const Tensor s = at::empty_like(a.x), y = at::empty_like(a.branch);
-        const Tensor stats = grad ? empty({2, a.N}, at::kFloat, x) : Tensor();           // mean, rstd
+        const Tensor stats = grad ? empty({2, a.N}, at::kFloat, x) : Tensor();
         float* const mean = fptr(stats);
         check(rwkv6_residual_norm_fwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
                                       ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), mean, mean ? mean + a.N : nullptr,
                                       a.N, a.C, stream_of(x)),
               "rwkv6_residual_norm_fwd");
-        if (grad) {
-            ctx->set_materialize_grads(false);
-            ctx->save_for_backward({x, branch, gt, cb, gamma, beta, stats});
-            put(ctx, {bits(scale)});
-        }
+        return {s, y, stats};
+    }
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& branch, const Tensor& gamma,
+                                 const Tensor& beta, const OptTensor& gate, const OptTensor& cbias, double eps,
+                                 double scale) {
+        const Tensor gt = gate.value_or(Tensor()), cb = cbias.value_or(Tensor());
+        const auto [s, y, stats] = run(x, branch, gamma, beta, gt, cb, eps, scale, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({x, branch, gt, cb, gamma, beta, stats});
+        put(ctx, {bits(scale)});
         return {s, y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -488,7 +493,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
                                       ptr(dga), ptr(dbe), dt, ptr(dcb), ptr(ws), a.N, a.C, stream_of(x)),
               "rwkv6_residual_norm_bwd");
         return {dx, same ? dx : db, sums ? cast(dga, gamma.scalar_type()) : dga, sums ? cast(dbe, beta.scalar_type()) : dbe, dg,
-                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor(), Tensor()};
+                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor()};
     }
     // A backward that is differentiated itself: the same formulas in torch's operators.
     static variable_list differentiable(const variable_list& sv, const Tensor& ds, const Tensor& dy, double scale) {
@@ -505,7 +510,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor dg = gate.defined() ? (df * f * sg * (1 - sg)).to(gate.scalar_type()) : Tensor();
         const Tensor dcb = cbias.defined() ? db.reshape({-1, x.size(-1)}).sum(0).to(cbias.scalar_type()) : Tensor();
         return {dS.to(x.scalar_type()), db.to(branch.scalar_type()), dga.to(gamma.scalar_type()), dbe.to(beta.scalar_type()),
-                dg, dcb, Tensor(), Tensor(), Tensor()};
+                dg, dcb, Tensor(), Tensor()};
     }
 };
 // None when the kernels do not take the call (only_plain: nor one that a mode or transform wants to see);
@@ -526,8 +531,16 @@ py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& ga
             return py::none();
     if (only_plain && !plain({&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})) return py::none();
     no_transforms();
-    const bool grad = recorded({&x, &branch, &gamma, &beta, gate ? &*gate : &x}, cbias);
-    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, grad); });
+    bool grad = recorded({&x, &branch, &gamma, &beta, gate ? &*gate : &x}, cbias);
+    for (const Tensor* t : {&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})
+        grad = grad || t->_fw_grad(0).defined();          // forward-mode derivatives are refused there
+    if (!grad) {
+        const auto o = unlocked([&] {
+            return ResidualNorm::run(x, branch, gamma, beta, gate.value_or(Tensor()), cbias.value_or(Tensor()), eps, scale, false);
+        });
+        return py::make_tuple(o[0], o[1]);
+    }
+    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale); });
     return py::make_tuple(o[0], o[1]);
 }
 

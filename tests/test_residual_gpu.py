@@ -232,6 +232,9 @@ def test_saved_tensors_and_transforms(rn):
         torch.autograd.grad(out, list(t.values()), (ds, dy))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda x: rn(x, t["branch"][0], t["weight"], t["bias"], EPS)[1])(t["x"])
+    x, branch, w, b = (t[n].detach() for n in ("x", "branch", "weight", "bias"))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        rn(torch.autograd.forward_ad.make_dual(x, x), branch, w, b, EPS)
 
 
 def test_graph_replays_and_another_stream(rn):
