@@ -287,21 +287,23 @@ int rwkv6_layer_norm_bwd(const void* x, const void* gamma, int gamma_dtype, cons
  *   f = (branch + branch_bias) * sigmoid(gate), s = x + scale * f, y = LayerNorm(s) * gamma + beta
  * x, s: [N,C] in x_dtype; branch, gate, y: [N,C] bf16; branch_bias [C] in bias_dtype and gate nullable;
  * gamma, beta: [C] in param_dtype; mean, rstd: [N] f32 for the backward (both NULL without one).  The
- * statistics and y are those of s before it is rounded to x_dtype.
+ * statistics and y are those of s before it is rounded to x_dtype; with stepwise != 0 the sum with
+ * the bias, the product with the gate and s are rounded (bf16, bf16, x_dtype) where separate operators
+ * would round them, and y is the norm of s as stored.
  *   bwd: ds [N,C] in x_dtype (nullable: zero), dy [N,C] bf16 -> dx in x_dtype, d_branch, d_gate bf16
  *        (d_gate NULL exactly when gate is), dgamma, dbeta in param_dtype and d_branch_bias in bias_dtype
  *        (all NULL: not wanted, no workspace; d_branch_bias NULL also when branch_bias is).  d_branch may
  *        be NULL where it equals dx: x_dtype bf16, scale 1, neither gate nor branch_bias.
  * ---------------------------------------------------------------------- */
 int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias,
-                            int bias_dtype, const void* gate, float scale, const void* gamma,
-                            const void* beta, int param_dtype, float eps, void* s, void* y,
-                            float* mean, float* rstd, int64_t N, int64_t C, void* stream);
+                            int bias_dtype, const void* gate, float scale, int stepwise,
+                            const void* gamma, const void* beta, int param_dtype, float eps, void* s,
+                            void* y, float* mean, float* rstd, int64_t N, int64_t C, void* stream);
 size_t rwkv6_residual_norm_bwd_workspace_bytes(int64_t N, int64_t C);
 int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias,
-                            int bias_dtype, const void* gate, float scale, const void* gamma,
-                            int gamma_dtype, const float* mean, const float* rstd, const void* ds,
-                            const void* dy, void* dx, void* d_branch, void* d_gate, void* dgamma,
+                            int bias_dtype, const void* gate, float scale, int stepwise,
+                            const void* gamma, int gamma_dtype, const float* mean, const float* rstd,
+                            const void* ds, const void* dy, void* dx, void* d_branch, void* d_gate, void* dgamma,
                             void* dbeta, int param_dtype, void* d_branch_bias, void* workspace,
                             int64_t N, int64_t C, void* stream);
 

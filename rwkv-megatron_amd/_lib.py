@@ -78,10 +78,10 @@ SIGNATURES = {
     "rwkv6_linear_f32": (_int, [_vp, _fp, _vp, _vp] + [_i64] * 3 + [_vp]),
     "rwkv6_layer_norm_fwd": (_int, [_vp] * 3 + [_int, _f32, _vp, _fp, _fp, _fp] + [_i64] * 2 + [_vp]),
     "rwkv6_layer_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64] * 2),
-    "rwkv6_residual_norm_fwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _vp, _vp, _int, _f32, _vp, _vp, _fp, _fp]
+    "rwkv6_residual_norm_fwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _int, _vp, _vp, _int, _f32, _vp, _vp, _fp, _fp]
                                 + [_i64] * 2 + [_vp]),
     "rwkv6_residual_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64] * 2),
-    "rwkv6_residual_norm_bwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _vp, _int, _fp, _fp] + [_vp] * 7
+    "rwkv6_residual_norm_bwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _int, _vp, _int, _fp, _fp] + [_vp] * 7
                                 + [_int, _vp, _vp] + [_i64] * 2 + [_vp]),
     "rwkv6_cross_entropy_fwd": (_int, [_vp, _int, _i64, _vp, _i64, _fp, _fp] + [_i64] * 2 + [_vp]),
     "rwkv6_cross_entropy_bwd": (_int, [_vp, _int, _i64, _vp, _i64, _fp, _fp, _vp] + [_i64] * 2 + [_vp]),

@@ -283,8 +283,8 @@ rwkv6_adamw_step_kernel(const StepTable tab, const Coef* __restrict__ coef, int6
             float tm = aw_top(mf), tv = aw_top(root);
             tm = tm < AW_TINY ? 0.f : tm;
             tv = tv < AW_TINY ? 0.f : tv;
-            aw_codes_store(m, i, n, vec, aw_encode(mf, tm > 0.f ? AW_F8_MAX / tm : 0.f));
-            aw_codes_store(v, i, n, vec, aw_encode(root, tv > 0.f ? AW_F8_MAX / tv : 0.f));
+            aw_codes_store(m, i, n, vec, aw_encode(mf, tm > 0.f ? (1.f / tm) * AW_F8_MAX : 0.f));
+            aw_codes_store(v, i, n, vec, aw_encode(root, tv > 0.f ? (1.f / tv) * AW_F8_MAX : 0.f));
             if ((threadIdx.x & 31) == 0) {
                 ms[0] = tm * (1.f / AW_F8_MAX);
                 vs[0] = tv * (1.f / AW_F8_MAX);

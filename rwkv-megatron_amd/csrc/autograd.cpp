@@ -445,7 +445,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     }
     // (s, y), and the rows' mean and rstd ([2, N]) where a backward will want them
     static std::array<Tensor, 3> run(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta,
-                                     const Tensor& gate, const Tensor& cbias, double eps, double scale, bool grad) {
+                                     const Tensor& gate, const Tensor& cbias, double eps, double scale, bool stepwise,
+                                     bool grad) {
         const Args a = args(x, branch, gate, cbias);
         Param ga = param(gamma), be = param(beta);
         if (ga.dt != be.dt) ga = {to_f32(gamma), RWKV6_F32}, be = {to_f32(beta), RWKV6_F32};
@@ -453,25 +454,26 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor stats = grad ? empty({2, a.N}, at::kFloat, x) : Tensor();
         float* const mean = fptr(stats);
         check(rwkv6_residual_norm_fwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
-                                      ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), mean, mean ? mean + a.N : nullptr,
+                                      stepwise, ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), mean, mean ? mean + a.N : nullptr,
                                       a.N, a.C, stream_of(x)),
               "rwkv6_residual_norm_fwd");
         return {s, y, stats};
     }
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& branch, const Tensor& gamma,
                                  const Tensor& beta, const OptTensor& gate, const OptTensor& cbias, double eps,
-                                 double scale) {
+                                 double scale, bool stepwise) {
         const Tensor gt = gate.value_or(Tensor()), cb = cbias.value_or(Tensor());
-        const auto [s, y, stats] = run(x, branch, gamma, beta, gt, cb, eps, scale, true);
+        const auto [s, y, stats] = run(x, branch, gamma, beta, gt, cb, eps, scale, stepwise, true);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({x, branch, gt, cb, gamma, beta, stats});
-        put(ctx, {bits(scale)});
+        put(ctx, {bits(scale), stepwise});
         return {s, y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const auto sv = ctx->get_saved_variables();
         const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2], &cbias = sv[3], &gamma = sv[4], &beta = sv[5];
-        const double scale = unbits(meta(ctx)[0]);
+        const auto m = meta(ctx);
+        const double scale = unbits(m[0]);
         // an output no loss uses has no gradient
         const Tensor dy = g[1].defined() ? to_bf16(g[1]) : at::zeros(branch.sizes(), branch.options());
         if (at::GradMode::is_enabled()) return differentiable(sv, g[0], g[1].defined() ? g[1] : dy, scale);
@@ -489,11 +491,11 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor dcb = sums && biased ? empty({a.C}, a.cbias.t.scalar_type(), x) : Tensor();
         const Tensor ws = sums ? bytes(rwkv6_residual_norm_bwd_workspace_bytes(a.N, a.C), x) : Tensor();
         check(rwkv6_residual_norm_bwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
-                                      ptr(ga.t), ga.dt, fptr(sv[6]), a.N ? fptr(sv[6]) + a.N : nullptr, ptr(ds), ptr(dy), ptr(dx), ptr(db), ptr(dg),
+                                      (int)m[1], ptr(ga.t), ga.dt, fptr(sv[6]), a.N ? fptr(sv[6]) + a.N : nullptr, ptr(ds), ptr(dy), ptr(dx), ptr(db), ptr(dg),
                                       ptr(dga), ptr(dbe), dt, ptr(dcb), ptr(ws), a.N, a.C, stream_of(x)),
               "rwkv6_residual_norm_bwd");
         return {dx, same ? dx : db, sums ? cast(dga, gamma.scalar_type()) : dga, sums ? cast(dbe, beta.scalar_type()) : dbe, dg,
-                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor()};
+                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor(), Tensor()};
     }
     // A backward that is differentiated itself: the same formulas in torch's operators.
     static variable_list differentiable(const variable_list& sv, const Tensor& ds, const Tensor& dy, double scale) {
@@ -510,13 +512,13 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor dg = gate.defined() ? (df * f * sg * (1 - sg)).to(gate.scalar_type()) : Tensor();
         const Tensor dcb = cbias.defined() ? db.reshape({-1, x.size(-1)}).sum(0).to(cbias.scalar_type()) : Tensor();
         return {dS.to(x.scalar_type()), db.to(branch.scalar_type()), dga.to(gamma.scalar_type()), dbe.to(beta.scalar_type()),
-                dg, dcb, Tensor(), Tensor()};
+                dg, dcb, Tensor(), Tensor(), Tensor()};
     }
 };
 // None when the kernels do not take the call (only_plain: nor one that a mode or transform wants to see);
 // the callers check and raise, or run torch's operators.
 py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta, double eps,
-                         const OptTensor& gate, const OptTensor& cbias, double scale, bool only_plain) {
+                         const OptTensor& gate, const OptTensor& cbias, double scale, bool stepwise, bool only_plain) {
     if (!x.is_cuda() || x.dim() < 1 || x.size(-1) < 1 || x.layout() != at::kStrided ||
         (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat))
         return py::none();
@@ -536,11 +538,11 @@ py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& ga
         grad = grad || t->_fw_grad(0).defined();          // forward-mode derivatives are refused there
     if (!grad) {
         const auto o = unlocked([&] {
-            return ResidualNorm::run(x, branch, gamma, beta, gate.value_or(Tensor()), cbias.value_or(Tensor()), eps, scale, false);
+            return ResidualNorm::run(x, branch, gamma, beta, gate.value_or(Tensor()), cbias.value_or(Tensor()), eps, scale, stepwise, false);
         });
         return py::make_tuple(o[0], o[1]);
     }
-    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale); });
+    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, stepwise); });
     return py::make_tuple(o[0], o[1]);
 }
 

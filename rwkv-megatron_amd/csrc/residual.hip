@@ -11,6 +11,10 @@
 //   dgamma = sum_rows dy xh, dbeta = sum_rows dy, d_branch_bias = sum_rows d_branch (fixed order)
 // s is rounded once, to x's type, on its way out.  The backward forms it again from the inputs: a
 // stored bf16 s would put its rounding, 2^-9 of s, into xh and so into an fp32 dgamma.
+// `stepwise` gives the numbers of the operators run one by one instead: the sum with the bias, the
+// product with the gate and s are rounded (bf16, bf16, x's type) before the next takes them, and y
+// is the norm of s as it is stored.  The layers and the model run that, so that fusing them changed
+// no forward value of theirs by more than the order of a row's sums does.
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 
@@ -71,7 +75,10 @@ struct RnIn {
     const void* cbias;
     int cdt;
     float scale;
+    int stepwise;
 };
+// Eight values rounded to bf16.
+__device__ __forceinline__ void round8(float* f) { unpack8(pack8(f), f); }
 
 }  // namespace
 
@@ -112,6 +119,7 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
                 load8(in.branch + row + c[i], f);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) f[j] += cb[i][j];
+                if (in.stepwise) round8(f);
                 if constexpr (GATE) {
                     float g[8];
                     load8(in.gate + row + c[i], g);
@@ -119,10 +127,13 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
                     for (int j = 0; j < 8; ++j) f[j] *= sigmoid(g[j]);
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[i][j] += in.scale * f[j];
-                    sum += v[i][j];
-                }
+                for (int j = 0; j < 8; ++j) f[j] *= in.scale;
+                if (in.stepwise) round8(f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] += f[j];
+                if (!XF && in.stepwise) round8(v[i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += v[i][j];
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
@@ -197,12 +208,24 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
             if constexpr (GATE) load8(in.gate + row + c[i], sg[i]);
             load8(dy + row + c[i], g[i]);
             if (ds) raw_f32<XF>(w_load<XF>(ds, row + c[i]), dS[i]);
+            if constexpr (CB) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[i][j] += cb[i][j];
+                if (in.stepwise) round8(f[i]);
+            }
+            float t[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if constexpr (CB) f[i][j] += cb[i][j];
                 if constexpr (GATE) sg[i][j] = sigmoid(sg[i][j]);
-                const float t = xh[i][j] + in.scale * (GATE ? f[i][j] * sg[i][j] : f[i][j]);
-                xh[i][j] = (t - mean) * rstd;
+                t[j] = (GATE ? f[i][j] * sg[i][j] : f[i][j]) * in.scale;
+            }
+            if (in.stepwise) round8(t);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] += xh[i][j];
+            if (!XF && in.stepwise) round8(t);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                xh[i][j] = (t[j] - mean) * rstd;
                 if (live) {
                     ag[i][j] += g[i][j] * xh[i][j];
                     ab[i][j] += g[i][j];
@@ -339,8 +362,8 @@ inline int64_t rn_parts(int64_t N, int RB) {
 extern "C" {
 
 int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
-                            const void* gate, float scale, const void* gamma, const void* beta, int param_dtype,
-                            float eps, void* s, void* y, float* mean, float* rstd, int64_t N, int64_t C, void* stream) {
+                            const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
+                            int param_dtype, float eps, void* s, void* y, float* mean, float* rstd, int64_t N, int64_t C, void* stream) {
     const int st = rn_check(N, C);
     if (st) return st;
     if (!dt_ok(x_dtype) || !dt_ok(param_dtype) || (branch_bias && !dt_ok(bias_dtype)) || (!mean != !rstd))
@@ -363,7 +386,7 @@ int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, cons
     const int64_t blocks = (N + h.RB - 1) / h.RB;
     hipLaunchKernelGGL(k, dim3((unsigned)(blocks < RN_FWD_BLOCKS ? blocks : RN_FWD_BLOCKS)), dim3(64 * h.W * h.RB), 0,
                        reinterpret_cast<hipStream_t>(stream),
-                       RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale}, gamma, beta,
+                       RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale, stepwise}, gamma, beta,
                        param_dtype, eps, s, (uint16_t*)y, mean, rstd, N, (int)C, h.W, h.RB, rn_stream(N, C));
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
@@ -374,7 +397,7 @@ size_t rwkv6_residual_norm_bwd_workspace_bytes(int64_t N, int64_t C) {
 }
 
 int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
-                            const void* gate, float scale, const void* gamma, int gamma_dtype, const float* mean,
+                            const void* gate, float scale, int stepwise, const void* gamma, int gamma_dtype, const float* mean,
                             const float* rstd, const void* ds, const void* dy, void* dx, void* d_branch, void* d_gate,
                             void* dgamma, void* dbeta, int param_dtype, void* d_branch_bias, void* workspace, int64_t N,
                             int64_t C, void* stream) {
@@ -409,7 +432,7 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
 #undef RN_PICK
 #undef RN_CB
         hipLaunchKernelGGL(k, dim3((unsigned)parts), dim3(64 * h.W * h.RB), sums && h.RB > 1 ? (size_t)M * 4 : 0, stm,
-                           RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale}, gamma,
+                           RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale, stepwise}, gamma,
                            gamma_dtype, mean, rstd, ds, (const uint16_t*)dy, dx, (uint16_t*)d_branch, (uint16_t*)d_gate, part,
                            N, (int)C, h.W, h.RB, rn_stream(N, C));
     }

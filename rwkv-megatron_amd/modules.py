@@ -323,10 +323,10 @@ class RWKV6ChannelMix(nn.Module):
 
 def _add_norm(norm, x, branch, bias=None, gate=None):
     """(s, LayerNorm(s)) for s = x + (branch + bias) sigmoid(gate): in one kernel (residual.residual_norm,
-    which rounds s and the norm once each) where it takes the call, else by the operators it stands
-    for.  A norm that is not this package's own class, or that has hooks, is called as a module."""
+    stepwise: rounded where the separate operators round) where it takes the call, else by the operators
+    it stands for.  A norm that is not this package's own class, or that has hooks, is called as a module."""
     if _plain_module(norm, LayerNorm) and norm.weight is not None and norm.bias is not None and x.is_cuda:
-        out = _lib.native().residual_norm(x, branch, norm.weight, norm.bias, norm.eps, gate, bias, 1.0, True)
+        out = _lib.native().residual_norm(x, branch, norm.weight, norm.bias, norm.eps, gate, bias, 1.0, True, True)
         if out is not None:
             return out
     if bias is not None:

@@ -242,9 +242,9 @@ def _encode(code, scale, value):
     b = b.view(-1, BLOCK)
     top = torch.where(b.isfinite(), b, 0).abs().amax(-1)
     top = torch.where(top < 2.0 ** -118, 0.0, top)
-    inv = torch.where(top > 0, 448.0 / top, 0.0)
+    inv = torch.where(top > 0, top.reciprocal() * 448.0, 0.0)
     _flat(code).copy_((b * inv[:, None]).to(torch.float8_e4m3fn).view(-1)[:n])
-    scale.copy_(top / 448.0)
+    scale.copy_(top * (1.0 / 448.0))
 
 
 def _moments(state):

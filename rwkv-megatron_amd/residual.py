@@ -22,17 +22,19 @@ from . import _lib
 MAX_CHANNELS = 8192
 
 
-def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, scale=1.0):
+def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, scale=1.0, stepwise=False):
     """(s, y) = (x + scale (branch + branch_bias) sigmoid(gate), LayerNorm(s) weight + bias).
 
     x [..., C] bf16 or fp32 (s comes back in the same type); branch and gate [..., C] bf16;
     weight, bias, branch_bias [C] in any of fp32, bf16, fp16; y [..., C] bf16.  Without a gate the
     factor is 1, without a branch_bias the term 0; scale is a number.  C is a multiple of 8 up to
-    8192.  s is rounded once, y is the norm of s before that rounding; inside, 32 bits.
+    8192.  s is rounded once, y is the norm of s before that rounding; inside, 32 bits.  With
+    stepwise=True the numbers are those of separate operators: the sum with the bias, the product with
+    the gate (bf16) and s (x's type) are rounded before they are used, y is the norm of s as returned.
 
     Gradients for x, branch, gate, weight, bias and branch_bias; sums over the rows run in a fixed
     order.  A backward that is differentiated again runs through torch's operators."""
-    out = _lib.native().residual_norm(x, branch, weight, bias, eps, gate, branch_bias, scale, False)
+    out = _lib.native().residual_norm(x, branch, weight, bias, eps, gate, branch_bias, scale, stepwise, False)
     return _refuse(x, branch, weight, bias, gate, branch_bias) if out is None else out
 
 

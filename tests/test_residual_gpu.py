@@ -88,6 +88,34 @@ def test_matches_float64(rn, shape, C, stream, param, gate, cbias, scale):
         assert near(got[n], want[n], slack[n]), (n, float((got[n].double() - want[n]).abs().max()))
 
 
+# Stepwise: the stream bit for bit that of the separate operators (a gate's sigmoid is the same function in
+# both); y up to the order of a row's sums, which moves a value by 2^-20 of the row's largest at most and so
+# over a rounding's edge now and then: one step of bf16 (2^-7 of it).  The separate gradients are rounded at
+# up to four places (2^-8 each, of d y, the norm's d s, the sum and the gate's product), the fused ones once.
+@pytest.mark.parametrize("C", [64, 512, 1024, 2056])
+@pytest.mark.parametrize("gate,cbias", [(False, False), (True, False), (False, True), (True, True)])
+def test_stepwise_is_the_operators_one_by_one(rn, C, gate, cbias):
+    pkg = importlib.import_module("rwkv-megatron_amd")
+    t, ds, dy = _inputs((37,), C, BF, F32, gate, cbias, seed=5)
+    if cbias:
+        t["branch_bias"] = t["branch_bias"].detach().to(BF).requires_grad_(True)
+    norm = pkg.modules.LayerNorm(C, eps=EPS, device=DEV)
+    norm.weight, norm.bias = torch.nn.Parameter(t["weight"].detach()), torch.nn.Parameter(t["bias"].detach())
+    f = t["branch"] + t["branch_bias"] if cbias else t["branch"]
+    s1 = t["x"] + (pkg.channelmix.sigmoid_gate(f, t["gate"]) if gate else f)
+    y1 = norm(s1)
+    names = [n for n in t if n not in ("weight", "bias")]
+    want = dict(zip([*names, "weight", "bias"], torch.autograd.grad((s1, y1), [*[t[n] for n in names], norm.weight, norm.bias], (ds, dy))))
+    s2, y2 = _call(rn, t, stepwise=True)
+    assert torch.equal(s1, s2)
+    a, b = y1.detach().double(), y2.detach().double()
+    assert bool(((a - b).abs() <= 2.0 ** -7 * a.abs() + 2.0 ** -18 * float(a.abs().max())).all())
+    assert C > 512 or torch.equal(y1, y2)                    # one wave a row in both
+    got = dict(zip(t, torch.autograd.grad((s2, y2), list(t.values()), (ds, dy))))
+    for n in t:
+        assert float((got[n].double() - want[n].double()).norm()) <= 4 * 2.0 ** -8 * float(want[n].double().norm()), n
+
+
 # L = <s, ds> + <y, dy> between two points along the gradient.  An output's rounding, half a step of bf16
 # (2^-9 of it on average), enters L at random: sqrt(N C) 2^-9 |y dy| at most, against a difference of 2 h
 # |grad|, |grad| >= sqrt(N C) / 2 here and h = 2: below 2^-8; the third derivative adds less than that.
