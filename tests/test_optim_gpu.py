@@ -346,6 +346,35 @@ def test_updates_are_seen_by_autograd_and_other_streams(opt):
     assert torch.equal(p, q)
 
 
+def test_a_tensor_past_32_bits(opt):
+    """Elements past 2^31 (and bytes past 2^32) of one tensor, 8-bit states, with a small one behind it."""
+    n = (1 << 31) + 3 * 2048 + 77
+    t = _lists([777], BF, BF, True)
+    big = {"p": torch.zeros(n, dtype=BF, device=DEV), "g": torch.zeros(n, dtype=BF, device=DEV),
+           "m": torch.zeros(n, dtype=torch.uint8, device=DEV).view(F8), "v": torch.zeros(n, dtype=torch.uint8, device=DEV).view(F8)}
+    scales = [torch.zeros(-(-n // 256), device=DEV) for _ in range(2)]
+    at = n - 77 - 700                                      # the last whole blocks and the ragged end, in a copy
+    at -= at % 256
+    small = _lists([n - at], BF, BF, True, seed=4)
+    for k in "pgmv":
+        big[k][at:].copy_(small[k][0])
+    for s, part in zip(scales, small["scales"]):
+        s[at // 256:] = part[0]
+    both = {k: [big[k], t[k][0].clone()] for k in "pgmv"}
+    opt.adamw_step(both["p"], both["g"], both["m"], both["v"], torch.full((), 6.0, device=DEV),
+                   scales=([scales[0], t["scales"][0][0].clone()], [scales[1], t["scales"][1][0].clone()]), **HYPER)
+    _call(opt, small)
+    _call(opt, t)
+    for k in "pmv":
+        assert torch.equal(big[k][at:].view(torch.uint8), small[k][0].view(torch.uint8))
+        assert torch.equal(both[k][1].view(torch.uint8), t[k][0].view(torch.uint8))
+    # the rest is 0 / (0 + eps) = 0 of a parameter of zero
+    assert not bool(big["p"][:at].any()) and not bool(scales[0][:at // 256].any())
+    norm = opt.grad_norm(both["g"])
+    want = sum(float(g.double().square().sum()) for g in (small["g"][0], t["g"][0])) ** 0.5
+    assert abs(float(norm) - want) <= 2.0 ** -23 * want
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_a_copy_of_the_optimizer_goes_on_by_itself(opt, bits):
     ps = _params(F32)

@@ -288,6 +288,52 @@ def test_graph_replays_and_another_stream(rn):
         assert all(torch.equal(a, b) for a, b in zip(want, out)), rep
 
 
+def test_a_single_row_without_batch_and_two_streams_at_once(rn):
+    t, ds, dy = _inputs((1,), 256, BF, F32, True, True)
+    a = _call(rn, t)
+    u = {n: (v.detach()[0] if v.dim() > 1 else v.detach()).requires_grad_(True) for n, v in t.items()}
+    b = _call(rn, u)
+    assert b[0].shape == (256,) and torch.equal(a[0][0], b[0]) and torch.equal(a[1][0], b[1])
+    ga = torch.autograd.grad(a, list(t.values()), (ds, dy))
+    gb = torch.autograd.grad(b, list(u.values()), (ds[0], dy[0]))
+    assert all(torch.equal(p.reshape(q.shape), q) for p, q in zip(ga, gb))
+
+    sets = [_inputs((3000,), 512, BF, F32, True, True, seed=k) for k in (11, 12)]
+    run = lambda t, ds, dy: torch.autograd.grad(_call(rn, t), list(t.values()), (ds, dy))
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [None, None]
+    for _ in range(3):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k] = run(*sets[k])
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(a, b) for a, b in zip(w, g))
+
+
+def test_offsets_past_32_bits(rn):
+    """Rows further than 2^31 elements (and 2^32 bytes) into the tensors."""
+    N, C = 540_000, 4096
+    x, branch, dy = (torch.zeros(N, C, device=DEV, dtype=BF) for _ in range(3))
+    rows = [0, 1, 262_143, 262_144, 524_287, 524_288, 539_999]
+    t, ds, g = _inputs((len(rows),), C, BF, F32, False, False)
+    with torch.no_grad():
+        for k, r in enumerate(rows):
+            x[r], branch[r], dy[r] = t["x"][k], t["branch"][k], g[k]
+    x.requires_grad_(True)
+    s, y = rn(x, branch, t["weight"].detach(), t["bias"].detach(), EPS)
+    small = rn(t["x"].detach().requires_grad_(True), t["branch"].detach(), t["weight"].detach(), t["bias"].detach(), EPS)
+    assert torch.equal(s[rows], small[0]) and torch.equal(y[rows], small[1])
+    assert not bool(s.detach().view(-1)[C * 2:C * 262_143].any())
+    xs = t["x"].detach().requires_grad_(True)
+    want = torch.autograd.grad(rn(xs, t["branch"].detach(), t["weight"].detach(), t["bias"].detach(), EPS)[1], xs, g)[0]
+    got = torch.autograd.grad(y, x, dy)[0]
+    assert torch.equal(got[rows], want) and not bool(got[2:262_143].any())
+
+
 def test_refusals(rn):
     t, _, _ = _inputs((4,), 64, BF, F32, True, True)
     a = {n: v.detach() for n, v in t.items()}
