@@ -289,7 +289,7 @@ int rwkv6_layer_norm_bwd(const void* x, const void* gamma, int gamma_dtype, cons
  * gamma, beta: [C] in param_dtype; mean, rstd: [N] f32 for the backward (both NULL without one).  The
  * statistics and y are those of s before it is rounded to x_dtype; with stepwise != 0 the sum with
  * the bias, the product with the gate and s are rounded (bf16, bf16, x_dtype) where separate operators
- * would round them, and y is the norm of s as stored.
+ * would round them, y is the norm of s as stored, and the backward rounds at the same places.
  *   bwd: ds [N,C] in x_dtype (nullable: zero), dy [N,C] bf16 -> dx in x_dtype, d_branch, d_gate bf16
  *        (d_gate NULL exactly when gate is), dgamma, dbeta in param_dtype and d_branch_bias in bias_dtype
  *        (all NULL: not wanted, no workspace; d_branch_bias NULL also when branch_bias is).  d_branch may

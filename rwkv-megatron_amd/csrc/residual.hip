@@ -12,9 +12,10 @@
 // s is rounded once, to x's type, on its way out.  The backward forms it again from the inputs: a
 // stored bf16 s would put its rounding, 2^-9 of s, into xh and so into an fp32 dgamma.
 // `stepwise` gives the numbers of the operators run one by one instead: the sum with the bias, the
-// product with the gate and s are rounded (bf16, bf16, x's type) before the next takes them, and y
-// is the norm of s as it is stored.  The layers and the model run that, so that fusing them changed
-// no forward value of theirs by more than the order of a row's sums does.
+// product with the gate and s are rounded (bf16, bf16, x's type) before the next takes them, y is the
+// norm of s as it is stored, and the gradients are rounded at the same places.  The layers and the
+// model run that, so that fusing them changed no value of theirs by more than the order of a row's
+// sums does.
 //
 // Bound by memory: bytes an element in bf16 8 forward (10 gated), 10 backward (16 gated).  16384 x 2048
 // forward and backward 112 us (46 + 62 and 4 for the parameters' sums), gated 160 us (57 + 95 + 4): 5.4 TB/s
@@ -60,7 +61,19 @@ __device__ __forceinline__ void store8_as(void* p, int64_t off, const float* f, 
         store8(reinterpret_cast<uint16_t*>(p) + off, f);
     }
 }
-__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + ex2(-RW_L2E * g)); }
+// sigmoid of eight values.  `near`: the reciprocal with a Newton step, as near as the separate operator's
+// division; without, the hardware's to 2^-23 (gated forward of 16384 x 2048 58 us, 66 with the step).
+__device__ __forceinline__ void sigmoid8(float* g, bool near) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        x[j] = 1.f + ex2(-RW_L2E * g[j]);
+        g[j] = __builtin_amdgcn_rcpf(x[j]);
+    }
+    if (near)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = x[j] == INFINITY ? 0.f : fmaf(fmaf(-x[j], g[j], 1.f), g[j], g[j]);
+}
 
 // Sum over the row's W waves, the same bits in each: `red` is [waves], one of two arrays that the
 // caller alternates, so one barrier a sum is enough.
@@ -89,7 +102,7 @@ __device__ __forceinline__ void round8(float* f) { unpack8(pack8(f), f); }
 
 // A row is W waves' (512 NV channels each, 8 a lane and piece); a block holds RB = 4 / W rows, one at
 // least, and strides over the rows.  The pieces of a row stay in registers.
-template <int NV, bool XF, bool GATE>
+template <int NV, bool XF, bool GATE, bool CB>
 __global__ void __launch_bounds__(64 * RN_MAX_WAVES)
 rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const void* __restrict__ beta, int pdt,
                                float eps, void* __restrict__ s, uint16_t* __restrict__ y,
@@ -99,16 +112,14 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, gr = wv / W, w = wv - gr * W;
     const float inv = 1.f / (float)C;
     int c[NV];
-    float ga[NV][8], be[NV][8], cb[NV][8];
+    float ga[NV][8], be[NV][8], cb[CB ? NV : 1][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         c[i] = 8 * (lane + 64 * (w + W * i));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ga[i][j] = be[i][j] = cb[i][j] = 0.f;
         if (c[i] < C) {
             load_param8(gamma, pdt, c[i], ga[i]);
             load_param8(beta, pdt, c[i], be[i]);
-            if (in.cbias) load_param8(in.cbias, in.cdt, c[i], cb[i]);
+            if constexpr (CB) load_param8(in.cbias, in.cdt, c[i], cb[i]);
         }
     }
     for (int64_t b0 = (int64_t)blockIdx.x * RB; b0 < N; b0 += (int64_t)gridDim.x * RB) {
@@ -122,14 +133,17 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
                 float f[8];
                 raw_f32<XF>(w_load<XF>(in.x, row + c[i]), v[i]);
                 load8(in.branch + row + c[i], f);
+                if constexpr (CB) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] += cb[i][j];
-                if (in.stepwise) round8(f);
+                    for (int j = 0; j < 8; ++j) f[j] += cb[i][j];
+                    if (in.stepwise) round8(f);
+                }
                 if constexpr (GATE) {
                     float g[8];
                     load8(in.gate + row + c[i], g);
+                    sigmoid8(g, in.stepwise);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] *= sigmoid(g[j]);
+                    for (int j = 0; j < 8; ++j) f[j] *= g[j];
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) f[j] *= in.scale;
@@ -218,12 +232,10 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
                 for (int j = 0; j < 8; ++j) f[i][j] += cb[i][j];
                 if (in.stepwise) round8(f[i]);
             }
+            if constexpr (GATE) sigmoid8(sg[i], in.stepwise);
             float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if constexpr (GATE) sg[i][j] = sigmoid(sg[i][j]);
-                t[j] = (GATE ? f[i][j] * sg[i][j] : f[i][j]) * in.scale;
-            }
+            for (int j = 0; j < 8; ++j) t[j] = (GATE ? f[i][j] * sg[i][j] : f[i][j]) * in.scale;
             if (in.stepwise) round8(t);
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[j] += xh[i][j];
@@ -235,9 +247,8 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
                     ag[i][j] += g[i][j] * xh[i][j];
                     ab[i][j] += g[i][j];
                 }
-                g[i][j] *= ga[i][j];
-                s1 += g[i][j];
-                s2 += g[i][j] * xh[i][j];
+                s1 += g[i][j] * ga[i][j];
+                s2 += g[i][j] * ga[i][j] * xh[i][j];
             }
         }
         s1 = wave_sum(s1);
@@ -258,21 +269,30 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (c[i] >= C) continue;
+            float e[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dS[i][j] += rstd * (g[i][j] - s1 - xh[i][j] * s2);
+            for (int j = 0; j < 8; ++j) e[j] = rstd * (g[i][j] * ga[i][j] - s1 - xh[i][j] * s2);
+            if (!XF && in.stepwise) round8(e);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dS[i][j] += e[j];
+            if (!XF && in.stepwise) round8(dS[i]);
             store8_as<XF>(dx, row + c[i], dS[i], nt);
             if (!db) continue;
             float o[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                dS[i][j] *= in.scale;
-                o[j] = GATE ? dS[i][j] * sg[i][j] : dS[i][j];
-                if constexpr (CB) ac[i][j] += o[j];
+            for (int j = 0; j < 8; ++j) dS[i][j] *= in.scale;
+            if (in.stepwise) round8(dS[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = GATE ? dS[i][j] * sg[i][j] : dS[i][j];
+            if constexpr (CB) {
+                if (in.stepwise) round8(o);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ac[i][j] += o[j];
             }
             store8_as<false>(db, row + c[i], o, nt);
             if constexpr (GATE) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = o[j] * f[i][j] * (1.f - sg[i][j]);
+                for (int j = 0; j < 8; ++j) o[j] = dS[i][j] * f[i][j] * sg[i][j] * (1.f - sg[i][j]);
                 store8_as<false>(dg, row + c[i], o, nt);
             }
         }
@@ -383,11 +403,12 @@ int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, cons
                   {{x, xs}, {branch, act}, {branch_bias, (size_t)C * param_bytes(bias_dtype)}, {gate, act}, {gamma, par}, {beta, par}}))
         return RWKV6_ERR_INVALID_ARG;
     const RnShape h = rn_shape(C);
-    const bool xf = x_dtype == RWKV6_F32, gt = gate != nullptr;
-#define RN_PICK(NV) (xf ? (gt ? rwkv6_residual_norm_fwd_kernel<NV, true, true> : rwkv6_residual_norm_fwd_kernel<NV, true, false>) \
-                        : (gt ? rwkv6_residual_norm_fwd_kernel<NV, false, true> : rwkv6_residual_norm_fwd_kernel<NV, false, false>))
+    const bool xf = x_dtype == RWKV6_F32, gt = gate != nullptr, cb = branch_bias != nullptr;
+#define RN_CB(NV, X, G) (cb ? rwkv6_residual_norm_fwd_kernel<NV, X, G, true> : rwkv6_residual_norm_fwd_kernel<NV, X, G, false>)
+#define RN_PICK(NV) (xf ? (gt ? RN_CB(NV, true, true) : RN_CB(NV, true, false)) : (gt ? RN_CB(NV, false, true) : RN_CB(NV, false, false)))
     auto k = h.NV == 1 ? RN_PICK(1) : RN_PICK(2);
 #undef RN_PICK
+#undef RN_CB
     const int64_t blocks = (N + h.RB - 1) / h.RB;
     hipLaunchKernelGGL(k, dim3((unsigned)(blocks < RN_FWD_BLOCKS ? blocks : RN_FWD_BLOCKS)), dim3(64 * h.W * h.RB), 0,
                        reinterpret_cast<hipStream_t>(stream),

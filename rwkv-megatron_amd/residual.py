@@ -30,7 +30,8 @@ def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, sca
     factor is 1, without a branch_bias the term 0; scale is a number.  C is a multiple of 8 up to
     8192.  s is rounded once, y is the norm of s before that rounding; inside, 32 bits.  With
     stepwise=True the numbers are those of separate operators: the sum with the bias, the product with
-    the gate (bf16) and s (x's type) are rounded before they are used, y is the norm of s as returned.
+    the gate (bf16) and s (x's type) are rounded before they are used, y is the norm of s as returned,
+    and the gradients are rounded at the same places.
 
     Gradients for x, branch, gate, weight, bias and branch_bias; sums over the rows run in a fixed
     order.  A backward that is differentiated again runs through torch's operators."""

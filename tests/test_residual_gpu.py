@@ -90,8 +90,9 @@ def test_matches_float64(rn, shape, C, stream, param, gate, cbias, scale):
 
 # Stepwise: the stream bit for bit that of the separate operators (a gate's sigmoid is the same function in
 # both); y up to the order of a row's sums, which moves a value by 2^-20 of the row's largest at most and so
-# over a rounding's edge now and then: one step of bf16 (2^-7 of it).  The separate gradients are rounded at
-# up to four places (2^-8 each, of d y, the norm's d s, the sum and the gate's product), the fused ones once.
+# over a rounding's edge now and then: one step of bf16 (2^-7 of it).  The gradients likewise: for a row in one
+# wave the order is the same, and the compiler's choice of fused multiply-adds may move a value by 2^-23
+# before its rounding, over an edge once in 2^15 values or so; the parameters' are sums in other orders.
 @pytest.mark.parametrize("C", [64, 512, 1024, 2056])
 @pytest.mark.parametrize("gate,cbias", [(False, False), (True, False), (False, True), (True, True)])
 def test_stepwise_is_the_operators_one_by_one(rn, C, gate, cbias):
@@ -112,8 +113,13 @@ def test_stepwise_is_the_operators_one_by_one(rn, C, gate, cbias):
     assert bool(((a - b).abs() <= 2.0 ** -7 * a.abs() + 2.0 ** -18 * float(a.abs().max())).all())
     assert C > 512 or torch.equal(y1, y2)                    # one wave a row in both
     got = dict(zip(t, torch.autograd.grad((s2, y2), list(t.values()), (ds, dy))))
-    for n in t:
-        assert float((got[n].double() - want[n].double()).norm()) <= 4 * 2.0 ** -8 * float(want[n].double().norm()), n
+    for n in ("x", "branch", *(["gate"] if gate else [])):
+        a, b = want[n].double(), got[n].double()
+        assert float((a != b).double().mean()) <= 2.0 ** -8, n
+        assert bool(((a - b).abs() <= 2.0 ** -6 * a.abs() + 2.0 ** -16 * float(a.abs().max())).all()), n
+    for n in ("weight", "bias", *(["branch_bias"] if cbias else [])):
+        half = 2.0 ** -7 if got[n].dtype == BF else 0
+        assert bool(((got[n].double() - want[n].double()).abs() <= half * want[n].double().abs() + 2.0 ** -12).all()), n
 
 
 # L = <s, ds> + <y, dy> between two points along the gradient.  An output's rounding, half a step of bf16
