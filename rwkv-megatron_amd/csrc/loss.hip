@@ -10,7 +10,7 @@
 //
 // Bound by memory: 2 bytes a logit in bf16 forward, 4 backward.  16384 x 65536: 344 us (6.2 TB/s) and 809
 // us (5.3 TB/s); 1024 x 65536: 38 and 47 us, the forward while what ran before it still writes its output
-// back (23 us without); 1001 x 50001 in fp32 54 and 68 us.  A copy of 2 GiB reaches 4.9 TB/s.  torch's
+// back (26 us without); 1001 x 50001 in fp32 54 and 68 us.  A copy of 2 GiB reaches 4.9 TB/s.  torch's
 // operators in 32 bits take 9.1 ms, 636 and 410 us for both ways.
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
@@ -233,9 +233,9 @@ int rwkv6_cross_entropy_fwd(const void* logits, int dtype, int64_t ld, const int
     const bool f32 = dtype == RWKV6_F32;
     // A wave for a short row, whose cost is the joining of the threads' sums, more for a long one; one row
     // of 1024 threads at a time streams best where the rows fill the device several times over.  Forward, us,
-    // with 64, 256, 512, 1024 threads: 65536 x 376 25, 74, 163, 338; 16384 x 4104 27, 36, 58, 103; 16384 x
-    // 8192 51, 44, 72, 116; 8192 x 32000 94, 93, 90, 116; 4096 x 65536 94, 96, 93, 87; 1024 x 65536 -, 41, 38,
-    // 40.
+    // with 64, 256, 512, 1024 threads: 65536 x 376 20, 61, 132, 261; 16384 x 4104 26, 35, 52, 86; 16384 x 8192
+    // 50, 45, 68, 96; 8192 x 32000 92, 91, 87, 107; 4096 x 65536 103, 94, 92, 86; 1024 x 65536 35, 28, 26, 26;
+    // 512 x 65536 24, 13, 13, 14.
     const int64_t pieces = V * (int64_t)param_bytes(dtype) / 16;
     const int thr = pieces < 1024 ? 64 : pieces < 4096 ? 256 : N < 2048 ? 512 : 1024;
 #define CE_PICK(F) (thr == 64 ? rwkv6_cross_entropy_fwd_kernel<F, 64> : thr == 256 ? rwkv6_cross_entropy_fwd_kernel<F, 256> \

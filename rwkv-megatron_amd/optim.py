@@ -81,6 +81,12 @@ def _check_hyper(lr, betas, eps, weight_decay, max_norm):
         raise ValueError(f"max_norm must be positive, got {max_norm}")
 
 
+def _not_captured(what):
+    """Raises where a captured step would make tensors that every replay makes anew."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: run one such step before it is captured in a graph")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay over bf16 or fp32 parameters on one GPU.
 
@@ -88,7 +94,7 @@ class AdamW(torch.optim.Optimizer):
     more; smaller ones (norms, biases, mixing coefficients) keep 32 bits.  max_norm clips by the norm of
     all gradients of the step, in all groups (`grad_norm` holds it afterwards, a 0-dim tensor); the
     gradients themselves stay as they are.  lr may be a one-element fp32 tensor on the GPU, which a
-    captured step reads on replay.
+    captured step reads on replay; a step is captured after one like it has run (the states exist then).
 
     State of a parameter: ``step`` (one tensor for all parameters that have made the same steps),
     ``exp_avg`` and ``exp_avg_sq`` (fp32), or in 8 bits ``exp_avg``, ``exp_avg_scale``, ``exp_avg_sq_root`` and
@@ -143,6 +149,7 @@ class AdamW(torch.optim.Optimizer):
                 if p.device.type != "cuda":
                     raise ValueError("parameters must live on the GPU")
                 if not self.state[p]:
+                    _not_captured("the first step of a parameter makes its states")
                     key = (p.device, self._eight(p))
                     if key not in new:
                         new[key] = torch.zeros((), dtype=torch.float32, device=p.device)
@@ -154,6 +161,7 @@ class AdamW(torch.optim.Optimizer):
                     lists.setdefault(key, []).append(p)
         for key, ps in lists.items():
             if len(ps) < sharing[key]:             # the others make no step: these go on with a count of their own
+                _not_captured("parameters that have made the same steps part")
                 step = self.state[ps[0]]["step"].clone()
                 for p in ps:
                     self.state[p]["step"] = step

@@ -327,6 +327,26 @@ def test_learning_rate_on_the_device_and_captured_steps(opt):
     assert all(float(a.state[p]["step"]) == 4 for p in ps)
 
 
+def test_a_first_step_is_not_captured(opt, monkeypatch):
+    """States made inside a capture would be made again, as zeros, by every replay."""
+    ps = _params(F32)
+    o = opt.AdamW(ps, **HYPER)
+    _grads(ps, 0)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="captured"):
+            o.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, _params(F32)))
+    o.step()
+    ps[1].grad = None
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="captured"):
+            o.step()
+    o.step()
+    assert [float(o.state[p]["step"]) for p in ps] == [2, 1, 2, 2]
+
+
 def test_updates_are_seen_by_autograd_and_other_streams(opt):
     p = torch.nn.Parameter(torch.ones(100, device=DEV))
     o = opt.AdamW([p], **HYPER)
