@@ -21,12 +21,13 @@
 //
 // Bound by memory: bytes a parameter 22 (bf16 p and g, fp32 states), 28 (all fp32), 10 and 16 with
 // 8-bit states, and once more the gradient where it is clipped.  Four layers of 2048 channels (218 M
-// bf16 parameters in 92 tensors): norm 130 us, step 941 us (5.1 TB/s), with 8-bit states 434 us (5.0
-// TB/s); two layers of 512 (7.3 M fp32): 8 + 5 + 34 us, the 5 the one block that forms the norm and
+// bf16 parameters in 92 tensors): norm 88 us (5.0 TB/s), step 865 us (5.6 TB/s), with 8-bit states 403 us
+// (5.5 TB/s); two layers of 512 (7.3 M fp32): 7 + 5 + 34 us, the 5 the one block that forms the norm and
 // the coefficients.  A copy of 2 GiB reaches 4.9 TB/s.  torch's operators in 32 bits on the same
-// parameters as one tensor take 8.0 ms, 11.7 ms and 313 us.  Tried and left: streamed loads (499 us
-// instead of 457 for 109 M parameters) and stores (the same), the norm's sums of eight squares in 32
-// bits (the same), the tensors in reverse so that the norm's last ones are still cached (the same).
+// parameters as one tensor take 8.0 ms, 11.7 ms and 313 us.  Tried and left: the step's loads past the
+// caches (499 us instead of 457 for 109 M parameters) and its stores (the same), the norm's sums of eight
+// squares in 32 bits (the same), the tensors in reverse so that the norm's last ones are still cached
+// (the same).
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 
@@ -37,6 +38,7 @@
 #define AW_STEP (8 * AW_THR)    // elements a block takes at once
 #define AW_PARTS 8192           // blocks of the norm's sums, at about
 #define AW_AHEAD 4              // steps of the norm's loads in flight
+#define AW_RUN (AW_AHEAD * AW_STEP)
 #define AW_T 60                 // tensors a launch: the arguments stay below 4 KB
 #define AW_BLK 256              // elements under one 8-bit scale: 32 lanes of 8
 #define AW_MAX ((int64_t)1 << 37)   // elements a call: a launch stays below 2^32 threads
@@ -93,6 +95,21 @@ __device__ __forceinline__ void aw_load8(const void* p, int dt, int64_t i, int64
             if (i + j < n)
                 f[j] = dt == RWKV6_BF16 ? bf2f(reinterpret_cast<const uint16_t*>(p)[i + j])
                                         : reinterpret_cast<const float*>(p)[i + j];
+        }
+    }
+}
+// Eight aligned elements past the caches.
+__device__ __forceinline__ void aw_load8_nt(const void* p, int dt, int64_t i, float* f) {
+    if (dt == RWKV6_BF16) {
+        const u32x4_t q = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(p) + i));
+        unpack8(make_uint4(q.x, q.y, q.z, q.w), f);
+    } else {
+        const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + i);
+        const f32x4 a = __builtin_nontemporal_load(q), b = __builtin_nontemporal_load(q + 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f[j] = a[j];
+            f[4 + j] = b[j];
         }
     }
 }
@@ -169,32 +186,35 @@ struct Coef {
 
 }  // namespace
 
-// Sum of squares of the blocks' elements, `per` of a tensor each: part[base + block].
+// Sums of squares: a tensor's blocks take its runs of AW_RUN elements in turn, so that together they
+// sweep it; part[base + block].
 __global__ void __launch_bounds__(AW_THR)
-rwkv6_grad_square_sums_kernel(const NormTable tab, int64_t per, double* __restrict__ part) {
+rwkv6_grad_square_sums_kernel(const NormTable tab, bool nt, double* __restrict__ part) {
     __shared__ double red[AW_THR / 64];
     const int k = aw_find(tab.first, tab.count, blockIdx.x);
-    const int64_t n = tab.n[k], i0 = (int64_t)((int)blockIdx.x - tab.first[k]) * per, i1 = min(n, i0 + per);
+    const int64_t n = tab.n[k];
+    const int j0 = (int)blockIdx.x - tab.first[k];
+    const int64_t stride = (int64_t)((k + 1 < tab.count ? tab.first[k + 1] : (int)gridDim.x) - tab.first[k]) * AW_RUN;
     const void* g = tab.g[k];
     const int dt = tab.dt[k];
     const bool vec = aw_al16(g);
     double sum[2] = {0., 0.};
-    int64_t i = i0 + 8 * threadIdx.x;
-    // whole steps, AW_AHEAD of them in flight
-    for (; vec && i + 8 + (AW_AHEAD - 1) * AW_STEP <= i1; i += AW_AHEAD * AW_STEP) {
+    for (int64_t i = (int64_t)j0 * AW_RUN + 8 * threadIdx.x; i < n; i += stride) {
         float f[AW_AHEAD][8];
+        if (vec && i + 8 + (AW_AHEAD - 1) * AW_STEP <= n) {
 #pragma unroll
-        for (int u = 0; u < AW_AHEAD; ++u) aw_load8(g, dt, i + u * AW_STEP, n, true, f[u]);
+            for (int u = 0; u < AW_AHEAD; ++u) {
+                if (nt) aw_load8_nt(g, dt, i + u * AW_STEP, f[u]);
+                else aw_load8(g, dt, i + u * AW_STEP, n, true, f[u]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < AW_AHEAD; ++u) aw_load8(g, dt, i + u * AW_STEP, n, vec, f[u]);
+        }
 #pragma unroll
         for (int u = 0; u < AW_AHEAD; ++u)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j & 1] = fma((double)f[u][j], (double)f[u][j], sum[j & 1]);
-    }
-    for (; i < i1; i += AW_STEP) {
-        float f[8];
-        aw_load8(g, dt, i, i1, vec, f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j & 1] = fma((double)f[j], (double)f[j], sum[j & 1]);
     }
     double acc = sum[0] + sum[1];
 #pragma unroll
@@ -304,13 +324,20 @@ rwkv6_adamw_step_kernel(const StepTable tab, const Coef* __restrict__ coef, int6
 }
 
 namespace {
-// Elements a block takes: `blocks` blocks over all tensors, in steps of AW_STEP.
-int64_t aw_per(const int64_t* numel, int64_t count, int64_t blocks, int64_t most) {
+// Elements that a block takes: `blocks` blocks over all tensors, in steps of AW_STEP.
+int64_t aw_per(const int64_t* numel, int64_t count, int64_t blocks) {
     int64_t total = 0;
     for (int64_t k = 0; k < count; ++k) total += numel[k];
-    int64_t per = (total / blocks + AW_STEP - 1) / AW_STEP * AW_STEP;
-    if (per < AW_STEP) per = AW_STEP;
-    return most && per > most ? most : per;
+    const int64_t per = (total / blocks + AW_STEP - 1) / AW_STEP * AW_STEP;
+    return per < AW_STEP ? AW_STEP : per;
+}
+// Of the step: all blocks at once (eight a CU) where that leaves each a few steps, else one step a block, so
+// that the blocks that run together sweep the tensors: 109 M parameters, bf16 with fp32 states, us, with 1,
+// 2, 4, 8 and 16 steps a block: 423, 447, 458, 469, 488; 55 M with fp32 and 8-bit states 160, 163, 171, 178, 184;
+// 7 M, 2 steps all at once and 1 step 33 and 35.
+int64_t aw_step_per(const int64_t* numel, int64_t count) {
+    const int64_t per = aw_per(numel, count, 2048);
+    return per > 2 * AW_STEP ? AW_STEP : per;
 }
 int64_t aw_blocks(int64_t n, int64_t per) { return (n + per - 1) / per; }
 bool aw_dt(int dt) { return dt == RWKV6_F32 || dt == RWKV6_BF16; }
@@ -326,7 +353,7 @@ int aw_sizes(const int64_t* numel, int64_t count) {
     return total > AW_MAX ? RWKV6_ERR_UNSUPPORTED : RWKV6_OK;
 }
 int64_t aw_partials(const int64_t* numel, int64_t count) {
-    const int64_t per = aw_per(numel, count, AW_PARTS, 0);
+    const int64_t per = aw_per(numel, count, AW_PARTS);
     int64_t P = 0;
     for (int64_t k = 0; k < count; ++k) P += aw_blocks(numel[k], per);
     return P;
@@ -366,15 +393,20 @@ int rwkv6_grad_norm_sums(const void* const* grad, const int* grad_dtype, const i
     const int st = aw_sizes(numel, count);
     if (st) return st;
     if (count && (!grad || !grad_dtype)) return RWKV6_ERR_INVALID_ARG;
-    const int64_t per = aw_per(numel, count, AW_PARTS, 0);
+    const int64_t per = aw_per(numel, count, AW_PARTS);
     const Span out = {partials, (size_t)aw_partials(numel, count) * 8};
+    int64_t bytes = 0;
     for (int64_t k = 0; k < count; ++k) {
         if (!aw_dt(grad_dtype[k]) || (numel[k] && (!grad[k] || !partials))) return RWKV6_ERR_INVALID_ARG;
         if (aw_misaligned(grad[k], param_bytes(grad_dtype[k]))) return RWKV6_ERR_ALIGNMENT;
+        bytes += numel[k] * (int64_t)param_bytes(grad_dtype[k]);
         if (spans_overlap(out, {grad[k], (size_t)numel[k] * param_bytes(grad_dtype[k])}))
             return RWKV6_ERR_INVALID_ARG;
     }
     if (aw_misaligned(partials, 8)) return RWKV6_ERR_ALIGNMENT;
+    // Gradients that the last cache (256 MB) cannot keep for the step anyway are read past it: kept there they
+    // push out what the kernels before have written.  437 MB: 117 us through the caches, 85 past them.
+    const bool nt = bytes > ((int64_t)1 << 28);
     NormTable tab;
     int blocks = 0, base = 0;
     tab.count = 0;
@@ -382,7 +414,7 @@ int rwkv6_grad_norm_sums(const void* const* grad, const int* grad_dtype, const i
         if (!blocks) return;
         tab.base = base;
         hipLaunchKernelGGL(rwkv6_grad_square_sums_kernel, dim3((unsigned)blocks), dim3(AW_THR), 0,
-                           reinterpret_cast<hipStream_t>(stream), tab, per, partials);
+                           reinterpret_cast<hipStream_t>(stream), tab, nt, partials);
         base += blocks;
         blocks = tab.count = 0;
     };
@@ -459,7 +491,7 @@ int rwkv6_adamw_step(void* const* param, const int* param_dtype, const void* con
     Coef* coef = (Coef*)workspace;
     hipLaunchKernelGGL(rwkv6_adamw_coef_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), partials,
                        partials ? (int)P : 0, max_norm, norm, step, lr_dev, lr, log(beta1), log(beta2), weight_decay, coef);
-    const int64_t per = aw_per(numel, count, 2048, 8 * AW_STEP);
+    const int64_t per = aw_step_per(numel, count);
     StepTable tab;
     int64_t blocks = 0;
     tab.count = 0;
