@@ -8,14 +8,14 @@
 // end, and keeps m and z of a row: (m, 1/z) instead of log z + m keeps the gradient's exponent free of
 // the rounding of a number of size 10.
 //
-// Bound by memory: 2 bytes a logit in bf16 forward, 4 backward.  16384 x 65536: 344 us (6.2 TB/s) and 809
-// us (5.3 TB/s); 1024 x 65536: 38 and 47 us, the forward while what ran before it still writes its output
-// back (26 us without); 1001 x 50001 in fp32 54 and 68 us.  A copy of 2 GiB reaches 4.9 TB/s.  torch's
+// Bound by memory: 2 bytes a logit in bf16 forward, 4 backward.  16384 x 65536: 344 us (6.2 TB/s) and 726
+// us (5.9 TB/s); 1024 x 65536: 38 and 41 us, the forward while what ran before it still writes its output
+// back (26 us without); 1001 x 50001 in fp32 54 and 69 us.  A copy of 2 GiB reaches 4.9 TB/s.  torch's
 // operators in 32 bits take 9.1 ms, 636 and 410 us for both ways.
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 
-#define CE_GRID (1 << 16)
+#define CE_GRID (1 << 22)
 
 namespace {
 
@@ -132,15 +132,20 @@ rwkv6_cross_entropy_fwd_kernel(const void* __restrict__ logits, int64_t ld, cons
     }
 }
 
-// THR threads a row as above; gridDim.y segments of a row's pieces.
+// THR threads a row as above, or a part of it: `seg` parts a row, a block each, in the order they lie in
+// memory, so that the blocks that run together sweep it.
 template <bool F32, int THR>
 __global__ void __launch_bounds__(CE_BLOCK(THR))
 rwkv6_cross_entropy_bwd_kernel(const void* __restrict__ logits, int64_t ld, const int64_t* __restrict__ target,
                                int64_t ignore, const float2* __restrict__ stats, const float* __restrict__ d_loss,
-                               void* __restrict__ d_logits, int64_t N, int V) {
+                               void* __restrict__ d_logits, int64_t N, int V, int seg) {
     constexpr int E = CeVec<F32>::E, ES = F32 ? 4 : 2, ROWS = CE_BLOCK(THR) / THR;
     const int tid = threadIdx.x % THR;
-    for (int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / THR; n < N; n += (int64_t)gridDim.x * ROWS) {
+    const int64_t all = (N + ROWS - 1) / ROWS * seg;
+    for (int64_t id = blockIdx.x; id < all; id += gridDim.x) {
+        const int part = seg > 1 ? (int)(id % seg) : 0;
+        const int64_t n = (seg > 1 ? id / seg : id) * ROWS + threadIdx.x / THR;
+        if (n >= N) return;
         const int64_t t = target[n];
         const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
         const char* row = reinterpret_cast<const char*>(logits) + n * ld * ES;
@@ -167,7 +172,7 @@ rwkv6_cross_entropy_bwd_kernel(const void* __restrict__ logits, int64_t ld, cons
         const int lead = ce_lead<F32>(out, V);
         const int pieces = (V - lead) / E, tail = lead + pieces * E;
         const bool vec = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-        const int per = (pieces + (int)gridDim.y - 1) / (int)gridDim.y, i0 = min(per * (int)blockIdx.y, pieces);
+        const int per = (pieces + seg - 1) / seg, i0 = min(per * part, pieces);
         const int i1 = min(i0 + per, pieces);
         int i = i0 + tid;
         for (; vec && i + (CE_U - 1) * THR < i1; i += CE_U * THR) {
@@ -198,7 +203,7 @@ rwkv6_cross_entropy_bwd_kernel(const void* __restrict__ logits, int64_t ld, cons
             put(j, v);
         }
         // fewer than 8 elements at either end
-        if (blockIdx.y == 0) {
+        if (part == 0) {
             if (tid < lead) put1(tid);
             if (tid < V - tail) put1(tail + tid);
         }
@@ -259,17 +264,17 @@ int rwkv6_cross_entropy_bwd(const void* logits, int dtype, int64_t ld, const int
     if (any_alias({{d_logits, (size_t)(N * V) * param_bytes(dtype)}},
                   {{logits, ce_span(ld, N, V, dtype)}, {target, (size_t)N * 8}, {stats, (size_t)N * 8}, {d_loss, (size_t)N * 4}}))
         return RWKV6_ERR_INVALID_ARG;
-    // a wave for a short row; a long one is cut until the blocks fill the device, each keeping a step of its
-    // 256 threads
-    const bool f32 = dtype == RWKV6_F32, wave = V * (int64_t)param_bytes(dtype) / 16 < 1024;
-    int seg = 1;
-    while (!wave && seg < 64 && N * seg < 2048 && V >= (int64_t)seg * 2 * 256 * 8) seg *= 2;
+    // A wave for a short row; a long one in parts of 1024 pieces, the CE_U a thread that are in flight at once.
+    // 16384 x 65536 bf16, us, with 256, 1024, 2048, 4096 pieces and whole rows a block: 936, 726, 775, 795, 807.
+    const int64_t pieces = V * (int64_t)param_bytes(dtype) / 16;
+    const bool f32 = dtype == RWKV6_F32, wave = pieces < 1024;
+    const int seg = wave ? 1 : (int)((pieces + 1023) / 1024);
     auto k = f32 ? (wave ? rwkv6_cross_entropy_bwd_kernel<true, 64> : rwkv6_cross_entropy_bwd_kernel<true, 256>)
                  : (wave ? rwkv6_cross_entropy_bwd_kernel<false, 64> : rwkv6_cross_entropy_bwd_kernel<false, 256>);
-    const int64_t blocks = wave ? (N + 3) / 4 : N;
-    hipLaunchKernelGGL(k, dim3((unsigned)(blocks < CE_GRID ? blocks : CE_GRID), (unsigned)seg), dim3(256), 0,
+    const int64_t blocks = wave ? (N + 3) / 4 : N * seg;
+    hipLaunchKernelGGL(k, dim3((unsigned)(blocks < CE_GRID ? blocks : CE_GRID)), dim3(256), 0,
                        reinterpret_cast<hipStream_t>(stream), logits, ld, target, ignore_index, (const float2*)stats, d_loss,
-                       d_logits, N, (int)V);
+                       d_logits, N, (int)V, seg);
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
 
