@@ -28,7 +28,9 @@
 #define RN_MAX_C 8192
 #define RN_MAX_WAVES 8
 #define RN_FWD_BLOCKS (1 << 20)
-#define RN_PART 512      // row ranges of the backward at most
+#define RN_BLOCKS 512    // blocks of the backward at most, with one run of rows each (see rn_runs)
+#define RN_TURN_BLOCKS 768   // and with runs of RN_TURN steps in turn
+#define RN_TURN 4
 
 namespace {
 
@@ -182,19 +184,19 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
     }
 }
 
-// Block p of P: rows [p N / P, (p + 1) N / P), RB at a time; part[p][CB ? 3 : 2][C] = its sums of dgamma, dbeta
+// Steps of RB rows; block p takes `run` of them, then skips the other blocks' runs.  part[p][CB ? 3 : 2][C] = its sums of dgamma, dbeta
 // and d_branch_bias (part null: none).  ds null: zero.  db null: d_branch equals dx, not stored twice.
 template <int NV, bool XF, bool GATE, bool CB>
 __global__ void __launch_bounds__(64 * RN_MAX_WAVES)
 rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt, const float* __restrict__ mean_in,
                                const float* __restrict__ rstd_in, const void* __restrict__ ds,
                                const uint16_t* __restrict__ dy, void* __restrict__ dx, uint16_t* __restrict__ db,
-                               uint16_t* __restrict__ dg, float* __restrict__ part, int64_t N, int C, int W, int RB, bool nt) {
+                               uint16_t* __restrict__ dg, float* __restrict__ part, int64_t N, int C, int W, int RB, int run,
+                               bool nt) {
     extern __shared__ __attribute__((aligned(16))) float rn_acc[];            // [CB ? 3 : 2][C]
     __shared__ float2 red[2][RN_MAX_WAVES];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, gr = wv / W, w = wv - gr * W;
     const float inv = 1.f / (float)C;
-    const int64_t n0 = N * blockIdx.x / gridDim.x, n1 = N * (blockIdx.x + 1) / gridDim.x;
     int c[NV];
     float ga[NV][8], cb[CB ? NV : 1][8], ag[NV][8], ab[NV][8], ac[CB ? NV : 1][8];
 #pragma unroll
@@ -211,9 +213,16 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
         }
     }
     int turn = 0;
-    for (int64_t b0 = n0; b0 < n1; b0 += RB, turn ^= 1) {
-        const bool live = b0 + gr < n1;
-        const int64_t n = live ? b0 + gr : n1 - 1, row = n * C;
+    const int64_t skip = ((int64_t)gridDim.x - 1) * run * RB;
+    int step = 0;
+    for (int64_t b0 = (int64_t)blockIdx.x * run * RB; b0 < N; turn ^= 1) {
+        const bool live = b0 + gr < N;
+        const int64_t n = live ? b0 + gr : N - 1, row = n * C;
+        b0 += RB;
+        if (++step == run) {
+            step = 0;
+            b0 += skip;
+        }
         const float mean = mean_in[n], rstd = rstd_in[n];
         float xh[NV][8], g[NV][8], f[NV][8], sg[NV][8], dS[NV][8];
         float s1 = 0.f, s2 = 0.f;
@@ -377,10 +386,20 @@ inline RnShape rn_shape(int64_t C) {
 // input: streamed too, the forward and backward in turn take 109 instead of 112 us, but a training step of
 // the 1.6B shape 168.2 instead of 167.5 ms (three runs each).  2049 x 4096, both ways the same.
 inline bool rn_stream(int64_t N, int64_t C) { return N * C >= (int64_t)1 << 24; }
-// Row ranges of the backward: RN_PART of them, two a CU, where that leaves each two steps of a block.
-inline int64_t rn_parts(int64_t N, int RB) {
-    const int64_t p = (N + 2 * RB - 1) / (2 * RB);
-    return p < 1 ? 1 : p < RN_PART ? p : RN_PART;
+// The backward's blocks, each with two steps or more, and the steps that a block takes in a row before it
+// leaves as many to each other block.  Without a gate and with work for them 768 blocks (three a CU) take
+// runs of 4 in turn, so that the rows in work lie together; otherwise 512 blocks take one run each.  us, in
+// turn and in one run: 8192 x 2048 31 and 36, 16384 x 2048 57 to 68 and 66 to 68 (by where the tensors lie),
+// 32768 x 2048 125 and 133; gated 57 and 52, 100 to 114 and 100 to 108, 210 and 212.
+struct RnRuns {
+    int64_t blocks;
+    int run;
+};
+inline RnRuns rn_runs(int64_t N, int RB, bool gate) {
+    const int64_t steps = (N + RB - 1) / RB, half = (steps + 1) / 2;
+    if (!gate && steps >= 2 * RN_TURN * RN_TURN_BLOCKS) return {RN_TURN_BLOCKS, RN_TURN};
+    const int64_t b = half < 1 ? 1 : half < RN_BLOCKS ? half : RN_BLOCKS, run = (steps + b - 1) / b;
+    return {b, (int)(run < 1 ? 1 : run)};
 }
 }  // namespace
 
@@ -419,7 +438,7 @@ int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, cons
 
 size_t rwkv6_residual_norm_bwd_workspace_bytes(int64_t N, int64_t C) {
     if (rn_check(N, C)) return 0;
-    return (size_t)(rn_parts(N, rn_shape(C).RB) * 3 * C) * sizeof(float);
+    return (size_t)(rn_runs(N, rn_shape(C).RB, false).blocks * 3 * C) * sizeof(float);
 }
 
 int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
@@ -449,7 +468,8 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
         return RWKV6_ERR_INVALID_ARG;
     hipStream_t stm = reinterpret_cast<hipStream_t>(stream);
     const RnShape h = rn_shape(C);
-    const int64_t parts = rn_parts(N, h.RB), M = (cb ? 3 : 2) * C;
+    const RnRuns r = rn_runs(N, h.RB, gt);
+    const int64_t M = (cb ? 3 : 2) * C;
     float* part = sums ? (float*)workspace : nullptr;
     if (N > 0) {
 #define RN_CB(NV, X, G) (cb ? rwkv6_residual_norm_bwd_kernel<NV, X, G, true> : rwkv6_residual_norm_bwd_kernel<NV, X, G, false>)
@@ -457,14 +477,14 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
         auto k = h.NV == 1 ? RN_PICK(1) : RN_PICK(2);
 #undef RN_PICK
 #undef RN_CB
-        hipLaunchKernelGGL(k, dim3((unsigned)parts), dim3(64 * h.W * h.RB), sums && h.RB > 1 ? (size_t)M * 4 : 0, stm,
+        hipLaunchKernelGGL(k, dim3((unsigned)r.blocks), dim3(64 * h.W * h.RB), sums && h.RB > 1 ? (size_t)M * 4 : 0, stm,
                            RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale, stepwise}, gamma,
                            gamma_dtype, mean, rstd, ds, (const uint16_t*)dy, dx, (uint16_t*)d_branch, (uint16_t*)d_gate, part,
-                           N, (int)C, h.W, h.RB, rn_stream(N, C));
+                           N, (int)C, h.W, h.RB, r.run, rn_stream(N, C));
     }
     if (sums)
         hipLaunchKernelGGL(rwkv6_residual_norm_sums_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, stm, part,
-                           N > 0 ? (int)parts : 0, (int)M, (int)C, dgamma, dbeta, param_dtype, d_branch_bias, bias_dtype);
+                           N > 0 ? (int)r.blocks : 0, (int)M, (int)C, dgamma, dbeta, param_dtype, d_branch_bias, bias_dtype);
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
 

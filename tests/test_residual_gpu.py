@@ -176,6 +176,32 @@ def test_inputs_that_need_a_copy(rn, form):
     assert all(torch.equal(a, b) for a, b in zip(base, got))
 
 
+# Rows enough for the backward's blocks to take them in turn (6144 steps of a block's four, two or one rows
+# and more), the last run cut short: a row's gradients are those that it has among few rows, bit for bit, and
+# the parameters' are the sums, each in 32 bits below 2^-17 of the magnitudes' sum (as above).
+@pytest.mark.parametrize("N,C", [(24578, 64), (12291, 1024), (6150, 2048), (6144, 4104)])
+@pytest.mark.parametrize("cbias", [False, True])
+def test_rows_in_turn(rn, N, C, cbias):
+    t, ds, dy = _inputs((N,), C, BF, F32, False, cbias)
+    rows, params = [n for n in t if t[n].dim() > 1], [n for n in t if t[n].dim() == 1]
+    got = dict(zip(t, torch.autograd.grad(_call(rn, t), list(t.values()), (ds, dy))))
+    for i in range(0, N, 1500):
+        u = {n: (v.detach()[i:i + 1500].requires_grad_(True) if n in rows else v) for n, v in t.items()}
+        part = torch.autograd.grad(_call(rn, u), [u[n] for n in rows], (ds[i:i + 1500], dy[i:i + 1500]))
+        assert all(torch.equal(a, got[n][i:i + 1500]) for a, n in zip(part, rows))
+    d, _, xh, _ = _formula(t, 1.0)
+    sums = {"weight": dy.double() * xh.detach(), "bias": dy.double(), "branch_bias": got["branch"].double()}
+    for n in params:
+        # xh itself is off by 2^-17 of the largest s / std at most, d_branch by half a step of bf16 a row
+        w = sums[n]
+        slack = 2.0 ** -17 * w.abs().sum(0)
+        if n == "weight":
+            slack = slack + 2.0 ** -17 * float(xh.detach().abs().max() + 1) * dy.double().abs().sum(0)
+        if n == "branch_bias":
+            slack = slack + 2.0 ** -9 * 1.01 * w.abs().sum(0)
+        assert bool(((got[n].double() - w.sum(0)).abs() <= slack).all()), n
+
+
 @pytest.mark.parametrize("used", ["s", "y"])
 @pytest.mark.parametrize("gate", [False, True])
 def test_an_output_no_loss_uses(rn, used, gate):
