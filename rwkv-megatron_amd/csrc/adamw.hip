@@ -21,7 +21,7 @@
 //
 // Bound by memory: bytes a parameter 22 (bf16 p and g, fp32 states), 28 (all fp32), 10 and 16 with
 // 8-bit states, and once more the gradient where it is clipped.  Four layers of 2048 channels (218 M
-// bf16 parameters in 92 tensors): norm 88 us (5.0 TB/s), step 865 us (5.6 TB/s), with 8-bit states 403 us
+// bf16 parameters in 92 tensors): norm 90 us (4.9 TB/s), step 883 us (5.4 TB/s), with 8-bit states 401 us
 // (5.5 TB/s); two layers of 512 (7.3 M fp32): 7 + 5 + 34 us, the 5 the one block that forms the norm and
 // the coefficients.  A copy of 2 GiB reaches 4.9 TB/s.  torch's operators in 32 bits on the same
 // parameters as one tensor take 8.0 ms, 11.7 ms and 313 us.  Tried and left: the step's loads past the

@@ -8,9 +8,9 @@
 // end, and keeps m and z of a row: (m, 1/z) instead of log z + m keeps the gradient's exponent free of
 // the rounding of a number of size 10.
 //
-// Bound by memory: 2 bytes a logit in bf16 forward, 4 backward.  16384 x 65536: 344 us (6.2 TB/s) and 726
-// us (5.9 TB/s); 1024 x 65536: 38 and 41 us, the forward while what ran before it still writes its output
-// back (26 us without); 1001 x 50001 in fp32 54 and 69 us.  A copy of 2 GiB reaches 4.9 TB/s.  torch's
+// Bound by memory: 2 bytes a logit in bf16 forward, 4 backward.  16384 x 65536: 341 us (6.3 TB/s) and 726
+// us (5.9 TB/s); 1024 x 65536: 38 and 40 us, the forward while what ran before it still writes its output
+// back (26 us without); 1001 x 50001 in fp32 53 and 70 us.  A copy of 2 GiB reaches 4.9 TB/s.  torch's
 // operators in 32 bits take 9.1 ms, 636 and 410 us for both ways.
 #include "common.h"
 #include "../../include/rwkv6_amd.h"

@@ -18,9 +18,9 @@
 // sums does.
 //
 // Bound by memory: bytes an element in bf16 8 forward (10 gated), 10 backward (16 gated).  16384 x 2048
-// forward and backward 113 us (kernels 46 + 66, and 4 for the parameters' sums), gated 160 us (57 + 102 +
-// 4): 5.4 TB/s of those bytes, where a copy of 2 GiB reaches 4.9; torch's operators in 32 bits take 1300 and
-// 1950.  Few rows are bound by the launches (8 rows of 2048: 4 us of kernel, 10 a call).
+// forward and backward 106 us (kernels 47 + 57, and 4 for the parameters' sums), gated 160 us (56 + 101 +
+// 4): 5.7 and 5.4 TB/s of those bytes, where a copy of 2 GiB reaches 4.9; torch's operators in 32 bits take
+// 1300 and 1950.  Few rows are bound by the launches (8 rows of 2048: 4 us of kernel, 10 a call).
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 
@@ -382,8 +382,8 @@ inline RnShape rn_shape(int64_t C) {
 }
 // Whether the outputs but y are stored past the caches: where the call's tensors do not fit the 256 MB of
 // the last one anyway.  Kept in it, they push out what the call still reads: 16384 x 2048 bf16, us, cached
-// and streamed: backward 72 and 62, gated 103 and 92, gated forward 64 and 57.  y is the next kernel's
-// input: streamed too, the forward and backward in turn take 109 instead of 112 us, but a training step of
+// and streamed: backward 75 and 57, gated 103 and 100, gated forward 64 and 57.  y is the next kernel's
+// input: streamed too, the forward and backward one after the other took 109 instead of 112 us, but a training step of
 // the 1.6B shape 168.2 instead of 167.5 ms (three runs each).  2049 x 4096, both ways the same.
 inline bool rn_stream(int64_t N, int64_t C) { return N * C >= (int64_t)1 << 24; }
 // The backward's blocks, each with two steps or more, and the steps that a block takes in a row before it
