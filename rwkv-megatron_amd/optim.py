@@ -195,7 +195,14 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Loads a state dict of this class or of torch.optim.AdamW; states keep their own types (torch's
-        loading would cast them to the parameters')."""
+        loading would cast them to the parameters').  A step of another kind (amsgrad, maximize, weight decay
+        added to the gradient) is refused."""
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize") or (g.get("weight_decay") and not g.get("decoupled_weight_decay", True)):
+                raise ValueError("the state dict is of a step with amsgrad, maximize or weight decay in the gradient")
+        for st in state_dict["state"].values():
+            if st and not ("step" in st and "exp_avg" in st and ("exp_avg_sq" in st or "exp_avg_sq_root" in st)):
+                raise ValueError(f"the state dict is not of an AdamW step: a state holds {sorted(st)}")
         super().load_state_dict(state_dict)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         ps = [p for g in self.param_groups for p in g["params"]]

@@ -146,3 +146,20 @@ def test_python_functions_refuse_cpu_tensors(pkg):
     p.grad = torch.zeros(4)
     with pytest.raises(ValueError, match="GPU"):
         o.step()
+
+
+def test_state_dicts_of_other_steps_are_refused(pkg):
+    p, q = (torch.nn.Parameter(torch.ones(4)) for _ in range(2))
+    o = pkg.optim.AdamW([p], lr=0.5)
+    q.grad = torch.ones(4)
+    for make in (lambda: torch.optim.AdamW([q], amsgrad=True), lambda: torch.optim.AdamW([q], maximize=True),
+                 lambda: torch.optim.Adam([q], weight_decay=0.1), lambda: torch.optim.SGD([q], momentum=0.9)):
+        other = make()
+        other.step()
+        with pytest.raises(ValueError):
+            o.load_state_dict(other.state_dict())
+        assert o.param_groups[0]["lr"] == 0.5 and not o.state
+    other = torch.optim.AdamW([q], lr=0.25)
+    other.step()
+    o.load_state_dict(other.state_dict())
+    assert o.param_groups[0]["lr"] == 0.25 and torch.equal(o.moments(p)[0], other.state[q]["exp_avg"])
