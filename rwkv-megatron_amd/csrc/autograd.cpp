@@ -17,6 +17,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/TracerMode.h>
 #include <ATen/autocast_mode.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
@@ -533,6 +534,7 @@ py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& ga
             return py::none();
     if (only_plain && !plain({&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})) return py::none();
     no_transforms();
+    const c10::DeviceGuard on(x.device());           // the default stream is the current device's
     bool grad = recorded({&x, &branch, &gamma, &beta, gate ? &*gate : &x}, cbias);
     for (const Tensor* t : {&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})
         grad = grad || t->_fw_grad(0).defined();          // forward-mode derivatives are refused there
@@ -591,6 +593,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
 };
 Tensor cross_entropy(const Tensor& logits, const Tensor& targets, int64_t ignore) {
     no_transforms();
+    const c10::DeviceGuard on(logits.device());
     return unlocked([&] { return CrossEntropy::apply(logits, targets, ignore); });
 }
 
@@ -629,6 +632,7 @@ Tensor grad_norm_sums(const std::vector<Tensor>& grads) {
         g.n.push_back(t.numel());
     }
     need(!grads.empty(), "no gradients");
+    const c10::DeviceGuard on(grads[0].device());
     const int64_t n = (int64_t)g.n.size();
     const Tensor part = empty({rwkv6_grad_norm_partials(g.n.data(), n)}, at::kDouble, grads[0]);
     unlocked([&] {
@@ -638,6 +642,7 @@ Tensor grad_norm_sums(const std::vector<Tensor>& grads) {
     return part;
 }
 Tensor grad_norm(const Tensor& partials) {
+    const c10::DeviceGuard on(partials.device());
     const Tensor norm = empty({}, at::kFloat, partials);
     check(rwkv6_grad_norm(static_cast<const double*>(ptr(partials)), partials.numel(), fptr(norm), stream_of(partials)),
           "rwkv6_grad_norm");
@@ -662,6 +667,7 @@ py::object adamw_step(const std::vector<Tensor>& params, const std::vector<Tenso
     std::vector<int64_t> num(n);
     const auto dev = params[0].device();
     need(step.device() == dev, "step must lie on the parameters' device");
+    const c10::DeviceGuard on(dev);
     for (size_t i = 0; i < n; ++i) {
         const Tensor &p = params[i], *g = &grads[i];
         need(p.is_cuda() && p.device() == dev, "parameters must live on one GPU");

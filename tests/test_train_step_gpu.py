@@ -181,3 +181,23 @@ def test_without_gradients_and_a_prompt_of_one_token(pkg):
         one = model(tokens[:, :1])
     # the first token does not depend on the later ones; kernels of few tokens sum in other orders
     assert float((one.double() - full[:1].double()).norm()) <= 2.0 ** -5 * float(full[:1].double().norm())
+
+
+# On tensors of a device that is not the current one the kernels run there, on that device's stream.
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one(pkg):
+    g = torch.Generator().manual_seed(2)
+    x, b = (torch.randn(33, 128, generator=g).to(BF) for _ in range(2))
+    w, t = torch.randn(128, generator=g), torch.randint(0, 128, (33,), generator=g)
+    got = []
+    for dev in ("cuda:0", "cuda:1"):
+        u = [v.to(dev).requires_grad_(True) for v in (x, b)]
+        p = torch.nn.Parameter(w.to(dev))
+        s, y = pkg.residual.residual_norm(*u, p, p, 1e-5)
+        loss = pkg.loss.cross_entropy(y, t.to(dev)).mean() + s.float().square().mean()
+        loss.backward()
+        opt = pkg.optim.AdamW([p], max_norm=0.1)
+        opt.step()
+        got.append([v.detach().cpu() for v in (s, y, loss, u[0].grad, u[1].grad, p, opt.grad_norm, pkg.optim.grad_norm([p.grad]))])
+    assert torch.cuda.current_device() == 0
+    assert all(torch.equal(a, b) for a, b in zip(*got))
