@@ -334,7 +334,11 @@ int rwkv6_cross_entropy_bwd(const void* logits, int dtype, int64_t ld, const int
  *                   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
  *                   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
  * exp_avg, exp_avg_sq: f32; or, with exp_avg_scale and exp_avg_sq_scale (ceil(n / 256) floats a tensor),
- * float8 e4m3 codes of m and of sqrt(v) in blocks of 256 elements, value = code * scale.  workspace: 16
+ * float8 e4m3 codes of m and of sqrt(v) in blocks of 256 elements, value = code * scale, each the
+ * nearest; with adamw_step_stochastic one of the two next to the value, so that m and v are right on
+ * average (a hash of t, the element's place and its gradient chooses: equal calls give equal bits).  That
+ * one is for runs of steps: the nearest codes do not follow a v that moves by less than half a code a
+ * step, which at b2 near 1 it always does.  workspace: 16
  * bytes.  No output may overlap another tensor of the call (a tensor listed twice:
  * RWKV6_ERR_INVALID_ARG).
  * ---------------------------------------------------------------------- */
@@ -349,6 +353,13 @@ int rwkv6_adamw_step(void* const* param, const int* param_dtype, const void* con
                      const float* lr_dev, double beta1, double beta2, double eps,
                      double weight_decay, const double* partials, int64_t P, float max_norm,
                      float* norm, void* workspace, void* stream);
+int rwkv6_adamw_step_stochastic(void* const* param, const int* param_dtype, const void* const* grad,
+                                const int* grad_dtype, void* const* exp_avg, void* const* exp_avg_sq,
+                                float* const* exp_avg_scale, float* const* exp_avg_sq_scale,
+                                const int64_t* numel, int64_t count, float* step, double lr,
+                                const float* lr_dev, double beta1, double beta2, double eps,
+                                double weight_decay, const double* partials, int64_t P,
+                                float max_norm, float* norm, void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------
  * Forward without a workspace argument.  No counterpart in the reference: for callers that

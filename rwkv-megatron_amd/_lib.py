@@ -89,6 +89,7 @@ SIGNATURES = {
     "rwkv6_grad_norm_sums": (_int, [_vp, _vp, _vp, _i64, _vp, _vp]),
     "rwkv6_grad_norm": (_int, [_vp, _i64, _fp, _vp]),
     "rwkv6_adamw_step": (_int, [_vp] * 9 + [_i64, _fp, _f64, _fp] + [_f64] * 4 + [_vp, _i64, _f32, _fp, _vp, _vp]),
+    "rwkv6_adamw_step_stochastic": (_int, [_vp] * 9 + [_i64, _fp, _f64, _fp] + [_f64] * 4 + [_vp, _i64, _f32, _fp, _vp, _vp]),
     "rwkv6_layer_norm_bwd": (_int, [_vp, _vp, _int, _fp, _fp] + [_vp] * 4 + [_int, _vp] + [_i64] * 2 + [_vp]),
 }
 

@@ -14,6 +14,13 @@
 // scale)^2, which doubles the range in the exponent (a code reaches from 448 to 2^-9: 2^-36 of the
 // block's largest v).  Values that are not finite do not enter the scale and become NaN codes, so that
 // they spoil no other element of the block; a block below 2^-118 stores zeros.
+// Codes are rounded to the nearest, or (`stochastic`) up or down so that m and v, not its root, come out
+// right on average.  A run of steps wants that: a step moves the root of v by (1 - b2) / 2 of it at most
+// downwards, far less than half a code (3 to 6 %), so that the nearest code is the old one step after step
+// and an element's v moves with its block's largest alone.  4000 steps of N(0, 1) gradients at b2 = 0.995
+// (test_optim_rounding_gpu.py has the like): where half a block's fall to a tenth, their root ends 10.5 times that of
+// 32 bits with the nearest codes, and 0.77 to 1.28 times it (5th to 95th percentile) on average right.
+// The choice is a hash of the step, the element and its gradient, so that equal calls give equal bits.
 //
 // The tensors' addresses travel in the kernels' arguments, AW_T tensors a launch: nothing is copied to
 // the device or kept between calls, and a captured call replays with the addresses it was made with.
@@ -22,7 +29,8 @@
 // Bound by memory: bytes a parameter 22 (bf16 p and g, fp32 states), 28 (all fp32), 10 and 16 with
 // 8-bit states, and once more the gradient where it is clipped.  Four layers of 2048 channels (218 M
 // bf16 parameters in 92 tensors): norm 90 us (4.9 TB/s), step 883 us (5.4 TB/s), with 8-bit states 401 us
-// (5.5 TB/s); two layers of 512 (7.3 M fp32): 7 + 5 + 34 us, the 5 the one block that forms the norm and
+// (5.5 TB/s), and 95 us more with codes right on average, whose arithmetic the bytes no longer hide (fp32
+// parameters: the same time); two layers of 512 (7.3 M fp32): 7 + 5 + 34 us, the 5 the one block that forms the norm and
 // the coefficients.  A copy of 2 GiB reaches 4.9 TB/s.  torch's operators in 32 bits on the same
 // parameters as one tensor take 8.0 ms, 11.7 ms and 313 us.  Tried and left: the step's loads past the
 // caches (499 us instead of 457 for 109 M parameters) and its stores (the same), the norm's sums of eight
@@ -43,6 +51,7 @@
 #define AW_BLK 256              // elements under one 8-bit scale: 32 lanes of 8
 #define AW_MAX ((int64_t)1 << 37)   // elements a call: a launch stays below 2^32 threads
 #define AW_F8_MAX 448.f
+#define AW_F8_BELOW 447.99988f  // 448 (1 - 2^-22): times a reciprocal and the value itself, below 448 after three roundings
 #define AW_TINY 0x1p-118f
 
 namespace {
@@ -180,6 +189,43 @@ __device__ __forceinline__ float aw_top(const float* f) {
     t = fmaxf(t, dpp_mov<0x140>(t));              // the other 8 of 16
     return fmaxf(t, lane_xor_swz<16>(t));
 }
+// What the random bits of eight elements start from: a multiply and shift hash, every bit of which depends on
+// every bit of the step, the element's place and the gradient.
+__device__ __forceinline__ uint32_t aw_seed(float t, int64_t i, float g) {
+    uint32_t h = (uint32_t)(i >> 3) * 0x9E3779B1u ^ (uint32_t)(i >> 35) * 0xC2B2AE3Du ^ __float_as_uint(t) * 0x85EBCA77u ^ __float_as_uint(g);
+    h = (h ^ h >> 16) * 0x7FEB352Du;
+    h = (h ^ h >> 15) * 0x846CA68Bu;
+    return h ^ h >> 16;
+}
+// Eight codes each of m and of the roots of v over their scales, rounded up or down to one of the two e4m3
+// numbers lo < hi around a value a: m up with probability (a - lo) / (hi - lo), a right on average, a root with
+// (a^2 - lo^2) / (hi^2 - lo^2), its square right on average.  The values lie below 448 (see AW_F8_BELOW); one
+// that is not finite becomes NaN.  Below 2^-6 the numbers lie 2^-9 apart, as from 2^-6 to 2^-5: `off` moves a
+// value there.  32 bits an element, the low 18 for the root, the 20 above the twelfth for m, whose weight lies
+// in the other 14.
+__device__ __forceinline__ void aw_encode_either(const float* m, float im, const float* root, float iv, uint32_t h, uint2* cm,
+                                                 uint2* cv) {
+    float qm[8], qv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        h += 0x9E3779B9u;
+        const uint32_t r = (h ^ h >> 15) * 0xD1D5F3A5u;
+        {
+            // the carry of the random bits below the code's last one
+            const float a = fabsf(m[j]) * im, off = a < 0x1p-6f ? 0x1p-6f : 0.f;
+            qm[j] = copysignf(__uint_as_float((__float_as_uint(a + off) + (r >> 12)) & 0xfff00000u) - off, m[j]);
+        }
+        {
+            const float a = root[j] * iv, off = a < 0x1p-6f ? 0x1p-6f : 0.f;
+            const uint32_t b = __float_as_uint(a + off) & 0xfff00000u;
+            const float gap = __uint_as_float((b & 0x7f800000u) - (3u << 23)), lo = __uint_as_float(b) - off, hi = lo + gap;
+            const float u = (float)(r & 0x3ffffu) * 0x1p-18f;
+            qv[j] = u * (gap * (hi + lo)) < (a - lo) * (a + lo) ? hi : lo;
+        }
+    }
+    *cm = aw_encode(qm, 1.f);
+    *cv = aw_encode(qv, 1.f);
+}
 struct Coef {
     float clip, keep, lr, rbc2;                   // c, 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
@@ -263,12 +309,14 @@ rwkv6_adamw_coef_kernel(const double* __restrict__ part, int P, float max_norm, 
 }
 
 // Block b: `per` elements of a tensor, 8 a thread and step.  32 lanes hold the 256 elements of one scale.
-template <bool F8>
+// SR: codes rounded up or down at random, right on average.
+template <bool F8, bool SR>
 __global__ void __launch_bounds__(AW_THR)
 rwkv6_adamw_step_kernel(const StepTable tab, const Coef* __restrict__ coef, int64_t per, float b1, float ob1, float b2,
-                        float ob2, float eps) {
+                        float ob2, float eps, const float* __restrict__ step) {
     const int k = aw_find(tab.first, tab.count, blockIdx.x);
     const Coef c = coef[0];
+    const float t = SR ? step[0] : 0.f;
     const int64_t n = tab.n[k], i0 = (int64_t)((int)blockIdx.x - tab.first[k]) * per, i1 = min(n, i0 + per);
     void *p = tab.p[k], *m = tab.m[k], *v = tab.v[k];
     const void* g = tab.g[k];
@@ -310,8 +358,17 @@ rwkv6_adamw_step_kernel(const StepTable tab, const Coef* __restrict__ coef, int6
             tm = tm < AW_TINY ? 0.f : tm;
             tv = tv < AW_TINY ? 0.f : tv;
             // scale = t (1 / 448), and the codes' factor 448 (1 / t)
-            aw_codes_store(m, i, n, vec, aw_encode(mf, tm > 0.f ? (1.f / tm) * AW_F8_MAX : 0.f));
-            aw_codes_store(v, i, n, vec, aw_encode(root, tv > 0.f ? (1.f / tv) * AW_F8_MAX : 0.f));
+            constexpr float top = SR ? AW_F8_BELOW : AW_F8_MAX;
+            const float im = tm > 0.f ? (1.f / tm) * top : 0.f, iv = tv > 0.f ? (1.f / tv) * top : 0.f;
+            uint2 cm, cv;
+            if constexpr (SR) {
+                aw_encode_either(mf, im, root, iv, aw_seed(t, i, gf[0]), &cm, &cv);
+            } else {
+                cm = aw_encode(mf, im);
+                cv = aw_encode(root, iv);
+            }
+            aw_codes_store(m, i, n, vec, cm);
+            aw_codes_store(v, i, n, vec, cv);
             if ((threadIdx.x & 31) == 0) {
                 ms[0] = tm * (1.f / AW_F8_MAX);
                 vs[0] = tv * (1.f / AW_F8_MAX);
@@ -380,6 +437,86 @@ bool aw_overlap(std::vector<Range>& r) {
     }
     return false;
 }
+int aw_step(bool stochastic, void* const* param, const int* param_dtype, const void* const* grad, const int* grad_dtype,
+            void* const* exp_avg, void* const* exp_avg_sq, float* const* exp_avg_scale,
+            float* const* exp_avg_sq_scale, const int64_t* numel, int64_t count, float* step, double lr,
+            const float* lr_dev, double beta1, double beta2, double eps, double weight_decay, const double* partials,
+            int64_t P, float max_norm, float* norm, void* workspace, void* stream) {
+    const int st = aw_sizes(numel, count);
+    if (st) return st;
+    const bool f8 = exp_avg_scale != nullptr;
+    if (!step || !workspace || P < 0 || (P && !partials)) return RWKV6_ERR_INVALID_ARG;
+    if (P > (1 << 30)) return RWKV6_ERR_UNSUPPORTED;
+    if (!(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1.)) return RWKV6_ERR_INVALID_ARG;
+    if (count && (!param || !param_dtype || !grad || !grad_dtype || !exp_avg || !exp_avg_sq)) return RWKV6_ERR_INVALID_ARG;
+    if (f8 != (exp_avg_sq_scale != nullptr)) return RWKV6_ERR_INVALID_ARG;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15u) || aw_misaligned(partials, 8) || aw_misaligned(step, 4) ||
+        aw_misaligned(lr_dev, 4) || aw_misaligned(norm, 4))
+        return RWKV6_ERR_ALIGNMENT;
+    try {
+        std::vector<Range> ranges;
+        ranges.reserve((size_t)count * 6 + 5);
+        aw_add(ranges, workspace, sizeof(Coef), true);
+        aw_add(ranges, step, 4, true);
+        aw_add(ranges, norm, 4, true);
+        aw_add(ranges, lr_dev, 4, false);
+        aw_add(ranges, partials, (size_t)P * 8, false);
+        for (int64_t k = 0; k < count; ++k) {
+            if (!aw_dt(param_dtype[k]) || !aw_dt(grad_dtype[k])) return RWKV6_ERR_INVALID_ARG;
+            if (numel[k] == 0) continue;
+            if (!param[k] || !grad[k] || !exp_avg[k] || !exp_avg_sq[k] || (f8 && (!exp_avg_scale[k] || !exp_avg_sq_scale[k])))
+                return RWKV6_ERR_INVALID_ARG;
+            const size_t n = (size_t)numel[k], ps = param_bytes(param_dtype[k]), gs = param_bytes(grad_dtype[k]), ss = f8 ? 1 : 4;
+            if (aw_misaligned(param[k], ps) || aw_misaligned(grad[k], gs) || aw_misaligned(exp_avg[k], ss) ||
+                aw_misaligned(exp_avg_sq[k], ss) || (f8 && (aw_misaligned(exp_avg_scale[k], 4) || aw_misaligned(exp_avg_sq_scale[k], 4))))
+                return RWKV6_ERR_ALIGNMENT;
+            aw_add(ranges, param[k], n * ps, true);
+            aw_add(ranges, grad[k], n * gs, false);
+            aw_add(ranges, exp_avg[k], n * ss, true);
+            aw_add(ranges, exp_avg_sq[k], n * ss, true);
+            if (f8) {
+                aw_add(ranges, exp_avg_scale[k], (n + AW_BLK - 1) / AW_BLK * 4, true);
+                aw_add(ranges, exp_avg_sq_scale[k], (n + AW_BLK - 1) / AW_BLK * 4, true);
+            }
+        }
+        if (aw_overlap(ranges)) return RWKV6_ERR_INVALID_ARG;
+    } catch (...) {                               // no host memory for the check
+        return RWKV6_ERR_LAUNCH;
+    }
+    Coef* coef = (Coef*)workspace;
+    hipLaunchKernelGGL(rwkv6_adamw_coef_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), partials,
+                       partials ? (int)P : 0, max_norm, norm, step, lr_dev, lr, log(beta1), log(beta2), weight_decay, coef);
+    const int64_t per = aw_step_per(numel, count);
+    StepTable tab;
+    int64_t blocks = 0;
+    tab.count = 0;
+    auto launch = [&] {
+        if (!blocks) return;
+        auto k = !f8 ? rwkv6_adamw_step_kernel<false, false>
+                     : stochastic ? rwkv6_adamw_step_kernel<true, true> : rwkv6_adamw_step_kernel<true, false>;
+        hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(AW_THR), 0, reinterpret_cast<hipStream_t>(stream), tab, (const Coef*)coef,
+                           per, (float)beta1, (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps, (const float*)step);
+        blocks = tab.count = 0;
+    };
+    for (int64_t k = 0; k < count; ++k) {
+        if (numel[k] == 0) continue;
+        const int64_t need = aw_blocks(numel[k], per);
+        if (tab.count == AW_T) launch();
+        const int i = tab.count++;
+        tab.p[i] = param[k];
+        tab.g[i] = grad[k];
+        tab.m[i] = exp_avg[k];
+        tab.v[i] = exp_avg_sq[k];
+        tab.ms[i] = f8 ? exp_avg_scale[k] : nullptr;
+        tab.vs[i] = f8 ? exp_avg_sq_scale[k] : nullptr;
+        tab.n[i] = numel[k];
+        tab.dt[i] = param_dtype[k] | grad_dtype[k] << 8;
+        tab.first[i] = (int)blocks;
+        blocks += need;
+    }
+    launch();
+    return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+}
 }  // namespace
 
 extern "C" {
@@ -447,79 +584,17 @@ int rwkv6_adamw_step(void* const* param, const int* param_dtype, const void* con
                      float* const* exp_avg_sq_scale, const int64_t* numel, int64_t count, float* step, double lr,
                      const float* lr_dev, double beta1, double beta2, double eps, double weight_decay, const double* partials,
                      int64_t P, float max_norm, float* norm, void* workspace, void* stream) {
-    const int st = aw_sizes(numel, count);
-    if (st) return st;
-    const bool f8 = exp_avg_scale != nullptr;
-    if (!step || !workspace || P < 0 || (P && !partials)) return RWKV6_ERR_INVALID_ARG;
-    if (P > (1 << 30)) return RWKV6_ERR_UNSUPPORTED;
-    if (!(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1.)) return RWKV6_ERR_INVALID_ARG;
-    if (count && (!param || !param_dtype || !grad || !grad_dtype || !exp_avg || !exp_avg_sq)) return RWKV6_ERR_INVALID_ARG;
-    if (f8 != (exp_avg_sq_scale != nullptr)) return RWKV6_ERR_INVALID_ARG;
-    if ((reinterpret_cast<uintptr_t>(workspace) & 15u) || aw_misaligned(partials, 8) || aw_misaligned(step, 4) ||
-        aw_misaligned(lr_dev, 4) || aw_misaligned(norm, 4))
-        return RWKV6_ERR_ALIGNMENT;
-    try {
-        std::vector<Range> ranges;
-        ranges.reserve((size_t)count * 6 + 5);
-        aw_add(ranges, workspace, sizeof(Coef), true);
-        aw_add(ranges, step, 4, true);
-        aw_add(ranges, norm, 4, true);
-        aw_add(ranges, lr_dev, 4, false);
-        aw_add(ranges, partials, (size_t)P * 8, false);
-        for (int64_t k = 0; k < count; ++k) {
-            if (!aw_dt(param_dtype[k]) || !aw_dt(grad_dtype[k])) return RWKV6_ERR_INVALID_ARG;
-            if (numel[k] == 0) continue;
-            if (!param[k] || !grad[k] || !exp_avg[k] || !exp_avg_sq[k] || (f8 && (!exp_avg_scale[k] || !exp_avg_sq_scale[k])))
-                return RWKV6_ERR_INVALID_ARG;
-            const size_t n = (size_t)numel[k], ps = param_bytes(param_dtype[k]), gs = param_bytes(grad_dtype[k]), ss = f8 ? 1 : 4;
-            if (aw_misaligned(param[k], ps) || aw_misaligned(grad[k], gs) || aw_misaligned(exp_avg[k], ss) ||
-                aw_misaligned(exp_avg_sq[k], ss) || (f8 && (aw_misaligned(exp_avg_scale[k], 4) || aw_misaligned(exp_avg_sq_scale[k], 4))))
-                return RWKV6_ERR_ALIGNMENT;
-            aw_add(ranges, param[k], n * ps, true);
-            aw_add(ranges, grad[k], n * gs, false);
-            aw_add(ranges, exp_avg[k], n * ss, true);
-            aw_add(ranges, exp_avg_sq[k], n * ss, true);
-            if (f8) {
-                aw_add(ranges, exp_avg_scale[k], (n + AW_BLK - 1) / AW_BLK * 4, true);
-                aw_add(ranges, exp_avg_sq_scale[k], (n + AW_BLK - 1) / AW_BLK * 4, true);
-            }
-        }
-        if (aw_overlap(ranges)) return RWKV6_ERR_INVALID_ARG;
-    } catch (...) {                               // no host memory for the check
-        return RWKV6_ERR_LAUNCH;
-    }
-    Coef* coef = (Coef*)workspace;
-    hipLaunchKernelGGL(rwkv6_adamw_coef_kernel, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), partials,
-                       partials ? (int)P : 0, max_norm, norm, step, lr_dev, lr, log(beta1), log(beta2), weight_decay, coef);
-    const int64_t per = aw_step_per(numel, count);
-    StepTable tab;
-    int64_t blocks = 0;
-    tab.count = 0;
-    auto launch = [&] {
-        if (!blocks) return;
-        hipLaunchKernelGGL(f8 ? rwkv6_adamw_step_kernel<true> : rwkv6_adamw_step_kernel<false>, dim3((unsigned)blocks),
-                           dim3(AW_THR), 0, reinterpret_cast<hipStream_t>(stream), tab, (const Coef*)coef, per, (float)beta1,
-                           (float)(1. - beta1), (float)beta2, (float)(1. - beta2), (float)eps);
-        blocks = tab.count = 0;
-    };
-    for (int64_t k = 0; k < count; ++k) {
-        if (numel[k] == 0) continue;
-        const int64_t need = aw_blocks(numel[k], per);
-        if (tab.count == AW_T) launch();
-        const int i = tab.count++;
-        tab.p[i] = param[k];
-        tab.g[i] = grad[k];
-        tab.m[i] = exp_avg[k];
-        tab.v[i] = exp_avg_sq[k];
-        tab.ms[i] = f8 ? exp_avg_scale[k] : nullptr;
-        tab.vs[i] = f8 ? exp_avg_sq_scale[k] : nullptr;
-        tab.n[i] = numel[k];
-        tab.dt[i] = param_dtype[k] | grad_dtype[k] << 8;
-        tab.first[i] = (int)blocks;
-        blocks += need;
-    }
-    launch();
-    return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+    return aw_step(false, param, param_dtype, grad, grad_dtype, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, numel, count, step, lr,
+                   lr_dev, beta1, beta2, eps, weight_decay, partials, P, max_norm, norm, workspace, stream);
+}
+
+int rwkv6_adamw_step_stochastic(void* const* param, const int* param_dtype, const void* const* grad, const int* grad_dtype,
+                                void* const* exp_avg, void* const* exp_avg_sq, float* const* exp_avg_scale,
+                                float* const* exp_avg_sq_scale, const int64_t* numel, int64_t count, float* step, double lr,
+                                const float* lr_dev, double beta1, double beta2, double eps, double weight_decay, const double* partials,
+                                int64_t P, float max_norm, float* norm, void* workspace, void* stream) {
+    return aw_step(true, param, param_dtype, grad, grad_dtype, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, numel, count, step, lr,
+                   lr_dev, beta1, beta2, eps, weight_decay, partials, P, max_norm, norm, workspace, stream);
 }
 
 }  // extern "C"

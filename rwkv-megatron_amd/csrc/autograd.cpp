@@ -653,7 +653,7 @@ Tensor grad_norm(const Tensor& partials) {
 py::object adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m,
                       const std::vector<Tensor>& v, const std::vector<Tensor>& ms, const std::vector<Tensor>& vs,
                       const Tensor& step, double lr, const OptTensor& lr_dev, double b1, double b2, double eps, double wd,
-                      double max_norm, const OptTensor& partials) {
+                      double max_norm, const OptTensor& partials, bool stochastic) {
     const size_t n = params.size();
     const bool f8 = !ms.empty() || !vs.empty();
     need(n > 0, "no parameters");
@@ -709,11 +709,12 @@ py::object adamw_step(const std::vector<Tensor>& params, const std::vector<Tenso
     if (clip) need(partials->device() == dev && partials->scalar_type() == at::kDouble && partials->is_contiguous(), "partial sums must be float64 on the parameters' device");
     const Tensor work = empty({4}, at::kFloat, step), norm = clip ? empty({}, at::kFloat, step) : Tensor();
     unlocked([&] {
-        check(rwkv6_adamw_step(pp.data(), pt.data(), pg.data(), gt.data(), pm.data(), pv.data(), f8 ? psm.data() : nullptr,
-                               f8 ? psv.data() : nullptr, num.data(), (int64_t)n, fptr(step), lr, lrp, b1, b2, eps, wd,
-                               clip ? static_cast<const double*>(ptr(*partials)) : nullptr, clip ? partials->numel() : 0,
-                               (float)max_norm, fptr(norm), fptr(work), stream_of(step)),
-              "rwkv6_adamw_step");
+        const auto fn = stochastic ? rwkv6_adamw_step_stochastic : rwkv6_adamw_step;
+        check(fn(pp.data(), pt.data(), pg.data(), gt.data(), pm.data(), pv.data(), f8 ? psm.data() : nullptr,
+                 f8 ? psv.data() : nullptr, num.data(), (int64_t)n, fptr(step), lr, lrp, b1, b2, eps, wd,
+                 clip ? static_cast<const double*>(ptr(*partials)) : nullptr, clip ? partials->numel() : 0,
+                 (float)max_norm, fptr(norm), fptr(work), stream_of(step)),
+              stochastic ? "rwkv6_adamw_step_stochastic" : "rwkv6_adamw_step");
     });
     // the tensors changed: a backward that still needs one of them as it was says so
     auto bump = [](const Tensor& t) {

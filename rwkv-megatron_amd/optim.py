@@ -13,9 +13,12 @@ The reference trains with AdamW, decoupled weight decay and a gradient clip
   parameter has no wider copy: where that matters keep the parameters in fp32, as the modules here
   take them.
 * 8-bit states: float8 (e4m3) codes and one fp32 scale for every 256 consecutive elements; the second
-  moment by its root, which doubles the range that a code covers.  A code rounds a value by 2^-4 of it
-  at most, and an element whose magnitude relative to its block's largest changes by less than that
-  in a step keeps its code: the second moments of a block rise and fall with the largest.
+  moment by its root, which doubles the range that a code covers.  ``AdamW`` rounds codes up or down so
+  that both moments are right on average, by less than 2^-3 of the value (the root's); over a run of steps the
+  root of the second moment then scatters by about a sixth of its value around that of 32 bits.
+  ``adamw_step`` alone rounds to the nearest code (2^-4 of the value at most) unless it is told otherwise:
+  the nearest code of a second moment that moves by less than half a code a step is the old one, so over
+  many such steps it follows its block's largest and not its own gradients.
 * A step is a handful of launches whatever the number of tensors, nothing is copied to or read from
   the device, and the step count lives there: a captured step (HIP graph) counts on replay.
 """
@@ -37,12 +40,13 @@ def grad_norm(grads):
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
-               max_norm=None, scales=None):
+               max_norm=None, scales=None, rounding="nearest"):
     """One AdamW step over lists of tensors, in place.
 
     params, grads: bf16 or fp32, dense in memory; exp_avgs, exp_avg_sqs: fp32 of the parameters' shapes,
     or with scales = (exp_avg_scales, exp_avg_sq_scales) float8_e4m3fn codes, the scales fp32
-    [ceil(numel / 256)] a tensor (exp_avg_sqs then stands for the roots: v = (code * scale)^2).  step: one
+    [ceil(numel / 256)] a tensor (exp_avg_sqs then stands for the roots: v = (code * scale)^2; rounding
+    "nearest", or "stochastic" for a run of steps, module docstring).  step: one
     fp32 number on the GPU, the steps done before; it is counted up.  lr is a number or a one-element fp32
     tensor on the GPU.  With max_norm the gradients count times min(1, max_norm / (norm + 1e-6)), without
     being changed, and the norm over all of them is returned (0-dim fp32), else None."""
@@ -51,16 +55,19 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     ms, vs = ([], []) if scales is None else (_tensors("scales", scales[0]), _tensors("scales", scales[1]))
     if scales is not None and not len(ms) == len(vs) == len(params):
         raise ValueError("lists of different lengths")
+    if rounding not in ("nearest", "stochastic"):
+        raise ValueError(f'rounding must be "nearest" or "stochastic", got {rounding!r}')
     _check_hyper(lr, betas, eps, weight_decay, max_norm)
     native = _lib.native()
     sums = None if max_norm is None else native.grad_norm_sums(grads)
-    return _step(native, params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, max_norm, sums)
+    return _step(native, params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, max_norm, sums,
+                 rounding == "stochastic")
 
 
-def _step(native, params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, max_norm, sums):
+def _step(native, params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, max_norm, sums, stochastic):
     tensor = isinstance(lr, torch.Tensor) and lr.is_cuda
     return native.adamw_step(params, grads, m, v, ms, vs, step, 0.0 if tensor else float(lr), lr if tensor else None,
-                             betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, sums)
+                             betas[0], betas[1], eps, weight_decay, 0.0 if max_norm is None else max_norm, sums, stochastic)
 
 
 def _tensors(name, ts):
@@ -90,10 +97,10 @@ def _not_captured(what):
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay over bf16 or fp32 parameters on one GPU.
 
-    state_bits=8 keeps the moments in 8 bits (module docstring) for tensors of min_8bit_numel elements and
-    more; smaller ones (norms, biases, mixing coefficients) keep 32 bits.  max_norm clips by the norm of
-    all gradients of the step, in all groups (`grad_norm` holds it afterwards, a 0-dim tensor); the
-    gradients themselves stay as they are.  lr may be a one-element fp32 tensor on the GPU, which a
+    state_bits=8 keeps the moments in 8 bits (module docstring; rounded right on average, the same bits for
+    the same step, gradient and state) for tensors of min_8bit_numel elements and more; smaller ones (norms,
+    biases, mixing coefficients) keep 32 bits.  max_norm clips by the norm of all gradients of the step, in
+    all groups (`grad_norm` holds it afterwards, a 0-dim tensor); the gradients themselves stay as they are.  lr may be a one-element fp32 tensor on the GPU, which a
     captured step reads on replay; a step is captured after one like it has run (the states exist then).
 
     State of a parameter: ``step`` (one tensor for all parameters that have made the same steps),
@@ -188,7 +195,7 @@ class AdamW(torch.optim.Optimizer):
             norm = _step(native, ps, [p.grad for p in ps], take("exp_avg"),
                          take("exp_avg_sq_root" if eight else "exp_avg_sq"), take("exp_avg_scale") if eight else [],
                          take("exp_avg_sq_scale") if eight else [], states[0]["step"], group["lr"], group["betas"],
-                         group["eps"], group["weight_decay"], self.max_norm, sums)
+                         group["eps"], group["weight_decay"], self.max_norm, sums, True)
         self.grad_norm = norm
         return loss
 

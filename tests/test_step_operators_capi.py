@@ -163,3 +163,18 @@ def test_state_dicts_of_other_steps_are_refused(pkg):
     other.step()
     o.load_state_dict(other.state_dict())
     assert o.param_groups[0]["lr"] == 0.25 and torch.equal(o.moments(p)[0], other.state[q]["exp_avg"])
+
+
+def test_the_stochastic_step_refuses_the_same_calls(pkg):
+    L = pkg._lib.load()
+
+    class Other:
+        rwkv6_adamw_step = L.rwkv6_adamw_step_stochastic
+
+    vp = ctypes.c_void_p
+    for kw in (dict(p=None), dict(step=None), dict(ws=None), dict(count=-1), dict(b2=1.0), dict(vs=None), dict(P=1),
+               dict(p=_arr(vp, [0x10000000, 0x10000000])), dict(step=_p(0x40000000))):
+        assert _step(Other, **kw) == INVALID, kw
+    assert _step(Other, ws=_p(0x71000008)) == ALIGNMENT and _step(Other, size=1 << 41) == UNSUPPORTED
+    with pytest.raises(ValueError, match="rounding"):
+        pkg.optim.adamw_step([torch.zeros(4)], [torch.zeros(4)], [torch.zeros(4)], [torch.zeros(4)], torch.zeros(()), lr=1.0, rounding="down")
