@@ -203,24 +203,33 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Loads a state dict of this class or of torch.optim.AdamW; states keep their own types (torch's
         loading would cast them to the parameters').  A step of another kind (amsgrad, maximize, weight decay
-        added to the gradient) is refused."""
+        added to the gradient) is refused, and so is a state that does not have its parameter's shape; the
+        optimizer is then as it was."""
+        loaded = self._loaded(state_dict)
+        super().load_state_dict({**state_dict, "state": {}})
+        self.state.update(loaded)
+
+    def _loaded(self, state_dict):
+        """The states that a state dict stands for, a parameter, as this optimizer keeps them."""
+        saved_groups = [g["params"] for g in state_dict["param_groups"]]
+        groups = [g["params"] for g in self.param_groups]
+        if [len(g) for g in saved_groups] != [len(g) for g in groups]:
+            raise ValueError("the state dict has other parameter groups than the optimizer")
         for g in state_dict["param_groups"]:
             if g.get("amsgrad") or g.get("maximize") or (g.get("weight_decay") and not g.get("decoupled_weight_decay", True)):
                 raise ValueError("the state dict is of a step with amsgrad, maximize or weight decay in the gradient")
+        pairs = [[(p, state_dict["state"][i]) for i, p in zip(ids, ps) if state_dict["state"].get(i)]
+                 for ids, ps in zip(saved_groups, groups)]
         for st in state_dict["state"].values():
-            if st and not ("step" in st and "exp_avg" in st and ("exp_avg_sq" in st or "exp_avg_sq_root" in st)):
-                raise ValueError(f"the state dict is not of an AdamW step: a state holds {sorted(st)}")
-        super().load_state_dict(state_dict)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        ps = [p for g in self.param_groups for p in g["params"]]
-        saved = {p: state_dict["state"][i] for i, p in zip(ids, ps) if i in state_dict["state"]}
-        self.state.clear()
-        for group in self.param_groups:
+            if st:
+                _check_names(st)
+        for p, st in (pair for group in pairs for pair in group):
+            _check_shapes(p, st)
+        loaded = {}
+        for group in pairs:
             steps = {}                             # one tensor for equal counts, as a run would have made them
-            for p in group["params"]:
-                if not saved.get(p):
-                    continue
-                state, old = self._new_state(p), saved[p]
+            for p, old in group:
+                state = self._new_state(p)
                 key = (float(old["step"]), p.device, "exp_avg_scale" in state)
                 if key not in steps:
                     steps[key] = torch.full((), key[0], dtype=torch.float32, device=p.device)
@@ -236,11 +245,31 @@ class AdamW(torch.optim.Optimizer):
                     else:
                         state["exp_avg"].copy_(m)
                         state["exp_avg_sq"].copy_(v)
-                self.state[p] = dict(step=steps[key], **state)
+                loaded[p] = dict(step=steps[key], **state)
+        return loaded
 
     def moments(self, p):
         """The fp32 values that a parameter's states stand for: (exp_avg, exp_avg_sq)."""
         return _moments(self.state[p])
+
+
+def _check_names(state):
+    """Raises for a state that is neither torch's AdamW's nor an 8-bit one of this class."""
+    eight = {"exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_scale"}
+    wanted = {"step", "exp_avg", *(eight if eight & set(state) else {"exp_avg_sq"})}
+    if not wanted <= set(state):
+        raise ValueError(f"the state dict is not of an AdamW step: a state holds {sorted(state)}")
+
+
+def _check_shapes(p, state):
+    for name in ("exp_avg", "exp_avg_sq", "exp_avg_sq_root"):
+        if name in state and state[name].shape != p.shape:
+            raise ValueError(f"a state's {name} has the shape {tuple(state[name].shape)}, its parameter {tuple(p.shape)}")
+    for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+        blocks = -(-p.numel() // BLOCK)
+        if name in state and tuple(state[name].shape) != (blocks,):
+            raise ValueError(f"{name} must be a scale for {BLOCK} elements of a shape {tuple(p.shape)}, {blocks} in all, "
+                             f"got {tuple(state[name].shape)}")
 
 
 def _flat(t):
