@@ -204,10 +204,20 @@ class AdamW(torch.optim.Optimizer):
         """Loads a state dict of this class or of torch.optim.AdamW; states keep their own types (torch's
         loading would cast them to the parameters').  A step of another kind (amsgrad, maximize, weight decay
         added to the gradient) is refused, and so is a state that does not have its parameter's shape; the
-        optimizer is then as it was."""
-        loaded = self._loaded(state_dict)
-        super().load_state_dict({**state_dict, "state": {}})
-        self.state.update(loaded)
+        optimizer is then as it was.  Pre-hooks may change the dict, post-hooks find the states loaded."""
+        loaded = {}
+
+        def take(_, sd):                           # the last pre-hook: sees what the others made of the dict
+            loaded.update(self._loaded(sd))
+            return {**sd, "state": {}}
+
+        hooks = [self.register_load_state_dict_pre_hook(take),
+                 self.register_load_state_dict_post_hook(lambda _: self.state.update(loaded), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
 
     def _loaded(self, state_dict):
         """The states that a state dict stands for, a parameter, as this optimizer keeps them."""

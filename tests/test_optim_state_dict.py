@@ -98,3 +98,36 @@ def test_states_that_fit_load(pkg):
         assert float(o.state[p]["step"]) == 1 and o.param_groups[0]["lr"] == 0.25
         o.load_state_dict(pkg.optim.AdamW([_param(3, 100)], lr=0.75).state_dict())
         assert not o.state and o.param_groups[0]["lr"] == 0.75
+
+
+# What a pre-hook returns is what is loaded; a post-hook sees the states; both stay registered, and nothing else does.
+@pytest.mark.parametrize("bits", [8, 32])
+def test_hooks_around_loading(pkg, bits):
+    p = _param(300)
+    o = pkg.optim.AdamW([p], state_bits=bits, min_8bit_numel=1)
+    seen = []
+
+    def twice(opt, sd):
+        sd = copy.deepcopy(sd)
+        sd["state"][0]["exp_avg"] *= 2
+        sd["state"][0]["step"] += 4
+        return sd
+
+    o.register_load_state_dict_pre_hook(twice)
+    o.register_load_state_dict_post_hook(lambda opt: seen.append({k: v.clone() for k, v in opt.state[p].items()}))
+    for k in range(2):
+        o.load_state_dict(_saved(pkg, (300,)))
+        m, _ = o.moments(p)
+        # 0.1 in 32 bits; the largest of its block, so exact in 8 bits up to the scale
+        assert bool(((m - 0.1).abs() <= 2.0 ** -20).all()) and float(o.state[p]["step"]) == 5
+        assert len(seen) == k + 1 and seen[k].keys() == o.state[p].keys() and all(torch.equal(v.float(), o.state[p][n].float()) for n, v in seen[k].items())
+    before = _look(o)
+    refuse = o.register_load_state_dict_pre_hook(lambda opt, sd: _saved(pkg, (4,)))
+    with pytest.raises(ValueError, match="shape"):
+        o.load_state_dict(_saved(pkg, (300,)))
+    assert _same(_look(o), before) and len(seen) == 2
+    refuse.remove()
+    # a copy, which has no hooks, loads too
+    other = copy.deepcopy(o)
+    other.load_state_dict(_saved(pkg, (300,)))
+    assert float(other.state[other.param_groups[0]["params"][0]]["step"]) == 1
