@@ -49,7 +49,8 @@
 #define AW_RUN (AW_AHEAD * AW_STEP)
 #define AW_T 60                 // tensors a launch: the arguments stay below 4 KB
 #define AW_BLK 256              // elements under one 8-bit scale: 32 lanes of 8
-#define AW_MAX ((int64_t)1 << 37)   // elements a call: a launch stays below 2^32 threads
+#define AW_MAX ((int64_t)1 << 37)   // elements a call
+#define AW_BLOCKS ((int64_t)1 << 23)    // blocks a launch, at about: fewer than 2^32 threads
 #define AW_F8_MAX 448.f
 #define AW_F8_BELOW 447.99988f  // 448 (1 - 2^-22): times a reciprocal and the value itself, below 448 after three roundings
 #define AW_TINY 0x1p-118f
@@ -393,8 +394,12 @@ int64_t aw_per(const int64_t* numel, int64_t count, int64_t blocks) {
 // 2, 4, 8 and 16 steps a block: 423, 447, 458, 469, 488; 55 M with fp32 and 8-bit states 160, 163, 171, 178, 184;
 // 7 M, 2 steps all at once and 1 step 33 and 35.
 int64_t aw_step_per(const int64_t* numel, int64_t count) {
-    const int64_t per = aw_per(numel, count, 2048);
-    return per > 2 * AW_STEP ? AW_STEP : per;
+    int64_t total = 0;
+    for (int64_t k = 0; k < count; ++k) total += numel[k];
+    int64_t per = aw_per(numel, count, 2048);
+    per = per > 2 * AW_STEP ? AW_STEP : per;
+    while (total / per > AW_BLOCKS) per *= 2;      // each tensor of a launch adds a block at most
+    return per;
 }
 int64_t aw_blocks(int64_t n, int64_t per) { return (n + per - 1) / per; }
 bool aw_dt(int dt) { return dt == RWKV6_F32 || dt == RWKV6_BF16; }
