@@ -15,7 +15,7 @@
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 
-#define CE_GRID (1 << 22)
+#define CE_GRID (1 << 21)      // blocks a launch, of up to 1024 threads: fewer than 2^32 threads
 
 namespace {
 

@@ -105,6 +105,15 @@ def test_a_call_past_the_limit_launches_nothing(look):
         assert look(f"adamw({sizes}, True)") == (2, []) == look(f"norm({sizes})")
 
 
+# 256 GiB of bf16 logits, and more rows than a grid's blocks at every number of threads a row.
+@pytest.mark.parametrize("N,V", [(1 << 21, 65536), (1 << 22, 32768), (1 << 23, 8192), (1 << 26, 512), (1 << 35, 8), (1 << 40, 1)])
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("dt", [0, 1])
+def test_cross_entropy(look, N, V, back, dt):
+    status, launches = look(f"loss({N}, {V}, {dt}, {back})")
+    assert status == 0 and len(launches) == 1 and 0 < launches[0][0] * launches[0][1] < 1 << 32, launches
+
+
 @pytest.mark.parametrize("N,C", [(1 << 37, 8), (1 << 32, 256), (1 << 30, 1024), (1 << 28, 4096), (1 << 27, 8192)])
 @pytest.mark.parametrize("gate", [False, True])
 def test_residual_norm(look, N, C, gate):
