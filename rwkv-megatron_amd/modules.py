@@ -336,10 +336,12 @@ def _add_norm(norm, x, branch, bias=None, gate=None):
 
 
 def _plain_module(m, cls):
-    """Whether calling m is calling cls.forward: no subclass, no hooks (a profiler's, a sharding
-    wrapper's), no forward of its own, no compiler that traces the call."""
+    """Whether calling m is calling the forward that cls has in this file: no subclass, no forward or call that a
+    program has put in its place (on the instance, the class or nn.Module), no hooks (a profiler's, a sharding
+    wrapper's), no compiler that traces the call."""
     hooks = torch.nn.modules.module
     return (type(m) is cls and "forward" not in m.__dict__
+            and cls.forward is _FORWARD[cls] and cls.__call__ is _CALL and nn.Module._call_impl is _CALL_IMPL
             and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
                      or hooks._global_forward_hooks or hooks._global_forward_pre_hooks
                      or hooks._global_backward_hooks or hooks._global_backward_pre_hooks)
@@ -377,6 +379,11 @@ class RWKV6Layer(nn.Module):
         x, h = self._time_mix(x, h)
         out, gate = self.mlp.ungated(h)
         return _add_norm(next_norm, x, out, gate=gate)
+
+
+# what _plain_module compares with
+_FORWARD = {cls: cls.forward for cls in (LayerNorm, RWKV6ChannelMix, RWKV6Layer)}
+_CALL, _CALL_IMPL = nn.Module.__call__, nn.Module._call_impl
 
 
 def get_rwkv6_layer_spec():
