@@ -293,7 +293,8 @@ int rwkv6_layer_norm_bwd(const void* x, const void* gamma, int gamma_dtype, cons
  *   bwd: ds [N,C] in x_dtype (nullable: zero), dy [N,C] bf16 -> dx in x_dtype, d_branch, d_gate bf16
  *        (d_gate NULL exactly when gate is), dgamma, dbeta in param_dtype and d_branch_bias in bias_dtype
  *        (all NULL: not wanted, no workspace; d_branch_bias NULL also when branch_bias is).  d_branch may
- *        be NULL where it equals dx: x_dtype bf16, scale 1, neither gate nor branch_bias.
+ *        be NULL where it equals dx: x_dtype bf16, scale 1, neither gate nor branch_bias.  branch may be
+ *        NULL where stepwise is set and gate is NULL: x is then the s that the forward wrote.
  * ---------------------------------------------------------------------- */
 int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias,
                             int bias_dtype, const void* gate, float scale, int stepwise,

@@ -441,7 +441,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     };
     static Args args(const Tensor& x, const Tensor& branch, const Tensor& gate, const Tensor& cbias) {
         const int64_t C = x.size(-1);
-        return {dense(x), dense(branch), gate.defined() ? dense(gate) : gate, cbias.defined() ? param(cbias) : Param{cbias, 0},
+        return {dense(x), branch.defined() ? dense(branch) : branch, gate.defined() ? dense(gate) : gate, cbias.defined() ? param(cbias) : Param{cbias, 0},
                 x.scalar_type() == at::kFloat ? RWKV6_F32 : RWKV6_BF16, C ? x.numel() / C : 0, C};
     }
     // (s, y), and the rows' mean and rstd ([2, N]) where a backward will want them
@@ -462,11 +462,14 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     }
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& branch, const Tensor& gamma,
                                  const Tensor& beta, const OptTensor& gate, const OptTensor& cbias, double eps,
-                                 double scale, bool stepwise) {
+                                 double scale, bool stepwise, bool layers) {
         const Tensor gt = gate.value_or(Tensor()), cb = cbias.value_or(Tensor());
         const auto [s, y, stats] = run(x, branch, gamma, beta, gt, cb, eps, scale, stepwise, true);
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({x, branch, gt, cb, gamma, beta, stats});
+        // In the layers s stays as it is and the next call holds it as its x: without a gate it is all that the
+        // backward needs.  Anyone else may change s in place.
+        if (layers && stepwise && !gt.defined()) ctx->save_for_backward({s, Tensor(), gt, cb, gamma, beta, stats});
+        else ctx->save_for_backward({x, branch, gt, cb, gamma, beta, stats});
         put(ctx, {bits(scale), stepwise});
         return {s, y};
     }
@@ -476,7 +479,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const auto m = meta(ctx);
         const double scale = unbits(m[0]);
         // an output no loss uses has no gradient
-        const Tensor dy = g[1].defined() ? to_bf16(g[1]) : at::zeros(branch.sizes(), branch.options());
+        const Tensor dy = g[1].defined() ? to_bf16(g[1]) : at::zeros(x.sizes(), x.options().dtype(at::kBFloat16));
         if (at::GradMode::is_enabled()) return differentiable(sv, g[0], g[1].defined() ? g[1] : dy, scale);
         const Args a = args(x, branch, gate, cbias);
         const Tensor ds = g[0].defined() ? dense(cast(g[0], x.scalar_type())) : Tensor();
@@ -485,7 +488,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         bool sums = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
         if (biased) sums = sums || ctx->needs_input_grad(gated ? 5 : 4);
         const bool same = a.xt == RWKV6_BF16 && scale == 1. && !gated && !biased;      // d_branch is dx
-        const Tensor dx = at::empty_like(a.x), db = same ? Tensor() : at::empty_like(a.branch);
+        const Tensor dx = at::empty_like(a.x), db = same ? Tensor() : at::empty_like(dy);
         const Tensor dg = gated ? at::empty_like(a.gate) : Tensor();
         const int dt = grad_code(gamma) == grad_code(beta) ? grad_code(gamma) : RWKV6_F32;
         const Tensor dga = sums ? empty({a.C}, param_type(dt), x) : Tensor(), dbe = sums ? at::empty_like(dga) : Tensor();
@@ -496,14 +499,17 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
                                       ptr(dga), ptr(dbe), dt, ptr(dcb), ptr(ws), a.N, a.C, stream_of(x)),
               "rwkv6_residual_norm_bwd");
         return {dx, same ? dx : db, sums ? cast(dga, gamma.scalar_type()) : dga, sums ? cast(dbe, beta.scalar_type()) : dbe, dg,
-                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor(), Tensor()};
+                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor(), Tensor(), Tensor()};
     }
     // A backward that is differentiated itself: the same formulas in torch's operators.
     static variable_list differentiable(const variable_list& sv, const Tensor& ds, const Tensor& dy, double scale) {
         const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2], &cbias = sv[3], &gamma = sv[4], &beta = sv[5];
-        const Tensor f = cbias.defined() ? branch.to(at::kFloat) + cbias.to(at::kFloat) : branch.to(at::kFloat);
-        const Tensor sg = gate.defined() ? at::sigmoid(gate.to(at::kFloat)) : Tensor();
-        const Tensor s = x.to(at::kFloat) + (gate.defined() ? f * sg : f) * scale;
+        Tensor s = x.to(at::kFloat), f, sg;
+        if (branch.defined()) {
+            f = cbias.defined() ? branch.to(at::kFloat) + cbias.to(at::kFloat) : branch.to(at::kFloat);
+            if (gate.defined()) sg = at::sigmoid(gate.to(at::kFloat));
+            s = s + (gate.defined() ? f * sg : f) * scale;
+        }
         std::vector<int64_t> st(x.sizes().begin(), x.sizes().end());
         st.back() = 1;
         auto [dS, dga, dbe] = at::native_layer_norm_backward(dy.to(at::kFloat), s, {x.size(-1)}, sv[6][0].view(st), sv[6][1].view(st),
@@ -512,14 +518,14 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor df = dS * scale, db = gate.defined() ? df * sg : df;
         const Tensor dg = gate.defined() ? (df * f * sg * (1 - sg)).to(gate.scalar_type()) : Tensor();
         const Tensor dcb = cbias.defined() ? db.reshape({-1, x.size(-1)}).sum(0).to(cbias.scalar_type()) : Tensor();
-        return {dS.to(x.scalar_type()), db.to(branch.scalar_type()), dga.to(gamma.scalar_type()), dbe.to(beta.scalar_type()),
-                dg, dcb, Tensor(), Tensor(), Tensor()};
+        return {dS.to(x.scalar_type()), db.to(at::kBFloat16), dga.to(gamma.scalar_type()), dbe.to(beta.scalar_type()),
+                dg, dcb, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
-// None when the kernels do not take the call (only_plain: nor one that a mode or transform wants to see);
+// None when the kernels do not take the call (layers: nor one that a mode or transform wants to see);
 // the callers check and raise, or run torch's operators.
 py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta, double eps,
-                         const OptTensor& gate, const OptTensor& cbias, double scale, bool stepwise, bool only_plain) {
+                         const OptTensor& gate, const OptTensor& cbias, double scale, bool stepwise, bool layers) {
     if (!x.is_cuda() || x.dim() < 1 || x.size(-1) < 1 || x.layout() != at::kStrided ||
         (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat))
         return py::none();
@@ -532,7 +538,7 @@ py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& ga
         if (t->device() != x.device() || t->sizes() != at::IntArrayRef({C}) ||
             (t->scalar_type() != at::kBFloat16 && t->scalar_type() != at::kFloat && t->scalar_type() != at::kHalf))
             return py::none();
-    if (only_plain && !plain({&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})) return py::none();
+    if (layers && !plain({&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})) return py::none();
     no_transforms();
     const c10::DeviceGuard on(x.device());           // the default stream is the current device's
     bool grad = recorded({&x, &branch, &gamma, &beta, gate ? &*gate : &x}, cbias);
@@ -544,7 +550,7 @@ py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& ga
         });
         return py::make_tuple(o[0], o[1]);
     }
-    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, stepwise); });
+    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, stepwise, layers); });
     return py::make_tuple(o[0], o[1]);
 }
 

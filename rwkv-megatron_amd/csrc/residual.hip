@@ -10,7 +10,8 @@
 //   dx = dS, d_branch = scale dS sg, d_gate = scale dS (branch + branch_bias) sg (1 - sg)
 //   dgamma = sum_rows dy xh, dbeta = sum_rows dy, d_branch_bias = sum_rows d_branch (fixed order)
 // s is rounded once, to x's type, on its way out.  The backward forms it again from the inputs: a
-// stored bf16 s would put its rounding, 2^-9 of s, into xh and so into an fp32 dgamma.
+// stored bf16 s would put its rounding, 2^-9 of s, into xh and so into an fp32 dgamma.  Where the norm was taken
+// of the stored s (stepwise, below) and there is no gate, it can take that s in place of x and the branch.
 // `stepwise` gives the numbers of the operators run one by one instead: the sum with the bias, the
 // product with the gate and s are rounded (bf16, bf16, x's type) before the next takes them, y is the
 // norm of s as it is stored, and the gradients are rounded at the same places.  The layers and the
@@ -185,8 +186,9 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
 }
 
 // Steps of RB rows; block p takes `run` of them, then skips the other blocks' runs.  part[p][CB ? 3 : 2][C] = its sums of dgamma, dbeta
-// and d_branch_bias (part null: none).  ds null: zero.  db null: d_branch equals dx, not stored twice.
-template <int NV, bool XF, bool GATE, bool CB>
+// and d_branch_bias (part null: none).  ds null: zero.  db null: d_branch equals dx, not stored twice.  SUM: x is the
+// sum s as the stepwise forward stored it, what its norm was taken of, and the branch is not read.
+template <int NV, bool XF, bool GATE, bool CB, bool SUM>
 __global__ void __launch_bounds__(64 * RN_MAX_WAVES)
 rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt, const float* __restrict__ mean_in,
                                const float* __restrict__ rstd_in, const void* __restrict__ ds,
@@ -209,7 +211,7 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
         }
         if (c[i] < C) {
             load_param8(gamma, pdt, c[i], ga[i]);
-            if constexpr (CB) load_param8(in.cbias, in.cdt, c[i], cb[i]);
+            if constexpr (CB && !SUM) load_param8(in.cbias, in.cdt, c[i], cb[i]);
         }
     }
     int turn = 0;
@@ -232,23 +234,28 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
             for (int j = 0; j < 8; ++j) xh[i][j] = g[i][j] = f[i][j] = sg[i][j] = dS[i][j] = 0.f;
             if (c[i] >= C) continue;
             raw_f32<XF>(w_load<XF>(in.x, row + c[i]), xh[i]);
-            load8(in.branch + row + c[i], f[i]);
+            if constexpr (!SUM) load8(in.branch + row + c[i], f[i]);
             if constexpr (GATE) load8(in.gate + row + c[i], sg[i]);
             load8(dy + row + c[i], g[i]);
             if (ds) raw_f32<XF>(w_load<XF>(ds, row + c[i]), dS[i]);
-            if constexpr (CB) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) f[i][j] += cb[i][j];
-                if (in.stepwise) round8(f[i]);
-            }
-            if constexpr (GATE) sigmoid8(sg[i], in.stepwise);
             float t[8];
+            if constexpr (SUM) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = (GATE ? f[i][j] * sg[i][j] : f[i][j]) * in.scale;
-            if (in.stepwise) round8(t);
+                for (int j = 0; j < 8; ++j) t[j] = xh[i][j];
+            } else {
+                if constexpr (CB) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] += xh[i][j];
-            if (!XF && in.stepwise) round8(t);
+                    for (int j = 0; j < 8; ++j) f[i][j] += cb[i][j];
+                    if (in.stepwise) round8(f[i]);
+                }
+                if constexpr (GATE) sigmoid8(sg[i], in.stepwise);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = (GATE ? f[i][j] * sg[i][j] : f[i][j]) * in.scale;
+                if (in.stepwise) round8(t);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] += xh[i][j];
+                if (!XF && in.stepwise) round8(t);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 xh[i][j] = (t[j] - mean) * rstd;
@@ -453,8 +460,9 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
     const bool sums = dgamma || dbeta, xf = x_dtype == RWKV6_F32, gt = gate != nullptr, cb = branch_bias != nullptr;
     // d_branch is dx itself, and not written, only where the two are the same numbers
     if (N > 0 && !d_branch && (gt || cb || xf || scale != 1.f)) return RWKV6_ERR_INVALID_ARG;
+    // no branch: x is the sum that the stepwise forward stored
     if (!gamma || (!dgamma != !dbeta) || (!d_branch_bias != !(cb && sums)) || (sums && !workspace) ||
-        (N > 0 && (!x || !branch || !mean || !rstd || !dy || !dx || !d_gate != !gt)))
+        (N > 0 && (!x || (!branch && (!stepwise || gt)) || !mean || !rstd || !dy || !dx || !d_gate != !gt)))
         return RWKV6_ERR_INVALID_ARG;
     for (const void* p : {x, branch, branch_bias, gate, gamma, ds, dy, (const void*)dx, (const void*)d_branch,
                           (const void*)d_gate, (const void*)workspace})
@@ -472,10 +480,12 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
     const int64_t M = (cb ? 3 : 2) * C;
     float* part = sums ? (float*)workspace : nullptr;
     if (N > 0) {
-#define RN_CB(NV, X, G) (cb ? rwkv6_residual_norm_bwd_kernel<NV, X, G, true> : rwkv6_residual_norm_bwd_kernel<NV, X, G, false>)
-#define RN_PICK(NV) (xf ? (gt ? RN_CB(NV, true, true) : RN_CB(NV, true, false)) : (gt ? RN_CB(NV, false, true) : RN_CB(NV, false, false)))
+#define RN_CB(NV, X, G, S) (cb ? rwkv6_residual_norm_bwd_kernel<NV, X, G, true, S> : rwkv6_residual_norm_bwd_kernel<NV, X, G, false, S>)
+#define RN_GATE(NV, X) (gt ? RN_CB(NV, X, true, false) : branch ? RN_CB(NV, X, false, false) : RN_CB(NV, X, false, true))
+#define RN_PICK(NV) (xf ? RN_GATE(NV, true) : RN_GATE(NV, false))
         auto k = h.NV == 1 ? RN_PICK(1) : RN_PICK(2);
 #undef RN_PICK
+#undef RN_GATE
 #undef RN_CB
         hipLaunchKernelGGL(k, dim3((unsigned)r.blocks), dim3(64 * h.W * h.RB), sums && h.RB > 1 ? (size_t)M * 4 : 0, stm,
                            RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale, stepwise}, gamma,

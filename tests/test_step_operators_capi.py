@@ -178,3 +178,10 @@ def test_the_stochastic_step_refuses_the_same_calls(pkg):
     assert _step(Other, ws=_p(0x71000008)) == ALIGNMENT and _step(Other, size=1 << 41) == UNSUPPORTED
     with pytest.raises(ValueError, match="rounding"):
         pkg.optim.adamw_step([torch.zeros(4)], [torch.zeros(4)], [torch.zeros(4)], [torch.zeros(4)], torch.zeros(()), lr=1.0, rounding="down")
+
+
+def test_residual_norm_backward_without_a_branch(pkg):
+    """Only where x can be the sum that the forward stored: stepwise, without a gate."""
+    L = pkg._lib.load()
+    for kw in (dict(step=0), dict(step=1, gate=A[11], dg=A[12]), dict(step=1, x=None), dict(step=1, N=0, ws=None)):
+        assert _bwd(L, branch=None, **kw) == INVALID, kw
