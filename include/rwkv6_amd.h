@@ -300,6 +300,13 @@ int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, cons
                             int bias_dtype, const void* gate, float scale, int stepwise,
                             const void* gamma, const void* beta, int param_dtype, float eps, void* s,
                             void* y, float* mean, float* rstd, int64_t N, int64_t C, void* stream);
+/* The same, and gamma_used [C] f32 = gamma (nullable; not written for N = 0): the backward of a gamma that
+ * may have changed by then takes it as its gamma. */
+int rwkv6_residual_norm_train_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias,
+                                  int bias_dtype, const void* gate, float scale, int stepwise,
+                                  const void* gamma, const void* beta, int param_dtype, float eps,
+                                  void* s, void* y, float* mean, float* rstd, float* gamma_used,
+                                  int64_t N, int64_t C, void* stream);
 size_t rwkv6_residual_norm_bwd_workspace_bytes(int64_t N, int64_t C);
 int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias,
                             int bias_dtype, const void* gate, float scale, int stepwise,

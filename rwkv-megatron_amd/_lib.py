@@ -80,6 +80,8 @@ SIGNATURES = {
     "rwkv6_layer_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64] * 2),
     "rwkv6_residual_norm_fwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _int, _vp, _vp, _int, _f32, _vp, _vp, _fp, _fp]
                                 + [_i64] * 2 + [_vp]),
+    "rwkv6_residual_norm_train_fwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _int, _vp, _vp, _int, _f32, _vp, _vp] + [_fp] * 3
+                                      + [_i64] * 2 + [_vp]),
     "rwkv6_residual_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64] * 2),
     "rwkv6_residual_norm_bwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _int, _vp, _int, _fp, _fp] + [_vp] * 7
                                 + [_int, _vp, _vp] + [_i64] * 2 + [_vp]),

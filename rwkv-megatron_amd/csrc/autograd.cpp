@@ -5,9 +5,9 @@
 // cost 40-80 us a direction.
 //
 // Every function keeps no state between calls; tensors whose values it needs again go through
-// save_for_backward (version checks, saved-tensor hooks and checkpointing apply; LayerNorm's
-// backward works on its own copy of a parameter wider than bf16 and keeps the parameters beside it
-// for their types and for a second derivative), kernels run on the current stream of the tensors'
+// save_for_backward (version checks, saved-tensor hooks and checkpointing apply; a norm's
+// backward, LayerNorm's and ResidualNorm's, works on its own copy of a weight wider than bf16 and keeps
+// the parameters beside it for their types and for a second derivative), kernels run on the current stream of the tensors'
 // device, and a call from forward-mode differentiation or a function transform is refused.
 //
 // Mathematics and reference lines: wkv.py, timemix.py, channelmix.py and modules.py, whose
@@ -444,8 +444,9 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         return {dense(x), branch.defined() ? dense(branch) : branch, gate.defined() ? dense(gate) : gate, cbias.defined() ? param(cbias) : Param{cbias, 0},
                 x.scalar_type() == at::kFloat ? RWKV6_F32 : RWKV6_BF16, C ? x.numel() / C : 0, C};
     }
-    // (s, y), and the rows' mean and rstd ([2, N]) where a backward will want them
-    static std::array<Tensor, 3> run(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta,
+    // (s, y), and where a backward will want them the rows' mean and rstd ([2, N]) and a copy of a gamma wider
+    // than bf16, so that an update of the parameter in between is not an error
+    static std::array<Tensor, 4> run(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta,
                                      const Tensor& gate, const Tensor& cbias, double eps, double scale, bool stepwise,
                                      bool grad) {
         const Args a = args(x, branch, gate, cbias);
@@ -453,37 +454,46 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         if (ga.dt != be.dt) ga = {to_f32(gamma), RWKV6_F32}, be = {to_f32(beta), RWKV6_F32};
         const Tensor s = at::empty_like(a.x), y = at::empty_like(a.branch);
         const Tensor stats = grad ? empty({2, a.N}, at::kFloat, x) : Tensor();
+        const Tensor used = grad && gamma.scalar_type() != at::kBFloat16 ? empty({a.C}, at::kFloat, x) : Tensor();
         float* const mean = fptr(stats);
-        check(rwkv6_residual_norm_fwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
-                                      stepwise, ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), mean, mean ? mean + a.N : nullptr,
-                                      a.N, a.C, stream_of(x)),
-              "rwkv6_residual_norm_fwd");
-        return {s, y, stats};
+        check(rwkv6_residual_norm_train_fwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
+                                            stepwise, ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), mean,
+                                            mean ? mean + a.N : nullptr, fptr(used), a.N, a.C, stream_of(x)),
+              "rwkv6_residual_norm_train_fwd");
+        return {s, y, stats, used};
     }
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& branch, const Tensor& gamma,
                                  const Tensor& beta, const OptTensor& gate, const OptTensor& cbias, double eps,
                                  double scale, bool stepwise, bool layers) {
         const Tensor gt = gate.value_or(Tensor()), cb = cbias.value_or(Tensor());
-        const auto [s, y, stats] = run(x, branch, gamma, beta, gt, cb, eps, scale, stepwise, true);
+        const auto [s, y, stats, used] = run(x, branch, gamma, beta, gt, cb, eps, scale, stepwise, true);
+        const Tensor& ga = used.defined() ? used : gamma;
         ctx->set_materialize_grads(false);
         // In the layers s stays as it is and the next call holds it as its x: without a gate it is all that the
         // backward needs.  Anyone else may change s in place.
-        if (layers && stepwise && !gt.defined()) ctx->save_for_backward({s, Tensor(), gt, cb, gamma, beta, stats});
-        else ctx->save_for_backward({x, branch, gt, cb, gamma, beta, stats});
+        const bool sum = layers && stepwise && !gt.defined();
+        if (sum) ctx->save_for_backward({s, Tensor(), gt, Tensor(), ga, stats});
+        else ctx->save_for_backward({x, branch, gt, cb, ga, stats});
+        // of these the backward wants the types, and in the second derivative the nodes
+        if (used.defined()) ctx->saved_data["gamma"] = gamma;
+        if (sum && cb.defined()) ctx->saved_data["bias"] = cb;
+        ctx->saved_data["beta"] = beta;
         put(ctx, {bits(scale), stepwise});
         return {s, y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const auto sv = ctx->get_saved_variables();
-        const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2], &cbias = sv[3], &gamma = sv[4], &beta = sv[5];
+        const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2];
+        const auto kept = [&](const char* key, const Tensor& t) { return ctx->saved_data.count(key) ? ctx->saved_data[key].toTensor() : t; };
+        const Tensor cbias = kept("bias", sv[3]), gamma = kept("gamma", sv[4]), beta = kept("beta", Tensor());
         const auto m = meta(ctx);
         const double scale = unbits(m[0]);
         // an output no loss uses has no gradient
         const Tensor dy = g[1].defined() ? to_bf16(g[1]) : at::zeros(x.sizes(), x.options().dtype(at::kBFloat16));
-        if (at::GradMode::is_enabled()) return differentiable(sv, g[0], g[1].defined() ? g[1] : dy, scale);
+        if (at::GradMode::is_enabled()) return differentiable(sv, cbias, gamma, beta, g[0], g[1].defined() ? g[1] : dy, scale);
         const Args a = args(x, branch, gate, cbias);
         const Tensor ds = g[0].defined() ? dense(cast(g[0], x.scalar_type())) : Tensor();
-        const Param ga = param(gamma);
+        const Param ga = param(sv[4]);
         const bool gated = gate.defined(), biased = cbias.defined();
         bool sums = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
         if (biased) sums = sums || ctx->needs_input_grad(gated ? 5 : 4);
@@ -495,15 +505,18 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor dcb = sums && biased ? empty({a.C}, a.cbias.t.scalar_type(), x) : Tensor();
         const Tensor ws = sums ? bytes(rwkv6_residual_norm_bwd_workspace_bytes(a.N, a.C), x) : Tensor();
         check(rwkv6_residual_norm_bwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
-                                      (int)m[1], ptr(ga.t), ga.dt, fptr(sv[6]), a.N ? fptr(sv[6]) + a.N : nullptr, ptr(ds), ptr(dy), ptr(dx), ptr(db), ptr(dg),
+                                      (int)m[1], ptr(ga.t), ga.dt, fptr(sv[5]), a.N ? fptr(sv[5]) + a.N : nullptr, ptr(ds), ptr(dy), ptr(dx), ptr(db), ptr(dg),
                                       ptr(dga), ptr(dbe), dt, ptr(dcb), ptr(ws), a.N, a.C, stream_of(x)),
               "rwkv6_residual_norm_bwd");
         return {dx, same ? dx : db, sums ? cast(dga, gamma.scalar_type()) : dga, sums ? cast(dbe, beta.scalar_type()) : dbe, dg,
                 dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor(), Tensor(), Tensor()};
     }
     // A backward that is differentiated itself: the same formulas in torch's operators.
-    static variable_list differentiable(const variable_list& sv, const Tensor& ds, const Tensor& dy, double scale) {
-        const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2], &cbias = sv[3], &gamma = sv[4], &beta = sv[5];
+    static variable_list differentiable(const variable_list& sv, const Tensor& cbias, const Tensor& gamma, const Tensor& beta,
+                                        const Tensor& ds, const Tensor& dy, double scale) {
+        const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2];
+        // the values that the forward used
+        const Tensor ga = gamma.is_same(sv[4]) ? gamma : gamma + (sv[4].to(gamma.scalar_type()) - gamma).detach();
         Tensor s = x.to(at::kFloat), f, sg;
         if (branch.defined()) {
             f = cbias.defined() ? branch.to(at::kFloat) + cbias.to(at::kFloat) : branch.to(at::kFloat);
@@ -512,8 +525,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         }
         std::vector<int64_t> st(x.sizes().begin(), x.sizes().end());
         st.back() = 1;
-        auto [dS, dga, dbe] = at::native_layer_norm_backward(dy.to(at::kFloat), s, {x.size(-1)}, sv[6][0].view(st), sv[6][1].view(st),
-                                                             gamma.to(at::kFloat), beta.to(at::kFloat), {true, true, true});
+        auto [dS, dga, dbe] = at::native_layer_norm_backward(dy.to(at::kFloat), s, {x.size(-1)}, sv[5][0].view(st), sv[5][1].view(st),
+                                                             ga.to(at::kFloat), beta.to(at::kFloat), {true, true, true});
         if (ds.defined()) dS = dS + ds.to(at::kFloat);
         const Tensor df = dS * scale, db = gate.defined() ? df * sg : df;
         const Tensor dg = gate.defined() ? (df * f * sg * (1 - sg)).to(gate.scalar_type()) : Tensor();

@@ -109,8 +109,8 @@ template <int NV, bool XF, bool GATE, bool CB>
 __global__ void __launch_bounds__(64 * RN_MAX_WAVES)
 rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const void* __restrict__ beta, int pdt,
                                float eps, void* __restrict__ s, uint16_t* __restrict__ y,
-                               float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t N, int C, int W,
-                               int RB, bool nt) {
+                               float* __restrict__ mean_out, float* __restrict__ rstd_out, float* __restrict__ gamma_used,
+                               int64_t N, int C, int W, int RB, bool nt) {
     __shared__ float red[2][RN_MAX_WAVES];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, gr = wv / W, w = wv - gr * W;
     const float inv = 1.f / (float)C;
@@ -123,6 +123,8 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
             load_param8(gamma, pdt, c[i], ga[i]);
             load_param8(beta, pdt, c[i], be[i]);
             if constexpr (CB) load_param8(in.cbias, in.cdt, c[i], cb[i]);
+            // for a backward after gamma has changed
+            if (gamma_used && blockIdx.x == 0 && gr == 0) store8_as<true>(gamma_used, c[i], ga[i]);
         }
     }
     for (int64_t b0 = (int64_t)blockIdx.x * RB; b0 < N; b0 += (int64_t)gridDim.x * RB) {
@@ -408,24 +410,20 @@ inline RnRuns rn_runs(int64_t N, int RB, bool gate) {
     const int64_t b = half < 1 ? 1 : half < RN_BLOCKS ? half : RN_BLOCKS, run = (steps + b - 1) / b;
     return {b, (int)(run < 1 ? 1 : run)};
 }
-}  // namespace
-
-extern "C" {
-
-int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
-                            const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
-                            int param_dtype, float eps, void* s, void* y, float* mean, float* rstd, int64_t N, int64_t C, void* stream) {
+int rn_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype, const void* gate,
+           float scale, int stepwise, const void* gamma, const void* beta, int param_dtype, float eps, void* s, void* y,
+           float* mean, float* rstd, float* gamma_used, int64_t N, int64_t C, void* stream) {
     const int st = rn_check(N, C);
     if (st) return st;
     if (!dt_ok(x_dtype) || !dt_ok(param_dtype) || (branch_bias && !dt_ok(bias_dtype)) || (!mean != !rstd))
         return RWKV6_ERR_INVALID_ARG;
     if (N == 0) return RWKV6_OK;
     if (!x || !branch || !gamma || !beta || !s || !y) return RWKV6_ERR_INVALID_ARG;
-    for (const void* p : {x, branch, branch_bias, gate, gamma, beta, (const void*)s, (const void*)y})
+    for (const void* p : {x, branch, branch_bias, gate, gamma, beta, (const void*)s, (const void*)y, (const void*)gamma_used})
         if (!al16(p)) return RWKV6_ERR_ALIGNMENT;
     const size_t act = (size_t)(N * C) * 2, xs = (size_t)(N * C) * param_bytes(x_dtype), st4 = (size_t)N * 4;
     const size_t par = (size_t)C * param_bytes(param_dtype);
-    if (any_alias({{s, xs}, {y, act}, {mean, st4}, {rstd, st4}},
+    if (any_alias({{s, xs}, {y, act}, {mean, st4}, {rstd, st4}, {gamma_used, (size_t)C * 4}},
                   {{x, xs}, {branch, act}, {branch_bias, (size_t)C * param_bytes(bias_dtype)}, {gate, act}, {gamma, par}, {beta, par}}))
         return RWKV6_ERR_INVALID_ARG;
     const RnShape h = rn_shape(C);
@@ -439,8 +437,26 @@ int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, cons
     hipLaunchKernelGGL(k, dim3((unsigned)(blocks < RN_FWD_BLOCKS ? blocks : RN_FWD_BLOCKS)), dim3(64 * h.W * h.RB), 0,
                        reinterpret_cast<hipStream_t>(stream),
                        RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale, stepwise}, gamma, beta,
-                       param_dtype, eps, s, (uint16_t*)y, mean, rstd, N, (int)C, h.W, h.RB, rn_stream(N, C));
+                       param_dtype, eps, s, (uint16_t*)y, mean, rstd, gamma_used, N, (int)C, h.W, h.RB, rn_stream(N, C));
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+}
+}  // namespace
+
+extern "C" {
+
+int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
+                            const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
+                            int param_dtype, float eps, void* s, void* y, float* mean, float* rstd, int64_t N, int64_t C, void* stream) {
+    return rn_fwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, beta, param_dtype, eps, s, y, mean, rstd,
+                  nullptr, N, C, stream);
+}
+
+int rwkv6_residual_norm_train_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
+                                  const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
+                                  int param_dtype, float eps, void* s, void* y, float* mean, float* rstd,
+                                  float* gamma_used, int64_t N, int64_t C, void* stream) {
+    return rn_fwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, beta, param_dtype, eps, s, y, mean, rstd,
+                  gamma_used, N, C, stream);
 }
 
 size_t rwkv6_residual_norm_bwd_workspace_bytes(int64_t N, int64_t C) {

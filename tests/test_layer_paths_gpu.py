@@ -128,3 +128,40 @@ def test_the_sum_of_a_public_call_may_be_changed_in_place(pkg):
         s, y = call()
         s.add_(1)
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad((s, y), list(t.values()), (ds, dy)), want))
+
+
+# A norm's backward uses the parameters that its forward saw; one of them changed in between (fp32, so the
+# kernels of the separate norm worked on a copy) is not an error.
+@pytest.mark.parametrize("bias", [False, True])
+def test_a_norm_changed_between_forward_and_backward(pkg, bias):
+    model, (tokens, labels) = _model(pkg, bias=bias), _batch()
+    norms = [m for m in model.modules() if isinstance(m, pkg.modules.LayerNorm)]
+    want = _grads(model, model(tokens, labels).mean())
+    loss = model(tokens, labels).mean()
+    with torch.no_grad():
+        for n in norms:
+            n.weight.mul_(2)
+            n.bias.add_(1)
+    for (n, a), b in zip(_grads(model, loss).items(), want.values()):
+        assert torch.equal(a, b), n
+
+
+# The same of the public call, in every type of a norm's parameters; a bf16 weight is held itself, as LayerNorm holds it.
+@pytest.mark.parametrize("param", [torch.float32, torch.float16, BF])
+@pytest.mark.parametrize("N,C", [(5, 64), (3, 2056), (2, 8192), (700, 512)])
+def test_the_public_norm_changed_between_forward_and_backward(pkg, param, N, C):
+    t, ds, dy = _inputs((N,), C, BF, param, True, False)
+    call = lambda: pkg.residual.residual_norm(t["x"], t["branch"], t["weight"], t["bias"], EPS, gate=t["gate"])
+    want = torch.autograd.grad(call(), list(t.values()), (ds, dy))
+    out = call()
+    with torch.no_grad():
+        t["bias"].add_(1)
+        if param != BF:
+            t["weight"].mul_(2)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, list(t.values()), (ds, dy)), want))
+    out = call()
+    with torch.no_grad():
+        t["weight"].mul_(2)
+    if param == BF:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, list(t.values()), (ds, dy))

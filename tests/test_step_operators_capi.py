@@ -185,3 +185,18 @@ def test_residual_norm_backward_without_a_branch(pkg):
     L = pkg._lib.load()
     for kw in (dict(step=0), dict(step=1, gate=A[11], dg=A[12]), dict(step=1, x=None), dict(step=1, N=0, ws=None)):
         assert _bwd(L, branch=None, **kw) == INVALID, kw
+
+
+def test_residual_norm_for_training_refuses_a_bad_copy_of_gamma(pkg):
+    L = pkg._lib.load()
+
+    def call(used, **kw):
+        a = dict(x=A[0], xt=BF16, branch=A[1], cb=None, cbt=F32, gate=None, scale=1.0, step=0, gamma=A[2], beta=A[3], pt=F32,
+                 eps=1e-5, s=A[4], y=A[5], mean=A[6], rstd=A[7], used=used, N=4, C=64, stream=None)
+        a.update(kw)
+        return L.rwkv6_residual_norm_train_fwd(*a.values())
+
+    assert call(A[8], N=0) == OK == call(None, N=0)
+    for used in (A[2], A[5], _p(0x40000000 - 16), A[7]):
+        assert call(used) == INVALID, used
+    assert call(_p(0x90000008)) == ALIGNMENT and call(A[8], C=12) == UNSUPPORTED
