@@ -116,3 +116,35 @@ def test_states_of_32_bits_and_refusals(opt):
     with pytest.raises(ValueError, match="rounding"):
         _call(opt, t, rounding="up")
     assert float(t["step"]) == 7
+
+
+# Step by step: every step of the optimizer is the formula's from the moments that it holds, so that a moment lost, negated
+# or scaled between two steps shows (each would move p by a good part of lr; the bound is 2^-20 of the step, as in
+# test_optim_gpu.py, and a rounding of p).
+@pytest.mark.parametrize("bits", [8, 32])
+def test_every_step_is_the_formula_of_the_moments_held(opt, bits):
+    g = torch.Generator(device=DEV).manual_seed(4)
+    ps = [torch.nn.Parameter(torch.randn(n, generator=g, device=DEV) * 0.1) for n in (5000, 100, 4096)]
+    o = opt.AdamW(ps, **HYPER, state_bits=bits)
+    lr, (b1, b2), eps, wd = HYPER["lr"], HYPER["betas"], HYPER["eps"], HYPER["weight_decay"]
+    held = [(torch.zeros_like(p, dtype=torch.float64),) * 2 for p in ps]
+    for k in range(1, 6):
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g, device=DEV) * 0.02
+        before = [p.detach().double() for p in ps]
+        o.step()
+        for i, p in enumerate(ps):
+            m, v = held[i]
+            gr = p.grad.double()
+            m, v = b1 * m + (1 - b1) * gr, b2 * v + (1 - b2) * gr * gr
+            u = lr / (1 - b1 ** k) * m / ((v / (1 - b2 ** k)).sqrt() + eps)
+            want = before[i] * (1 - lr * wd) - u
+            # m itself takes roundings of its two terms, which may cancel
+            slack = lr / (1 - b1 ** k) * 2.0 ** -22 * (held[i][0].abs() + gr.abs()) / ((v / (1 - b2 ** k)).sqrt() + eps)
+            assert bool(((p.detach().double() - want).abs() <= 2.0 ** -20 * u.abs() + 2.0 ** -22 * want.abs() + slack).all()), (k, i)
+            now = [t.double() for t in o.moments(p)]
+            if bits == 8 and p.numel() >= 4096:
+                for got, exact, name in ((now[0], m, "exp_avg_scale"), (now[1].sqrt(), v.sqrt(), "exp_avg_sq_scale")):
+                    unit = o.state[p][name].double().repeat_interleave(256)[:p.numel()]
+                    assert bool(((got - exact).abs() <= 1.001 * _gap(exact, unit) + 2.0 ** -18 * unit).all()), (k, i, name)
+            held[i] = now

@@ -200,3 +200,10 @@ def test_residual_norm_for_training_refuses_a_bad_copy_of_gamma(pkg):
     for used in (A[2], A[5], _p(0x40000000 - 16), A[7]):
         assert call(used) == INVALID, used
     assert call(_p(0x90000008)) == ALIGNMENT and call(A[8], C=12) == UNSUPPORTED
+
+
+def test_the_partial_sums_of_the_largest_call(pkg):
+    """768 blocks' sums of three rows of C."""
+    L = pkg._lib.load()
+    for C in (1024, 2048, 4096, 8192):
+        assert L.rwkv6_residual_norm_bwd_workspace_bytes(1 << 20, C) == 768 * 3 * C * 4 == L.rwkv6_residual_norm_bwd_workspace_bytes(1 << 27, C)
