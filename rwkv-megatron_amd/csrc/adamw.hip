@@ -29,7 +29,7 @@
 // Bound by memory: bytes a parameter 22 (bf16 p and g, fp32 states), 28 (all fp32), 10 and 16 with
 // 8-bit states, and once more the gradient where it is clipped.  Four layers of 2048 channels (218 M
 // bf16 parameters in 92 tensors): norm 90 us (4.9 TB/s), step 883 us (5.4 TB/s), with 8-bit states 401 us
-// (5.5 TB/s), and 95 us more with codes right on average, whose arithmetic the bytes no longer hide (fp32
+// (5.5 TB/s), and 66 us more with codes right on average, whose arithmetic the bytes no longer hide (fp32
 // parameters: the same time); two layers of 512 (7.3 M fp32): 7 + 5 + 34 us, the 5 the one block that forms the norm and
 // the coefficients.  A copy of 2 GiB reaches 4.9 TB/s.  torch's operators in 32 bits on the same
 // parameters as one tensor take 8.0 ms, 11.7 ms and 313 us.  Tried and left: the step's loads past the
@@ -202,15 +202,15 @@ __device__ __forceinline__ uint32_t aw_seed(float t, int64_t i, float g) {
 // numbers lo < hi around a value a: m up with probability (a - lo) / (hi - lo), a right on average, a root with
 // (a^2 - lo^2) / (hi^2 - lo^2), its square right on average.  The values lie below 448 (see AW_F8_BELOW); one
 // that is not finite becomes NaN.  Below 2^-6 the numbers lie 2^-9 apart, as from 2^-6 to 2^-5: `off` moves a
-// value there.  32 bits an element, the low 18 for the root, the 20 above the twelfth for m, whose weight lies
-// in the other 14.
+// value there.  An e4m3 number has the low 20 bits of a float zero.  32 random bits an element, m's from the
+// top, the root's from the 23rd.
 __device__ __forceinline__ void aw_encode_either(const float* m, float im, const float* root, float iv, uint32_t h, uint2* cm,
                                                  uint2* cv) {
     float qm[8], qv[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         h += 0x9E3779B9u;
-        const uint32_t r = (h ^ h >> 15) * 0xD1D5F3A5u;
+        const uint32_t r = __umul24(h ^ h >> 15, 0xD1D5F3u);
         {
             // the carry of the random bits below the code's last one
             const float a = fabsf(m[j]) * im, off = a < 0x1p-6f ? 0x1p-6f : 0.f;
@@ -219,9 +219,10 @@ __device__ __forceinline__ void aw_encode_either(const float* m, float im, const
         {
             const float a = root[j] * iv, off = a < 0x1p-6f ? 0x1p-6f : 0.f;
             const uint32_t b = __float_as_uint(a + off) & 0xfff00000u;
-            const float gap = __uint_as_float((b & 0x7f800000u) - (3u << 23)), lo = __uint_as_float(b) - off, hi = lo + gap;
-            const float u = (float)(r & 0x3ffffu) * 0x1p-18f;
-            qv[j] = u * (gap * (hi + lo)) < (a - lo) * (a + lo) ? hi : lo;
+            const float lo = __uint_as_float(b) - off, hi = __uint_as_float(b + 0x100000u) - off;
+            const float low2 = lo * lo, all = fmaf(hi, hi, -low2);
+            const float u1 = __uint_as_float((r & 0x7fffffu) | 0x3f800000u);          // 1 + u
+            qv[j] = fmaf(u1, all, -all) < fmaf(a, a, -low2) ? hi : lo;
         }
     }
     *cm = aw_encode(qm, 1.f);
