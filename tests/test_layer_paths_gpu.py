@@ -4,6 +4,7 @@ import importlib
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from test_residual_gpu import EPS, _inputs
 from test_train_step_gpu import _batch, _grads, _model
@@ -165,3 +166,37 @@ def test_the_public_norm_changed_between_forward_and_backward(pkg, param, N, C):
     if param == BF:
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(out, list(t.values()), (ds, dy))
+
+
+# The saved sum is an output of its own node: offloaded, checkpointed, used twice, and freed with the graph.
+def test_offloading_checkpoints_and_two_backwards(pkg):
+    layer, x = _layer(pkg, True)
+    leaves = [x, *layer.parameters()]
+    grads = lambda y, **kw: torch.autograd.grad(y.float().square().mean(), leaves, **kw)
+    want = grads(layer(x))
+    same = lambda got: all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(DEV)):
+        y = layer(x)
+    assert same(grads(y))
+    assert same(grads(torch.utils.checkpoint.checkpoint(layer, x, use_reentrant=False)))
+    y = layer(x)
+    assert same(grads(y, retain_graph=True)) and same(grads(y))
+    with pytest.raises(RuntimeError, match="second time"):
+        grads(y)
+
+
+def test_a_graph_without_a_backward_is_freed(pkg):
+    model, (tokens, labels) = _model(pkg), _batch()
+    model(tokens, labels)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    for _ in range(3):
+        loss = model(tokens, labels)
+        assert torch.cuda.memory_allocated() > held
+        del loss
+        assert torch.cuda.memory_allocated() == held
+    loss = model(tokens, labels).mean()
+    loss.backward()
+    model.zero_grad(set_to_none=True)
+    del loss
+    assert torch.cuda.memory_allocated() == held
