@@ -29,9 +29,9 @@
 // Bound by memory: bytes a parameter 22 (bf16 p and g, fp32 states), 28 (all fp32), 10 and 16 with
 // 8-bit states, and once more the gradient where it is clipped.  Four layers of 2048 channels (218 M
 // bf16 parameters in 92 tensors): norm 90 us (4.9 TB/s), step 883 us (5.4 TB/s), with 8-bit states 401 us
-// (5.5 TB/s), and 66 us more with codes right on average, whose arithmetic the bytes no longer hide (fp32
-// parameters: the same time); two layers of 512 (7.3 M fp32): 7 + 5 + 34 us, the 5 the one block that forms the norm and
-// the coefficients.  A copy of 2 GiB reaches 4.9 TB/s.  torch's operators in 32 bits on the same
+// (5.5 TB/s), with codes right on average 465 us, whose arithmetic the bytes no longer hide (55 M fp32 parameters
+// 160 us either way); two layers of 512 (7.3 M fp32): 7 + 5 + 34 us, the 5 the one block that forms the norm and
+// the coefficients.  A sum of two 1 GiB tensors reaches 6.1 TB/s.  torch's operators in 32 bits on the same
 // parameters as one tensor take 8.0 ms, 11.7 ms and 313 us.  Tried and left: the step's loads past the
 // caches (499 us instead of 457 for 109 M parameters) and its stores (the same), the norm's sums of eight
 // squares in 32 bits (the same), the tensors in reverse so that the norm's last ones are still cached
@@ -44,7 +44,7 @@
 
 #define AW_THR 256
 #define AW_STEP (8 * AW_THR)    // elements a block takes at once
-#define AW_PARTS 8192           // blocks of the norm's sums, at about
+#define AW_PARTS 8192           // blocks of the norm's sums, at about; below 50 M elements some of them have no run
 #define AW_AHEAD 4              // steps of the norm's loads in flight
 #define AW_RUN (AW_AHEAD * AW_STEP)
 #define AW_T 60                 // tensors a launch: the arguments stay below 4 KB

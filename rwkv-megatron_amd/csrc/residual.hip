@@ -20,8 +20,9 @@
 //
 // Bound by memory: bytes an element in bf16 8 forward (10 gated), 10 backward (16 gated).  16384 x 2048
 // forward and backward 106 us (kernels 47 + 57, and 4 for the parameters' sums), gated 160 us (56 + 101 +
-// 4): 5.7 and 5.4 TB/s of those bytes, where a copy of 2 GiB reaches 4.9; torch's operators in 32 bits take
-// 1300 and 1950.  Few rows are bound by the launches (8 rows of 2048: 4 us of kernel, 10 a call).
+// 4): 5.7 and 5.4 TB/s of those bytes, where a sum of two 1 GiB tensors reaches 6.1; torch's operators in 32
+// bits take 1300 and 1950.  Stepwise, the layers' form: 110 to 114 us (51, 59 from the stored sum, 5), gated 167
+// (61 + 103 + 5).  Few rows are bound by the launches (8 rows of 2048: 4 us of kernel, 10 a call).
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 
@@ -65,7 +66,8 @@ __device__ __forceinline__ void store8_as(void* p, int64_t off, const float* f, 
     }
 }
 // sigmoid of eight values.  `near`: the reciprocal with a Newton step, as near as the separate operator's
-// division; without, the hardware's to 2^-23 (gated forward of 16384 x 2048 57 us, 66 with the step).
+// division; without, the hardware's to 2^-23 (gated forward of 16384 x 2048 56 us, 61 with the step and the other
+// roundings of `stepwise`).
 __device__ __forceinline__ void sigmoid8(float* g, bool near) {
     float x[8];
 #pragma unroll
