@@ -412,6 +412,41 @@ int rwkv6_wkv_bwd_ex(const void* r, const void* k, const void* v, const void* w,
                      int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, float scale,
                      void* stream, void* const* phase_events);
 
+/* ------------------------------------------------------------------------
+ * The gated delta rule, a recurrent mixer beside WKV6 (no counterpart in the reference):
+ *   S' = e^g S,  e = v - S'^T k,  S = S' + beta k e^T,  o = scale S^T q        (a token of a head)
+ *   q, k : [B,H,T,K] bf16;  v : [B,HV,T,V] bf16;  HV a multiple of H, value head h reads key head h / (HV/H)
+ *   g    : [B,HV,T] f32, the log decay (at most 0 for a bounded state);  beta [B,HV,T] in beta_dtype
+ *   h0, hT : [B,HV,K,V] f32, each nullable;  o : [B,HV,T,V] bf16
+ * K is 64 or 128, V a multiple of 64 up to 512, T >= 0.  q, k, v (and d_o) may be strided: `strides` is a host
+ * array of three element strides (sequence, head, token) for each of them in turn, multiples of 8; their
+ * channels are adjacent.  Everything else is dense.
+ * `saved` (rwkv6_gated_delta_saved_bytes) receives what the backward reads; NULL when none follows, and then
+ * `workspace` (rwkv6_gated_delta_workspace_bytes, for_bwd 0) is used.  bwd: gradients of losses on o (d_o) and on
+ * the final state (dhT, nullable); dq, dk [B,H,T,K] (the sums over the value heads of a key head), dv [B,HV,T,V]
+ * bf16, dg f32, dbeta in beta_dtype [B,HV,T], dh0 f32 nullable.
+ * hT, dh0, dg and dbeta have the precision of 32-bit arithmetic.
+ * step: the same for a few tokens, `state` [B,HV,K,V] f32 updated where it lies: state_strides are a sequence's
+ * and a head's (multiples of 4); states that overlap each other are refused.
+ * A caller that captures a call into a graph makes one eager call of fwd on the device first.
+ * ---------------------------------------------------------------------- */
+size_t rwkv6_gated_delta_saved_bytes(int64_t B, int64_t HV, int64_t T, int64_t K, int64_t V);
+size_t rwkv6_gated_delta_workspace_bytes(int64_t B, int64_t HV, int64_t T, int64_t K, int64_t V,
+                                         int for_bwd);
+int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
+                          const float* g, const void* beta, int beta_dtype, const float* h0, void* o,
+                          float* hT, void* saved, void* workspace, int64_t B, int64_t H, int64_t HV,
+                          int64_t T, int64_t K, int64_t V, float scale, void* stream);
+int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const void* d_o,
+                          const int64_t* strides, const void* beta, int beta_dtype, const float* dhT,
+                          const void* saved, void* dq, void* dk, void* dv, float* dg, void* dbeta,
+                          float* dh0, void* workspace, int64_t B, int64_t H, int64_t HV, int64_t T,
+                          int64_t K, int64_t V, float scale, void* stream);
+int rwkv6_gated_delta_step(const void* q, const void* k, const void* v, const int64_t* strides,
+                           const float* g, const void* beta, int beta_dtype, float* state,
+                           const int64_t* state_strides, void* o, int64_t B, int64_t H, int64_t HV,
+                           int64_t T, int64_t K, int64_t V, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

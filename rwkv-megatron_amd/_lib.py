@@ -92,6 +92,11 @@ SIGNATURES = {
     "rwkv6_grad_norm": (_int, [_vp, _i64, _fp, _vp]),
     "rwkv6_adamw_step": (_int, [_vp] * 9 + [_i64, _fp, _f64, _fp] + [_f64] * 4 + [_vp, _i64, _f32, _fp, _vp, _vp]),
     "rwkv6_adamw_step_stochastic": (_int, [_vp] * 9 + [_i64, _fp, _f64, _fp] + [_f64] * 4 + [_vp, _i64, _f32, _fp, _vp, _vp]),
+    "rwkv6_gated_delta_saved_bytes": (ctypes.c_size_t, [_i64] * 5),
+    "rwkv6_gated_delta_workspace_bytes": (ctypes.c_size_t, [_i64] * 5 + [_int]),
+    "rwkv6_gated_delta_fwd": (_int, [_vp] * 4 + [_fp, _vp, _int, _fp, _vp, _fp, _vp, _vp] + [_i64] * 6 + [_f32, _vp]),
+    "rwkv6_gated_delta_bwd": (_int, [_vp] * 6 + [_int, _fp] + [_vp] * 4 + [_fp, _vp, _fp, _vp] + [_i64] * 6 + [_f32, _vp]),
+    "rwkv6_gated_delta_step": (_int, [_vp] * 4 + [_fp, _vp, _int, _fp, _vp, _vp] + [_i64] * 6 + [_f32, _vp]),
     "rwkv6_layer_norm_bwd": (_int, [_vp, _vp, _int, _fp, _fp] + [_vp] * 4 + [_int, _vp] + [_i64] * 2 + [_vp]),
 }
 

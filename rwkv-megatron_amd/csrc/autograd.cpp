@@ -209,6 +209,133 @@ py::tuple wkv6_seqfirst(const Tensor& r, const Tensor& k, const Tensor& v, const
 }
 
 // ---------------------------------------------------------------------------------------
+// The gated delta rule (q, k [B,H,T,K]; v [B,HV,T,V]; g, beta [B,HV,T])
+// ---------------------------------------------------------------------------------------
+// A tensor as those kernels read it: bf16, its channels adjacent, the other strides as they are where they
+// are multiples of 8 (a view of a projection's output is read where it lies).
+struct Strided {
+    Tensor t;
+    std::array<int64_t, 3> s;
+};
+Strided strided(const Tensor& x) {
+    Tensor t = cast(x, at::kBFloat16);
+    const auto fits = [](const Tensor& y) {
+        for (int64_t d = 0; d < 3; ++d)
+            if (y.size(d) > 1 && y.stride(d) % 8) return false;
+        return (y.size(3) == 1 || y.stride(3) == 1) && reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0;
+    };
+    if (!fits(t)) t = dense(t);
+    std::array<int64_t, 3> s;
+    for (int64_t d = 0; d < 3; ++d) s[d] = t.size(d) > 1 ? t.stride(d) : 0;
+    return {t, s};
+}
+template <size_t N> std::array<int64_t, 3 * N> all_strides(const std::array<const Strided*, N>& ts) {
+    std::array<int64_t, 3 * N> s;
+    for (size_t i = 0; i < N; ++i) std::copy(ts[i]->s.begin(), ts[i]->s.end(), s.begin() + 3 * i);
+    return s;
+}
+
+struct GatedDelta : torch::autograd::Function<GatedDelta> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                 const Tensor& beta, const OptTensor& h0, double scale, bool final_state, bool grad) {
+        const int64_t B = q.size(0), H = q.size(1), T = q.size(2), K = q.size(3), HV = v.size(1), V = v.size(3);
+        const Strided qs = strided(q), ks = strided(k), vs = strided(v);
+        const Tensor gf = to_f32(g);
+        const Param be = param(beta);
+        const bool state = h0.has_value() && h0->defined();
+        const Tensor h0f = state ? to_f32(*h0) : Tensor();
+        const Tensor saved = grad ? bytes(rwkv6_gated_delta_saved_bytes(B, HV, T, K, V), gf) : Tensor();
+        const Tensor work = grad ? Tensor() : bytes(rwkv6_gated_delta_workspace_bytes(B, HV, T, K, V, 0), gf);
+        const Tensor o = empty({B, HV, T, V}, at::kBFloat16, gf);
+        const Tensor hT = final_state ? empty({B, HV, K, V}, at::kFloat, gf) : Tensor();
+        const auto st = all_strides<3>({&qs, &ks, &vs});
+        check(rwkv6_gated_delta_fwd(ptr(qs.t), ptr(ks.t), ptr(vs.t), st.data(), fptr(gf), ptr(be.t), be.dt, fptr(h0f), ptr(o),
+                                    fptr(hT), ptr(saved), ptr(work), B, H, HV, T, K, V, (float)scale, stream_of(gf)),
+              "rwkv6_gated_delta_fwd");
+        if (grad) {
+            ctx->set_materialize_grads(false);
+            ctx->save_for_backward({qs.t, ks.t, vs.t, be.t, saved});
+            put(ctx, {bits(scale), be.dt, state, code(q), code(k), code(v), code(g), code(beta), state ? code(*h0) : 0});
+        }
+        const Tensor out = cast(o, v.scalar_type());
+        if (final_state) return {out, hT};
+        return {out};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list gr) {
+        if (at::GradMode::is_enabled())
+            C10_THROW_ERROR(NotImplementedError, "the gated delta rule's backward cannot be differentiated (create_graph=True)");
+        const auto s = ctx->get_saved_variables();
+        const auto m = meta(ctx);
+        const Strided qs = strided(s[0]), ks = strided(s[1]), vs = strided(s[2]);
+        const Tensor &be = s[3], &saved = s[4];
+        const int64_t B = qs.t.size(0), H = qs.t.size(1), T = qs.t.size(2), K = qs.t.size(3), HV = vs.t.size(1), V = vs.t.size(3);
+        // an output no loss uses has no gradient: zeros for o, nothing for the final state
+        const Strided os = strided(gr[0].defined() ? gr[0] : at::zeros({B, HV, T, V}, vs.t.options()));
+        const Tensor dht = gr.size() > 1 && gr[1].defined() ? to_f32(gr[1]) : Tensor();
+        const Tensor dq = empty({B, H, T, K}, at::kBFloat16, be), dk = at::empty_like(dq), dv = empty({B, HV, T, V}, at::kBFloat16, be);
+        const Tensor dg = empty({B, HV, T}, at::kFloat, be), db = empty({B, HV, T}, param_type((int)m[1]), be);
+        const Tensor dh0 = m[2] && ctx->needs_input_grad(5) ? empty({B, HV, K, V}, at::kFloat, be) : Tensor();
+        const Tensor work = bytes(rwkv6_gated_delta_workspace_bytes(B, HV, T, K, V, 1), be);
+        const auto st = all_strides<4>({&qs, &ks, &vs, &os});
+        check(rwkv6_gated_delta_bwd(ptr(qs.t), ptr(ks.t), ptr(vs.t), ptr(os.t), st.data(), ptr(be), (int)m[1], fptr(dht), ptr(saved),
+                                    ptr(dq), ptr(dk), ptr(dv), fptr(dg), ptr(db), fptr(dh0), ptr(work), B, H, HV, T, K, V,
+                                    (float)unbits(m[0]), stream_of(be)),
+              "rwkv6_gated_delta_bwd");
+        return {cast(dq, type(m[3])), cast(dk, type(m[4])), cast(dv, type(m[5])), cast(dg, type(m[6])), cast(db, type(m[7])),
+                dh0.defined() ? cast(dh0, type(m[8])) : dh0, Tensor(), Tensor(), Tensor()};
+    }
+};
+// Whether the arguments fit together; gated_delta.py says which does not.
+bool delta_fits(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta) {
+    for (const Tensor* t : {&q, &k, &v, &g, &beta})
+        if (!wkv_type(*t) || t->device() != q.device() || t->layout() != at::kStrided) return false;
+    if (q.dim() != 4 || k.sizes() != q.sizes() || v.dim() != 4 || v.size(0) != q.size(0) || v.size(2) != q.size(2)) return false;
+    const int64_t B = q.size(0), H = q.size(1), T = q.size(2), K = q.size(3), HV = v.size(1), V = v.size(3);
+    if (H < 1 || HV < 1 || HV % H || (K != 64 && K != 128) || V < 64 || V % 64 || V > 512) return false;
+    return g.sizes() == at::IntArrayRef({B, HV, T}) && beta.sizes() == g.sizes();
+}
+// None when an argument does not fit.
+py::object gated_delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
+                            const OptTensor& h0, double scale, bool final_state) {
+    if (!delta_fits(q, k, v, g, beta)) return py::none();
+    if (h0 && (h0->device() != q.device() || !h0->is_floating_point() ||
+               h0->sizes() != at::IntArrayRef({q.size(0), v.size(1), q.size(3), v.size(3)})))
+        return py::none();
+    no_transforms();
+    const c10::DeviceGuard on(q.device());
+    const variable_list out = unlocked([&] {
+        return GatedDelta::apply(q, k, v, g, beta, h0, scale, final_state, recorded({&q, &k, &v, &g, &beta}, h0));
+    });
+    if (final_state) return py::make_tuple(out[0], out[1]);
+    return py::make_tuple(out[0], py::none());
+}
+// The same over a few tokens, the state updated in place; None when an argument does not fit.
+py::object gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
+                            const Tensor& state, double scale) {
+    if (!delta_fits(q, k, v, g, beta)) return py::none();
+    const int64_t B = q.size(0), H = q.size(1), T = q.size(2), K = q.size(3), HV = v.size(1), V = v.size(3);
+    if (state.device() != q.device() || state.scalar_type() != at::kFloat || state.layout() != at::kStrided ||
+        state.sizes() != at::IntArrayRef({B, HV, K, V}) || state.stride(3) != 1 || state.stride(2) != V || state.requires_grad() ||
+        recorded({&q, &k, &v, &g, &beta}, OptTensor()))
+        return py::none();
+    no_transforms();
+    const c10::DeviceGuard on(q.device());
+    return py::cast(unlocked([&] {
+        const Strided qs = strided(q), ks = strided(k), vs = strided(v);
+        const Tensor gf = to_f32(g);
+        const Param be = param(beta);
+        const Tensor o = empty({B, HV, T, V}, at::kBFloat16, gf);
+        const auto st = all_strides<3>({&qs, &ks, &vs});
+        const std::array<int64_t, 2> ss = {state.stride(0), state.stride(1)};
+        check(rwkv6_gated_delta_step(ptr(qs.t), ptr(ks.t), ptr(vs.t), st.data(), fptr(gf), ptr(be.t), be.dt, fptr(state), ss.data(),
+                                     ptr(o), B, H, HV, T, K, V, (float)scale, stream_of(gf)),
+              "rwkv6_gated_delta_step");
+        if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+        return cast(o, v.scalar_type());
+    }));
+}
+
+// ---------------------------------------------------------------------------------------
 // The time mix's bottlenecks: maa given, the token shift's (5 mixes); else the decay's
 // ---------------------------------------------------------------------------------------
 struct Weights {
@@ -930,6 +1057,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("set_error", [](py::object cls) { g_error = cls.release().ptr(); });
     m.def("wkv6", torch::wrap_pybind_function(wkv6));
     m.def("wkv6_seqfirst", torch::wrap_pybind_function(wkv6_seqfirst));
+    m.def("gated_delta_rule", torch::wrap_pybind_function(gated_delta_rule));
+    m.def("gated_delta_step", torch::wrap_pybind_function(gated_delta_step));
     m.def("token_shift_mix", torch::wrap_pybind_function(token_shift_mix));
     m.def("decay_lora", torch::wrap_pybind_function(decay_lora));
     m.def("group_norm_gate", torch::wrap_pybind_function(group_norm_gate));
