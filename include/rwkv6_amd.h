@@ -412,6 +412,26 @@ int rwkv6_wkv_bwd_ex(const void* r, const void* k, const void* v, const void* w,
                      int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, float scale,
                      void* stream, void* const* phase_events);
 
+/* residual_norm with dropout of probability p on f (the reference's bias-dropout-add, rwkv6_layer_specs.py:545,
+ * :548): element e of f [N,C] is kept and scaled by 1 / (1 - p) where the 16-bit number e % 8 of Philox4x32-10
+ * with counter e / 8 and key *seed (a device pointer; low halves of the four words first) is at least 65536 p,
+ * which is rounded to a whole number below 65536.  seed_used (nullable) gets the seed's value for a backward after
+ * the seed has changed; the backward draws the same numbers, no mask is stored.  p = 0 is the call without. */
+int rwkv6_residual_norm_dropout_fwd(const void* x, int x_dtype, const void* branch,
+                                    const void* branch_bias, int bias_dtype, const void* gate,
+                                    float scale, int stepwise, const void* gamma, const void* beta,
+                                    int param_dtype, float eps, void* s, void* y, float* mean,
+                                    float* rstd, float* gamma_used, const int64_t* seed, double p,
+                                    int64_t* seed_used, int64_t N, int64_t C, void* stream);
+int rwkv6_residual_norm_dropout_bwd(const void* x, int x_dtype, const void* branch,
+                                    const void* branch_bias, int bias_dtype, const void* gate,
+                                    float scale, int stepwise, const void* gamma, int gamma_dtype,
+                                    const float* mean, const float* rstd, const void* ds,
+                                    const void* dy, void* dx, void* d_branch, void* d_gate,
+                                    void* dgamma, void* dbeta, int param_dtype, void* d_branch_bias,
+                                    void* workspace, const int64_t* seed, double p, int64_t N,
+                                    int64_t C, void* stream);
+
 /* ------------------------------------------------------------------------
  * The gated delta rule, a recurrent mixer beside WKV6 (no counterpart in the reference):
  *   S' = e^g S,  e = v - S'^T k,  S = S' + beta k e^T,  o = scale S^T q        (a token of a head)

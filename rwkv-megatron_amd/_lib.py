@@ -85,6 +85,10 @@ SIGNATURES = {
     "rwkv6_residual_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64] * 2),
     "rwkv6_residual_norm_bwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _int, _vp, _int, _fp, _fp] + [_vp] * 7
                                 + [_int, _vp, _vp] + [_i64] * 2 + [_vp]),
+    "rwkv6_residual_norm_dropout_fwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _int, _vp, _vp, _int, _f32, _vp, _vp] + [_fp] * 3
+                                        + [_vp, _f64, _vp] + [_i64] * 2 + [_vp]),
+    "rwkv6_residual_norm_dropout_bwd": (_int, [_vp, _int, _vp, _vp, _int, _vp, _f32, _int, _vp, _int, _fp, _fp] + [_vp] * 7
+                                        + [_int, _vp, _vp, _vp, _f64] + [_i64] * 2 + [_vp]),
     "rwkv6_cross_entropy_fwd": (_int, [_vp, _int, _i64, _vp, _i64, _fp, _fp] + [_i64] * 2 + [_vp]),
     "rwkv6_cross_entropy_bwd": (_int, [_vp, _int, _i64, _vp, _i64, _fp, _fp, _vp] + [_i64] * 2 + [_vp]),
     "rwkv6_grad_norm_partials": (_i64, [_vp, _i64]),

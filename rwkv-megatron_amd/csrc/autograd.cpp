@@ -56,6 +56,7 @@ void check(int status, const char* what) {
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
+int64_t* iptr(const Tensor& t) { return static_cast<int64_t*>(ptr(t)); }
 
 // dense and 16-byte aligned, as the kernels read tensors
 Tensor dense(const Tensor& t) {
@@ -575,7 +576,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     // than bf16, so that an update of the parameter in between is not an error
     static std::array<Tensor, 4> run(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta,
                                      const Tensor& gate, const Tensor& cbias, double eps, double scale, bool stepwise,
-                                     bool grad) {
+                                     bool grad, double p, const Tensor& seed, const Tensor& seed_used) {
         const Args a = args(x, branch, gate, cbias);
         Param ga = param(gamma), be = param(beta);
         if (ga.dt != be.dt) ga = {to_f32(gamma), RWKV6_F32}, be = {to_f32(beta), RWKV6_F32};
@@ -583,17 +584,20 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor stats = grad ? empty({2, a.N}, at::kFloat, x) : Tensor();
         const Tensor used = grad && gamma.scalar_type() != at::kBFloat16 ? empty({a.C}, at::kFloat, x) : Tensor();
         float* const mean = fptr(stats);
-        check(rwkv6_residual_norm_train_fwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
+        check(rwkv6_residual_norm_dropout_fwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
                                             stepwise, ptr(ga.t), ptr(be.t), ga.dt, (float)eps, ptr(s), ptr(y), mean,
-                                            mean ? mean + a.N : nullptr, fptr(used), a.N, a.C, stream_of(x)),
-              "rwkv6_residual_norm_train_fwd");
+                                            mean ? mean + a.N : nullptr, fptr(used), iptr(seed), p, iptr(seed_used), a.N, a.C, stream_of(x)),
+              "rwkv6_residual_norm_dropout_fwd");
         return {s, y, stats, used};
     }
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& branch, const Tensor& gamma,
                                  const Tensor& beta, const OptTensor& gate, const OptTensor& cbias, double eps,
-                                 double scale, bool stepwise, bool layers) {
+                                 double scale, bool stepwise, bool layers, double p, const OptTensor& key_in) {
+        const Tensor seed = key_in.value_or(Tensor());
         const Tensor gt = gate.value_or(Tensor()), cb = cbias.value_or(Tensor());
-        const auto [s, y, stats, used] = run(x, branch, gamma, beta, gt, cb, eps, scale, stepwise, true);
+        // the backward draws with the seed's value of now
+        const Tensor key = seed.defined() ? at::empty_like(seed) : Tensor();
+        const auto [s, y, stats, used] = run(x, branch, gamma, beta, gt, cb, eps, scale, stepwise, true, p, seed, key);
         const Tensor& ga = used.defined() ? used : gamma;
         ctx->set_materialize_grads(false);
         // In the layers s stays as it is and the next call holds it as its x: without a gate it is all that the
@@ -605,7 +609,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         if (used.defined()) ctx->saved_data["gamma"] = gamma;
         if (sum && cb.defined()) ctx->saved_data["bias"] = cb;
         ctx->saved_data["beta"] = beta;
-        put(ctx, {bits(scale), stepwise});
+        if (key.defined()) ctx->saved_data["seed"] = key;
+        put(ctx, {bits(scale), stepwise, bits(p)});
         return {s, y};
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -614,58 +619,69 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const auto kept = [&](const char* key, const Tensor& t) { return ctx->saved_data.count(key) ? ctx->saved_data[key].toTensor() : t; };
         const Tensor cbias = kept("bias", sv[3]), gamma = kept("gamma", sv[4]), beta = kept("beta", Tensor());
         const auto m = meta(ctx);
-        const double scale = unbits(m[0]);
+        const double scale = unbits(m[0]), p = unbits(m[2]);
+        const Tensor seed = kept("seed", Tensor());
         // an output no loss uses has no gradient
         const Tensor dy = g[1].defined() ? to_bf16(g[1]) : at::zeros(x.sizes(), x.options().dtype(at::kBFloat16));
-        if (at::GradMode::is_enabled()) return differentiable(sv, cbias, gamma, beta, g[0], g[1].defined() ? g[1] : dy, scale);
+        if (at::GradMode::is_enabled()) return differentiable(sv, cbias, gamma, beta, g[0], g[1].defined() ? g[1] : dy, scale, p, seed);
         const Args a = args(x, branch, gate, cbias);
         const Tensor ds = g[0].defined() ? dense(cast(g[0], x.scalar_type())) : Tensor();
         const Param ga = param(sv[4]);
         const bool gated = gate.defined(), biased = cbias.defined();
         bool sums = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
         if (biased) sums = sums || ctx->needs_input_grad(gated ? 5 : 4);
-        const bool same = a.xt == RWKV6_BF16 && scale == 1. && !gated && !biased;      // d_branch is dx
+        const bool same = a.xt == RWKV6_BF16 && scale == 1. && !gated && !biased && p == 0.;      // d_branch is dx
         const Tensor dx = at::empty_like(a.x), db = same ? Tensor() : at::empty_like(dy);
         const Tensor dg = gated ? at::empty_like(a.gate) : Tensor();
         const int dt = grad_code(gamma) == grad_code(beta) ? grad_code(gamma) : RWKV6_F32;
         const Tensor dga = sums ? empty({a.C}, param_type(dt), x) : Tensor(), dbe = sums ? at::empty_like(dga) : Tensor();
         const Tensor dcb = sums && biased ? empty({a.C}, a.cbias.t.scalar_type(), x) : Tensor();
         const Tensor ws = sums ? bytes(rwkv6_residual_norm_bwd_workspace_bytes(a.N, a.C), x) : Tensor();
-        check(rwkv6_residual_norm_bwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
+        check(rwkv6_residual_norm_dropout_bwd(ptr(a.x), a.xt, ptr(a.branch), ptr(a.cbias.t), a.cbias.dt, ptr(a.gate), (float)scale,
                                       (int)m[1], ptr(ga.t), ga.dt, fptr(sv[5]), a.N ? fptr(sv[5]) + a.N : nullptr, ptr(ds), ptr(dy), ptr(dx), ptr(db), ptr(dg),
-                                      ptr(dga), ptr(dbe), dt, ptr(dcb), ptr(ws), a.N, a.C, stream_of(x)),
-              "rwkv6_residual_norm_bwd");
+                                      ptr(dga), ptr(dbe), dt, ptr(dcb), ptr(ws), iptr(seed), p, a.N, a.C, stream_of(x)),
+              "rwkv6_residual_norm_dropout_bwd");
         return {dx, same ? dx : db, sums ? cast(dga, gamma.scalar_type()) : dga, sums ? cast(dbe, beta.scalar_type()) : dbe, dg,
-                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor(), Tensor(), Tensor()};
+                dcb.defined() ? cast(dcb, cbias.scalar_type()) : dcb, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
     // A backward that is differentiated itself: the same formulas in torch's operators.
     static variable_list differentiable(const variable_list& sv, const Tensor& cbias, const Tensor& gamma, const Tensor& beta,
-                                        const Tensor& ds, const Tensor& dy, double scale) {
+                                        const Tensor& ds, const Tensor& dy, double scale, double p, const Tensor& seed) {
         const Tensor &x = sv[0], &branch = sv[1], &gate = sv[2];
+        const Tensor drop = p > 0. ? factors(x, sv[4], p, seed) : Tensor();
         // the values that the forward used
         const Tensor ga = gamma.is_same(sv[4]) ? gamma : gamma + (sv[4].to(gamma.scalar_type()) - gamma).detach();
         Tensor s = x.to(at::kFloat), f, sg;
         if (branch.defined()) {
             f = cbias.defined() ? branch.to(at::kFloat) + cbias.to(at::kFloat) : branch.to(at::kFloat);
             if (gate.defined()) sg = at::sigmoid(gate.to(at::kFloat));
-            s = s + (gate.defined() ? f * sg : f) * scale;
+            const Tensor fg = gate.defined() ? f * sg : f;
+            s = s + (drop.defined() ? fg * drop : fg) * scale;
         }
         std::vector<int64_t> st(x.sizes().begin(), x.sizes().end());
         st.back() = 1;
         auto [dS, dga, dbe] = at::native_layer_norm_backward(dy.to(at::kFloat), s, {x.size(-1)}, sv[5][0].view(st), sv[5][1].view(st),
                                                              ga.to(at::kFloat), beta.to(at::kFloat), {true, true, true});
         if (ds.defined()) dS = dS + ds.to(at::kFloat);
-        const Tensor df = dS * scale, db = gate.defined() ? df * sg : df;
+        const Tensor df = drop.defined() ? dS * scale * drop : dS * scale, db = gate.defined() ? df * sg : df;
         const Tensor dg = gate.defined() ? (df * f * sg * (1 - sg)).to(gate.scalar_type()) : Tensor();
         const Tensor dcb = cbias.defined() ? db.reshape({-1, x.size(-1)}).sum(0).to(cbias.scalar_type()) : Tensor();
         return {dS.to(x.scalar_type()), db.to(at::kBFloat16), dga.to(gamma.scalar_type()), dbe.to(beta.scalar_type()),
-                dg, dcb, Tensor(), Tensor(), Tensor(), Tensor()};
+                dg, dcb, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+    // dropout's factors, 0 or 1 / (1 - p): what the forward makes of ones added to zeros
+    static Tensor factors(const Tensor& x, const Tensor& gamma, double p, const Tensor& seed) {
+        const at::NoGradGuard none;
+        const Tensor zero = at::zeros(x.sizes(), x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+        const Tensor one = at::ones(x.sizes(), x.options().dtype(at::kBFloat16).memory_format(at::MemoryFormat::Contiguous));
+        return run(zero, one, gamma.detach(), gamma.detach(), Tensor(), Tensor(), 1., 1., false, false, p, seed, Tensor())[0];
     }
 };
 // None when the kernels do not take the call (layers: nor one that a mode or transform wants to see);
 // the callers check and raise, or run torch's operators.
-py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta, double eps,
-                         const OptTensor& gate, const OptTensor& cbias, double scale, bool stepwise, bool layers) {
+py::object residual_norm_dropout(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta, double eps,
+                                 const OptTensor& gate, const OptTensor& cbias, double scale, bool stepwise, bool layers, double p,
+                                 const OptTensor& seed_in) {
     if (!x.is_cuda() || x.dim() < 1 || x.size(-1) < 1 || x.layout() != at::kStrided ||
         (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat))
         return py::none();
@@ -678,6 +694,9 @@ py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& ga
         if (t->device() != x.device() || t->sizes() != at::IntArrayRef({C}) ||
             (t->scalar_type() != at::kBFloat16 && t->scalar_type() != at::kFloat && t->scalar_type() != at::kHalf))
             return py::none();
+    if (p != 0. && (!seed_in || seed_in->device() != x.device() || seed_in->scalar_type() != at::kLong || seed_in->numel() != 1))
+        return py::none();
+    const Tensor seed = p != 0. ? *seed_in : Tensor();
     if (layers && !plain({&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})) return py::none();
     no_transforms();
     const c10::DeviceGuard on(x.device());           // the default stream is the current device's
@@ -686,12 +705,17 @@ py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& ga
         grad = grad || t->_fw_grad(0).defined();          // forward-mode derivatives are refused there
     if (!grad) {
         const auto o = unlocked([&] {
-            return ResidualNorm::run(x, branch, gamma, beta, gate.value_or(Tensor()), cbias.value_or(Tensor()), eps, scale, stepwise, false);
+            return ResidualNorm::run(x, branch, gamma, beta, gate.value_or(Tensor()), cbias.value_or(Tensor()), eps, scale, stepwise, false, p,
+                                     seed, Tensor());
         });
         return py::make_tuple(o[0], o[1]);
     }
-    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, stepwise, layers); });
+    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, stepwise, layers, p, p != 0. ? seed_in : OptTensor()); });
     return py::make_tuple(o[0], o[1]);
+}
+py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta, double eps,
+                         const OptTensor& gate, const OptTensor& cbias, double scale, bool stepwise, bool layers) {
+    return residual_norm_dropout(x, branch, gamma, beta, eps, gate, cbias, scale, stepwise, layers, 0., OptTensor());
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1063,6 +1087,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("decay_lora", torch::wrap_pybind_function(decay_lora));
     m.def("group_norm_gate", torch::wrap_pybind_function(group_norm_gate));
     m.def("layer_norm", torch::wrap_pybind_function(layer_norm));
+    m.def("residual_norm_dropout", torch::wrap_pybind_function(residual_norm_dropout));
     m.def("residual_norm", torch::wrap_pybind_function(residual_norm));
     m.def("cross_entropy", torch::wrap_pybind_function(cross_entropy));
     m.def("grad_norm_sums", torch::wrap_pybind_function(grad_norm_sums));

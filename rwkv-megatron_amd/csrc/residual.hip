@@ -18,6 +18,12 @@
 // model run that, so that fusing them changed no value of theirs by more than the order of a row's
 // sums does.
 //
+// With dropout f is kept with probability 1 - p and scaled by 1 / (1 - p), after the gate and before the scale.
+// Whether an element is kept comes from a counter-based generator (Philox4x32-10, Salmon et al. 2011): the counter is
+// the element's place over 8, the key the call's seed, and an element of the eight has 16 of the 128 bits, so
+// p is taken to the nearest 2^-16 and 1 / (1 - p) of that.  The mask is never stored: the backward draws it
+// again.  Ten rounds are 20 products of 32 bits for 8 elements, a piece of a lane.
+//
 // Bound by memory: bytes an element in bf16 8 forward (10 gated), 10 backward (16 gated).  16384 x 2048
 // forward and backward 106 us (kernels 47 + 57, and 4 for the parameters' sums), gated 160 us (56 + 101 +
 // 4): 5.7 and 5.4 TB/s of those bytes, where a sum of two 1 GiB tensors reaches 6.1; torch's operators in 32
@@ -99,7 +105,27 @@ struct RnIn {
     int cdt;
     float scale;
     int stepwise;
+    const int64_t* seed;      // dropout: the key, the number of 65536 draws that drop, 1 / (1 - p)
+    uint32_t cut;
+    float keep;
 };
+// Factors 0 or `keep` of the eight elements of piece `at` of a tensor.
+__device__ __forceinline__ void drop8(uint64_t at, uint64_t seed, uint32_t cut, float keep, float* f) {
+    uint32_t c0 = (uint32_t)at, c1 = (uint32_t)(at >> 32), c2 = 0, c3 = 0, k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
+        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)b;
+        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)a;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    const uint32_t w[4] = {c0, c1, c2, c3};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu) >= cut ? keep : 0.f;
+}
 // Eight values rounded to bf16.
 __device__ __forceinline__ void round8(float* f) { unpack8(pack8(f), f); }
 
@@ -107,15 +133,17 @@ __device__ __forceinline__ void round8(float* f) { unpack8(pack8(f), f); }
 
 // A row is W waves' (512 NV channels each, 8 a lane and piece); a block holds RB = 4 / W rows, one at
 // least, and strides over the rows.  The pieces of a row stay in registers.
-template <int NV, bool XF, bool GATE, bool CB>
+template <int NV, bool XF, bool GATE, bool CB, bool DROP>
 __global__ void __launch_bounds__(64 * RN_MAX_WAVES)
 rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const void* __restrict__ beta, int pdt,
                                float eps, void* __restrict__ s, uint16_t* __restrict__ y,
                                float* __restrict__ mean_out, float* __restrict__ rstd_out, float* __restrict__ gamma_used,
-                               int64_t N, int C, int W, int RB, bool nt) {
+                               int64_t* __restrict__ seed_used, int64_t N, int C, int W, int RB, bool nt) {
     __shared__ float red[2][RN_MAX_WAVES];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, gr = wv / W, w = wv - gr * W;
     const float inv = 1.f / (float)C;
+    const uint64_t seed = DROP ? (uint64_t)*in.seed : 0;
+    if (DROP && seed_used && blockIdx.x == 0 && threadIdx.x == 0) *seed_used = (int64_t)seed;
     int c[NV];
     float ga[NV][8], be[NV][8], cb[CB ? NV : 1][8];
 #pragma unroll
@@ -151,6 +179,14 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
                     sigmoid8(g, in.stepwise);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) f[j] *= g[j];
+                }
+                if constexpr (DROP) {
+                    float d[8];
+                    drop8((uint64_t)(row + c[i]) >> 3, seed, in.cut, in.keep, d);
+                    if (GATE && in.stepwise) round8(f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = d[j] != 0.f ? f[j] * d[j] : 0.f;
+                    if (in.stepwise) round8(f);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) f[j] *= in.scale;
@@ -192,7 +228,7 @@ rwkv6_residual_norm_fwd_kernel(RnIn in, const void* __restrict__ gamma, const vo
 // Steps of RB rows; block p takes `run` of them, then skips the other blocks' runs.  part[p][CB ? 3 : 2][C] = its sums of dgamma, dbeta
 // and d_branch_bias (part null: none).  ds null: zero.  db null: d_branch equals dx, not stored twice.  SUM: x is the
 // sum s as the stepwise forward stored it, what its norm was taken of, and the branch is not read.
-template <int NV, bool XF, bool GATE, bool CB, bool SUM>
+template <int NV, bool XF, bool GATE, bool CB, bool SUM, bool DROP>
 __global__ void __launch_bounds__(64 * RN_MAX_WAVES)
 rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt, const float* __restrict__ mean_in,
                                const float* __restrict__ rstd_in, const void* __restrict__ ds,
@@ -203,6 +239,7 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
     __shared__ float2 red[2][RN_MAX_WAVES];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, gr = wv / W, w = wv - gr * W;
     const float inv = 1.f / (float)C;
+    const uint64_t seed = DROP ? (uint64_t)*in.seed : 0;
     int c[NV];
     float ga[NV][8], cb[CB ? NV : 1][8], ag[NV][8], ab[NV][8], ac[CB ? NV : 1][8];
 #pragma unroll
@@ -230,7 +267,7 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
             b0 += skip;
         }
         const float mean = mean_in[n], rstd = rstd_in[n];
-        float xh[NV][8], g[NV][8], f[NV][8], sg[NV][8], dS[NV][8];
+        float xh[NV][8], g[NV][8], f[NV][8], sg[NV][8], dS[NV][8], dr[DROP ? NV : 1][8];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -242,6 +279,7 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
             if constexpr (GATE) load8(in.gate + row + c[i], sg[i]);
             load8(dy + row + c[i], g[i]);
             if (ds) raw_f32<XF>(w_load<XF>(ds, row + c[i]), dS[i]);
+            if constexpr (DROP) drop8((uint64_t)(row + c[i]) >> 3, seed, in.cut, in.keep, dr[i]);
             float t[8];
             if constexpr (SUM) {
 #pragma unroll
@@ -254,7 +292,15 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
                 }
                 if constexpr (GATE) sigmoid8(sg[i], in.stepwise);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) t[j] = (GATE ? f[i][j] * sg[i][j] : f[i][j]) * in.scale;
+                for (int j = 0; j < 8; ++j) t[j] = GATE ? f[i][j] * sg[i][j] : f[i][j];
+                if constexpr (DROP) {
+                    if (GATE && in.stepwise) round8(t);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t[j] = dr[i][j] != 0.f ? t[j] * dr[i][j] : 0.f;
+                    if (in.stepwise) round8(t);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] *= in.scale;
                 if (in.stepwise) round8(t);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) t[j] += xh[i][j];
@@ -302,6 +348,11 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
 #pragma unroll
             for (int j = 0; j < 8; ++j) dS[i][j] *= in.scale;
             if (in.stepwise) round8(dS[i]);
+            if constexpr (DROP) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) dS[i][j] = dr[i][j] != 0.f ? dS[i][j] * dr[i][j] : 0.f;
+                if (in.stepwise) round8(dS[i]);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[j] = GATE ? dS[i][j] * sg[i][j] : dS[i][j];
             if constexpr (CB) {
@@ -412,11 +463,24 @@ inline RnRuns rn_runs(int64_t N, int RB, bool gate) {
     const int64_t b = half < 1 ? 1 : half < RN_BLOCKS ? half : RN_BLOCKS, run = (steps + b - 1) / b;
     return {b, (int)(run < 1 ? 1 : run)};
 }
+// Dropout with probability p: the draws of 65536 that drop; -1 for a p that is none, or whose 16 bits drop everything.
+int rn_cut(double p) {
+    if (!(p >= 0. && p <= 1.)) return -1;
+    const int cut = (int)(p * 65536. + .5);
+    return cut < 65536 ? cut : -1;
+}
+RnIn rn_in(const void* x, const void* branch, const void* gate, const void* cbias, int cdt, float scale, int stepwise,
+           const int64_t* seed, int cut) {
+    return {x, (const uint16_t*)branch, (const uint16_t*)gate, cbias, cdt, scale, stepwise, seed, (uint32_t)cut,
+            (float)(65536. / (65536. - cut))};
+}
 int rn_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype, const void* gate,
            float scale, int stepwise, const void* gamma, const void* beta, int param_dtype, float eps, void* s, void* y,
-           float* mean, float* rstd, float* gamma_used, int64_t N, int64_t C, void* stream) {
-    const int st = rn_check(N, C);
+           float* mean, float* rstd, float* gamma_used, const int64_t* seed, double p, int64_t* seed_used, int64_t N, int64_t C,
+           void* stream) {
+    const int st = rn_check(N, C), cut = rn_cut(p);
     if (st) return st;
+    if (cut < 0 || (cut > 0 && !seed)) return RWKV6_ERR_INVALID_ARG;
     if (!dt_ok(x_dtype) || !dt_ok(param_dtype) || (branch_bias && !dt_ok(bias_dtype)) || (!mean != !rstd))
         return RWKV6_ERR_INVALID_ARG;
     if (N == 0) return RWKV6_OK;
@@ -425,59 +489,41 @@ int rn_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bi
         if (!al16(p)) return RWKV6_ERR_ALIGNMENT;
     const size_t act = (size_t)(N * C) * 2, xs = (size_t)(N * C) * param_bytes(x_dtype), st4 = (size_t)N * 4;
     const size_t par = (size_t)C * param_bytes(param_dtype);
-    if (any_alias({{s, xs}, {y, act}, {mean, st4}, {rstd, st4}, {gamma_used, (size_t)C * 4}},
-                  {{x, xs}, {branch, act}, {branch_bias, (size_t)C * param_bytes(bias_dtype)}, {gate, act}, {gamma, par}, {beta, par}}))
+    if (any_alias({{s, xs}, {y, act}, {mean, st4}, {rstd, st4}, {gamma_used, (size_t)C * 4}, {seed_used, 8}},
+                  {{seed, 8}, {x, xs}, {branch, act}, {branch_bias, (size_t)C * param_bytes(bias_dtype)}, {gate, act}, {gamma, par}, {beta, par}}))
         return RWKV6_ERR_INVALID_ARG;
     const RnShape h = rn_shape(C);
     const bool xf = x_dtype == RWKV6_F32, gt = gate != nullptr, cb = branch_bias != nullptr;
-#define RN_CB(NV, X, G) (cb ? rwkv6_residual_norm_fwd_kernel<NV, X, G, true> : rwkv6_residual_norm_fwd_kernel<NV, X, G, false>)
+#define RN_DROP(NV, X, G, B) (cut ? rwkv6_residual_norm_fwd_kernel<NV, X, G, B, true> : rwkv6_residual_norm_fwd_kernel<NV, X, G, B, false>)
+#define RN_CB(NV, X, G) (cb ? RN_DROP(NV, X, G, true) : RN_DROP(NV, X, G, false))
 #define RN_PICK(NV) (xf ? (gt ? RN_CB(NV, true, true) : RN_CB(NV, true, false)) : (gt ? RN_CB(NV, false, true) : RN_CB(NV, false, false)))
     auto k = h.NV == 1 ? RN_PICK(1) : RN_PICK(2);
 #undef RN_PICK
 #undef RN_CB
+#undef RN_DROP
     const int64_t blocks = (N + h.RB - 1) / h.RB;
     hipLaunchKernelGGL(k, dim3((unsigned)(blocks < RN_FWD_BLOCKS ? blocks : RN_FWD_BLOCKS)), dim3(64 * h.W * h.RB), 0,
                        reinterpret_cast<hipStream_t>(stream),
-                       RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale, stepwise}, gamma, beta,
-                       param_dtype, eps, s, (uint16_t*)y, mean, rstd, gamma_used, N, (int)C, h.W, h.RB, rn_stream(N, C));
+                       rn_in(x, branch, gate, branch_bias, bias_dtype, scale, stepwise, seed, cut), gamma, beta,
+                       param_dtype, eps, s, (uint16_t*)y, mean, rstd, gamma_used, seed_used, N, (int)C, h.W, h.RB, rn_stream(N, C));
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
-}  // namespace
-
-extern "C" {
-
-int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
-                            const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
-                            int param_dtype, float eps, void* s, void* y, float* mean, float* rstd, int64_t N, int64_t C, void* stream) {
-    return rn_fwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, beta, param_dtype, eps, s, y, mean, rstd,
-                  nullptr, N, C, stream);
+size_t rn_bwd_bytes(int64_t N, int64_t C) {
+    return rn_check(N, C) ? 0 : (size_t)(rn_runs(N, rn_shape(C).RB, false).blocks * 3 * C) * sizeof(float);
 }
-
-int rwkv6_residual_norm_train_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
-                                  const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
-                                  int param_dtype, float eps, void* s, void* y, float* mean, float* rstd,
-                                  float* gamma_used, int64_t N, int64_t C, void* stream) {
-    return rn_fwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, beta, param_dtype, eps, s, y, mean, rstd,
-                  gamma_used, N, C, stream);
-}
-
-size_t rwkv6_residual_norm_bwd_workspace_bytes(int64_t N, int64_t C) {
-    if (rn_check(N, C)) return 0;
-    return (size_t)(rn_runs(N, rn_shape(C).RB, false).blocks * 3 * C) * sizeof(float);
-}
-
-int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
+int rn_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
                             const void* gate, float scale, int stepwise, const void* gamma, int gamma_dtype, const float* mean,
                             const float* rstd, const void* ds, const void* dy, void* dx, void* d_branch, void* d_gate,
-                            void* dgamma, void* dbeta, int param_dtype, void* d_branch_bias, void* workspace, int64_t N,
-                            int64_t C, void* stream) {
-    const int st = rn_check(N, C);
+                            void* dgamma, void* dbeta, int param_dtype, void* d_branch_bias, void* workspace, const int64_t* seed,
+                            double p, int64_t N, int64_t C, void* stream) {
+    const int st = rn_check(N, C), cut = rn_cut(p);
     if (st) return st;
+    if (cut < 0 || (cut > 0 && !seed)) return RWKV6_ERR_INVALID_ARG;
     if (!dt_ok(x_dtype) || !dt_ok(gamma_dtype) || !dt_ok(param_dtype) || (branch_bias && !dt_ok(bias_dtype)))
         return RWKV6_ERR_INVALID_ARG;
     const bool sums = dgamma || dbeta, xf = x_dtype == RWKV6_F32, gt = gate != nullptr, cb = branch_bias != nullptr;
     // d_branch is dx itself, and not written, only where the two are the same numbers
-    if (N > 0 && !d_branch && (gt || cb || xf || scale != 1.f)) return RWKV6_ERR_INVALID_ARG;
+    if (N > 0 && !d_branch && (cut || gt || cb || xf || scale != 1.f)) return RWKV6_ERR_INVALID_ARG;
     // no branch: x is the sum that the stepwise forward stored
     if (!gamma || (!dgamma != !dbeta) || (!d_branch_bias != !(cb && sums)) || (sums && !workspace) ||
         (N > 0 && (!x || (!branch && (!stepwise || gt)) || !mean || !rstd || !dy || !dx || !d_gate != !gt)))
@@ -488,8 +534,8 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
     const size_t act = (size_t)(N * C) * 2, xs = (size_t)(N * C) * param_bytes(x_dtype), st4 = (size_t)N * 4;
     const size_t par = (size_t)C * param_bytes(param_dtype), cbs = cb ? (size_t)C * param_bytes(bias_dtype) : 0;
     if (any_alias({{dx, xs}, {d_branch, act}, {d_gate, act}, {dgamma, par}, {dbeta, par}, {d_branch_bias, cbs},
-                   {sums ? workspace : nullptr, rwkv6_residual_norm_bwd_workspace_bytes(N, C)}},
-                  {{x, xs}, {branch, act}, {branch_bias, cbs}, {gate, act}, {gamma, (size_t)C * param_bytes(gamma_dtype)},
+                   {sums ? workspace : nullptr, rn_bwd_bytes(N, C)}},
+                  {{seed, 8}, {x, xs}, {branch, act}, {branch_bias, cbs}, {gate, act}, {gamma, (size_t)C * param_bytes(gamma_dtype)},
                    {mean, st4}, {rstd, st4}, {ds, xs}, {dy, act}}))
         return RWKV6_ERR_INVALID_ARG;
     hipStream_t stm = reinterpret_cast<hipStream_t>(stream);
@@ -498,15 +544,17 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
     const int64_t M = (cb ? 3 : 2) * C;
     float* part = sums ? (float*)workspace : nullptr;
     if (N > 0) {
-#define RN_CB(NV, X, G, S) (cb ? rwkv6_residual_norm_bwd_kernel<NV, X, G, true, S> : rwkv6_residual_norm_bwd_kernel<NV, X, G, false, S>)
+#define RN_DROP(NV, X, G, B, S) (cut ? rwkv6_residual_norm_bwd_kernel<NV, X, G, B, S, true> : rwkv6_residual_norm_bwd_kernel<NV, X, G, B, S, false>)
+#define RN_CB(NV, X, G, S) (cb ? RN_DROP(NV, X, G, true, S) : RN_DROP(NV, X, G, false, S))
 #define RN_GATE(NV, X) (gt ? RN_CB(NV, X, true, false) : branch ? RN_CB(NV, X, false, false) : RN_CB(NV, X, false, true))
 #define RN_PICK(NV) (xf ? RN_GATE(NV, true) : RN_GATE(NV, false))
         auto k = h.NV == 1 ? RN_PICK(1) : RN_PICK(2);
 #undef RN_PICK
 #undef RN_GATE
 #undef RN_CB
+#undef RN_DROP
         hipLaunchKernelGGL(k, dim3((unsigned)r.blocks), dim3(64 * h.W * h.RB), sums && h.RB > 1 ? (size_t)M * 4 : 0, stm,
-                           RnIn{x, (const uint16_t*)branch, (const uint16_t*)gate, branch_bias, bias_dtype, scale, stepwise}, gamma,
+                           rn_in(x, branch, gate, branch_bias, bias_dtype, scale, stepwise, seed, cut), gamma,
                            gamma_dtype, mean, rstd, ds, (const uint16_t*)dy, dx, (uint16_t*)d_branch, (uint16_t*)d_gate, part,
                            N, (int)C, h.W, h.RB, r.run, rn_stream(N, C));
     }
@@ -514,6 +562,54 @@ int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, cons
         hipLaunchKernelGGL(rwkv6_residual_norm_sums_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, stm, part,
                            N > 0 ? (int)r.blocks : 0, (int)M, (int)C, dgamma, dbeta, param_dtype, d_branch_bias, bias_dtype);
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
+}
+}  // namespace
+
+extern "C" {
+
+int rwkv6_residual_norm_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
+                            const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
+                            int param_dtype, float eps, void* s, void* y, float* mean, float* rstd, int64_t N, int64_t C, void* stream) {
+    return rn_fwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, beta, param_dtype, eps, s, y, mean, rstd,
+                  nullptr, nullptr, 0., nullptr, N, C, stream);
+}
+
+int rwkv6_residual_norm_train_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
+                                  const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
+                                  int param_dtype, float eps, void* s, void* y, float* mean, float* rstd,
+                                  float* gamma_used, int64_t N, int64_t C, void* stream) {
+    return rn_fwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, beta, param_dtype, eps, s, y, mean, rstd,
+                  gamma_used, nullptr, 0., nullptr, N, C, stream);
+}
+
+int rwkv6_residual_norm_dropout_fwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
+                                    const void* gate, float scale, int stepwise, const void* gamma, const void* beta,
+                                    int param_dtype, float eps, void* s, void* y, float* mean, float* rstd, float* gamma_used,
+                                    const int64_t* seed, double p, int64_t* seed_used, int64_t N, int64_t C, void* stream) {
+    return rn_fwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, beta, param_dtype, eps, s, y, mean, rstd,
+                  gamma_used, seed, p, seed_used, N, C, stream);
+}
+
+size_t rwkv6_residual_norm_bwd_workspace_bytes(int64_t N, int64_t C) {
+    return rn_bwd_bytes(N, C);
+}
+
+int rwkv6_residual_norm_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
+                            const void* gate, float scale, int stepwise, const void* gamma, int gamma_dtype, const float* mean,
+                            const float* rstd, const void* ds, const void* dy, void* dx, void* d_branch, void* d_gate,
+                            void* dgamma, void* dbeta, int param_dtype, void* d_branch_bias, void* workspace, int64_t N,
+                            int64_t C, void* stream) {
+    return rn_bwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, gamma_dtype, mean, rstd, ds, dy, dx, d_branch,
+                  d_gate, dgamma, dbeta, param_dtype, d_branch_bias, workspace, nullptr, 0., N, C, stream);
+}
+
+int rwkv6_residual_norm_dropout_bwd(const void* x, int x_dtype, const void* branch, const void* branch_bias, int bias_dtype,
+                            const void* gate, float scale, int stepwise, const void* gamma, int gamma_dtype, const float* mean,
+                            const float* rstd, const void* ds, const void* dy, void* dx, void* d_branch, void* d_gate,
+                            void* dgamma, void* dbeta, int param_dtype, void* d_branch_bias, void* workspace, const int64_t* seed, double p, int64_t N,
+                            int64_t C, void* stream) {
+    return rn_bwd(x, x_dtype, branch, branch_bias, bias_dtype, gate, scale, stepwise, gamma, gamma_dtype, mean, rstd, ds, dy, dx, d_branch,
+                  d_gate, dgamma, dbeta, param_dtype, d_branch_bias, workspace, seed, p, N, C, stream);
 }
 
 }  // extern "C"

@@ -29,7 +29,7 @@ read here is one of those, or is read with getattr and a default:
   params_dtype, perform_initialization, init_method_std, token_shift_bottleneck_size,
   decay_bottleneck_size; optional: init_method / output_layer_init_method (callables, as
   Megatron's config sets them; else normal(0, std) and normal(0, std / sqrt(2 L))),
-  add_bias_linear / add_qkv_bias (default False), sequence_parallel (must be False: one
+  add_bias_linear / add_qkv_bias (default False), hidden_dropout (default 0), sequence_parallel (must be False: one
   GPU, no token-shift halo), rwkv_lm_decay_init (this package's own switch, default False).
 
 Deliberate differences, all documented in the reference's own terms:
@@ -72,6 +72,7 @@ class TransformerConfig:
     add_bias_linear: bool = False                # example_config.yaml:20
     add_qkv_bias: bool = False                   # example_config.yaml:22
     sequence_parallel: bool = False              # one GPU: no sequence-parallel token shift
+    hidden_dropout: float = 0.0                  # example_config.yaml:13, of the blocks' outputs in training
     # The reference initialises the decay bottleneck's bias uniform(-1, 1) (:173-175).  True
     # selects RWKV-LM's per-channel ramp -6 + 5 (c/(C-1))^(0.7 + 1.3 l/(L-1)) instead (the
     # tiny-LM benchmark configuration asks for it).  Not a Megatron field: read with getattr.
@@ -321,17 +322,21 @@ class RWKV6ChannelMix(nn.Module):
         return out, self.linear_gate(mixed_gate)[0]
 
 
-def _add_norm(norm, x, branch, bias=None, gate=None):
-    """(s, LayerNorm(s)) for s = x + (branch + bias) sigmoid(gate): in one kernel (residual.residual_norm,
-    stepwise: rounded where the separate operators round) where it takes the call, else by the operators
-    it stands for.  A norm that is not this package's own class, or that has hooks, is called as a module."""
+def _add_norm(norm, x, branch, bias=None, gate=None, dropout=0.0):
+    """(s, LayerNorm(s)) for s = x + dropout((branch + bias) sigmoid(gate)): in one kernel
+    (residual.residual_norm, stepwise: rounded where the separate operators round) where it takes the call,
+    else by the operators it stands for.  A norm that is not this package's own class, or that has hooks, is
+    called as a module.  Dropout's seed is drawn from torch's generator of the device, once a call."""
     if _plain_module(norm, LayerNorm) and norm.weight is not None and norm.bias is not None and x.is_cuda:
-        out = _lib.native().residual_norm(x, branch, norm.weight, norm.bias, norm.eps, gate, bias, 1.0, True, True)
+        seed = torch.randint(2 ** 63 - 1, (1,), device=x.device) if dropout else None
+        out = _lib.native().residual_norm_dropout(x, branch, norm.weight, norm.bias, norm.eps, gate, bias, 1.0, True, True,
+                                                  dropout, seed)
         if out is not None:
             return out
     if bias is not None:
         branch = branch + bias
-    x = x + (branch if gate is None else channelmix.sigmoid_gate(branch, gate))
+    branch = branch if gate is None else channelmix.sigmoid_gate(branch, gate)
+    x = x + (F.dropout(branch, dropout) if dropout else branch)
     return x, norm(x)
 
 
@@ -350,7 +355,8 @@ def _plain_module(m, cls):
 
 class RWKV6Layer(nn.Module):
     """The TransformerLayer that get_rwkv6_layer_spec() builds (:539-550):
-    LN -> time mix -> residual -> LN -> channel mix -> residual (dropout 0)."""
+    LN -> time mix -> residual -> LN -> channel mix -> residual, with the config's hidden_dropout on what the
+    residuals add, in training."""
 
     def __init__(self, config, layer_number=1, device=None):
         super().__init__()
@@ -361,24 +367,31 @@ class RWKV6Layer(nn.Module):
         self.pre_mlp_layernorm = LayerNorm(C, eps=config.layernorm_epsilon, device=device,
                                            dtype=config.params_dtype)
         self.mlp = RWKV6ChannelMix(config, layer_number, device)
+        self.hidden_dropout = float(getattr(config, "hidden_dropout", 0.0) or 0.0)
+        if not 0 <= self.hidden_dropout < 1 - 2.0 ** -17:
+            raise ValueError(f"hidden_dropout must be in [0, 1 - 2^-17), got {self.hidden_dropout}")
+
+    def _dropout(self):
+        return self.hidden_dropout if self.training else 0.0
 
     def forward(self, x):
         x, h = self._time_mix(x, self.input_layernorm(x))
         m, _ = self.mlp(h)
-        return x + m
+        p = self._dropout()
+        return x + (F.dropout(m, p) if p else m)
 
     def _time_mix(self, x, h):
         """The stream after the time mix of h = input_layernorm(x), and its norm for the channel mix
-        (bias-dropout-add, dropout 0)."""
+        (bias-dropout-add)."""
         a, a_bias = self.self_attention(h, None)
-        return _add_norm(self.pre_mlp_layernorm, x, a, a_bias)
+        return _add_norm(self.pre_mlp_layernorm, x, a, a_bias, dropout=self._dropout())
 
     def chained(self, x, h, next_norm):
         """forward from h = input_layernorm(x), with the norm that follows this layer: (forward(x),
         next_norm(forward(x))), the channel mix's gate, the residual and that norm in one kernel."""
         x, h = self._time_mix(x, h)
         out, gate = self.mlp.ungated(h)
-        return _add_norm(next_norm, x, out, gate=gate)
+        return _add_norm(next_norm, x, out, gate=gate, dropout=self._dropout())
 
 
 # what _plain_module compares with

@@ -8,6 +8,9 @@ mix's output is gated by a sigmoid before that (:533-536):
     s = x + scale * f
     y = LayerNorm(s) * weight + bias
 
+and in training drops elements of f out (the layer's hidden_dropout, a bias-dropout-add), from a
+counter-based generator whose numbers the backward draws again: no mask is stored.
+
 ``residual_norm`` is one kernel forward and two backward (the gradients of everything, and the sums
 over the rows for the parameters') where torch runs an add, a product and a LayerNorm of which each
 reads and writes the stream.  modules.RWKV6Layer and RWKV6Model call it.  The autograd function is
@@ -22,7 +25,7 @@ from . import _lib
 MAX_CHANNELS = 8192
 
 
-def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, scale=1.0, stepwise=False):
+def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, scale=1.0, stepwise=False, dropout=0.0, seed=None):
     """(s, y) = (x + scale (branch + branch_bias) sigmoid(gate), LayerNorm(s) weight + bias).
 
     x [..., C] bf16 or fp32 (s comes back in the same type); branch and gate [..., C] bf16;
@@ -33,13 +36,24 @@ def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, sca
     the gate (bf16) and s (x's type) are rounded before they are used, y is the norm of s as returned,
     and the gradients are rounded at the same places.
 
+    dropout=p keeps an element of f with probability 1 - p and scales it by 1 / (1 - p), p taken to the nearest
+    2^-16.  seed is an int64 tensor of one element on the GPU, read when the kernel runs: the same seed gives
+    the same mask for a tensor of the same sizes, so every call wants one of its own (torch.randint's, say, which a
+    captured graph draws anew on each replay); what the backward uses is the value that the forward read.
+    Element e of f is kept where the 16-bit number e % 8 of Philox4x32-10(counter e // 8, key seed) is at
+    least 65536 p.  stepwise rounds the dropped-out product too.
+
     Gradients for x, branch, gate, weight, bias and branch_bias; sums over the rows run in a fixed
     order.  A backward that is differentiated again runs through torch's operators."""
-    out = _lib.native().residual_norm(x, branch, weight, bias, eps, gate, branch_bias, scale, stepwise, False)
-    return _refuse(x, branch, weight, bias, gate, branch_bias) if out is None else out
+    if not 0 <= dropout < 1 - 2.0 ** -17:
+        raise ValueError(f"dropout must be in [0, 1 - 2^-17), got {dropout}")
+    if dropout and not isinstance(seed, torch.Tensor):
+        raise TypeError("dropout needs a seed: an int64 tensor of one element on the GPU")
+    out = _lib.native().residual_norm_dropout(x, branch, weight, bias, eps, gate, branch_bias, scale, stepwise, False, dropout, seed)
+    return _refuse(x, branch, weight, bias, gate, branch_bias, seed if dropout else None) if out is None else out
 
 
-def _refuse(x, branch, weight, bias, gate, branch_bias):
+def _refuse(x, branch, weight, bias, gate, branch_bias, seed):
     """Raises for a call that the kernels do not take, and says why."""
     for name, t in (("x", x), ("branch", branch), ("gate", gate)):
         if t is None:
@@ -62,6 +76,8 @@ def _refuse(x, branch, weight, bias, gate, branch_bias):
             raise TypeError(f"{name} must be a bfloat16, float32 or float16 tensor")
         if tuple(t.shape) != (C,):
             raise ValueError(f"{name} must be [C] = {(C,)}, got {tuple(t.shape)}")
-    if len({t.device for t in (x, branch, gate, weight, bias, branch_bias) if t is not None}) != 1:
+    if seed is not None and (seed.dtype != torch.int64 or seed.numel() != 1):
+        raise TypeError(f"seed must be an int64 tensor of one element, got {seed.dtype} {tuple(seed.shape)}")
+    if len({t.device for t in (x, branch, gate, weight, bias, branch_bias, seed) if t is not None}) != 1:
         raise ValueError("all tensors must be on the same device")
     raise NotImplementedError("residual_norm takes dense (strided) tensors of at most 2^40 elements")
