@@ -17,16 +17,22 @@
 //   d_g = the suffix sums of d_G in the chunk.
 //
 // Kernels: `prep` (G and T, a block a chunk), `fwd` (a walk over the chunks), `bwd` (the walk back,
-// for d_v and D), `grads` (the rest, a block a chunk), `step` (a few tokens).  Only k S, T (..) and k^T (..)
-// follow one another in a walk.  Its columns are independent of each other: a wave keeps 16 columns of S in
-// its accumulators, and since an accumulator's rows are what the next product contracts over, it hands every
-// intermediate on in registers (the contraction's order is permuted to the accumulators' one, see `rows`).
+// for d_v and D), `grads` (the rest, a block a chunk), `step` (a few tokens).
 //
-// Numbers.  q, k, v and d_o are bf16 and enter the products as they are.  Everything computed (S, T, n,
-// P, ...) is 32 bits and enters as a sum of two bf16, 2^-17 of the value off at most: one product where
-// torch would run one in 32 bits becomes two (bf16 times computed) or three (computed times computed, without
-// the two low halves), 5 to 8 times the rate of the matrix instructions in 32 bits.  Final states and the
-// gradients of g and beta so have the precision of 32-bit arithmetic, not of bf16.
+// A walk.  Only k S, T (..) and k^T (..) follow one another from chunk to chunk, and their columns are
+// independent of each other: a wave keeps 16 columns of S in its accumulators, and since an accumulator's rows are
+// what the next product contracts over, it hands every intermediate on in registers (the contraction's order is
+// permuted to the accumulators' one, see `GD_POS`) and meets the others only for what they share.  Four such
+// waves have a block; four more bring the next chunk in and form P, so that the chain's waves issue nothing else: a walk
+// is bound by the instructions of that one wave a SIMD.
+//
+// Numbers.  q, k, v and d_o are bf16 and enter the products as they are.  Everything computed (S, n, T, P,
+// ...) is 32 bits and enters as a sum of three bf16 numbers, nothing of it lost: a product that torch would run in
+// 32 bits becomes three of bf16 (bf16 times computed) or six (computed times computed, without the halves that
+// lie below 2^-24), 5 and 2.5 times the rate of the matrix instructions in 32 bits; T (..), whose operands would both
+// have to be taken apart, runs in those.  What ends in a bf16 output alone (o; p and m of d_q and d_k) is
+// taken as two numbers, 2^-16 off at most.  Final states and the gradients of g and beta so have the precision of
+// 32-bit arithmetic, not of bf16.
 // G is summed in 64 bits and kept as a pair of floats: decays between neighbours late in a chunk are
 // differences of large sums.
 #include "common.h"
@@ -34,7 +40,9 @@
 
 #define GD_C 64                 // tokens of a chunk
 #define GD_PAD 8                // elements behind a row of an LDS tile
-#define GD_TS (GD_C + GD_PAD)   // row of a tile of 64 columns
+#define GD_TS (GD_C + GD_PAD)   // row of a bf16 tile of 64 columns
+#define GD_TF (GD_C + 4)        // row of T in 32 bits
+#define GD_TB 2560              // T in memory: the ten 16 x 16 blocks of its triangle
 #define GD_FLOOR (-1024.f)      // log decays below are this one: e^-1024 is 0 in 32 bits
 #define GD_STEP_WAVES 4
 
@@ -48,48 +56,77 @@ struct GdShape {
     int H, HV, T, NC, V;        // key heads, value heads, tokens, chunks, value channels
     int64_t BH;                 // sequences times value heads
 };
-struct Pair {                   // a computed operand: hi + lo
+struct Two {                    // a computed operand: h + l, 2^-16 off at most
     bf16x8 h, l;
 };
+struct Three {                  // h + m + l, exact
+    bf16x8 h, m, l;
+};
 
-__device__ __forceinline__ Pair split8(const float* x) {
-    float f[8], d[8];
-    const uint4 h = pack8(x);
+__device__ __forceinline__ uint4 rest8(float* x, uint4 h) {        // x less what h holds of it, and that as bf16
+    float f[8];
     unpack8(h, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) d[j] = x[j] - f[j];
-    return {__builtin_bit_cast(bf16x8, h), __builtin_bit_cast(bf16x8, pack8(d))};
+    for (int j = 0; j < 8; ++j) x[j] -= f[j];
+    return pack8(x);
 }
-__device__ __forceinline__ Pair split_tiles(f32x4 a, f32x4 b) {
-    const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    return split8(x);
+__device__ __forceinline__ Three three(f32x4 a, f32x4 b) {
+    float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    const uint4 h = pack8(x), m = rest8(x, h), l = rest8(x, m);
+    return {__builtin_bit_cast(bf16x8, h), __builtin_bit_cast(bf16x8, m), __builtin_bit_cast(bf16x8, l)};
 }
-// one computed operand, one of bf16
-__device__ __forceinline__ f32x4 mm(bf16x8 a, const Pair& b, f32x4 c) { return mfma32(a, b.h, mfma32(a, b.l, c)); }
-__device__ __forceinline__ f32x4 mm(const Pair& a, bf16x8 b, f32x4 c) { return mfma32(a.h, b, mfma32(a.l, b, c)); }
-// both computed
-__device__ __forceinline__ f32x4 mm(const Pair& a, const Pair& b, f32x4 c) {
+__device__ __forceinline__ Two two(f32x4 a, f32x4 b) {
+    float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    const uint4 h = pack8(x);
+    return {__builtin_bit_cast(bf16x8, h), __builtin_bit_cast(bf16x8, rest8(x, h))};
+}
+// four values in parts of bf16, 8 bytes each
+__device__ __forceinline__ uint2 rest4(float* x, uint2 h) {
+    float f[4];
+    unpack4(h, f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] -= f[j];
+    return make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
+}
+__device__ __forceinline__ f32x4 mm(bf16x8 a, const Two& b, f32x4 c) { return mfma32(a, b.h, mfma32(a, b.l, c)); }
+__device__ __forceinline__ f32x4 mm(const Two& a, bf16x8 b, f32x4 c) { return mfma32(a.h, b, mfma32(a.l, b, c)); }
+__device__ __forceinline__ f32x4 mm(const Two& a, const Two& b, f32x4 c) {
     return mfma32(a.h, b.h, mfma32(a.h, b.l, mfma32(a.l, b.h, c)));
 }
+__device__ __forceinline__ f32x4 mm(bf16x8 a, const Three& b, f32x4 c) {
+    return mfma32(a, b.h, mfma32(a, b.m, mfma32(a, b.l, c)));
+}
+__device__ __forceinline__ f32x4 mm(const Three& a, bf16x8 b, f32x4 c) {
+    return mfma32(a.h, b, mfma32(a.m, b, mfma32(a.l, b, c)));
+}
+__device__ __forceinline__ f32x4 mm(const Three& a, const Three& b, f32x4 c) {
+    c = mfma32(a.m, b.m, mfma32(a.h, b.l, mfma32(a.l, b.h, c)));
+    return mfma32(a.h, b.h, mfma32(a.h, b.m, mfma32(a.m, b.h, c)));
+}
 
-// Operand of 16 rows of a row-major tile, contracted over its columns c0 .. c0 + 31 in the accumulators'
-// order: slot 8q + j stands for column c0 + 16 (j / 4) + 4q + j % 4, so that two accumulator tiles, whose lane
-// holds rows 4q .. 4q + 3, are the other operand as they are.
+// The walks' contraction order: slot 8q + j of 32 stands for index 16 (j / 4) + 4q + j % 4, so that two accumulator
+// tiles, whose lane holds rows 4q .. 4q + 3, are an operand as they are.  q and k lie in LDS with their columns in
+// that order: column c at place GD_POS(c) of its row.
+#define GD_POS(c) (((c) & ~31) + 8 * (((c) >> 2) & 3) + 4 * (((c) >> 4) & 1) + ((c) & 3))
+// Operand of 16 rows of such a tile, contracted over its columns c0 .. c0 + 31.
+__device__ __forceinline__ bf16x8 prows(const uint16_t* X, int stride, int r0, int c0, int lane) {
+    return ld_bf16x8(X + (r0 + (lane & 15)) * stride + c0 + 8 * (lane >> 4));
+}
+// Its transposed: 16 columns, contracted over the rows r0 .. r0 + 31 in the walks' order.
+__device__ __forceinline__ bf16x8 pcols(const uint16_t* X, int stride, int r0, int c0, int lane) {
+    const int L = lane & 15, q = lane >> 4;
+    const uint16_t* p = X + (r0 + 4 * q + (L >> 2)) * stride + GD_POS(c0) + 8 * (L & 3);
+    return cat_bf16x8(lds_tr16(p), lds_tr16(p + 16 * stride));
+}
+// The same two of a tile in plain order.
 __device__ __forceinline__ bf16x8 rows(const uint16_t* X, int stride, int r0, int c0, int lane) {
     const uint16_t* p = X + (r0 + (lane & 15)) * stride + c0 + 4 * (lane >> 4);
     return cat_bf16x8(ld_bf16x4(p), ld_bf16x4(p + 16));
 }
-// The transposed one: 16 columns, contracted over the rows r0 .. r0 + 31, in the same order.
 __device__ __forceinline__ bf16x8 cols(const uint16_t* X, int stride, int r0, int c0, int lane) {
     const int L = lane & 15, q = lane >> 4;
     const uint16_t* p = X + (r0 + 4 * q + (L >> 2)) * stride + c0 + 4 * (L & 3);
     return cat_bf16x8(lds_tr16(p), lds_tr16(p + 16 * stride));
-}
-__device__ __forceinline__ Pair rows2(const uint16_t* H, const uint16_t* L, int stride, int r0, int c0, int lane) {
-    return {rows(H, stride, r0, c0, lane), rows(L, stride, r0, c0, lane)};
-}
-__device__ __forceinline__ Pair cols2(const uint16_t* H, const uint16_t* L, int stride, int r0, int c0, int lane) {
-    return {cols(H, stride, r0, c0, lane), cols(L, stride, r0, c0, lane)};
 }
 // Rows r0 + 4q .. + 3 of column c0 + lr: a bf16 tile's values as an accumulator tile's lane holds them.
 __device__ __forceinline__ f32x4 as_acc(const uint16_t* X, int stride, int r0, int c0, int lane) {
@@ -99,75 +136,94 @@ __device__ __forceinline__ f32x4 as_acc(const uint16_t* X, int stride, int r0, i
     unpack4(x, f);
     return f32x4{f[0], f[1], f[2], f[3]};
 }
+__device__ __forceinline__ f32x4 at4(const float* p, int i) { return *reinterpret_cast<const f32x4*>(p + i); }
+// T X (or T^T X, T lying transposed): tile I from the tiles up to the diagonal (or from it), in 32 bits.  Step r of
+// a tile contracts over its rows 4q + r.
+__device__ __forceinline__ f32x4 mul_t(const float* T, int I, int J, const f32x4& x, f32x4 c, int lane) {
+    const f32x4 a = at4(T, (16 * I + (lane & 15)) * GD_TF + 16 * J + 4 * (lane >> 4));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], x[r], c, 0, 0, 0);
+    return c;
+}
 __device__ __forceinline__ float gd_gap(float2 a, float2 b) { return (a.x - b.x) + (a.y - b.y); }
 __device__ __forceinline__ float gd_beta(const void* p, int dt, int64_t i) {
     return dt == RWKV6_BF16 ? bf2f(reinterpret_cast<const uint16_t*>(p)[i]) : reinterpret_cast<const float*>(p)[i];
 }
-// Operands in memory as the walks hold them: [chunk][16 columns][32 contracted][hi, lo][lane][8].
-__device__ __forceinline__ void put_pair(uint16_t* base, int64_t n, int lane, const Pair& p) {
-    uint4* d = reinterpret_cast<uint4*>(base) + n * 128 + lane;
-    d[0] = __builtin_bit_cast(uint4, p.h);
-    d[64] = __builtin_bit_cast(uint4, p.l);
-}
+__device__ __forceinline__ int gd_block_row(int t) { return t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0; }
+// Accumulator tiles in memory: [chunk][16 columns][tile][lane][4].
+__device__ __forceinline__ void put_tiles(float* p, f32x4 x, int lane) { *reinterpret_cast<f32x4*>(p + 4 * lane) = x; }
 
-// N 16-byte pieces a thread of a [64][8 * per_row] tile (zeros behind the last token), and into LDS.
+// 16-byte pieces of 256 threads of a [64][COLS] tile, zeros behind the last token.
 template <int COLS> struct TileRegs {
     uint4 q[COLS / 32];
 };
 template <int COLS>
 __device__ __forceinline__ TileRegs<COLS> tile_load(const uint16_t* p, int64_t st, int t0, int T, int tid) {
+    constexpr int per = COLS / 8, step = 256 / per;            // pieces of a row, rows of a step
     TileRegs<COLS> r;
+    const int row = tid / per;
+    const uint16_t* x = p + (int64_t)(t0 + row) * st + 8 * (tid % per);
+    if (t0 + GD_C <= T) {
 #pragma unroll
-    for (int i = 0; i < COLS / 32; ++i) {
-        const int n = tid + 256 * i, row = n / (COLS / 8), col = 8 * (n % (COLS / 8)), t = t0 + row;
-        r.q[i] = *reinterpret_cast<const uint4*>(p + (int64_t)(t < T ? t : T - 1) * st + col);
-        if (t >= T) r.q[i] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < COLS / 32; ++i, x += step * st) r.q[i] = *reinterpret_cast<const uint4*>(x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < COLS / 32; ++i, x += step * st) {
+            r.q[i] = make_uint4(0, 0, 0, 0);
+            if (t0 + row + step * i < T) r.q[i] = *reinterpret_cast<const uint4*>(x);
+        }
     }
     return r;
 }
-template <int COLS>
+template <int COLS, bool PERMUTED>
 __device__ __forceinline__ void tile_store(const TileRegs<COLS>& r, uint16_t* X, int tid) {
+    constexpr int per = COLS / 8, step = 256 / per;
+    const int col = 8 * (tid % per);
+    uint16_t* p = X + (tid / per) * (COLS + GD_PAD) + (PERMUTED ? GD_POS(col) : col);
 #pragma unroll
-    for (int i = 0; i < COLS / 32; ++i) {
-        const int n = tid + 256 * i, row = n / (COLS / 8), col = 8 * (n % (COLS / 8));
-        *reinterpret_cast<uint4*>(X + row * (COLS + GD_PAD) + col) = r.q[i];
+    for (int i = 0; i < COLS / 32; ++i, p += step * (COLS + GD_PAD)) {
+        if constexpr (PERMUTED) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(r.q[i].x, r.q[i].y);
+            *reinterpret_cast<uint2*>(p + 8) = make_uint2(r.q[i].z, r.q[i].w);
+        } else {
+            *reinterpret_cast<uint4*>(p) = r.q[i];
+        }
     }
 }
 
-// P of a chunk as hi and lo tiles [i][j], by four waves: tile t of the triangle's ten by wave t % 4, formed
+// P of a chunk in N parts, tiles [i][j], by four waves: tile t of the triangle's ten by wave t % 4, formed
 // transposed, so that a lane has four adjacent j.  The blocks right of the diagonal are zeroed by `gd_zero_p`.
-template <int K>
-__device__ __forceinline__ void gd_p(const uint16_t* Qt, const uint16_t* Kt, const float2* G, float scale, uint16_t* Ph,
-                                     uint16_t* Pl, int wave, int lane) {
+template <int K, int N>
+__device__ __forceinline__ void gd_p(const uint16_t* Qt, const uint16_t* Kt, const float2* G, float scale, uint16_t* P, int wave,
+                                     int lane) {
     const int lr = lane & 15, q = lane >> 4;
 #pragma unroll
     for (int u = 0; u < 3; ++u) {
         const int t = wave + 4 * u;
         if (t >= 10) break;
-        const int I = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0, J = t - I * (I + 1) / 2;
+        const int I = gd_block_row(t), J = t - I * (I + 1) / 2;
         f32x4 a = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < K / 32; ++s)
-            a = mfma32(rows(Kt, K + GD_PAD, 16 * J, 32 * s, lane), rows(Qt, K + GD_PAD, 16 * I, 32 * s, lane), a);
+            a = mfma32(prows(Kt, K + GD_PAD, 16 * J, 32 * s, lane), prows(Qt, K + GD_PAD, 16 * I, 32 * s, lane), a);
         const int i = 16 * I + lr, j = 16 * J + 4 * q;
         const float2 gi = G[i];
-        float x[4], d[4], f[4];
+        float x[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = i >= j + r ? scale * ex2(gd_gap(gi, G[j + r])) * a[r] : 0.f;
-        const uint2 h = make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
-        unpack4(h, f);
+        uint2 part = make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) d[r] = x[r] - f[r];
-        *reinterpret_cast<uint2*>(Ph + i * GD_TS + j) = h;
-        *reinterpret_cast<uint2*>(Pl + i * GD_TS + j) = make_uint2(pk2(d[0], d[1]), pk2(d[2], d[3]));
+        for (int m = 0; m < N; ++m) {
+            *reinterpret_cast<uint2*>(P + m * GD_C * GD_TS + i * GD_TS + j) = part;
+            if (m + 1 < N) part = rest4(x, part);
+        }
     }
 }
-__device__ __forceinline__ void gd_zero_p(uint16_t* Ph, uint16_t* Pl, int tid) {
-    // blocks (0,1) and (2,3): 2 x 16 rows of 32 bytes, hi and lo
-    if (tid < 128) {
+template <int N> __device__ __forceinline__ void gd_zero_p(uint16_t* P, int tid) {
+    // blocks (0,1) and (2,3): 2 x 16 rows of 32 bytes a part
+    if (tid < 64 * N) {
         const int row = (tid >> 1) & 15, b = (tid >> 5) & 1, half = tid & 1;
-        uint16_t* P = tid & 64 ? Pl : Ph;
-        *reinterpret_cast<uint4*>(P + (32 * b + row) * GD_TS + 32 * b + 16 + 8 * half) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(P + (tid >> 6) * GD_C * GD_TS + (32 * b + row) * GD_TS + 32 * b + 16 + 8 * half) = make_uint4(0, 0, 0, 0);
     }
 }
 
@@ -176,12 +232,12 @@ __device__ __forceinline__ void gd_zero_p(uint16_t* Ph, uint16_t* Pl, int tid) {
 // G and T of a chunk.  Wave w forms the rows of its 16-token block of A = beta L k k^T, inverts the block
 // on the diagonal by substitution, and then column w of the blocks below it, in the 32-bit matrix instructions:
 // T_IJ = -T_II sum_{J<=l<I} A_Il T_lJ.  Out: G [chunk][64] as pairs of floats in base-2 units, T [chunk]
-// [hi, lo][64][64].
+// [10 blocks][16][16].
 template <int K>
 __global__ void __launch_bounds__(256)
 rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const void* __restrict__ beta, int beta_dt,
-                              float2* __restrict__ G_out, uint16_t* __restrict__ T_out, GdShape n) {
-    __shared__ __attribute__((aligned(16))) float As[GD_C][GD_C + 4], Ts[GD_C][GD_C + 4];
+                              float2* __restrict__ G_out, float* __restrict__ T_out, GdShape n) {
+    __shared__ __attribute__((aligned(16))) float As[GD_C][GD_TF], Ts[GD_C][GD_TF];
     __shared__ float2 G[GD_C];
     __shared__ float be[GD_C];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q = lane >> 4;
@@ -221,14 +277,13 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
         for (int J = 0; J <= I; ++J) {
             f32x4 a = {0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < K / 32; ++s) a = mfma32(f[I][s], f[J][s], a);
-            const int j = 16 * J + lr;
-            const float2 gj = G[j];
+            for (int s = 0; s < K / 32; ++s) a = mfma32(f[J][s], f[I][s], a);        // transposed: row i = lr
+            const int i = 16 * I + lr, j = 16 * J + 4 * q;
+            const float2 gi = G[i];
+            f32x4 x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * I + 4 * q + r;
-                As[i][j] = i > j ? be[i] * ex2(gd_gap(G[i], gj)) * a[r] : 0.f;
-            }
+            for (int r = 0; r < 4; ++r) x[r] = i > j + r ? be[i] * ex2(gd_gap(gi, G[j + r])) * a[r] : 0.f;
+            *reinterpret_cast<f32x4*>(&As[i][j]) = x;
         }
     }
     __syncthreads();
@@ -240,8 +295,9 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
             float a[16], s0 = r == lr ? 1.f : 0.f, s1 = 0.f;
 #pragma unroll
             for (int s = 0; s < r; s += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(&As[b + r][b + s]);
-                a[s] = v.x, a[s + 1] = v.y, a[s + 2] = v.z, a[s + 3] = v.w;
+                const f32x4 v = at4(&As[b + r][b + s], 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[s + j] = v[j];
             }
 #pragma unroll
             for (int s = 0; s < r; ++s) (s & 1 ? s1 : s0) -= a[s] * x[s];
@@ -260,94 +316,99 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
         for (int I = J + 1; I < 4; ++I) {
             f32x4 a = {0, 0, 0, 0}, d = {0, 0, 0, 0};
 #pragma unroll
-            for (int l = J; l < I; ++l) {
-                const float4 v = *reinterpret_cast<const float4*>(&As[16 * I + lr][16 * l + 4 * q]);
-                const float w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int r = 0; r < 4; ++r) a = __builtin_amdgcn_mfma_f32_16x16x4f32(w[r], t[l][r], a, 0, 0, 0);
-            }
-            const float4 v = *reinterpret_cast<const float4*>(&Ts[16 * I + lr][16 * I + 4 * q]);
-            const float w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int r = 0; r < 4; ++r) d = __builtin_amdgcn_mfma_f32_16x16x4f32(w[r], a[r], d, 0, 0, 0);
+            for (int l = J; l < I; ++l) a = mul_t(&As[0][0], I, l, t[l], a, lane);
+            d = mul_t(&Ts[0][0], I, I, a, d, lane);
             t[I] = -d;
 #pragma unroll
             for (int r = 0; r < 4; ++r) Ts[16 * I + 4 * q + r][16 * J + lr] = t[I][r];
         }
     }
     __syncthreads();
-    const int row = tid >> 2, cb = tid & 3;
-    uint4* out = reinterpret_cast<uint4*>(T_out + chunk * (2 * GD_C * GD_C) + row * GD_C + 16 * cb);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = cb <= (row >> 4) ? Ts[row][16 * cb + 8 * h + j] : 0.f;
-        const Pair p = split8(x);
-        out[h] = __builtin_bit_cast(uint4, p.h);
-        out[h + GD_C * GD_C / 8] = __builtin_bit_cast(uint4, p.l);
+    for (int i = tid; i < GD_TB / 4; i += 256) {
+        const int t = i >> 6, I = gd_block_row(t), J = t - I * (I + 1) / 2;
+        reinterpret_cast<f32x4*>(T_out + chunk * GD_TB)[i] = at4(&Ts[16 * I + ((i >> 2) & 15)][16 * J + 4 * (i & 3)], 0);
     }
 }
 
 namespace {
-// LDS of the walks: two buffers of q, k, v (or d_o), T hi and lo, G, e^G, e^{G_C - G}, beta; then P hi and lo.
-template <int K> struct WalkLds {
-    static constexpr int qk = GD_C * (K + GD_PAD), t = GD_C * GD_TS;
-    static constexpr int buf = 2 * qk + 3 * t + (8 + 3 * 4) / 2 * GD_C;          // in elements of 2 bytes
-    static constexpr size_t bytes = (size_t)(2 * buf + 2 * t) * 2;
+// LDS of the walks: two buffers of q, k, v (or d_o), T, G, e^G, e^{G_C - G}, beta; then P in NP parts.
+template <int K, int NP> struct WalkLds {
+    static constexpr int qk = GD_C * (K + GD_PAD), t = GD_C * GD_TS, tf = GD_C * GD_TF * 2;
+    static constexpr int buf = 2 * qk + t + tf + (8 + 3 * 4) / 2 * GD_C;          // in elements of 2 bytes
+    static constexpr size_t bytes = (size_t)(2 * buf + NP * t) * 2;
 };
 struct WalkBuf {
-    uint16_t *Q, *K, *V, *Th, *Tl;
+    uint16_t *Q, *K, *V;
+    float* T;
     float2* G;
     float *eG, *eL, *be;
 };
 template <int K> __device__ __forceinline__ WalkBuf walk_buf(uint16_t* p) {
-    using L = WalkLds<K>;
+    using L = WalkLds<K, 0>;
     WalkBuf b;
     b.Q = p;
     b.K = p + L::qk;
     b.V = p + 2 * L::qk;
-    b.Th = b.V + L::t;
-    b.Tl = b.Th + L::t;
-    b.G = reinterpret_cast<float2*>(b.Tl + L::t);
+    b.T = reinterpret_cast<float*>(b.V + L::t);
+    b.G = reinterpret_cast<float2*>(b.T + GD_C * GD_TF);
     b.eG = reinterpret_cast<float*>(b.G + GD_C);
     b.eL = b.eG + GD_C;
     b.be = b.eL + GD_C;
     return b;
 }
-// One chunk's inputs on their way from memory to LDS.
+// One chunk's inputs on their way from memory to LDS, in 256 threads.
 template <int K> struct WalkRegs {
     TileRegs<K> q, k;
-    TileRegs<64> v, th, tl;
+    TileRegs<64> v;
+    f32x4 t[3];
     float2 G, GC;
     float be;
 };
+struct WalkIn {
+    const uint16_t *q, *k, *v;
+    int64_t qs, ks, vs;
+    const float* T;
+    const float2* G;
+    const void* beta;
+    int beta_dt;
+    int64_t bh;
+};
 template <int K>
-__device__ __forceinline__ WalkRegs<K> walk_load(const uint16_t* qp, int64_t qs, const uint16_t* kp, int64_t ks, const uint16_t* vp,
-                                                 int64_t vs, const uint16_t* T, const float2* G, const void* beta, int beta_dt,
-                                                 int64_t bh, int c, const GdShape& n, int tid) {
+__device__ __forceinline__ WalkRegs<K> walk_load(const WalkIn& w, int c, const GdShape& n, int tid) {
     WalkRegs<K> r;
     const int t0 = c * GD_C;
-    const int64_t chunk = bh * n.NC + c;
-    r.k = tile_load<K>(kp, ks, t0, n.T, tid);
-    r.th = tile_load<64>(T + chunk * (2 * GD_C * GD_C), GD_C, 0, GD_C, tid);
-    r.tl = tile_load<64>(T + chunk * (2 * GD_C * GD_C) + GD_C * GD_C, GD_C, 0, GD_C, tid);
-    r.v = tile_load<64>(vp, vs, t0, n.T, tid);
-    r.q = tile_load<K>(qp, qs, t0, n.T, tid);
+    const int64_t chunk = w.bh * n.NC + c;
+    r.k = tile_load<K>(w.k, w.ks, t0, n.T, tid);
+    r.q = tile_load<K>(w.q, w.qs, t0, n.T, tid);
+    const f32x4* T = reinterpret_cast<const f32x4*>(w.T + chunk * GD_TB);
+    r.t[0] = T[tid];
+    r.t[1] = T[tid + 256];
+    if (tid < GD_TB / 4 - 512) r.t[2] = T[tid + 512];
+    r.v = tile_load<64>(w.v, w.vs, t0, n.T, tid);
     if (tid < GD_C) {
-        r.G = G[chunk * GD_C + tid];
-        r.GC = G[chunk * GD_C + GD_C - 1];
-        r.be = t0 + tid < n.T ? gd_beta(beta, beta_dt, bh * n.T + t0 + tid) : 0.f;
+        r.G = w.G[chunk * GD_C + tid];
+        r.GC = w.G[chunk * GD_C + GD_C - 1];
+        r.be = t0 + tid < n.T ? gd_beta(w.beta, w.beta_dt, w.bh * n.T + t0 + tid) : 0.f;
     }
     return r;
 }
-template <int K>
+template <int K, bool TRANSPOSED>
 __device__ __forceinline__ void walk_store(const WalkRegs<K>& r, const WalkBuf& L, int tid) {
-    tile_store<K>(r.q, L.Q, tid);
-    tile_store<K>(r.k, L.K, tid);
-    tile_store<64>(r.v, L.V, tid);
-    tile_store<64>(r.th, L.Th, tid);
-    tile_store<64>(r.tl, L.Tl, tid);
+    tile_store<K, true>(r.k, L.K, tid);
+    tile_store<K, true>(r.q, L.Q, tid);
+    tile_store<64, false>(r.v, L.V, tid);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        if (i == 2 && tid >= GD_TB / 4 - 512) break;
+        const int p = tid + 256 * i, t = p >> 6, I = gd_block_row(t), J = t - I * (I + 1) / 2;
+        const int row = 16 * I + ((p >> 2) & 15), col = 16 * J + 4 * (p & 3);
+        if constexpr (TRANSPOSED) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) L.T[(col + j) * GD_TF + row] = r.t[i][j];
+        } else {
+            *reinterpret_cast<f32x4*>(L.T + row * GD_TF + col) = r.t[i];
+        }
+    }
     if (tid < GD_C) {
         L.G[tid] = r.G;
         L.eG[tid] = ex2(r.G.x);
@@ -355,269 +416,301 @@ __device__ __forceinline__ void walk_store(const WalkRegs<K>& r, const WalkBuf& 
         L.be[tid] = r.be;
     }
 }
+// Which head and 64 columns a block walks: blocks of a head's other columns follow a multiple of 8 later where the
+// heads are one, on the same XCD, and find its q, k and T in that L2.
+struct WalkAt {
+    int64_t bh, b;
+    int hv, hk, v0;
+};
+__device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
+    WalkAt w;
+    w.bh = blockIdx.x % n.BH;
+    w.b = w.bh / n.HV;
+    w.hv = (int)(w.bh % n.HV);
+    w.hk = w.hv / (n.HV / n.H);
+    w.v0 = 64 * (int)(blockIdx.x / n.BH);
+    return w;
+}
 }  // namespace
 
-// A block walks one head's chunks with 64 columns of the state, a wave 16 of them.  S_save and n_save (the
-// backward's, or null) get the state entering each chunk and the values it writes.
+// A block walks one head's chunks with 64 columns of the state.  S_save and n_save (the backward's, or null) get
+// the state entering each chunk and the values it writes.
 template <int K>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const void* __restrict__ beta, int beta_dt,
-                             const float2* __restrict__ G, const uint16_t* __restrict__ T, const float* __restrict__ h0,
-                             uint16_t* __restrict__ o, float* __restrict__ hT, uint16_t* __restrict__ S_save,
-                             uint16_t* __restrict__ n_save, GdShape n, float scale) {
+                             const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ h0,
+                             uint16_t* __restrict__ o, float* __restrict__ hT, float* __restrict__ S_save,
+                             float* __restrict__ n_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
-    uint16_t *const Ph = gd_lds + 2 * WalkLds<K>::buf, *const Pl = Ph + WalkLds<K>::t;
+    using M = WalkLds<K, 2>;
+    uint16_t* const P = gd_lds + 2 * M::buf;
     constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
-    const int64_t bh = blockIdx.x % n.BH, b = bh / n.HV;
-    const int hv = (int)(bh % n.HV), hk = hv / (n.HV / n.H), v0 = 64 * (int)(blockIdx.x / n.BH), ct = v0 / 16 + wave;
-    const uint16_t *qp = q.p + b * q.sb + hk * q.sh, *kp = k.p + b * k.sb + hk * k.sh, *vp = v.p + b * v.sb + hv * v.sh + v0;
-    const int col = v0 + 16 * wave + lr;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, lr = lane & 15, lq = lane >> 4;
+    const WalkAt w = walk_at(n);
+    if (threadIdx.x >= 256) {                              // the next chunk, and P of this one
+        const int tid = threadIdx.x - 256;
+        const WalkIn in = {q.p + w.b * q.sb + w.hk * q.sh, k.p + w.b * k.sb + w.hk * k.sh, v.p + w.b * v.sb + w.hv * v.sh + w.v0,
+                           q.st, k.st, v.st, T, G, beta, beta_dt, w.bh};
+        gd_zero_p<2>(P, tid);
+        if (n.NC) walk_store<K, false>(walk_load<K>(in, 0, n, tid), walk_buf<K>(gd_lds), tid);
+        for (int c = 0; c < n.NC; ++c) {
+            const int u = c & 1;
+            const WalkBuf L = walk_buf<K>(gd_lds + u * M::buf);
+            __syncthreads();
+            WalkRegs<K> next;
+            if (c + 1 < n.NC) next = walk_load<K>(in, c + 1, n, tid);
+            gd_p<K, 2>(L.Q, L.K, L.G, scale, P, wave, lane);
+            __syncthreads();
+            if (c + 1 < n.NC) walk_store<K, false>(next, walk_buf<K>(gd_lds + (u ^ 1) * M::buf), tid);
+        }
+        return;
+    }
+    const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
     f32x4 S[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[d][r] = h0 ? h0[(bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
-    gd_zero_p(Ph, Pl, tid);
-    if (n.NC) walk_store<K>(walk_load<K>(qp, q.st, kp, k.st, vp, v.st, T, G, beta, beta_dt, bh, 0, n, tid), walk_buf<K>(gd_lds), tid);
+        for (int r = 0; r < 4; ++r) S[d][r] = h0 ? h0[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
     for (int c = 0; c < n.NC; ++c) {
-        const int u = c & 1;
-        const WalkBuf L = walk_buf<K>(gd_lds + u * WalkLds<K>::buf);
-        const int64_t chunk = bh * n.NC + c;
-        __syncthreads();
-        const bool more = c + 1 < n.NC;
-        WalkRegs<K> next;
-        if (more) next = walk_load<K>(qp, q.st, kp, k.st, vp, v.st, T, G, beta, beta_dt, bh, c + 1, n, tid);
-        gd_p<K>(L.Q, L.K, L.G, scale, Ph, Pl, wave, lane);
-        Pair Sp[NS];
+        const WalkBuf L = walk_buf<K>(gd_lds + (c & 1) * M::buf);
+        const int64_t at = (w.bh * n.NC + c) * (n.V / 16) + ct;
+        Three Sp[NS];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            Sp[s] = split_tiles(S[2 * s], S[2 * s + 1]);
-            if (S_save) put_pair(S_save, (chunk * (n.V / 16) + ct) * NS + s, lane, Sp[s]);
-        }
-        f32x4 E[4];
+        for (int s = 0; s < NS; ++s) Sp[s] = three(S[2 * s], S[2 * s + 1]);
+        if (S_save)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) put_tiles(S_save + (at * ND + d) * 256, S[d], lane);
+        __syncthreads();
+        f32x4 E[4], N[4];
 #pragma unroll
         for (int I = 0; I < 4; ++I) {
             f32x4 a = {0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < NS; ++s) a = mm(rows(L.K, KS, 16 * I, 32 * s, lane), Sp[s], a);
+            for (int s = 0; s < NS; ++s) a = mm(prows(L.K, KS, 16 * I, 32 * s, lane), Sp[s], a);
             const f32x4 x = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * I + 4 * lq + r;
-                E[I][r] = L.be[i] * (x[r] - L.eG[i] * a[r]);
-            }
+            E[I] = at4(L.be, 16 * I + 4 * lq) * (x - at4(L.eG, 16 * I + 4 * lq) * a);
         }
-        Pair Ep[2] = {split_tiles(E[0], E[1]), split_tiles(E[2], E[3])};
-        f32x4 N[4];
 #pragma unroll
         for (int I = 0; I < 4; ++I) {
             N[I] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s <= I / 2; ++s) N[I] = mm(rows2(L.Th, L.Tl, GD_TS, 16 * I, 32 * s, lane), Ep[s], N[I]);
+            for (int J = 0; J <= I; ++J) N[I] = mul_t(L.T, I, J, E[J], N[I], lane);
         }
-        Pair Np[2] = {split_tiles(N[0], N[1]), split_tiles(N[2], N[3])};
-        if (n_save) {
-            put_pair(n_save, (chunk * (n.V / 16) + ct) * 2, lane, Np[0]);
-            put_pair(n_save, (chunk * (n.V / 16) + ct) * 2 + 1, lane, Np[1]);
-        }
+        if (n_save)
 #pragma unroll
-        for (int I = 0; I < 4; ++I)
+            for (int I = 0; I < 4; ++I) put_tiles(n_save + (at * 4 + I) * 256, N[I], lane);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) N[I][r] *= L.eL[16 * I + 4 * lq + r];
-        Ep[0] = split_tiles(N[0], N[1]);
-        Ep[1] = split_tiles(N[2], N[3]);
+        for (int I = 0; I < 4; ++I) E[I] = N[I] * at4(L.eL, 16 * I + 4 * lq);
+        const Three Ep[2] = {three(E[0], E[1]), three(E[2], E[3])};
         const float eC = L.eG[GD_C - 1];
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             S[d] *= eC;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) S[d] = mm(cols(L.K, KS, 32 * s, 16 * d, lane), Ep[s], S[d]);
+            for (int s = 0; s < 2; ++s) S[d] = mm(pcols(L.K, KS, 32 * s, 16 * d, lane), Ep[s], S[d]);
         }
+        const Two Np[2] = {two(N[0], N[1]), two(N[2], N[3])};
         __syncthreads();                                   // P
         // o transposed: a lane has four adjacent channels of a token
 #pragma unroll
         for (int I = 0; I < 4; ++I) {
             f32x4 a = {0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < NS; ++s) a = mm(Sp[s], rows(L.Q, KS, 16 * I, 32 * s, lane), a);
+            for (int s = 0; s < NS; ++s) a = mm(Two{Sp[s].h, Sp[s].m}, prows(L.Q, KS, 16 * I, 32 * s, lane), a);
             a *= scale * L.eG[16 * I + lr];
 #pragma unroll
-            for (int s = 0; s <= I / 2; ++s) a = mm(Np[s], rows2(Ph, Pl, GD_TS, 16 * I, 32 * s, lane), a);
+            for (int s = 0; s <= I / 2; ++s)
+                a = mm(Np[s], Two{rows(P, GD_TS, 16 * I, 32 * s, lane), rows(P + GD_C * GD_TS, GD_TS, 16 * I, 32 * s, lane)}, a);
             const int t = c * GD_C + 16 * I + lr;
             if (t < n.T)
-                *reinterpret_cast<uint2*>(o + (bh * n.T + t) * n.V + v0 + 16 * wave + 4 * lq) = make_uint2(pk2(a[0], a[1]), pk2(a[2], a[3]));
+                *reinterpret_cast<uint2*>(o + (w.bh * n.T + t) * n.V + w.v0 + 16 * wave + 4 * lq) = make_uint2(pk2(a[0], a[1]), pk2(a[2], a[3]));
         }
-        if (more) walk_store<K>(next, walk_buf<K>(gd_lds + (u ^ 1) * WalkLds<K>::buf), tid);
     }
     if (hT)
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) hT[(bh * K + 16 * d + 4 * lq + r) * n.V + col] = S[d][r];
+            for (int r = 0; r < 4; ++r) hT[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] = S[d][r];
 }
 
 // The walk back: d_v, and for the other gradients r and the gradient D of the state that each chunk leaves.
 template <int K>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const void* __restrict__ beta, int beta_dt,
-                             const float2* __restrict__ G, const uint16_t* __restrict__ T, const float* __restrict__ dhT,
-                             uint16_t* __restrict__ dv, float* __restrict__ dh0, uint16_t* __restrict__ D_save,
-                             uint16_t* __restrict__ r_save, GdShape n, float scale) {
+                             const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ dhT,
+                             uint16_t* __restrict__ dv, float* __restrict__ dh0, float* __restrict__ D_save,
+                             float* __restrict__ r_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
-    uint16_t *const Ph = gd_lds + 2 * WalkLds<K>::buf, *const Pl = Ph + WalkLds<K>::t;
-    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
-    const int64_t bh = blockIdx.x % n.BH, b = bh / n.HV;
-    const int hv = (int)(bh % n.HV), hk = hv / (n.HV / n.H), v0 = 64 * (int)(blockIdx.x / n.BH), ct = v0 / 16 + wave;
-    const uint16_t *qp = q.p + b * q.sb + hk * q.sh, *kp = k.p + b * k.sb + hk * k.sh, *op = d_o.p + b * d_o.sb + hv * d_o.sh + v0;
-    const int col = v0 + 16 * wave + lr;
+    using M = WalkLds<K, 3>;
+    uint16_t* const P = gd_lds + 2 * M::buf;
+    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS;
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, lr = lane & 15, lq = lane >> 4;
+    const WalkAt w = walk_at(n);
+    if (threadIdx.x >= 256) {
+        const int tid = threadIdx.x - 256;
+        const WalkIn in = {q.p + w.b * q.sb + w.hk * q.sh, k.p + w.b * k.sb + w.hk * k.sh, d_o.p + w.b * d_o.sb + w.hv * d_o.sh + w.v0,
+                           q.st, k.st, d_o.st, T, G, beta, beta_dt, w.bh};
+        gd_zero_p<3>(P, tid);
+        if (n.NC) walk_store<K, true>(walk_load<K>(in, n.NC - 1, n, tid), walk_buf<K>(gd_lds), tid);
+        for (int c = n.NC - 1, u = 0; c >= 0; --c, u ^= 1) {
+            const WalkBuf L = walk_buf<K>(gd_lds + u * M::buf);
+            __syncthreads();
+            WalkRegs<K> next;
+            if (c) next = walk_load<K>(in, c - 1, n, tid);
+            gd_p<K, 3>(L.Q, L.K, L.G, scale, P, wave, lane);
+            __syncthreads();
+            if (c) walk_store<K, true>(next, walk_buf<K>(gd_lds + (u ^ 1) * M::buf), tid);
+        }
+        return;
+    }
+    const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
     f32x4 D[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) D[d][r] = dhT ? dhT[(bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
-    gd_zero_p(Ph, Pl, tid);
-    if (n.NC) walk_store<K>(walk_load<K>(qp, q.st, kp, k.st, op, d_o.st, T, G, beta, beta_dt, bh, n.NC - 1, n, tid), walk_buf<K>(gd_lds), tid);
+        for (int r = 0; r < 4; ++r) D[d][r] = dhT ? dhT[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
     for (int c = n.NC - 1, u = 0; c >= 0; --c, u ^= 1) {
-        const WalkBuf L = walk_buf<K>(gd_lds + u * WalkLds<K>::buf);
-        const int64_t chunk = bh * n.NC + c;
-        __syncthreads();
-        WalkRegs<K> next;
-        if (c) next = walk_load<K>(qp, q.st, kp, k.st, op, d_o.st, T, G, beta, beta_dt, bh, c - 1, n, tid);
-        gd_p<K>(L.Q, L.K, L.G, scale, Ph, Pl, wave, lane);
-        Pair Dp[NS];
+        const WalkBuf L = walk_buf<K>(gd_lds + u * M::buf);
+        const int64_t at = (w.bh * n.NC + c) * (n.V / 16) + ct;
+        Three Dp[NS];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            Dp[s] = split_tiles(D[2 * s], D[2 * s + 1]);
-            put_pair(D_save, (chunk * (n.V / 16) + ct) * NS + s, lane, Dp[s]);
-        }
-        const float eC = L.eG[GD_C - 1];
+        for (int s = 0; s < NS; ++s) Dp[s] = three(D[2 * s], D[2 * s + 1]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) put_tiles(D_save + (at * ND + d) * 256, D[d], lane);
+        __syncthreads();
         f32x4 X[4], Y[4];                                  // d_n; scale e^G d_o
 #pragma unroll
         for (int I = 0; I < 4; ++I) {
             X[I] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < NS; ++s) X[I] = mm(rows(L.K, KS, 16 * I, 32 * s, lane), Dp[s], X[I]);
-            Y[I] = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * I + 4 * lq + r;
-                X[I][r] *= L.eL[i];
-                Y[I][r] *= scale * L.eG[i];
-            }
+            for (int s = 0; s < NS; ++s) X[I] = mm(prows(L.K, KS, 16 * I, 32 * s, lane), Dp[s], X[I]);
+            X[I] *= at4(L.eL, 16 * I + 4 * lq);
+            Y[I] = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane) * (scale * at4(L.eG, 16 * I + 4 * lq));
         }
-        const Pair Yp[2] = {split_tiles(Y[0], Y[1]), split_tiles(Y[2], Y[3])};
+        const Three Yp[2] = {three(Y[0], Y[1]), three(Y[2], Y[3])};
+        const float eC = L.eG[GD_C - 1];
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             D[d] *= eC;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) D[d] = mm(cols(L.Q, KS, 32 * s, 16 * d, lane), Yp[s], D[d]);
+            for (int s = 0; s < 2; ++s) D[d] = mm(pcols(L.Q, KS, 32 * s, 16 * d, lane), Yp[s], D[d]);
         }
-        __syncthreads();                                   // P
         const bf16x8 dof[2] = {cols(L.V, GD_TS, 0, 16 * wave, lane), cols(L.V, GD_TS, 32, 16 * wave, lane)};
+        __syncthreads();                                   // P
 #pragma unroll
         for (int I = 0; I < 4; ++I)
 #pragma unroll
-            for (int s = I / 2; s < 2; ++s) X[I] = mm(cols2(Ph, Pl, GD_TS, 32 * s, 16 * I, lane), dof[s], X[I]);
-        const Pair Xp[2] = {split_tiles(X[0], X[1]), split_tiles(X[2], X[3])};
+            for (int s = I / 2; s < 2; ++s)
+                X[I] = mm(Three{cols(P, GD_TS, 32 * s, 16 * I, lane), cols(P + PS, GD_TS, 32 * s, 16 * I, lane),
+                                cols(P + 2 * PS, GD_TS, 32 * s, 16 * I, lane)}, dof[s], X[I]);
         f32x4 R[4];
 #pragma unroll
         for (int I = 0; I < 4; ++I) {
             R[I] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int s = I / 2; s < 2; ++s) R[I] = mm(cols2(L.Th, L.Tl, GD_TS, 32 * s, 16 * I, lane), Xp[s], R[I]);
+            for (int J = I; J < 4; ++J) R[I] = mul_t(L.T, I, J, X[J], R[I], lane);
+            put_tiles(r_save + (at * 4 + I) * 256, R[I], lane);
+            R[I] *= at4(L.be, 16 * I + 4 * lq);
         }
-        put_pair(r_save, (chunk * (n.V / 16) + ct) * 2, lane, split_tiles(R[0], R[1]));
-        put_pair(r_save, (chunk * (n.V / 16) + ct) * 2 + 1, lane, split_tiles(R[2], R[3]));
 #pragma unroll
-        for (int I = 0; I < 4; ++I)
+        for (int I = 0; I < 4; ++I) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = 16 * I + 4 * lq + r, t = c * GD_C + i;
-                const float x = L.be[i] * R[I][r];
-                if (t < n.T) dv[(bh * n.T + t) * n.V + col] = f2bf(x);
-                R[I][r] = -L.eG[i] * x;
+                const int t = c * GD_C + 16 * I + 4 * lq + r;
+                if (t < n.T) dv[(w.bh * n.T + t) * n.V + col] = f2bf(R[I][r]);
             }
-        const Pair Rp[2] = {split_tiles(R[0], R[1]), split_tiles(R[2], R[3])};
+            R[I] *= -at4(L.eG, 16 * I + 4 * lq);
+        }
+        const Three Rp[2] = {three(R[0], R[1]), three(R[2], R[3])};
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) D[d] = mm(cols(L.K, KS, 32 * s, 16 * d, lane), Rp[s], D[d]);
-        if (c) walk_store<K>(next, walk_buf<K>(gd_lds + (u ^ 1) * WalkLds<K>::buf), tid);
+            for (int s = 0; s < 2; ++s) D[d] = mm(pcols(L.K, KS, 32 * s, 16 * d, lane), Rp[s], D[d]);
     }
     if (dh0)
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) dh0[(bh * K + 16 * d + 4 * lq + r) * n.V + col] = D[d][r];
+            for (int r = 0; r < 4; ++r) dh0[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] = D[d][r];
 }
 
 namespace {
-// LDS of the gradients: q and k; 32 value channels of n, r [32][64 tokens] and S, D [32][K] as hi and lo, in
-// whose place p and m [64][64] hi and lo come afterwards; sums.
+// LDS of the gradients: q and k; 32 value channels of n, r [32][64 tokens] and S, D [32][K] in three parts, in
+// whose place p and m [64][64] in two parts come afterwards; sums.
 template <int K> struct GradLds {
     static constexpr int qk = GD_C * (K + GD_PAD), nv = 32 * GD_TS, sv = 32 * (K + GD_PAD), pm = GD_C * GD_TS;
-    static constexpr int shared_ = 4 * nv + 4 * sv > 4 * pm ? 4 * nv + 4 * sv : 4 * pm;
-    static constexpr size_t bytes = (size_t)(2 * qk + shared_) * 2 + GD_C * 8 + (GD_C * 3 + 4 * GD_C + GD_C + 8) * 4;
+    static constexpr int shared_ = 6 * nv + 6 * sv > 4 * pm ? 6 * nv + 6 * sv : 4 * pm;
+    static constexpr int sums = 3 + 4 + 2 * 3 + 1;         // of 64: e^G, e^{G_C - G}, beta; columns; rows' three by half; rest
+    static constexpr size_t bytes = (size_t)(2 * qk + shared_) * 2 + GD_C * 8 + sums * GD_C * 4;
 };
-// Two 16-column tiles of operands in the walks' layout, STEPS steps of 32 each, into tiles [32 columns][contracted].
-template <int STEPS> struct PairRegs {
-    uint4 q[STEPS];
-};
-template <int STEPS>
-__device__ __forceinline__ PairRegs<STEPS> pairs_load(const uint16_t* base, int64_t n0, int tid) {
-    PairRegs<STEPS> r;
+// Two 16-column tiles of 16 TILES rows in 512 threads, and into three parts [32 columns][16 TILES].
+template <int TILES>
+__device__ __forceinline__ void tiles_load(const float* base, int64_t at, int tid, f32x4* x) {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) r.q[i] = reinterpret_cast<const uint4*>(base)[n0 * 128 + tid + 256 * i];
-    return r;
+    for (int i = 0; i < TILES / 4; ++i) x[i] = reinterpret_cast<const f32x4*>(base)[at * (64 * TILES) + tid + 512 * i];
 }
-template <int STEPS>
-__device__ __forceinline__ void pairs_store(const PairRegs<STEPS>& x, uint16_t* H, uint16_t* Lo, int tid) {
+template <int TILES>
+__device__ __forceinline__ void tiles_store(const f32x4* v, uint16_t* X, int tid) {
+    constexpr int stride = 16 * TILES + GD_PAD;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        const int m = tid + 256 * i, lane = m & 63, step = (m >> 7) % STEPS, tile = (m >> 7) / STEPS;
-        uint16_t* p = (m & 64 ? Lo : H) + (16 * tile + (lane & 15)) * (32 * STEPS + GD_PAD) + 32 * step + 4 * (lane >> 4);
-        *reinterpret_cast<uint2*>(p) = make_uint2(x.q[i].x, x.q[i].y);
-        *reinterpret_cast<uint2*>(p + 16) = make_uint2(x.q[i].z, x.q[i].w);
+    for (int i = 0; i < TILES / 4; ++i) {
+        const int m = tid + 512 * i, lane = m & 63, d = (m >> 6) % TILES, tile = (m >> 6) / TILES;
+        uint16_t* p = X + (16 * tile + (lane & 15)) * stride + 16 * d + 4 * (lane >> 4);
+        float x[4] = {v[i][0], v[i][1], v[i][2], v[i][3]};
+        uint2 part = make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            *reinterpret_cast<uint2*>(p + j * 32 * stride) = part;
+            if (j < 2) part = rest4(x, part);
+        }
     }
 }
-__device__ __forceinline__ Pair tr8(const uint16_t* H, const uint16_t* L, int stride, int c0, int lane) {
-    return {lds_tr8(H, stride, 0, c0, lane), lds_tr8(L, stride, 0, c0, lane)};
+// Operand of 16 columns c0 .. of such a tile, contracted over the 32 value channels.
+__device__ __forceinline__ Three tr3(const uint16_t* X, int stride, int c0, int lane) {
+    return {lds_tr8(X, stride, 0, c0, lane), lds_tr8(X + 32 * stride, stride, 0, c0, lane),
+            lds_tr8(X + 64 * stride, stride, 0, c0, lane)};
 }
 __device__ __forceinline__ float sum16(float v) {          // over the 16 lanes of a row
     v = sum8lanes(v);
     return v + dpp_mov<0x140>(v);
 }
+__device__ __forceinline__ float sum_rows(float v) {       // over the four rows of 16 lanes
+    const RowSums r = row_sums(v);
+    return r.lo + r.hi;
+}
+__device__ __forceinline__ bf16x8 plain_rows(const uint16_t* X, int stride, int r0, int c0, int lane) {
+    return ld_bf16x8(X + (r0 + (lane & 15)) * stride + c0 + 8 * (lane >> 4));
+}
 }  // namespace
 
-// d_q, d_k, d_g and d_beta of a chunk of a key head, its value heads one after the other; wave w has the rows
-// of tokens 16w .. 16w + 15.
+// d_q, d_k, d_g and d_beta of a chunk of a key head, its value heads one after the other.  Wave (I, half) has the
+// tokens 16 I .. 16 I + 15 against half of the key channels, and of the columns of p and m those of its parity; every
+// product is formed transposed, so that a lane has one token and four adjacent channels.
 template <int K>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o, const void* __restrict__ beta, int beta_dt,
-                               const float2* __restrict__ G_in, const uint16_t* __restrict__ S_save,
-                               const uint16_t* __restrict__ n_save, const uint16_t* __restrict__ D_save,
-                               const uint16_t* __restrict__ r_save, uint16_t* __restrict__ dq, uint16_t* __restrict__ dk,
+                               const float2* __restrict__ G_in, const float* __restrict__ S_save,
+                               const float* __restrict__ n_save, const float* __restrict__ D_save,
+                               const float* __restrict__ r_save, uint16_t* __restrict__ dq, uint16_t* __restrict__ dk,
                                float* __restrict__ dg, void* __restrict__ dbeta, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
     using M = GradLds<K>;
-    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32;
+    constexpr int KS = K + GD_PAD, ND = K / 32, NS = K / 32;              // ND: a half's channel tiles
     uint16_t *Qt = gd_lds, *Kt = Qt + M::qk, *X = Kt + M::qk;
-    uint16_t *Nh = X, *Nl = Nh + M::nv, *Rh = Nl + M::nv, *Rl = Rh + M::nv;
-    uint16_t *Sh = Rl + M::nv, *Sl = Sh + M::sv, *Dh = Sl + M::sv, *Dl = Dh + M::sv;
-    uint16_t *ph = X, *pl = ph + M::pm, *mh = pl + M::pm, *ml = mh + M::pm;
+    uint16_t *Nt = X, *Rt = Nt + 3 * M::nv, *St = Rt + 3 * M::nv, *Dt = St + 3 * M::sv;
+    uint16_t *pt = X, *mt = pt + 2 * M::pm;
     float2* G = reinterpret_cast<float2*>(X + M::shared_);
-    float *eG = reinterpret_cast<float*>(G + GD_C), *eL = eG + GD_C, *be = eL + GD_C, *colsum = be + GD_C, *dG = colsum + 4 * GD_C,
-          *part = dG + GD_C;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
+    float *eG = reinterpret_cast<float*>(G + GD_C), *eL = eG + GD_C, *be = eL + GD_C, *colsum = be + GD_C;
+    float *own_ = colsum + 4 * GD_C, *kept_ = own_ + 2 * GD_C, *db_ = kept_ + 2 * GD_C, *part = db_ + 2 * GD_C;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4, I = wave & 3, half = wave >> 2;
     const int group = n.HV / n.H;
     const int64_t kc = blockIdx.x, bk = kc / n.NC, b = bk / n.H;
     const int c = (int)(kc - bk * n.NC), hk = (int)(bk % n.H), t0 = c * GD_C;
-    const uint16_t *qp = q.p + b * q.sb + hk * q.sh, *kp = k.p + b * k.sb + hk * k.sh;
-    tile_store<K>(tile_load<K>(qp, q.st, t0, n.T, tid), Qt, tid);
-    tile_store<K>(tile_load<K>(kp, k.st, t0, n.T, tid), Kt, tid);
-    const int row = t0 + 16 * wave + lr;                   // the token whose operands this lane reads
+    if (half)
+        tile_store<K, false>(tile_load<K>(q.p + b * q.sb + hk * q.sh, q.st, t0, n.T, tid - 256), Qt, tid - 256);
+    else
+        tile_store<K, false>(tile_load<K>(k.p + b * k.sb + hk * k.sh, k.st, t0, n.T, tid), Kt, tid);
+    const int i = 16 * I + lr, row = t0 + i, d0 = ND * half;              // this lane's token
     f32x4 aq[ND], ak[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) aq[d] = ak[d] = f32x4{0, 0, 0, 0};
@@ -632,178 +725,174 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
             eL[tid] = ex2(gd_gap(gC, g));
             be[tid] = t0 + tid < n.T ? gd_beta(beta, beta_dt, bh * n.T + t0 + tid) : 0.f;
         }
-        f32x4 P[4], R[4], Z[ND], Y[ND], W[ND], RV = {0, 0, 0, 0};
+        f32x4 P[2], R[2], Z[ND], Y[ND], W[ND], RV = {0, 0, 0, 0};
         float sd = 0.f;
-#pragma unroll
-        for (int J = 0; J < 4; ++J) P[J] = R[J] = f32x4{0, 0, 0, 0};
+        P[0] = P[1] = R[0] = R[1] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < ND; ++d) Z[d] = Y[d] = W[d] = f32x4{0, 0, 0, 0};
         for (int vb = 0; vb < n.V / 32; ++vb) {
-            const int64_t ct = chunk * (n.V / 16) + 2 * vb;
-            const PairRegs<2> xn = pairs_load<2>(n_save, ct * 2, tid), xr = pairs_load<2>(r_save, ct * 2, tid);
-            const PairRegs<NS> xs = pairs_load<NS>(S_save, ct * NS, tid), xd = pairs_load<NS>(D_save, ct * NS, tid);
-            uint4 ov = *reinterpret_cast<const uint4*>(op + (int64_t)(row < n.T ? row : n.T - 1) * d_o.st + 32 * vb + 8 * lq);
-            uint4 vv = *reinterpret_cast<const uint4*>(vp + (int64_t)(row < n.T ? row : n.T - 1) * v.st + 32 * vb + 8 * lq);
-            if (row >= n.T) ov = vv = make_uint4(0, 0, 0, 0);
-            const bf16x8 fo = __builtin_bit_cast(bf16x8, ov), fv = __builtin_bit_cast(bf16x8, vv);
-            __syncthreads();                               // the last block's operands, or p and m, are done with
-            pairs_store<2>(xn, Nh, Nl, tid);
-            pairs_store<2>(xr, Rh, Rl, tid);
-            pairs_store<NS>(xs, Sh, Sl, tid);
-            pairs_store<NS>(xd, Dh, Dl, tid);
-            __syncthreads();
-            for (int i = tid; i < 32 * K / 4; i += 256) {
-                const int at = (i / (K / 4)) * KS + 4 * (i % (K / 4));
-                float a[4], a2[4], d[4], d2[4];
-                unpack4(*reinterpret_cast<const uint2*>(Sh + at), a);
-                unpack4(*reinterpret_cast<const uint2*>(Sl + at), a2);
-                unpack4(*reinterpret_cast<const uint2*>(Dh + at), d);
-                unpack4(*reinterpret_cast<const uint2*>(Dl + at), d2);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sd += (a[j] + a2[j]) * (d[j] + d2[j]);
+            const int64_t at = chunk * (n.V / 16) + 2 * vb;
+            f32x4 xn[1], xr[1], xs[K / 64], xd[K / 64];
+            tiles_load<4>(n_save, at, tid, xn);
+            tiles_load<4>(r_save, at, tid, xr);
+            tiles_load<K / 16>(S_save, at, tid, xs);
+            tiles_load<K / 16>(D_save, at, tid, xd);
+            uint4 ov = make_uint4(0, 0, 0, 0), vv = ov;
+            if (row < n.T) {
+                ov = *reinterpret_cast<const uint4*>(op + row * d_o.st + 32 * vb + 8 * lq);
+                vv = *reinterpret_cast<const uint4*>(vp + row * v.st + 32 * vb + 8 * lq);
             }
-            const Pair fr = tr8(Rh, Rl, GD_TS, 16 * wave, lane), fn = tr8(Nh, Nl, GD_TS, 16 * wave, lane);
-            RV = mm(fr, fv, RV);
+            const bf16x8 fo = __builtin_bit_cast(bf16x8, ov), fv = __builtin_bit_cast(bf16x8, vv);
 #pragma unroll
-            for (int J = 0; J < 4; ++J) {
-                if (J > wave) continue;
-                const Pair nj = tr8(Nh, Nl, GD_TS, 16 * J, lane);
-                P[J] = mm(fo, nj, P[J]);
-                R[J] = mm(fr, nj, R[J]);
+            for (int j = 0; j < K / 64; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sd += xs[j][r] * xd[j][r];
+            __syncthreads();                               // the last block's operands, or p and m, are done with
+            tiles_store<4>(xn, Nt, tid);
+            tiles_store<4>(xr, Rt, tid);
+            tiles_store<K / 16>(xs, St, tid);
+            tiles_store<K / 16>(xd, Dt, tid);
+            __syncthreads();
+            const Three fr = tr3(Rt, GD_TS, 16 * I, lane), fn = tr3(Nt, GD_TS, 16 * I, lane);
+            if (half) RV = mm(fr, fv, RV);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int J = 2 * u + half;
+                if (J > I) continue;
+                const Three nj = tr3(Nt, GD_TS, 16 * J, lane);
+                P[u] = mm(nj, fo, P[u]);
+                R[u] = mm(nj, fr, R[u]);
             }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const Pair sp = tr8(Sh, Sl, KS, 16 * d, lane), dp = tr8(Dh, Dl, KS, 16 * d, lane);
-                Z[d] = mm(fo, sp, Z[d]);
-                Y[d] = mm(fr, sp, Y[d]);
-                W[d] = mm(fn, dp, W[d]);
+                const Three sp = tr3(St, KS, 16 * (d0 + d), lane);
+                Z[d] = mm(sp, fo, Z[d]);
+                Y[d] = mm(sp, fr, Y[d]);
+                W[d] = mm(tr3(Dt, KS, 16 * (d0 + d), lane), fn, W[d]);
             }
         }
         sd = wave_sum(sd);
         if (lane == 0) part[wave] = sd;
         __syncthreads();                                   // p and m take the operands' place
-        float own[4] = {0, 0, 0, 0}, kept[4] = {0, 0, 0, 0}, db[4] = {0, 0, 0, 0};
+        float own = 0.f, kept = 0.f, db = 0.f;
+        const float gi = eG[i], bi = be[i], li = eL[i];
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d) {
+            float qv[4], kv[4];
+            unpack4(*reinterpret_cast<const uint2*>(Qt + i * KS + 16 * (d0 + d) + 4 * lq), qv);
+            unpack4(*reinterpret_cast<const uint2*>(Kt + i * KS + 16 * (d0 + d) + 4 * lq), kv);
+            Z[d] *= scale * gi;
+            Y[d] *= gi;
+            W[d] *= li;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = 16 * wave + 4 * lq + r;
-                const float qv = bf2f(Qt[i * KS + 16 * d + lr]), kv = bf2f(Kt[i * KS + 16 * d + lr]);
-                Z[d][r] *= scale * eG[i];
-                Y[d][r] *= eG[i];
-                W[d][r] *= eL[i];
-                db[r] -= Y[d][r] * kv;
-                own[r] += Z[d][r] * qv - be[i] * Y[d][r] * kv;
-                kept[r] += W[d][r] * kv;
-                aq[d][r] += Z[d][r];
-                ak[d][r] += W[d][r] - be[i] * Y[d][r];
+                const float yk = Y[d][r] * kv[r];
+                db -= yk;
+                own += Z[d][r] * qv[r] - bi * yk;
+                kept += W[d][r] * kv[r];
             }
+            aq[d] += Z[d];
+            ak[d] += W[d] - bi * Y[d];
+        }
 #pragma unroll
-        for (int J = 0; J < 4; ++J) {
-            const int j = 16 * J + lr;
-            float cs = 0.f;
-            if (J <= wave) {
+        for (int u = 0; u < 2; ++u) {
+            const int J = 2 * u + half, j = 16 * J + 4 * lq;
+            float cs[4] = {0, 0, 0, 0}, p[4] = {0, 0, 0, 0}, m[4] = {0, 0, 0, 0};
+            if (J <= I) {
                 f32x4 qk = {0, 0, 0, 0}, kk = {0, 0, 0, 0};
 #pragma unroll
                 for (int s = 0; s < NS; ++s) {
-                    const bf16x8 kj = rows(Kt, KS, 16 * J, 32 * s, lane);
-                    qk = mfma32(rows(Qt, KS, 16 * wave, 32 * s, lane), kj, qk);
-                    kk = mfma32(rows(Kt, KS, 16 * wave, 32 * s, lane), kj, kk);
+                    const bf16x8 kj = plain_rows(Kt, KS, 16 * J, 32 * s, lane);
+                    qk = mfma32(kj, plain_rows(Qt, KS, 16 * I, 32 * s, lane), qk);
+                    kk = mfma32(kj, plain_rows(Kt, KS, 16 * I, 32 * s, lane), kk);
                 }
-                const float2 gj = G[j];
+                const float2 g = G[i];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * wave + 4 * lq + r;
-                    const float l = ex2(gd_gap(G[i], gj));
-                    const float p = i >= j ? scale * l * P[J][r] : 0.f, w = i > j ? -l * R[J][r] : 0.f, m = be[i] * w;
-                    const float x = p * qk[r] + m * kk[r];
-                    own[r] += x;
-                    cs += x;
-                    db[r] += w * kk[r];
-                    const uint16_t hp = f2bf(p), hm = f2bf(m);
-                    ph[i * GD_TS + j] = hp;
-                    pl[i * GD_TS + j] = f2bf(p - bf2f(hp));
-                    mh[i * GD_TS + j] = hm;
-                    ml[i * GD_TS + j] = f2bf(m - bf2f(hm));
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int at = (16 * wave + 4 * lq + r) * GD_TS + j;
-                    ph[at] = pl[at] = mh[at] = ml[at] = 0;
+                    const float l = ex2(gd_gap(g, G[j + r])), w = i > j + r ? -l * R[u][r] : 0.f;
+                    p[r] = i >= j + r ? scale * l * P[u][r] : 0.f;
+                    m[r] = bi * w;
+                    cs[r] = p[r] * qk[r] + m[r] * kk[r];
+                    own += cs[r];
+                    db += w * kk[r];
                 }
             }
-            const RowSums rs = row_sums(cs);
-            if (lq == 0) colsum[wave * GD_C + j] = rs.lo + rs.hi;
-        }
-        float all = 0.f;
+            uint2 hp = make_uint2(pk2(p[0], p[1]), pk2(p[2], p[3])), hm = make_uint2(pk2(m[0], m[1]), pk2(m[2], m[3]));
+            *reinterpret_cast<uint2*>(pt + i * GD_TS + j) = hp;
+            *reinterpret_cast<uint2*>(mt + i * GD_TS + j) = hm;
+            *reinterpret_cast<uint2*>(pt + M::pm + i * GD_TS + j) = rest4(p, hp);
+            *reinterpret_cast<uint2*>(mt + M::pm + i * GD_TS + j) = rest4(m, hm);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = 16 * wave + 4 * lq + r;
-            if (lr == 4 * lq + r) db[r] += RV[r];          // the diagonal of r v^T
-            own[r] = sum16(own[r]);
-            kept[r] = sum16(kept[r]);
-            db[r] = sum16(db[r]);
-            all += kept[r];
-            if (lr == 0) {
-                dG[i] = own[r] - kept[r];
-                if (t0 + i < n.T) {
-                    const int64_t at = bh * n.T + t0 + i;
-                    if (beta_dt == RWKV6_BF16) reinterpret_cast<uint16_t*>(dbeta)[at] = f2bf(db[r]);
-                    else reinterpret_cast<float*>(dbeta)[at] = db[r];
-                }
-            }
+            for (int r = 0; r < 4; ++r) cs[r] = sum16(cs[r]);
+            if (lr == 0) *reinterpret_cast<float4*>(colsum + I * GD_C + j) = make_float4(cs[0], cs[1], cs[2], cs[3]);
         }
-        const RowSums ks = row_sums(all);
-        if (lane == 0) part[4 + wave] = ks.lo + ks.hi;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (half && lr == 4 * lq + r) db += RV[r];     // the diagonal of r v^T
+        own = sum_rows(own);
+        kept = sum_rows(kept);
+        db = sum_rows(db);
+        if (lq == 0) {
+            own_[half * GD_C + i] = own;
+            kept_[half * GD_C + i] = kept;
+            db_[half * GD_C + i] = db;
+        }
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             // own rows: columns up to the diagonal; transposed: rows from it
-            const bool left = 2 * s <= wave, right = 2 * s + 1 >= wave;
-            Pair p0, m0, p1, m1;
+            const bool left = 2 * s <= I, right = 2 * s + 1 >= I;
+            Two p0, m0, p1, m1;
             if (left) {
-                p0 = rows2(ph, pl, GD_TS, 16 * wave, 32 * s, lane);
-                m0 = rows2(mh, ml, GD_TS, 16 * wave, 32 * s, lane);
+                p0 = {plain_rows(pt, GD_TS, 16 * I, 32 * s, lane), plain_rows(pt + M::pm, GD_TS, 16 * I, 32 * s, lane)};
+                m0 = {plain_rows(mt, GD_TS, 16 * I, 32 * s, lane), plain_rows(mt + M::pm, GD_TS, 16 * I, 32 * s, lane)};
             }
             if (right) {
-                p1 = cols2(ph, pl, GD_TS, 32 * s, 16 * wave, lane);
-                m1 = cols2(mh, ml, GD_TS, 32 * s, 16 * wave, lane);
+                p1 = {lds_tr8(pt, GD_TS, 32 * s, 16 * I, lane), lds_tr8(pt + M::pm, GD_TS, 32 * s, 16 * I, lane)};
+                m1 = {lds_tr8(mt, GD_TS, 32 * s, 16 * I, lane), lds_tr8(mt + M::pm, GD_TS, 32 * s, 16 * I, lane)};
             }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const bf16x8 fk = cols(Kt, KS, 32 * s, 16 * d, lane);
+                const bf16x8 fk = lds_tr8(Kt, KS, 32 * s, 16 * (d0 + d), lane);
                 if (left) {
-                    aq[d] = mm(p0, fk, aq[d]);
-                    ak[d] = mm(m0, fk, ak[d]);
+                    aq[d] = mm(fk, p0, aq[d]);
+                    ak[d] = mm(fk, m0, ak[d]);
                 }
                 if (right) {
-                    ak[d] = mm(p1, cols(Qt, KS, 32 * s, 16 * d, lane), ak[d]);
-                    ak[d] = mm(m1, fk, ak[d]);
+                    ak[d] = mm(lds_tr8(Qt, KS, 32 * s, 16 * (d0 + d), lane), p1, ak[d]);
+                    ak[d] = mm(fk, m1, ak[d]);
                 }
             }
         }
         if (wave == 0) {                                   // d_g: suffix sums over the chunk's tokens
-            double x = (double)dG[lane] - ((double)colsum[lane] + colsum[GD_C + lane] + colsum[2 * GD_C + lane] + colsum[3 * GD_C + lane]);
-            if (lane == GD_C - 1)
-                x += (double)part[4] + part[5] + part[6] + part[7] + (double)eG[GD_C - 1] * ((double)part[0] + part[1] + part[2] + part[3]);
+            const double kept2 = (double)kept_[lane] + kept_[GD_C + lane];
+            double x = (double)own_[lane] + own_[GD_C + lane] - kept2, all = kept2;
+            x -= (double)colsum[lane] + colsum[GD_C + lane] + colsum[2 * GD_C + lane] + colsum[3 * GD_C + lane];
+            for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+            if (lane == GD_C - 1) {
+                double s = 0;
+                for (int j = 0; j < 8; ++j) s += part[j];
+                x += all + (double)eG[GD_C - 1] * s;
+            }
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_down(x, d);
                 if (lane + d < 64) x += o;
             }
             if (t0 + lane < n.T) dg[bh * n.T + t0 + lane] = (float)x;
+        } else if (wave == 4 && t0 + lane < n.T) {
+            const float x = db_[lane] + db_[GD_C + lane];
+            const int64_t at = bh * n.T + t0 + lane;
+            if (beta_dt == RWKV6_BF16) reinterpret_cast<uint16_t*>(dbeta)[at] = f2bf(x);
+            else reinterpret_cast<float*>(dbeta)[at] = x;
         }
         __syncthreads();                                   // the sums and G are written again
     }
+    if (row < n.T)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int t = t0 + 16 * wave + 4 * lq + r;
-            if (t >= n.T) continue;
-            const int64_t at = (bk * n.T + t) * K + 16 * d + lr;
-            dq[at] = f2bf(aq[d][r]);
-            dk[at] = f2bf(ak[d][r]);
+        for (int d = 0; d < ND; ++d) {
+            const int64_t at = (bk * n.T + row) * K + 16 * (d0 + d) + 4 * lq;
+            *reinterpret_cast<uint2*>(dq + at) = make_uint2(pk2(aq[d][0], aq[d][1]), pk2(aq[d][2], aq[d][3]));
+            *reinterpret_cast<uint2*>(dk + at) = make_uint2(pk2(ak[d][0], ak[d][1]), pk2(ak[d][2], ak[d][3]));
         }
 }
 
@@ -873,8 +962,8 @@ inline bool gd_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15
 int gd_shape(int64_t B, int64_t H, int64_t HV, int64_t T, int64_t K, int64_t V, GdShape* n) {
     if (B < 0 || H < 1 || HV < 1 || T < 0 || K < 1 || V < 1 || HV % H) return RWKV6_ERR_INVALID_ARG;
     if ((K != 64 && K != 128) || V % 64 || V > 512) return RWKV6_ERR_UNSUPPORTED;
-    // a launch holds fewer than 2^32 threads, 256 a chunk and head, and 64 a wave of a step
-    const int64_t most = ((int64_t)1 << 24) - 1;
+    // a launch holds fewer than 2^32 threads, 512 a chunk and head, and 64 a wave of a step
+    const int64_t most = ((int64_t)1 << 23) - 1;
     if (HV > most || B > most / HV || T > ((int64_t)1 << 30)) return RWKV6_ERR_UNSUPPORTED;
     const int64_t NC = (T + GD_C - 1) / GD_C;
     if (B * HV * (NC > V / 8 ? NC : V / 8) > most) return RWKV6_ERR_UNSUPPORTED;
@@ -899,7 +988,7 @@ struct GdSaved {
     GdSaved(const GdShape& n, int64_t K) {
         const size_t chunks = (size_t)n.BH * n.NC;
         T = 0;
-        G = T + chunks * 4 * GD_C * GD_C;
+        G = T + chunks * 4 * GD_TB;
         S = G + chunks * 8 * GD_C;
         N = S + chunks * 4 * K * n.V;
         end = N + chunks * 4 * GD_C * n.V;
@@ -916,10 +1005,10 @@ int gd_limits(hipStream_t stream) {
         auto raise = [&](const void* f, size_t bytes) {
             if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         };
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<64>), WalkLds<64>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<128>), WalkLds<128>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<64>), WalkLds<64>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<128>), WalkLds<128>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<64>), WalkLds<64, 2>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<128>), WalkLds<128, 2>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<64>), WalkLds<64, 3>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<128>), WalkLds<128, 3>::bytes);
         raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<64>), GradLds<64>::bytes);
         raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<128>), GradLds<128>::bytes);
         return e;
@@ -968,15 +1057,16 @@ int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int
     if ((st = gd_limits(s))) return st;
     char* base = static_cast<char*>(saved ? saved : workspace);
     float2* G = reinterpret_cast<float2*>(base + at.G);
-    uint16_t *Tm = reinterpret_cast<uint16_t*>(base), *S = saved ? reinterpret_cast<uint16_t*>(base + at.S) : nullptr,
-             *N = saved ? reinterpret_cast<uint16_t*>(base + at.N) : nullptr;
+    float *Tm = reinterpret_cast<float*>(base), *S = saved ? reinterpret_cast<float*>(base + at.S) : nullptr,
+          *N = saved ? reinterpret_cast<float*>(base + at.N) : nullptr;
     if (T > 0) {
         auto prep = K == 64 ? rwkv6_gated_delta_prep_kernel<64> : rwkv6_gated_delta_prep_kernel<128>;
         hipLaunchKernelGGL(prep, dim3((unsigned)(n.BH * n.NC)), dim3(256), 0, s, kt, g, beta, beta_dtype, G, Tm, n);
     }
     if (T > 0 || hT) {
+        const size_t lds = K == 64 ? WalkLds<64, 2>::bytes : WalkLds<128, 2>::bytes;
         auto walk = K == 64 ? rwkv6_gated_delta_fwd_kernel<64> : rwkv6_gated_delta_fwd_kernel<128>;
-        hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / 64))), dim3(256), K == 64 ? WalkLds<64>::bytes : WalkLds<128>::bytes, s,
+        hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / 64))), dim3(512), lds, s,
                            qt, kt, vt, beta, beta_dtype, G, Tm, h0, (uint16_t*)o, hT, S, N, n, scale);
     }
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
@@ -1010,17 +1100,18 @@ int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const voi
     if ((st = gd_limits(s))) return st;
     const char* base = static_cast<const char*>(saved);
     const float2* G = reinterpret_cast<const float2*>(base + at.G);
-    const uint16_t *Tm = reinterpret_cast<const uint16_t*>(base), *S = reinterpret_cast<const uint16_t*>(base + at.S),
-                   *N = reinterpret_cast<const uint16_t*>(base + at.N);
-    uint16_t *D = static_cast<uint16_t*>(workspace), *R = D + (at.N - at.S) / 2;
+    const float *Tm = reinterpret_cast<const float*>(base), *S = reinterpret_cast<const float*>(base + at.S),
+                *N = reinterpret_cast<const float*>(base + at.N);
+    float *D = static_cast<float*>(workspace), *R = D + (at.N - at.S) / 4;
     if (T > 0 || dh0) {
+        const size_t lds = K == 64 ? WalkLds<64, 3>::bytes : WalkLds<128, 3>::bytes;
         auto walk = K == 64 ? rwkv6_gated_delta_bwd_kernel<64> : rwkv6_gated_delta_bwd_kernel<128>;
-        hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / 64))), dim3(256), K == 64 ? WalkLds<64>::bytes : WalkLds<128>::bytes, s,
+        hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / 64))), dim3(512), lds, s,
                            qt, kt, ot, beta, beta_dtype, G, Tm, dhT, (uint16_t*)dv, dh0, D, R, n, scale);
     }
     if (T > 0) {
         auto grads = K == 64 ? rwkv6_gated_delta_grads_kernel<64> : rwkv6_gated_delta_grads_kernel<128>;
-        hipLaunchKernelGGL(grads, dim3((unsigned)(B * H * n.NC)), dim3(256), K == 64 ? GradLds<64>::bytes : GradLds<128>::bytes, s,
+        hipLaunchKernelGGL(grads, dim3((unsigned)(B * H * n.NC)), dim3(512), K == 64 ? GradLds<64>::bytes : GradLds<128>::bytes, s,
                            qt, kt, vt, ot, beta, beta_dtype, G, S, N, D, R, (uint16_t*)dq, (uint16_t*)dk, dg, dbeta, n, scale);
     }
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
