@@ -29,8 +29,9 @@
 // Numbers.  q, k, v and d_o are bf16 and enter the products as they are.  Everything computed (S, n, T, P,
 // ...) is 32 bits and enters as a sum of three bf16 numbers, nothing of it lost: a product that torch would run in
 // 32 bits becomes three of bf16 (bf16 times computed) or six (computed times computed, without the halves that
-// lie below 2^-24), 5 and 2.5 times the rate of the matrix instructions in 32 bits; T (..), whose operands would both
-// have to be taken apart, runs in those.  What ends in a bf16 output alone (o; p and m of d_q and d_k) is
+// lie below 2^-24), 5 and 2.5 times the rate of the matrix instructions in 32 bits, which also keep a wave's other
+// instructions from running beside them (33 cycles each and 6 for each of five multiply-adds between two of them
+// took 61; the bf16 ones, of 17 cycles, hide theirs).  What ends in a bf16 output alone (o; p and m of d_q and d_k) is
 // taken as two numbers, 2^-16 off at most.  Final states and the gradients of g and beta so have the precision of
 // 32-bit arithmetic, not of bf16.
 // G is summed in 64 bits and kept as a pair of floats: decays between neighbours late in a chunk are
@@ -42,7 +43,9 @@
 #define GD_PAD 8                // elements behind a row of an LDS tile
 #define GD_TS (GD_C + GD_PAD)   // row of a bf16 tile of 64 columns
 #define GD_TF (GD_C + 4)        // row of T in 32 bits
-#define GD_TB 2560              // T in memory: the ten 16 x 16 blocks of its triangle
+#define GD_TB 7680              // T in memory: the ten 16 x 16 blocks of its triangle in three parts
+#define GD_TP 3584              // a part of T in LDS: 32 rows of 32 columns, 32 of 64
+#define GD_TROW(i) ((i) < 32 ? (i) * 40 : 1280 + ((i) - 32) * GD_TS)
 #define GD_FLOOR (-1024.f)      // log decays below are this one: e^-1024 is 0 in 32 bits
 #define GD_STEP_WAVES 4
 
@@ -89,13 +92,6 @@ __device__ __forceinline__ uint2 rest4(float* x, uint2 h) {
     return make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
 }
 __device__ __forceinline__ f32x4 mm(bf16x8 a, const Two& b, f32x4 c) { return mfma32(a, b.h, mfma32(a, b.l, c)); }
-__device__ __forceinline__ f32x4 mm(const Two& a, bf16x8 b, f32x4 c) { return mfma32(a.h, b, mfma32(a.l, b, c)); }
-__device__ __forceinline__ f32x4 mm(const Two& a, const Two& b, f32x4 c) {
-    return mfma32(a.h, b.h, mfma32(a.h, b.l, mfma32(a.l, b.h, c)));
-}
-__device__ __forceinline__ f32x4 mm(bf16x8 a, const Three& b, f32x4 c) {
-    return mfma32(a, b.h, mfma32(a, b.m, mfma32(a, b.l, c)));
-}
 __device__ __forceinline__ f32x4 mm(const Three& a, bf16x8 b, f32x4 c) {
     return mfma32(a.h, b, mfma32(a.m, b, mfma32(a.l, b, c)));
 }
@@ -118,11 +114,7 @@ __device__ __forceinline__ bf16x8 pcols(const uint16_t* X, int stride, int r0, i
     const uint16_t* p = X + (r0 + 4 * q + (L >> 2)) * stride + GD_POS(c0) + 8 * (L & 3);
     return cat_bf16x8(lds_tr16(p), lds_tr16(p + 16 * stride));
 }
-// The same two of a tile in plain order.
-__device__ __forceinline__ bf16x8 rows(const uint16_t* X, int stride, int r0, int c0, int lane) {
-    const uint16_t* p = X + (r0 + (lane & 15)) * stride + c0 + 4 * (lane >> 4);
-    return cat_bf16x8(ld_bf16x4(p), ld_bf16x4(p + 16));
-}
+// The same of a tile in plain order.
 __device__ __forceinline__ bf16x8 cols(const uint16_t* X, int stride, int r0, int c0, int lane) {
     const int L = lane & 15, q = lane >> 4;
     const uint16_t* p = X + (r0 + 4 * q + (L >> 2)) * stride + c0 + 4 * (L & 3);
@@ -137,13 +129,38 @@ __device__ __forceinline__ f32x4 as_acc(const uint16_t* X, int stride, int r0, i
     return f32x4{f[0], f[1], f[2], f[3]};
 }
 __device__ __forceinline__ f32x4 at4(const float* p, int i) { return *reinterpret_cast<const f32x4*>(p + i); }
-// T X (or T^T X, T lying transposed): tile I from the tiles up to the diagonal (or from it), in 32 bits.  Step r of
-// a tile contracts over its rows 4q + r.
-__device__ __forceinline__ f32x4 mul_t(const float* T, int I, int J, const f32x4& x, f32x4 c, int lane) {
-    const f32x4 a = at4(T, (16 * I + (lane & 15)) * GD_TF + 16 * J + 4 * (lane >> 4));
+// Block (I, l) of a 32-bit tile times an accumulator tile, in 32 bits.  Step r contracts over rows 4q + r.
+__device__ __forceinline__ f32x4 mul_f32(const float* T, int I, int l, const f32x4& x, f32x4 c, int lane) {
+    const f32x4 t = at4(T, (16 * I + (lane & 15)) * GD_TF + 16 * l + 4 * (lane >> 4));
 #pragma unroll
-    for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], x[r], c, 0, 0, 0);
+    for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(t[r], x[r], c, 0, 0, 0);
     return c;
+}
+// T's rows 16 I .. against its columns 32 s .., and T^T's.
+__device__ __forceinline__ Three t_rows(const uint16_t* T, int I, int s, int lane) {
+    const uint16_t* p = T + GD_TROW(16 * I);
+    const int st = I < 2 ? 40 : GD_TS;
+    return {prows(p, st, 0, 32 * s, lane), prows(p + GD_TP, st, 0, 32 * s, lane), prows(p + 2 * GD_TP, st, 0, 32 * s, lane)};
+}
+__device__ __forceinline__ Three t_cols(const uint16_t* T, int I, int s, int lane) {
+    const uint16_t* p = T + GD_TROW(32 * s);
+    const int st = s ? GD_TS : 40;
+    return {pcols(p, st, 0, 16 * I, lane), pcols(p + GD_TP, st, 0, 16 * I, lane), pcols(p + 2 * GD_TP, st, 0, 16 * I, lane)};
+}
+// tiles I0 .. I1 - 1 of c += a b, both computed, side by side
+template <int I0, int I1> __device__ __forceinline__ void mm_tiles(const Three* a, const Three& b, f32x4* c) {
+#pragma unroll
+    for (int I = I0; I < I1; ++I) c[I] = mfma32(a[I].l, b.h, c[I]);
+#pragma unroll
+    for (int I = I0; I < I1; ++I) c[I] = mfma32(a[I].h, b.l, c[I]);
+#pragma unroll
+    for (int I = I0; I < I1; ++I) c[I] = mfma32(a[I].m, b.m, c[I]);
+#pragma unroll
+    for (int I = I0; I < I1; ++I) c[I] = mfma32(a[I].m, b.h, c[I]);
+#pragma unroll
+    for (int I = I0; I < I1; ++I) c[I] = mfma32(a[I].h, b.m, c[I]);
+#pragma unroll
+    for (int I = I0; I < I1; ++I) c[I] = mfma32(a[I].h, b.h, c[I]);
 }
 __device__ __forceinline__ float gd_gap(float2 a, float2 b) { return (a.x - b.x) + (a.y - b.y); }
 __device__ __forceinline__ float gd_beta(const void* p, int dt, int64_t i) {
@@ -153,7 +170,8 @@ __device__ __forceinline__ int gd_block_row(int t) { return t >= 6 ? 3 : t >= 3 
 // Accumulator tiles in memory: [chunk][16 columns][tile][lane][4].
 __device__ __forceinline__ void put_tiles(float* p, f32x4 x, int lane) { *reinterpret_cast<f32x4*>(p + 4 * lane) = x; }
 
-// 16-byte pieces of 256 threads of a [64][COLS] tile, zeros behind the last token.
+// 16-byte pieces of 256 threads of a [64][COLS] tile.  Rows behind the last token read that one and are made zero on
+// their way into LDS: loads under a branch would be waited for where it ends.
 template <int COLS> struct TileRegs {
     uint4 q[COLS / 32];
 };
@@ -161,38 +179,32 @@ template <int COLS>
 __device__ __forceinline__ TileRegs<COLS> tile_load(const uint16_t* p, int64_t st, int t0, int T, int tid) {
     constexpr int per = COLS / 8, step = 256 / per;            // pieces of a row, rows of a step
     TileRegs<COLS> r;
-    const int row = tid / per;
-    const uint16_t* x = p + (int64_t)(t0 + row) * st + 8 * (tid % per);
-    if (t0 + GD_C <= T) {
+    const int row = t0 + tid / per;
+    const uint16_t* x = p + 8 * (tid % per);
 #pragma unroll
-        for (int i = 0; i < COLS / 32; ++i, x += step * st) r.q[i] = *reinterpret_cast<const uint4*>(x);
-    } else {
-#pragma unroll
-        for (int i = 0; i < COLS / 32; ++i, x += step * st) {
-            r.q[i] = make_uint4(0, 0, 0, 0);
-            if (t0 + row + step * i < T) r.q[i] = *reinterpret_cast<const uint4*>(x);
-        }
-    }
+    for (int i = 0; i < COLS / 32; ++i) r.q[i] = *reinterpret_cast<const uint4*>(x + min(row + step * i, T - 1) * st);
     return r;
 }
 template <int COLS, bool PERMUTED>
-__device__ __forceinline__ void tile_store(const TileRegs<COLS>& r, uint16_t* X, int tid) {
+__device__ __forceinline__ void tile_store(const TileRegs<COLS>& r, uint16_t* X, int t0, int T, int tid) {
     constexpr int per = COLS / 8, step = 256 / per;
-    const int col = 8 * (tid % per);
+    const int col = 8 * (tid % per), row = t0 + tid / per;
     uint16_t* p = X + (tid / per) * (COLS + GD_PAD) + (PERMUTED ? GD_POS(col) : col);
 #pragma unroll
     for (int i = 0; i < COLS / 32; ++i, p += step * (COLS + GD_PAD)) {
+        const uint4 z = make_uint4(0, 0, 0, 0), x = row + step * i < T ? r.q[i] : z;
         if constexpr (PERMUTED) {
-            *reinterpret_cast<uint2*>(p) = make_uint2(r.q[i].x, r.q[i].y);
-            *reinterpret_cast<uint2*>(p + 8) = make_uint2(r.q[i].z, r.q[i].w);
+            *reinterpret_cast<uint2*>(p) = make_uint2(x.x, x.y);
+            *reinterpret_cast<uint2*>(p + 8) = make_uint2(x.z, x.w);
         } else {
-            *reinterpret_cast<uint4*>(p) = r.q[i];
+            *reinterpret_cast<uint4*>(p) = x;
         }
     }
 }
 
-// P of a chunk in N parts, tiles [i][j], by four waves: tile t of the triangle's ten by wave t % 4, formed
-// transposed, so that a lane has four adjacent j.  The blocks right of the diagonal are zeroed by `gd_zero_p`.
+// P of a chunk in N parts, tiles [i][j] with j in the walks' order, by four waves: tile t of the triangle's ten by wave
+// t % 4, formed transposed, so that a lane has four adjacent j.  The blocks right of the diagonal are zeroed by
+// `gd_zero_p`.
 template <int K, int N>
 __device__ __forceinline__ void gd_p(const uint16_t* Qt, const uint16_t* Kt, const float2* G, float scale, uint16_t* P, int wave,
                                      int lane) {
@@ -201,42 +213,48 @@ __device__ __forceinline__ void gd_p(const uint16_t* Qt, const uint16_t* Kt, con
     for (int u = 0; u < 3; ++u) {
         const int t = wave + 4 * u;
         if (t >= 10) break;
-        const int I = gd_block_row(t), J = t - I * (I + 1) / 2;
+        const int I = gd_block_row(t), J = t - I * (I + 1) / 2, i = 16 * I + lr, j = 16 * J + 4 * q;
+        const float2 gi = G[i];
+        const f32x4 g0 = *reinterpret_cast<const f32x4*>(G + j), g1 = *reinterpret_cast<const f32x4*>(G + j + 2);
         f32x4 a = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < K / 32; ++s)
             a = mfma32(prows(Kt, K + GD_PAD, 16 * J, 32 * s, lane), prows(Qt, K + GD_PAD, 16 * I, 32 * s, lane), a);
-        const int i = 16 * I + lr, j = 16 * J + 4 * q;
-        const float2 gi = G[i];
+        const float2 gj[4] = {{g0[0], g0[1]}, {g0[2], g0[3]}, {g1[0], g1[1]}, {g1[2], g1[3]}};
         float x[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = i >= j + r ? scale * ex2(gd_gap(gi, G[j + r])) * a[r] : 0.f;
+        for (int r = 0; r < 4; ++r) {
+            x[r] = scale * ex2(gd_gap(gi, gj[r])) * a[r];
+            x[r] = i >= j + r ? x[r] : 0.f;
+        }
         uint2 part = make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
 #pragma unroll
         for (int m = 0; m < N; ++m) {
-            *reinterpret_cast<uint2*>(P + m * GD_C * GD_TS + i * GD_TS + j) = part;
+            *reinterpret_cast<uint2*>(P + m * GD_C * GD_TS + i * GD_TS + GD_POS(j)) = part;
             if (m + 1 < N) part = rest4(x, part);
         }
     }
 }
 template <int N> __device__ __forceinline__ void gd_zero_p(uint16_t* P, int tid) {
-    // blocks (0,1) and (2,3): 2 x 16 rows of 32 bytes a part
-    if (tid < 64 * N) {
-        const int row = (tid >> 1) & 15, b = (tid >> 5) & 1, half = tid & 1;
-        *reinterpret_cast<uint4*>(P + (tid >> 6) * GD_C * GD_TS + (32 * b + row) * GD_TS + 32 * b + 16 + 8 * half) = make_uint4(0, 0, 0, 0);
-    }
+    // blocks (0,1) and (2,3): 2 x 16 rows of four 8-byte pieces a part
+#pragma unroll
+    for (int m = 0; m < N; ++m)
+        if (tid < 128) {
+            const int row = (tid >> 2) & 15, b = tid >> 6, j = 32 * b + 16 + 4 * (tid & 3);
+            *reinterpret_cast<uint2*>(P + m * GD_C * GD_TS + (32 * b + row) * GD_TS + GD_POS(j)) = make_uint2(0, 0);
+        }
 }
 
 }  // namespace
 
 // G and T of a chunk.  Wave w forms the rows of its 16-token block of A = beta L k k^T, inverts the block
 // on the diagonal by substitution, and then column w of the blocks below it, in the 32-bit matrix instructions:
-// T_IJ = -T_II sum_{J<=l<I} A_Il T_lJ.  Out: G [chunk][64] as pairs of floats in base-2 units, T [chunk]
-// [10 blocks][16][16].
+// T_IJ = -T_II sum_{J<=l<I} A_Il T_lJ.  Out: G [chunk][64] as pairs of floats in base-2 units, beta
+// in 32 bits, T [chunk][10 blocks][3 parts][16][16].
 template <int K>
 __global__ void __launch_bounds__(256)
 rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const void* __restrict__ beta, int beta_dt,
-                              float2* __restrict__ G_out, float* __restrict__ T_out, GdShape n) {
+                              float2* __restrict__ G_out, float* __restrict__ b_out, uint16_t* __restrict__ T_out, GdShape n) {
     __shared__ __attribute__((aligned(16))) float As[GD_C][GD_TF], Ts[GD_C][GD_TF];
     __shared__ float2 G[GD_C];
     __shared__ float be[GD_C];
@@ -268,6 +286,7 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
         G[lane] = make_float2(hi, (float)(s - hi));
         G_out[chunk * GD_C + lane] = G[lane];
         be[lane] = t < n.T ? gd_beta(beta, beta_dt, bh * n.T + t) : 0.f;
+        b_out[chunk * GD_C + lane] = be[lane];
     }
     __syncthreads();
 #pragma unroll
@@ -316,30 +335,34 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
         for (int I = J + 1; I < 4; ++I) {
             f32x4 a = {0, 0, 0, 0}, d = {0, 0, 0, 0};
 #pragma unroll
-            for (int l = J; l < I; ++l) a = mul_t(&As[0][0], I, l, t[l], a, lane);
-            d = mul_t(&Ts[0][0], I, I, a, d, lane);
+            for (int l = J; l < I; ++l) a = mul_f32(&As[0][0], I, l, t[l], a, lane);
+            d = mul_f32(&Ts[0][0], I, I, a, d, lane);
             t[I] = -d;
 #pragma unroll
             for (int r = 0; r < 4; ++r) Ts[16 * I + 4 * q + r][16 * J + lr] = t[I][r];
         }
     }
     __syncthreads();
-    for (int i = tid; i < GD_TB / 4; i += 256) {
-        const int t = i >> 6, I = gd_block_row(t), J = t - I * (I + 1) / 2;
-        reinterpret_cast<f32x4*>(T_out + chunk * GD_TB)[i] = at4(&Ts[16 * I + ((i >> 2) & 15)][16 * J + 4 * (i & 3)], 0);
+    for (int i = tid; i < 320; i += 256) {
+        const int t = i >> 5, row = (i >> 1) & 15, half = i & 1, I = gd_block_row(t), J = t - I * (I + 1) / 2;
+        const float* p = &Ts[16 * I + row][16 * J + 8 * half];
+        const Three x = three(at4(p, 0), at4(p, 4));
+        uint4* out = reinterpret_cast<uint4*>(T_out + chunk * GD_TB) + 96 * t + 2 * row + half;
+        out[0] = __builtin_bit_cast(uint4, x.h);
+        out[32] = __builtin_bit_cast(uint4, x.m);
+        out[64] = __builtin_bit_cast(uint4, x.l);
     }
 }
 
 namespace {
 // LDS of the walks: two buffers of q, k, v (or d_o), T, G, e^G, e^{G_C - G}, beta; then P in NP parts.
 template <int K, int NP> struct WalkLds {
-    static constexpr int qk = GD_C * (K + GD_PAD), t = GD_C * GD_TS, tf = GD_C * GD_TF * 2;
-    static constexpr int buf = 2 * qk + t + tf + (8 + 3 * 4) / 2 * GD_C;          // in elements of 2 bytes
+    static constexpr int qk = GD_C * (K + GD_PAD), t = GD_C * GD_TS;
+    static constexpr int buf = 2 * qk + t + 3 * GD_TP + (8 + 3 * 4) / 2 * GD_C;          // in elements of 2 bytes
     static constexpr size_t bytes = (size_t)(2 * buf + NP * t) * 2;
 };
 struct WalkBuf {
-    uint16_t *Q, *K, *V;
-    float* T;
+    uint16_t *Q, *K, *V, *T;
     float2* G;
     float *eG, *eL, *be;
 };
@@ -349,8 +372,8 @@ template <int K> __device__ __forceinline__ WalkBuf walk_buf(uint16_t* p) {
     b.Q = p;
     b.K = p + L::qk;
     b.V = p + 2 * L::qk;
-    b.T = reinterpret_cast<float*>(b.V + L::t);
-    b.G = reinterpret_cast<float2*>(b.T + GD_C * GD_TF);
+    b.T = b.V + L::t;
+    b.G = reinterpret_cast<float2*>(b.T + 3 * GD_TP);
     b.eG = reinterpret_cast<float*>(b.G + GD_C);
     b.eL = b.eG + GD_C;
     b.be = b.eL + GD_C;
@@ -360,54 +383,46 @@ template <int K> __device__ __forceinline__ WalkBuf walk_buf(uint16_t* p) {
 template <int K> struct WalkRegs {
     TileRegs<K> q, k;
     TileRegs<64> v;
-    f32x4 t[3];
+    uint4 t[4];
     float2 G, GC;
     float be;
 };
 struct WalkIn {
     const uint16_t *q, *k, *v;
     int64_t qs, ks, vs;
-    const float* T;
+    const uint16_t* T;          // of the head's first chunk
+    const float* beta;
     const float2* G;
-    const void* beta;
-    int beta_dt;
-    int64_t bh;
+    int tokens;
 };
 template <int K>
-__device__ __forceinline__ WalkRegs<K> walk_load(const WalkIn& w, int c, const GdShape& n, int tid) {
+__device__ __forceinline__ WalkRegs<K> walk_load(const WalkIn& w, int c, int tid) {
     WalkRegs<K> r;
     const int t0 = c * GD_C;
-    const int64_t chunk = w.bh * n.NC + c;
-    r.k = tile_load<K>(w.k, w.ks, t0, n.T, tid);
-    r.q = tile_load<K>(w.q, w.qs, t0, n.T, tid);
-    const f32x4* T = reinterpret_cast<const f32x4*>(w.T + chunk * GD_TB);
-    r.t[0] = T[tid];
-    r.t[1] = T[tid + 256];
-    if (tid < GD_TB / 4 - 512) r.t[2] = T[tid + 512];
-    r.v = tile_load<64>(w.v, w.vs, t0, n.T, tid);
-    if (tid < GD_C) {
-        r.G = w.G[chunk * GD_C + tid];
-        r.GC = w.G[chunk * GD_C + GD_C - 1];
-        r.be = t0 + tid < n.T ? gd_beta(w.beta, w.beta_dt, w.bh * n.T + t0 + tid) : 0.f;
-    }
+    r.k = tile_load<K>(w.k, w.ks, t0, w.tokens, tid);
+    r.q = tile_load<K>(w.q, w.qs, t0, w.tokens, tid);
+    r.v = tile_load<64>(w.v, w.vs, t0, w.tokens, tid);
+    const uint4* T = reinterpret_cast<const uint4*>(w.T + (int64_t)c * GD_TB);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.t[i] = T[min(tid + 256 * i, GD_TB / 8 - 1)];
+    r.G = w.G[t0 + (tid & 63)];
+    r.GC = w.G[t0 + GD_C - 1];
+    r.be = w.beta[t0 + (tid & 63)];
     return r;
 }
-template <int K, bool TRANSPOSED>
-__device__ __forceinline__ void walk_store(const WalkRegs<K>& r, const WalkBuf& L, int tid) {
-    tile_store<K, true>(r.k, L.K, tid);
-    tile_store<K, true>(r.q, L.Q, tid);
-    tile_store<64, false>(r.v, L.V, tid);
+template <int K>
+__device__ __forceinline__ void walk_store(const WalkRegs<K>& r, const WalkIn& w, int c, const WalkBuf& L, int tid) {
+    const int t0 = c * GD_C;
+    tile_store<K, true>(r.k, L.K, t0, w.tokens, tid);
+    tile_store<K, true>(r.q, L.Q, t0, w.tokens, tid);
+    tile_store<64, false>(r.v, L.V, t0, w.tokens, tid);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        if (i == 2 && tid >= GD_TB / 4 - 512) break;
-        const int p = tid + 256 * i, t = p >> 6, I = gd_block_row(t), J = t - I * (I + 1) / 2;
-        const int row = 16 * I + ((p >> 2) & 15), col = 16 * J + 4 * (p & 3);
-        if constexpr (TRANSPOSED) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) L.T[(col + j) * GD_TF + row] = r.t[i][j];
-        } else {
-            *reinterpret_cast<f32x4*>(L.T + row * GD_TF + col) = r.t[i];
-        }
+    for (int i = 0; i < 4; ++i) {
+        if (i == 3 && tid >= GD_TB / 8 - 768) break;
+        const int p = tid + 256 * i, t = p / 96, part = (p >> 5) % 3, I = gd_block_row(t), J = t - I * (I + 1) / 2;
+        uint16_t* x = L.T + part * GD_TP + GD_TROW(16 * I + ((p >> 1) & 15)) + GD_POS(16 * J + 8 * (p & 1));
+        *reinterpret_cast<uint2*>(x) = make_uint2(r.t[i].x, r.t[i].y);
+        *reinterpret_cast<uint2*>(x + 8) = make_uint2(r.t[i].z, r.t[i].w);
     }
     if (tid < GD_C) {
         L.G[tid] = r.G;
@@ -433,36 +448,69 @@ __device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
 }
 }  // namespace
 
-// A block walks one head's chunks with 64 columns of the state.  S_save and n_save (the backward's, or null) get
-// the state entering each chunk and the values it writes.
-template <int K>
-__global__ void __launch_bounds__(512)
-rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const void* __restrict__ beta, int beta_dt,
-                             const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ h0,
+namespace {
+// What the four helper waves of a walk do: chunk c is in LDS before the first barrier of its step and P of it before
+// the second; the loads of the chunk after the next are in flight meanwhile.
+template <int K, int NP, bool BACK>
+__device__ __forceinline__ void walk_help(const WalkIn& in, int NC, float scale, uint16_t* lds, int tid) {
+    using M = WalkLds<K, NP>;
+    uint16_t* const P = lds + 2 * M::buf;
+    const int lane = tid & 63, wave = tid >> 6;
+    const auto at = [&](int x) { return BACK ? NC - 1 - min(x, NC - 1) : min(x, NC - 1); };
+    gd_zero_p<NP>(P, tid);
+    if (tid < 128)                                         // the blocks of T right of the diagonal that a step of 32 takes in
+#pragma unroll
+        for (int m = 0; m < 6; ++m) {
+            const int b = tid >> 6;
+            uint16_t* T = walk_buf<K>(lds + (m / 3) * M::buf).T + (m % 3) * GD_TP;
+            *reinterpret_cast<uint2*>(T + GD_TROW(32 * b + ((tid >> 2) & 15)) + GD_POS(32 * b + 16 + 4 * (tid & 3))) = make_uint2(0, 0);
+        }
+    if (!NC) return;
+    walk_store<K>(walk_load<K>(in, at(0), tid), in, at(0), walk_buf<K>(lds), tid);
+    WalkRegs<K> next = walk_load<K>(in, at(1), tid);
+    for (int x = 0; x < NC; ++x) {
+        const int u = x & 1;
+        const WalkBuf L = walk_buf<K>(lds + u * M::buf);
+        __syncthreads();
+        const WalkRegs<K> later = walk_load<K>(in, at(x + 2), tid);
+        gd_p<K, NP>(L.Q, L.K, L.G, scale, P, wave, lane);
+        __syncthreads();
+        if (x + 1 < NC) walk_store<K>(next, in, at(x + 1), walk_buf<K>(lds + (u ^ 1) * M::buf), tid);
+        next = later;
+    }
+}
+// Everything before stays before, for the compiler: it would put each LDS read next to its use, and wait for it there.
+__device__ __forceinline__ void gd_issued() { __builtin_amdgcn_sched_barrier(0); }
+// The order of the instructions since: N matrix instructions with V others after each, so that a wave has both pipes at
+// work.
+template <int N, int V> __device__ __forceinline__ void gd_weave() {
+    if constexpr (N > 0) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, V, 0);
+        gd_weave<N - 1, V>();
+    }
+}
+}  // namespace
+
+// A block walks one head's chunks with 64 columns of the state.  SAVE: S_save and n_save get the state entering each
+// chunk and the values it writes, for the backward.
+template <int K, bool SAVE>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
+                             const float2* __restrict__ G, const uint16_t* __restrict__ T, const float* __restrict__ h0,
                              uint16_t* __restrict__ o, float* __restrict__ hT, float* __restrict__ S_save,
                              float* __restrict__ n_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
     using M = WalkLds<K, 2>;
     uint16_t* const P = gd_lds + 2 * M::buf;
-    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32;
+    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS;
     const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, lr = lane & 15, lq = lane >> 4;
     const WalkAt w = walk_at(n);
-    if (threadIdx.x >= 256) {                              // the next chunk, and P of this one
-        const int tid = threadIdx.x - 256;
+    if (threadIdx.x >= 256) {
+        const int64_t first = w.bh * n.NC;
         const WalkIn in = {q.p + w.b * q.sb + w.hk * q.sh, k.p + w.b * k.sb + w.hk * k.sh, v.p + w.b * v.sb + w.hv * v.sh + w.v0,
-                           q.st, k.st, v.st, T, G, beta, beta_dt, w.bh};
-        gd_zero_p<2>(P, tid);
-        if (n.NC) walk_store<K, false>(walk_load<K>(in, 0, n, tid), walk_buf<K>(gd_lds), tid);
-        for (int c = 0; c < n.NC; ++c) {
-            const int u = c & 1;
-            const WalkBuf L = walk_buf<K>(gd_lds + u * M::buf);
-            __syncthreads();
-            WalkRegs<K> next;
-            if (c + 1 < n.NC) next = walk_load<K>(in, c + 1, n, tid);
-            gd_p<K, 2>(L.Q, L.K, L.G, scale, P, wave, lane);
-            __syncthreads();
-            if (c + 1 < n.NC) walk_store<K, false>(next, walk_buf<K>(gd_lds + (u ^ 1) * M::buf), tid);
-        }
+                           q.st, k.st, v.st, T + first * GD_TB, beta + first * GD_C, G + first * GD_C, n.T};
+        walk_help<K, 2, false>(in, n.NC, scale, gd_lds, threadIdx.x - 256);
         return;
     }
     const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
@@ -471,60 +519,145 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const void* __r
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[d][r] = h0 ? h0[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
-    for (int c = 0; c < n.NC; ++c) {
+    Three Sp[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) Sp[s] = three(S[2 * s], S[2 * s + 1]);
+    uint16_t* po = o + (w.bh * n.T + lr) * n.V + w.v0 + 16 * wave + 4 * lq;
+    const f32x4 zero = {0, 0, 0, 0};
+    for (int c = 0; c < n.NC; ++c, po += (int64_t)GD_C * n.V) {
         const WalkBuf L = walk_buf<K>(gd_lds + (c & 1) * M::buf);
         const int64_t at = (w.bh * n.NC + c) * (n.V / 16) + ct;
-        Three Sp[NS];
-#pragma unroll
-        for (int s = 0; s < NS; ++s) Sp[s] = three(S[2 * s], S[2 * s + 1]);
-        if (S_save)
+        if constexpr (SAVE)
 #pragma unroll
             for (int d = 0; d < ND; ++d) put_tiles(S_save + (at * ND + d) * 256, S[d], lane);
         __syncthreads();
-        f32x4 E[4], N[4];
+        bf16x8 f[NS][4], kc[ND];
+        f32x4 E[4], N[4], x[4], be[4], eg[4], el[4];
+        Three t0[4], t1[4];                                // T's columns 0 .. 31 and 32 .. 63
 #pragma unroll
-        for (int I = 0; I < 4; ++I) {
-            f32x4 a = {0, 0, 0, 0};
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int s = 0; s < NS; ++s) a = mm(prows(L.K, KS, 16 * I, 32 * s, lane), Sp[s], a);
-            const f32x4 x = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane);
-            E[I] = at4(L.be, 16 * I + 4 * lq) * (x - at4(L.eG, 16 * I + 4 * lq) * a);
+            for (int I = 0; I < 4; ++I) f[s][I] = prows(L.K, KS, 16 * I, 32 * s, lane);
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) E[I] = N[I] = zero;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            if (s == NS / 2) {                             // what comes next, once half of k's registers are free
+#pragma unroll
+                for (int I = 0; I < 4; ++I) {
+                    x[I] = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane);
+                    be[I] = at4(L.be, 16 * I + 4 * lq);
+                    eg[I] = at4(L.eG, 16 * I + 4 * lq);
+                }
+#pragma unroll
+                for (int I = 0; I < 4; ++I) t0[I] = t_rows(L.T, I, 0, lane);
+                gd_issued();
+            }
+#pragma unroll
+            for (int I = 0; I < 4; ++I) E[I] = mfma32(f[s][I], Sp[s].l, E[I]);
+#pragma unroll
+            for (int I = 0; I < 4; ++I) E[I] = mfma32(f[s][I], Sp[s].m, E[I]);
+#pragma unroll
+            for (int I = 0; I < 4; ++I) E[I] = mfma32(f[s][I], Sp[s].h, E[I]);
         }
+        gd_issued();
 #pragma unroll
-        for (int I = 0; I < 4; ++I) {
-            N[I] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int J = 0; J <= I; ++J) N[I] = mul_t(L.T, I, J, E[J], N[I], lane);
-        }
-        if (n_save)
-#pragma unroll
-            for (int I = 0; I < 4; ++I) put_tiles(n_save + (at * 4 + I) * 256, N[I], lane);
-#pragma unroll
-        for (int I = 0; I < 4; ++I) E[I] = N[I] * at4(L.eL, 16 * I + 4 * lq);
-        const Three Ep[2] = {three(E[0], E[1]), three(E[2], E[3])};
+        for (int I = 0; I < 4; ++I) el[I] = at4(L.eL, 16 * I + 4 * lq);
         const float eC = L.eG[GD_C - 1];
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            S[d] *= eC;
+        for (int d = 0; d < ND; ++d) kc[d] = pcols(L.K, KS, 0, 16 * d, lane);
+        gd_issued();
 #pragma unroll
-            for (int s = 0; s < 2; ++s) S[d] = mm(pcols(L.K, KS, 32 * s, 16 * d, lane), Ep[s], S[d]);
-        }
-        const Two Np[2] = {two(N[0], N[1]), two(N[2], N[3])};
-        __syncthreads();                                   // P
+        for (int I = 0; I < 4; ++I) E[I] = be[I] * (x[I] - eg[I] * E[I]);
+        const Three e0 = three(E[0], E[1]);
+        gd_issued();
+        // T (..): the first two tiles of n, then the other two beside taking the first ones apart
+        mm_tiles<0, 2>(t0, e0, N);
+        const Three e1 = three(E[2], E[3]);
+        gd_weave<12, 4>();
+        gd_issued();
+        for (int I = 2; I < 4; ++I) t1[I] = t_rows(L.T, I, 1, lane);
+        gd_issued();
+        mm_tiles<2, 4>(t0, e0, N);
+        const Three w0 = three(N[0] * el[0], N[1] * el[1]);
+        gd_weave<12, 5>();
+        gd_issued();
+        mm_tiles<2, 4>(t1, e1, N);
+        const Two n0 = two(N[0], N[1]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] *= eC;
+        gd_weave<12, 4>();
+        gd_issued();
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w0.l, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w0.m, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w0.h, S[d]);
+        const Three w1 = three(N[2] * el[2], N[3] * el[3]);
+        gd_weave<3 * ND, K == 64 ? 5 : 2>();
+        gd_issued();
+#pragma unroll
+        for (int d = 0; d < ND; ++d) kc[d] = pcols(L.K, KS, 32, 16 * d, lane);
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int I = 0; I < 4; ++I) f[s][I] = prows(L.Q, KS, 16 * I, 32 * s, lane);
+        float qg[4];
+#pragma unroll
+        for (int I = 0; I < 4; ++I) qg[I] = L.eG[16 * I + lr];
+        gd_issued();
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w1.l, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w1.m, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w1.h, S[d]);
         // o transposed: a lane has four adjacent channels of a token
 #pragma unroll
-        for (int I = 0; I < 4; ++I) {
-            f32x4 a = {0, 0, 0, 0};
+        for (int I = 0; I < 4; ++I) E[I] = zero;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) a = mm(Two{Sp[s].h, Sp[s].m}, prows(L.Q, KS, 16 * I, 32 * s, lane), a);
-            a *= scale * L.eG[16 * I + lr];
+        for (int s = 0; s < NS; ++s) {
 #pragma unroll
-            for (int s = 0; s <= I / 2; ++s)
-                a = mm(Np[s], Two{rows(P, GD_TS, 16 * I, 32 * s, lane), rows(P + GD_C * GD_TS, GD_TS, 16 * I, 32 * s, lane)}, a);
-            const int t = c * GD_C + 16 * I + lr;
-            if (t < n.T)
-                *reinterpret_cast<uint2*>(o + (w.bh * n.T + t) * n.V + w.v0 + 16 * wave + 4 * lq) = make_uint2(pk2(a[0], a[1]), pk2(a[2], a[3]));
+            for (int I = 0; I < 4; ++I) E[I] = mfma32(Sp[s].m, f[s][I], E[I]);
+#pragma unroll
+            for (int I = 0; I < 4; ++I) E[I] = mfma32(Sp[s].h, f[s][I], E[I]);
         }
+        if constexpr (SAVE)
+#pragma unroll
+            for (int I = 0; I < 4; ++I) put_tiles(n_save + (at * 4 + I) * 256, N[I], lane);
+        const Two n1 = two(N[2], N[3]);
+        __syncthreads();                                   // P
+        Two pp[4][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int I = 2 * s; I < 4; ++I) pp[I][s] = {prows(P, GD_TS, 16 * I, 32 * s, lane), prows(P + PS, GD_TS, 16 * I, 32 * s, lane)};
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) E[I] *= scale * qg[I];
+#pragma unroll
+        for (int I = 0; I < 4; ++I) E[I] = mfma32(n0.l, pp[I][0].h, E[I]);
+#pragma unroll
+        for (int I = 0; I < 4; ++I) E[I] = mfma32(n0.h, pp[I][0].l, E[I]);
+#pragma unroll
+        for (int I = 0; I < 4; ++I) E[I] = mfma32(n0.h, pp[I][0].h, E[I]);
+#pragma unroll
+        for (int I = 2; I < 4; ++I) E[I] = mfma32(n1.l, pp[I][1].h, E[I]);
+#pragma unroll
+        for (int I = 2; I < 4; ++I) E[I] = mfma32(n1.h, pp[I][1].l, E[I]);
+#pragma unroll
+        for (int I = 2; I < 4; ++I) E[I] = mfma32(n1.h, pp[I][1].h, E[I]);
+        // beside them the next chunk's state is taken apart
+#pragma unroll
+        for (int s = 0; s < NS; ++s) Sp[s] = three(S[2 * s], S[2 * s + 1]);
+        gd_weave<18, K == 64 ? 5 : 10>();
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 4; ++I)
+            if (c * GD_C + 16 * I + lr < n.T)
+                *reinterpret_cast<uint2*>(po + (int64_t)16 * I * n.V) = make_uint2(pk2(E[I][0], E[I][1]), pk2(E[I][2], E[I][3]));
     }
     if (hT)
 #pragma unroll
@@ -535,9 +668,9 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const void* __r
 
 // The walk back: d_v, and for the other gradients r and the gradient D of the state that each chunk leaves.
 template <int K>
-__global__ void __launch_bounds__(512)
-rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const void* __restrict__ beta, int beta_dt,
-                             const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ dhT,
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* __restrict__ beta,
+                             const float2* __restrict__ G, const uint16_t* __restrict__ T, const float* __restrict__ dhT,
                              uint16_t* __restrict__ dv, float* __restrict__ dh0, float* __restrict__ D_save,
                              float* __restrict__ r_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
@@ -547,20 +680,10 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const void* _
     const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, lr = lane & 15, lq = lane >> 4;
     const WalkAt w = walk_at(n);
     if (threadIdx.x >= 256) {
-        const int tid = threadIdx.x - 256;
+        const int64_t first = w.bh * n.NC;
         const WalkIn in = {q.p + w.b * q.sb + w.hk * q.sh, k.p + w.b * k.sb + w.hk * k.sh, d_o.p + w.b * d_o.sb + w.hv * d_o.sh + w.v0,
-                           q.st, k.st, d_o.st, T, G, beta, beta_dt, w.bh};
-        gd_zero_p<3>(P, tid);
-        if (n.NC) walk_store<K, true>(walk_load<K>(in, n.NC - 1, n, tid), walk_buf<K>(gd_lds), tid);
-        for (int c = n.NC - 1, u = 0; c >= 0; --c, u ^= 1) {
-            const WalkBuf L = walk_buf<K>(gd_lds + u * M::buf);
-            __syncthreads();
-            WalkRegs<K> next;
-            if (c) next = walk_load<K>(in, c - 1, n, tid);
-            gd_p<K, 3>(L.Q, L.K, L.G, scale, P, wave, lane);
-            __syncthreads();
-            if (c) walk_store<K, true>(next, walk_buf<K>(gd_lds + (u ^ 1) * M::buf), tid);
-        }
+                           q.st, k.st, d_o.st, T + first * GD_TB, beta + first * GD_C, G + first * GD_C, n.T};
+        walk_help<K, 3, true>(in, n.NC, scale, gd_lds, threadIdx.x - 256);
         return;
     }
     const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
@@ -578,54 +701,136 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const void* _
 #pragma unroll
         for (int d = 0; d < ND; ++d) put_tiles(D_save + (at * ND + d) * 256, D[d], lane);
         __syncthreads();
-        f32x4 X[4], Y[4];                                  // d_n; scale e^G d_o
+        bf16x8 f[NS][4], fc[2][ND], dof[2];
+        f32x4 X[4], Y[4], el[4], eg[4], be[4];             // X: d_n; Y: scale e^G d_o
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int I = 0; I < 4; ++I) f[s][I] = prows(L.K, KS, 16 * I, 32 * s, lane);
 #pragma unroll
         for (int I = 0; I < 4; ++I) {
-            X[I] = f32x4{0, 0, 0, 0};
+            Y[I] = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane);
+            el[I] = at4(L.eL, 16 * I + 4 * lq);
+            eg[I] = at4(L.eG, 16 * I + 4 * lq);
+        }
+        gd_issued();
 #pragma unroll
-            for (int s = 0; s < NS; ++s) X[I] = mm(prows(L.K, KS, 16 * I, 32 * s, lane), Dp[s], X[I]);
-            X[I] *= at4(L.eL, 16 * I + 4 * lq);
-            Y[I] = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane) * (scale * at4(L.eG, 16 * I + 4 * lq));
+        for (int I = 0; I < 4; ++I) X[I] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            if (s == NS / 2) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) fc[r][d] = pcols(L.Q, KS, 32 * r, 16 * d, lane);
+                gd_issued();
+            }
+#pragma unroll
+            for (int I = 0; I < 4; ++I) X[I] = mfma32(f[s][I], Dp[s].l, X[I]);
+#pragma unroll
+            for (int I = 0; I < 4; ++I) X[I] = mfma32(f[s][I], Dp[s].m, X[I]);
+#pragma unroll
+            for (int I = 0; I < 4; ++I) X[I] = mfma32(f[s][I], Dp[s].h, X[I]);
+        }
+#pragma unroll
+        for (int I = 0; I < 4; ++I) {
+            X[I] *= el[I];
+            Y[I] *= scale * eg[I];
         }
         const Three Yp[2] = {three(Y[0], Y[1]), three(Y[2], Y[3])};
         const float eC = L.eG[GD_C - 1];
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            D[d] *= eC;
+        for (int d = 0; d < ND; ++d) D[d] *= eC;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) D[d] = mm(pcols(L.Q, KS, 32 * s, 16 * d, lane), Yp[s], D[d]);
-        }
-        const bf16x8 dof[2] = {cols(L.V, GD_TS, 0, 16 * wave, lane), cols(L.V, GD_TS, 32, 16 * wave, lane)};
+        for (int s = 0; s < 2; ++s) dof[s] = cols(L.V, GD_TS, 32 * s, 16 * wave, lane);
         __syncthreads();                                   // P
+        Three pp[4][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int I = 0; I < 2 * s + 2; ++I)
+                pp[I][s] = {pcols(P, GD_TS, 32 * s, 16 * I, lane), pcols(P + PS, GD_TS, 32 * s, 16 * I, lane),
+                            pcols(P + 2 * PS, GD_TS, 32 * s, 16 * I, lane)};
+        gd_issued();
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[s][d], Yp[s].l, D[d]);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[s][d], Yp[s].m, D[d]);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[s][d], Yp[s].h, D[d]);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int I = 0; I < 2 * s + 2; ++I) X[I] = mfma32(pp[I][s].l, dof[s], X[I]);
+#pragma unroll
+            for (int I = 0; I < 2 * s + 2; ++I) X[I] = mfma32(pp[I][s].m, dof[s], X[I]);
+#pragma unroll
+            for (int I = 0; I < 2 * s + 2; ++I) X[I] = mfma32(pp[I][s].h, dof[s], X[I]);
+        }
+        Three t0[4], t1[4];                                // T^T's columns 0 .. 31 and 32 .. 63
+#pragma unroll
+        for (int I = 0; I < 4; ++I) t1[I] = t_cols(L.T, I, 1, lane);
+#pragma unroll
+        for (int I = 0; I < 4; ++I) be[I] = at4(L.be, 16 * I + 4 * lq);
+        const Three x1 = three(X[2], X[3]);
+        gd_issued();
+        f32x4 R[4];
+#pragma unroll
+        for (int I = 0; I < 4; ++I) R[I] = f32x4{0, 0, 0, 0};
+        mm_tiles<2, 4>(t1, x1, R);
+        const Three x0 = three(X[0], X[1]);
+        gd_weave<12, 4>();
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 2; ++I) t0[I] = t_cols(L.T, I, 0, lane);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) fc[0][d] = pcols(L.K, KS, 32, 16 * d, lane);
+        gd_issued();
+        mm_tiles<0, 2>(t1, x1, R);
+        f32x4 V[4];
+#pragma unroll
+        for (int I = 2; I < 4; ++I) {
+            V[I] = be[I] * R[I];
+            X[I] = -eg[I] * V[I];
+        }
+        const Three r1 = three(X[2], X[3]);
+        gd_weave<12, 5>();
+        gd_issued();
+        mm_tiles<0, 2>(t0, x0, R);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) fc[1][d] = pcols(L.K, KS, 0, 16 * d, lane);
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) put_tiles(r_save + (at * 4 + I) * 256, R[I], lane);
+#pragma unroll
+        for (int I = 0; I < 2; ++I) {
+            V[I] = be[I] * R[I];
+            X[I] = -eg[I] * V[I];
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[0][d], r1.l, D[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[0][d], r1.m, D[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[0][d], r1.h, D[d]);
+        const Three r0 = three(X[0], X[1]);
+        gd_weave<3 * ND, K == 64 ? 5 : 3>();
+        gd_issued();
+#pragma unroll
+        for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[1][d], r0.l, D[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[1][d], r0.m, D[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[1][d], r0.h, D[d]);
+        uint16_t* pv = dv + (w.bh * n.T + c * GD_C + 4 * lq) * n.V + col;
 #pragma unroll
         for (int I = 0; I < 4; ++I)
 #pragma unroll
-            for (int s = I / 2; s < 2; ++s)
-                X[I] = mm(Three{cols(P, GD_TS, 32 * s, 16 * I, lane), cols(P + PS, GD_TS, 32 * s, 16 * I, lane),
-                                cols(P + 2 * PS, GD_TS, 32 * s, 16 * I, lane)}, dof[s], X[I]);
-        f32x4 R[4];
-#pragma unroll
-        for (int I = 0; I < 4; ++I) {
-            R[I] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int J = I; J < 4; ++J) R[I] = mul_t(L.T, I, J, X[J], R[I], lane);
-            put_tiles(r_save + (at * 4 + I) * 256, R[I], lane);
-            R[I] *= at4(L.be, 16 * I + 4 * lq);
-        }
-#pragma unroll
-        for (int I = 0; I < 4; ++I) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int t = c * GD_C + 16 * I + 4 * lq + r;
-                if (t < n.T) dv[(w.bh * n.T + t) * n.V + col] = f2bf(R[I][r]);
-            }
-            R[I] *= -at4(L.eG, 16 * I + 4 * lq);
-        }
-        const Three Rp[2] = {three(R[0], R[1]), three(R[2], R[3])};
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) D[d] = mm(pcols(L.K, KS, 32 * s, 16 * d, lane), Rp[s], D[d]);
+            for (int r = 0; r < 4; ++r)
+                if (c * GD_C + 16 * I + 4 * lq + r < n.T) pv[(int64_t)(16 * I + r) * n.V] = f2bf(V[I][r]);
     }
     if (dh0)
 #pragma unroll
@@ -688,7 +893,7 @@ __device__ __forceinline__ bf16x8 plain_rows(const uint16_t* X, int stride, int 
 // product is formed transposed, so that a lane has one token and four adjacent channels.
 template <int K>
 __global__ void __launch_bounds__(512)
-rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o, const void* __restrict__ beta, int beta_dt,
+rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o, const float* __restrict__ beta, int beta_dt,
                                const float2* __restrict__ G_in, const float* __restrict__ S_save,
                                const float* __restrict__ n_save, const float* __restrict__ D_save,
                                const float* __restrict__ r_save, uint16_t* __restrict__ dq, uint16_t* __restrict__ dk,
@@ -707,9 +912,9 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
     const int64_t kc = blockIdx.x, bk = kc / n.NC, b = bk / n.H;
     const int c = (int)(kc - bk * n.NC), hk = (int)(bk % n.H), t0 = c * GD_C;
     if (half)
-        tile_store<K, false>(tile_load<K>(q.p + b * q.sb + hk * q.sh, q.st, t0, n.T, tid - 256), Qt, tid - 256);
+        tile_store<K, false>(tile_load<K>(q.p + b * q.sb + hk * q.sh, q.st, t0, n.T, tid - 256), Qt, t0, n.T, tid - 256);
     else
-        tile_store<K, false>(tile_load<K>(k.p + b * k.sb + hk * k.sh, k.st, t0, n.T, tid), Kt, tid);
+        tile_store<K, false>(tile_load<K>(k.p + b * k.sb + hk * k.sh, k.st, t0, n.T, tid), Kt, t0, n.T, tid);
     const int i = 16 * I + lr, row = t0 + i, d0 = ND * half;              // this lane's token
     f32x4 aq[ND], ak[ND];
 #pragma unroll
@@ -723,7 +928,7 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
             G[tid] = g;
             eG[tid] = ex2(g.x);
             eL[tid] = ex2(gd_gap(gC, g));
-            be[tid] = t0 + tid < n.T ? gd_beta(beta, beta_dt, bh * n.T + t0 + tid) : 0.f;
+            be[tid] = beta[chunk * GD_C + tid];
         }
         f32x4 P[2], R[2], Z[ND], Y[ND], W[ND], RV = {0, 0, 0, 0};
         float sd = 0.f;
@@ -982,14 +1187,15 @@ int gd_tensor(const void* p, const int64_t* s, int64_t B, int64_t heads, int64_t
     span->n = (size_t)((B - 1) * s[0] + (heads - 1) * s[1] + (T - 1) * s[2] + C) * 2;
     return RWKV6_OK;
 }
-// What the forward leaves for the backward (or uses itself): T, G, and the states and written values.
+// What the forward leaves for the backward (or uses itself): T, G, beta, and the states and written values.
 struct GdSaved {
-    size_t T, G, S, N, end;
+    size_t T, G, B, S, N, end;
     GdSaved(const GdShape& n, int64_t K) {
         const size_t chunks = (size_t)n.BH * n.NC;
         T = 0;
-        G = T + chunks * 4 * GD_TB;
-        S = G + chunks * 8 * GD_C;
+        G = T + chunks * 2 * GD_TB;
+        B = G + chunks * 8 * GD_C;
+        S = B + chunks * 4 * GD_C;
         N = S + chunks * 4 * K * n.V;
         end = N + chunks * 4 * GD_C * n.V;
     }
@@ -1005,8 +1211,10 @@ int gd_limits(hipStream_t stream) {
         auto raise = [&](const void* f, size_t bytes) {
             if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         };
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<64>), WalkLds<64, 2>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<128>), WalkLds<128, 2>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<64, false>), WalkLds<64, 2>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<64, true>), WalkLds<64, 2>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<128, false>), WalkLds<128, 2>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<128, true>), WalkLds<128, 2>::bytes);
         raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<64>), WalkLds<64, 3>::bytes);
         raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<128>), WalkLds<128, 3>::bytes);
         raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<64>), GradLds<64>::bytes);
@@ -1028,7 +1236,7 @@ size_t rwkv6_gated_delta_workspace_bytes(int64_t B, int64_t HV, int64_t T, int64
     GdShape n;
     if (gd_shape(B, 1, HV, T, K, V, &n)) return 0;
     const GdSaved s(n, K);
-    return for_bwd ? s.end - s.S : s.S;                   // D and r have the sizes of S and N; T and G
+    return for_bwd ? s.end - s.S : s.S;                   // D and r have the sizes of S and N; T, G, beta
 }
 
 int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const float* g,
@@ -1057,17 +1265,19 @@ int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int
     if ((st = gd_limits(s))) return st;
     char* base = static_cast<char*>(saved ? saved : workspace);
     float2* G = reinterpret_cast<float2*>(base + at.G);
-    float *Tm = reinterpret_cast<float*>(base), *S = saved ? reinterpret_cast<float*>(base + at.S) : nullptr,
+    uint16_t* Tm = reinterpret_cast<uint16_t*>(base);
+    float *be = reinterpret_cast<float*>(base + at.B), *S = saved ? reinterpret_cast<float*>(base + at.S) : nullptr,
           *N = saved ? reinterpret_cast<float*>(base + at.N) : nullptr;
     if (T > 0) {
         auto prep = K == 64 ? rwkv6_gated_delta_prep_kernel<64> : rwkv6_gated_delta_prep_kernel<128>;
-        hipLaunchKernelGGL(prep, dim3((unsigned)(n.BH * n.NC)), dim3(256), 0, s, kt, g, beta, beta_dtype, G, Tm, n);
+        hipLaunchKernelGGL(prep, dim3((unsigned)(n.BH * n.NC)), dim3(256), 0, s, kt, g, beta, beta_dtype, G, be, Tm, n);
     }
     if (T > 0 || hT) {
         const size_t lds = K == 64 ? WalkLds<64, 2>::bytes : WalkLds<128, 2>::bytes;
-        auto walk = K == 64 ? rwkv6_gated_delta_fwd_kernel<64> : rwkv6_gated_delta_fwd_kernel<128>;
+        auto walk = K == 64 ? (saved ? rwkv6_gated_delta_fwd_kernel<64, true> : rwkv6_gated_delta_fwd_kernel<64, false>)
+                            : (saved ? rwkv6_gated_delta_fwd_kernel<128, true> : rwkv6_gated_delta_fwd_kernel<128, false>);
         hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / 64))), dim3(512), lds, s,
-                           qt, kt, vt, beta, beta_dtype, G, Tm, h0, (uint16_t*)o, hT, S, N, n, scale);
+                           qt, kt, vt, be, G, Tm, h0, (uint16_t*)o, hT, S, N, n, scale);
     }
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
@@ -1100,19 +1310,20 @@ int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const voi
     if ((st = gd_limits(s))) return st;
     const char* base = static_cast<const char*>(saved);
     const float2* G = reinterpret_cast<const float2*>(base + at.G);
-    const float *Tm = reinterpret_cast<const float*>(base), *S = reinterpret_cast<const float*>(base + at.S),
+    const uint16_t* Tm = reinterpret_cast<const uint16_t*>(base);
+    const float *be = reinterpret_cast<const float*>(base + at.B), *S = reinterpret_cast<const float*>(base + at.S),
                 *N = reinterpret_cast<const float*>(base + at.N);
     float *D = static_cast<float*>(workspace), *R = D + (at.N - at.S) / 4;
     if (T > 0 || dh0) {
         const size_t lds = K == 64 ? WalkLds<64, 3>::bytes : WalkLds<128, 3>::bytes;
         auto walk = K == 64 ? rwkv6_gated_delta_bwd_kernel<64> : rwkv6_gated_delta_bwd_kernel<128>;
         hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / 64))), dim3(512), lds, s,
-                           qt, kt, ot, beta, beta_dtype, G, Tm, dhT, (uint16_t*)dv, dh0, D, R, n, scale);
+                           qt, kt, ot, be, G, Tm, dhT, (uint16_t*)dv, dh0, D, R, n, scale);
     }
     if (T > 0) {
         auto grads = K == 64 ? rwkv6_gated_delta_grads_kernel<64> : rwkv6_gated_delta_grads_kernel<128>;
         hipLaunchKernelGGL(grads, dim3((unsigned)(B * H * n.NC)), dim3(512), K == 64 ? GradLds<64>::bytes : GradLds<128>::bytes, s,
-                           qt, kt, vt, ot, beta, beta_dtype, G, S, N, D, R, (uint16_t*)dq, (uint16_t*)dk, dg, dbeta, n, scale);
+                           qt, kt, vt, ot, be, beta_dtype, G, S, N, D, R, (uint16_t*)dq, (uint16_t*)dk, dg, dbeta, n, scale);
     }
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
