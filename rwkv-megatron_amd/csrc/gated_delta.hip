@@ -36,6 +36,8 @@
 // 32-bit arithmetic, not of bf16.
 // G is summed in 64 bits and kept as a pair of floats: decays between neighbours late in a chunk are
 // differences of large sums.
+#include <type_traits>
+
 #include "common.h"
 #include "../../include/rwkv6_amd.h"
 
@@ -173,7 +175,7 @@ __device__ __forceinline__ void put_tiles(float* p, f32x4 x, int lane) { *reinte
 // 16-byte pieces of 256 threads of a [64][COLS] tile.  Rows behind the last token read that one and are made zero on
 // their way into LDS: loads under a branch would be waited for where it ends.
 template <int COLS> struct TileRegs {
-    uint4 q[COLS / 32];
+    uint4 q[(COLS + 31) / 32];
 };
 template <int COLS>
 __device__ __forceinline__ TileRegs<COLS> tile_load(const uint16_t* p, int64_t st, int t0, int T, int tid) {
@@ -182,7 +184,7 @@ __device__ __forceinline__ TileRegs<COLS> tile_load(const uint16_t* p, int64_t s
     const int row = t0 + tid / per;
     const uint16_t* x = p + 8 * (tid % per);
 #pragma unroll
-    for (int i = 0; i < COLS / 32; ++i) r.q[i] = *reinterpret_cast<const uint4*>(x + min(row + step * i, T - 1) * st);
+    for (int i = 0; i < (COLS + 31) / 32; ++i) r.q[i] = *reinterpret_cast<const uint4*>(x + min(row + step * i, T - 1) * st);
     return r;
 }
 template <int COLS, bool PERMUTED>
@@ -190,8 +192,9 @@ __device__ __forceinline__ void tile_store(const TileRegs<COLS>& r, uint16_t* X,
     constexpr int per = COLS / 8, step = 256 / per;
     const int col = 8 * (tid % per), row = t0 + tid / per;
     uint16_t* p = X + (tid / per) * (COLS + GD_PAD) + (PERMUTED ? GD_POS(col) : col);
+    if (COLS < 32 && tid >= GD_C * per) return;
 #pragma unroll
-    for (int i = 0; i < COLS / 32; ++i, p += step * (COLS + GD_PAD)) {
+    for (int i = 0; i < (COLS + 31) / 32; ++i, p += step * (COLS + GD_PAD)) {
         const uint4 z = make_uint4(0, 0, 0, 0), x = row + step * i < T ? r.q[i] : z;
         if constexpr (PERMUTED) {
             *reinterpret_cast<uint2*>(p) = make_uint2(x.x, x.y);
@@ -356,9 +359,9 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
 
 namespace {
 // LDS of the walks: two buffers of q, k, v (or d_o), T, G, e^G, e^{G_C - G}, beta; then P in NP parts.
-template <int K, int NP> struct WalkLds {
-    static constexpr int qk = GD_C * (K + GD_PAD), t = GD_C * GD_TS;
-    static constexpr int buf = 2 * qk + t + 3 * GD_TP + (8 + 3 * 4) / 2 * GD_C;          // in elements of 2 bytes
+template <int K, int NW, int NP> struct WalkLds {
+    static constexpr int qk = GD_C * (K + GD_PAD), t = GD_C * GD_TS, v = GD_C * (16 * NW + GD_PAD);
+    static constexpr int buf = 2 * qk + v + 3 * GD_TP + (8 + 3 * 4) / 2 * GD_C;          // in elements of 2 bytes
     static constexpr size_t bytes = (size_t)(2 * buf + NP * t) * 2;
 };
 struct WalkBuf {
@@ -366,13 +369,13 @@ struct WalkBuf {
     float2* G;
     float *eG, *eL, *be;
 };
-template <int K> __device__ __forceinline__ WalkBuf walk_buf(uint16_t* p) {
-    using L = WalkLds<K, 0>;
+template <int K, int NW> __device__ __forceinline__ WalkBuf walk_buf(uint16_t* p) {
+    using L = WalkLds<K, NW, 0>;
     WalkBuf b;
     b.Q = p;
     b.K = p + L::qk;
     b.V = p + 2 * L::qk;
-    b.T = b.V + L::t;
+    b.T = b.V + L::v;
     b.G = reinterpret_cast<float2*>(b.T + 3 * GD_TP);
     b.eG = reinterpret_cast<float*>(b.G + GD_C);
     b.eL = b.eG + GD_C;
@@ -380,9 +383,9 @@ template <int K> __device__ __forceinline__ WalkBuf walk_buf(uint16_t* p) {
     return b;
 }
 // One chunk's inputs on their way from memory to LDS, in 256 threads.
-template <int K> struct WalkRegs {
+template <int K, int NW> struct WalkRegs {
     TileRegs<K> q, k;
-    TileRegs<64> v;
+    TileRegs<16 * NW> v;
     uint4 t[4];
     float2 G, GC;
     float be;
@@ -395,13 +398,13 @@ struct WalkIn {
     const float2* G;
     int tokens;
 };
-template <int K>
-__device__ __forceinline__ WalkRegs<K> walk_load(const WalkIn& w, int c, int tid) {
-    WalkRegs<K> r;
+template <int K, int NW>
+__device__ __forceinline__ WalkRegs<K, NW> walk_load(const WalkIn& w, int c, int tid) {
+    WalkRegs<K, NW> r;
     const int t0 = c * GD_C;
     r.k = tile_load<K>(w.k, w.ks, t0, w.tokens, tid);
     r.q = tile_load<K>(w.q, w.qs, t0, w.tokens, tid);
-    r.v = tile_load<64>(w.v, w.vs, t0, w.tokens, tid);
+    r.v = tile_load<16 * NW>(w.v, w.vs, t0, w.tokens, tid);
     const uint4* T = reinterpret_cast<const uint4*>(w.T + (int64_t)c * GD_TB);
 #pragma unroll
     for (int i = 0; i < 4; ++i) r.t[i] = T[min(tid + 256 * i, GD_TB / 8 - 1)];
@@ -410,12 +413,12 @@ __device__ __forceinline__ WalkRegs<K> walk_load(const WalkIn& w, int c, int tid
     r.be = w.beta[t0 + (tid & 63)];
     return r;
 }
-template <int K>
-__device__ __forceinline__ void walk_store(const WalkRegs<K>& r, const WalkIn& w, int c, const WalkBuf& L, int tid) {
+template <int K, int NW>
+__device__ __forceinline__ void walk_store(const WalkRegs<K, NW>& r, const WalkIn& w, int c, const WalkBuf& L, int tid) {
     const int t0 = c * GD_C;
     tile_store<K, true>(r.k, L.K, t0, w.tokens, tid);
     tile_store<K, true>(r.q, L.Q, t0, w.tokens, tid);
-    tile_store<64, false>(r.v, L.V, t0, w.tokens, tid);
+    tile_store<16 * NW, false>(r.v, L.V, t0, w.tokens, tid);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i == 3 && tid >= GD_TB / 8 - 768) break;
@@ -431,29 +434,38 @@ __device__ __forceinline__ void walk_store(const WalkRegs<K>& r, const WalkIn& w
         L.be[tid] = r.be;
     }
 }
-// Which head and 64 columns a block walks: blocks of a head's other columns follow a multiple of 8 later where the
+// Which head and 16 NW columns a block walks: blocks of a head's other columns follow a multiple of 8 later where the
 // heads are one, on the same XCD, and find its q, k and T in that L2.
 struct WalkAt {
     int64_t bh, b;
     int hv, hk, v0;
 };
-__device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
+template <int NW> __device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
     WalkAt w;
     w.bh = blockIdx.x % n.BH;
     w.b = w.bh / n.HV;
     w.hv = (int)(w.bh % n.HV);
     w.hk = w.hv / (n.HV / n.H);
-    w.v0 = 64 * (int)(blockIdx.x / n.BH);
+    w.v0 = 16 * NW * (int)(blockIdx.x / n.BH);
     return w;
+}
+// A block's waves: NW walk (the first), four help.  Wave w runs on SIMD w % 4, so with fewer walking the helpers are
+// placed on the other SIMDs and the waves between, which have nothing to do, end at once.
+template <int NW> constexpr int walk_threads = NW == 1 ? 384 : 512;
+template <int NW> __device__ __forceinline__ int walk_role(int wave) {       // -1: walks, -2: nothing, else the helper's number
+    if (wave < NW) return -1;
+    if constexpr (NW == 4) return wave - 4;
+    if constexpr (NW == 2) return wave < 4 ? wave - 2 : wave < 6 ? -2 : wave - 4;
+    return wave < 4 ? wave - 1 : wave == 4 ? -2 : 3;
 }
 }  // namespace
 
 namespace {
 // What the four helper waves of a walk do: chunk c is in LDS before the first barrier of its step and P of it before
 // the second; the loads of the chunk after the next are in flight meanwhile.
-template <int K, int NP, bool BACK>
+template <int K, int NW, int NP, bool BACK>
 __device__ __forceinline__ void walk_help(const WalkIn& in, int NC, float scale, uint16_t* lds, int tid) {
-    using M = WalkLds<K, NP>;
+    using M = WalkLds<K, NW, NP>;
     uint16_t* const P = lds + 2 * M::buf;
     const int lane = tid & 63, wave = tid >> 6;
     const auto at = [&](int x) { return BACK ? NC - 1 - min(x, NC - 1) : min(x, NC - 1); };
@@ -462,20 +474,20 @@ __device__ __forceinline__ void walk_help(const WalkIn& in, int NC, float scale,
 #pragma unroll
         for (int m = 0; m < 6; ++m) {
             const int b = tid >> 6;
-            uint16_t* T = walk_buf<K>(lds + (m / 3) * M::buf).T + (m % 3) * GD_TP;
+            uint16_t* T = walk_buf<K, NW>(lds + (m / 3) * M::buf).T + (m % 3) * GD_TP;
             *reinterpret_cast<uint2*>(T + GD_TROW(32 * b + ((tid >> 2) & 15)) + GD_POS(32 * b + 16 + 4 * (tid & 3))) = make_uint2(0, 0);
         }
     if (!NC) return;
-    walk_store<K>(walk_load<K>(in, at(0), tid), in, at(0), walk_buf<K>(lds), tid);
-    WalkRegs<K> next = walk_load<K>(in, at(1), tid);
+    walk_store<K, NW>(walk_load<K, NW>(in, at(0), tid), in, at(0), walk_buf<K, NW>(lds), tid);
+    WalkRegs<K, NW> next = walk_load<K, NW>(in, at(1), tid);
     for (int x = 0; x < NC; ++x) {
         const int u = x & 1;
-        const WalkBuf L = walk_buf<K>(lds + u * M::buf);
+        const WalkBuf L = walk_buf<K, NW>(lds + u * M::buf);
         __syncthreads();
-        const WalkRegs<K> later = walk_load<K>(in, at(x + 2), tid);
+        const WalkRegs<K, NW> later = walk_load<K, NW>(in, at(x + 2), tid);
         gd_p<K, NP>(L.Q, L.K, L.G, scale, P, wave, lane);
         __syncthreads();
-        if (x + 1 < NC) walk_store<K>(next, in, at(x + 1), walk_buf<K>(lds + (u ^ 1) * M::buf), tid);
+        if (x + 1 < NC) walk_store<K, NW>(next, in, at(x + 1), walk_buf<K, NW>(lds + (u ^ 1) * M::buf), tid);
         next = later;
     }
 }
@@ -492,25 +504,27 @@ template <int N, int V> __device__ __forceinline__ void gd_weave() {
 }
 }  // namespace
 
-// A block walks one head's chunks with 64 columns of the state.  SAVE: S_save and n_save get the state entering each
+// A block walks one head's chunks with 16 NW columns of the state.  SAVE: S_save and n_save get the state entering each
 // chunk and the values it writes, for the backward.
-template <int K, bool SAVE>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int K, int NW, bool SAVE>
+__global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
                              const float2* __restrict__ G, const uint16_t* __restrict__ T, const float* __restrict__ h0,
                              uint16_t* __restrict__ o, float* __restrict__ hT, float* __restrict__ S_save,
                              float* __restrict__ n_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
-    using M = WalkLds<K, 2>;
+    using M = WalkLds<K, NW, 2>;
     uint16_t* const P = gd_lds + 2 * M::buf;
-    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS;
-    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, lr = lane & 15, lq = lane >> 4;
-    const WalkAt w = walk_at(n);
-    if (threadIdx.x >= 256) {
+    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS, VS = 16 * NW + GD_PAD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+    const WalkAt w = walk_at<NW>(n);
+    const int role = walk_role<NW>(__builtin_amdgcn_readfirstlane(wave));
+    if (role == -2) return;
+    if (role >= 0) {
         const int64_t first = w.bh * n.NC;
         const WalkIn in = {q.p + w.b * q.sb + w.hk * q.sh, k.p + w.b * k.sb + w.hk * k.sh, v.p + w.b * v.sb + w.hv * v.sh + w.v0,
                            q.st, k.st, v.st, T + first * GD_TB, beta + first * GD_C, G + first * GD_C, n.T};
-        walk_help<K, 2, false>(in, n.NC, scale, gd_lds, threadIdx.x - 256);
+        walk_help<K, NW, 2, false>(in, n.NC, scale, gd_lds, 64 * role + lane);
         return;
     }
     const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
@@ -525,7 +539,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
     uint16_t* po = o + (w.bh * n.T + lr) * n.V + w.v0 + 16 * wave + 4 * lq;
     const f32x4 zero = {0, 0, 0, 0};
     for (int c = 0; c < n.NC; ++c, po += (int64_t)GD_C * n.V) {
-        const WalkBuf L = walk_buf<K>(gd_lds + (c & 1) * M::buf);
+        const WalkBuf L = walk_buf<K, NW>(gd_lds + (c & 1) * M::buf);
         const int64_t at = (w.bh * n.NC + c) * (n.V / 16) + ct;
         if constexpr (SAVE)
 #pragma unroll
@@ -546,7 +560,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
             if (s == NS / 2) {                             // what comes next, once half of k's registers are free
 #pragma unroll
                 for (int I = 0; I < 4; ++I) {
-                    x[I] = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane);
+                    x[I] = as_acc(L.V, VS, 16 * I, 16 * wave, lane);
                     be[I] = at4(L.be, 16 * I + 4 * lq);
                     eg[I] = at4(L.eG, 16 * I + 4 * lq);
                 }
@@ -667,23 +681,25 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
 }
 
 // The walk back: d_v, and for the other gradients r and the gradient D of the state that each chunk leaves.
-template <int K>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int K, int NW>
+__global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* __restrict__ beta,
                              const float2* __restrict__ G, const uint16_t* __restrict__ T, const float* __restrict__ dhT,
                              uint16_t* __restrict__ dv, float* __restrict__ dh0, float* __restrict__ D_save,
                              float* __restrict__ r_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
-    using M = WalkLds<K, 3>;
+    using M = WalkLds<K, NW, 3>;
     uint16_t* const P = gd_lds + 2 * M::buf;
-    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS;
-    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, lr = lane & 15, lq = lane >> 4;
-    const WalkAt w = walk_at(n);
-    if (threadIdx.x >= 256) {
+    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS, VS = 16 * NW + GD_PAD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+    const WalkAt w = walk_at<NW>(n);
+    const int role = walk_role<NW>(__builtin_amdgcn_readfirstlane(wave));
+    if (role == -2) return;
+    if (role >= 0) {
         const int64_t first = w.bh * n.NC;
         const WalkIn in = {q.p + w.b * q.sb + w.hk * q.sh, k.p + w.b * k.sb + w.hk * k.sh, d_o.p + w.b * d_o.sb + w.hv * d_o.sh + w.v0,
                            q.st, k.st, d_o.st, T + first * GD_TB, beta + first * GD_C, G + first * GD_C, n.T};
-        walk_help<K, 3, true>(in, n.NC, scale, gd_lds, threadIdx.x - 256);
+        walk_help<K, NW, 3, true>(in, n.NC, scale, gd_lds, 64 * role + lane);
         return;
     }
     const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
@@ -693,7 +709,7 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
 #pragma unroll
         for (int r = 0; r < 4; ++r) D[d][r] = dhT ? dhT[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
     for (int c = n.NC - 1, u = 0; c >= 0; --c, u ^= 1) {
-        const WalkBuf L = walk_buf<K>(gd_lds + u * M::buf);
+        const WalkBuf L = walk_buf<K, NW>(gd_lds + u * M::buf);
         const int64_t at = (w.bh * n.NC + c) * (n.V / 16) + ct;
         Three Dp[NS];
 #pragma unroll
@@ -709,7 +725,7 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
             for (int I = 0; I < 4; ++I) f[s][I] = prows(L.K, KS, 16 * I, 32 * s, lane);
 #pragma unroll
         for (int I = 0; I < 4; ++I) {
-            Y[I] = as_acc(L.V, GD_TS, 16 * I, 16 * wave, lane);
+            Y[I] = as_acc(L.V, VS, 16 * I, 16 * wave, lane);
             el[I] = at4(L.eL, 16 * I + 4 * lq);
             eg[I] = at4(L.eG, 16 * I + 4 * lq);
         }
@@ -742,7 +758,7 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
 #pragma unroll
         for (int d = 0; d < ND; ++d) D[d] *= eC;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) dof[s] = cols(L.V, GD_TS, 32 * s, 16 * wave, lane);
+        for (int s = 0; s < 2; ++s) dof[s] = cols(L.V, VS, 32 * s, 16 * wave, lane);
         __syncthreads();                                   // P
         Three pp[4][2];
 #pragma unroll
@@ -892,7 +908,7 @@ __device__ __forceinline__ bf16x8 plain_rows(const uint16_t* X, int stride, int 
 // tokens 16 I .. 16 I + 15 against half of the key channels, and of the columns of p and m those of its parity; every
 // product is formed transposed, so that a lane has one token and four adjacent channels.
 template <int K>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, K == 64 ? 4 : 2)
 rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o, const float* __restrict__ beta, int beta_dt,
                                const float2* __restrict__ G_in, const float* __restrict__ S_save,
                                const float* __restrict__ n_save, const float* __restrict__ D_save,
@@ -907,7 +923,18 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
     float2* G = reinterpret_cast<float2*>(X + M::shared_);
     float *eG = reinterpret_cast<float*>(G + GD_C), *eL = eG + GD_C, *be = eL + GD_C, *colsum = be + GD_C;
     float *own_ = colsum + 4 * GD_C, *kept_ = own_ + 2 * GD_C, *db_ = kept_ + 2 * GD_C, *part = db_ + 2 * GD_C;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4, I = wave & 3, half = wave >> 2;
+    // lane and tid are taken anew from an opaque copy where a phase begins: hoisted out of the loops, the addresses
+    // of all of them at once would not fit the registers
+    int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), I = wave & 3, half = wave >> 2;
+    const auto anew = [&] {
+        int x = threadIdx.x;
+        asm volatile("" : "+v"(x));
+        tid = x;
+        lane = x & 63;
+        lr = x & 15;
+        lq = lane >> 4;
+    };
     const int group = n.HV / n.H;
     const int64_t kc = blockIdx.x, bk = kc / n.NC, b = bk / n.H;
     const int c = (int)(kc - bk * n.NC), hk = (int)(bk % n.H), t0 = c * GD_C;
@@ -915,7 +942,7 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
         tile_store<K, false>(tile_load<K>(q.p + b * q.sb + hk * q.sh, q.st, t0, n.T, tid - 256), Qt, t0, n.T, tid - 256);
     else
         tile_store<K, false>(tile_load<K>(k.p + b * k.sb + hk * k.sh, k.st, t0, n.T, tid), Kt, t0, n.T, tid);
-    const int i = 16 * I + lr, row = t0 + i, d0 = ND * half;              // this lane's token
+    const int d0 = ND * half;
     f32x4 aq[ND], ak[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) aq[d] = ak[d] = f32x4{0, 0, 0, 0};
@@ -923,6 +950,7 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
         const int hv = hk * group + e;
         const int64_t bh = b * n.HV + hv, chunk = bh * n.NC + c;
         const uint16_t *vp = v.p + b * v.sb + hv * v.sh, *op = d_o.p + b * d_o.sb + hv * d_o.sh;
+        anew();
         if (tid < GD_C) {
             const float2 g = G_in[chunk * GD_C + tid], gC = G_in[chunk * GD_C + GD_C - 1];
             G[tid] = g;
@@ -942,11 +970,10 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
             tiles_load<4>(r_save, at, tid, xr);
             tiles_load<K / 16>(S_save, at, tid, xs);
             tiles_load<K / 16>(D_save, at, tid, xd);
-            uint4 ov = make_uint4(0, 0, 0, 0), vv = ov;
-            if (row < n.T) {
-                ov = *reinterpret_cast<const uint4*>(op + row * d_o.st + 32 * vb + 8 * lq);
-                vv = *reinterpret_cast<const uint4*>(vp + row * v.st + 32 * vb + 8 * lq);
-            }
+            const int row = t0 + 16 * I + lr, in = min(row, n.T - 1);
+            uint4 ov = *reinterpret_cast<const uint4*>(op + in * d_o.st + 32 * vb + 8 * lq);
+            uint4 vv = *reinterpret_cast<const uint4*>(vp + in * v.st + 32 * vb + 8 * lq);
+            if (row >= n.T) ov = vv = make_uint4(0, 0, 0, 0);
             const bf16x8 fo = __builtin_bit_cast(bf16x8, ov), fv = __builtin_bit_cast(bf16x8, vv);
 #pragma unroll
             for (int j = 0; j < K / 64; ++j)
@@ -958,27 +985,38 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
             tiles_store<K / 16>(xs, St, tid);
             tiles_store<K / 16>(xd, Dt, tid);
             __syncthreads();
-            const Three fr = tr3(Rt, GD_TS, 16 * I, lane), fn = tr3(Nt, GD_TS, 16 * I, lane);
-            if (half) RV = mm(fr, fv, RV);
+            {
+                const Three fr = tr3(Rt, GD_TS, 16 * I, lane);
+                if (half) RV = mm(fr, fv, RV);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int J = 2 * u + half;
-                if (J > I) continue;
-                const Three nj = tr3(Nt, GD_TS, 16 * J, lane);
-                P[u] = mm(nj, fo, P[u]);
-                R[u] = mm(nj, fr, R[u]);
+                for (int u = 0; u < 2; ++u) {
+                    const int J = 2 * u + half;
+                    if (J > I) continue;
+                    const Three nj = tr3(Nt, GD_TS, 16 * J, lane);
+                    P[u] = mm(nj, fo, P[u]);
+                    R[u] = mm(nj, fr, R[u]);
+                }
+                gd_issued();
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const Three sp = tr3(St, KS, 16 * (d0 + d), lane);
+                    Z[d] = mm(sp, fo, Z[d]);
+                    Y[d] = mm(sp, fr, Y[d]);
+                    gd_issued();
+                }
             }
+            const Three fn = tr3(Nt, GD_TS, 16 * I, lane);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const Three sp = tr3(St, KS, 16 * (d0 + d), lane);
-                Z[d] = mm(sp, fo, Z[d]);
-                Y[d] = mm(sp, fr, Y[d]);
                 W[d] = mm(tr3(Dt, KS, 16 * (d0 + d), lane), fn, W[d]);
+                gd_issued();
             }
         }
         sd = wave_sum(sd);
+        anew();
         if (lane == 0) part[wave] = sd;
         __syncthreads();                                   // p and m take the operands' place
+        const int i = 16 * I + lr;                         // this lane's token
         float own = 0.f, kept = 0.f, db = 0.f;
         const float gi = eG[i], bi = be[i], li = eL[i];
 #pragma unroll
@@ -1043,6 +1081,7 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
             db_[half * GD_C + i] = db;
         }
         __syncthreads();
+        anew();
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             // own rows: columns up to the diagonal; transposed: rows from it
@@ -1092,6 +1131,8 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
         }
         __syncthreads();                                   // the sums and G are written again
     }
+    anew();
+    const int row = t0 + 16 * I + lr;
     if (row < n.T)
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
@@ -1200,6 +1241,24 @@ struct GdSaved {
         end = N + chunks * 4 * GD_C * n.V;
     }
 };
+// How a head's columns are dealt to blocks: a block of 4 waves of 16 columns, or of fewer where all blocks still find a
+// CU of their own.  A wave then has its SIMD and the CU's LDS to itself.
+inline int gd_waves(const GdShape& n) {
+    const int64_t tiles = n.BH * (n.V / 16);
+    return tiles <= 256 ? 1 : tiles <= 512 ? 2 : 4;
+}
+// f(integral constants of the key channels and of gd_waves)
+template <class F> void gd_walks(const GdShape& n, int64_t K, F&& f) {
+    const auto by_waves = [&](auto k) {
+        switch (gd_waves(n)) {
+        case 1: f(k, std::integral_constant<int, 1>()); break;
+        case 2: f(k, std::integral_constant<int, 2>()); break;
+        default: f(k, std::integral_constant<int, 4>());
+        }
+    };
+    if (K == 64) by_waves(std::integral_constant<int, 64>());
+    else by_waves(std::integral_constant<int, 128>());
+}
 // The walks' and gradients' LDS is past what a launch gets by itself: raised once on each device.
 int gd_limits(hipStream_t stream) {
     static DeviceOnce once[kMaxDevices];
@@ -1211,12 +1270,12 @@ int gd_limits(hipStream_t stream) {
         auto raise = [&](const void* f, size_t bytes) {
             if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         };
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<64, false>), WalkLds<64, 2>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<64, true>), WalkLds<64, 2>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<128, false>), WalkLds<128, 2>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<128, true>), WalkLds<128, 2>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<64>), WalkLds<64, 3>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<128>), WalkLds<128, 3>::bytes);
+#define GD_RAISE(K, NW)                                                                                              \
+    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, false>), WalkLds<K, NW, 2>::bytes);       \
+    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, true>), WalkLds<K, NW, 2>::bytes);        \
+    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<K, NW>), WalkLds<K, NW, 3>::bytes);
+        GD_RAISE(64, 1) GD_RAISE(64, 2) GD_RAISE(64, 4) GD_RAISE(128, 1) GD_RAISE(128, 2) GD_RAISE(128, 4)
+#undef GD_RAISE
         raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<64>), GradLds<64>::bytes);
         raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<128>), GradLds<128>::bytes);
         return e;
@@ -1272,13 +1331,14 @@ int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int
         auto prep = K == 64 ? rwkv6_gated_delta_prep_kernel<64> : rwkv6_gated_delta_prep_kernel<128>;
         hipLaunchKernelGGL(prep, dim3((unsigned)(n.BH * n.NC)), dim3(256), 0, s, kt, g, beta, beta_dtype, G, be, Tm, n);
     }
-    if (T > 0 || hT) {
-        const size_t lds = K == 64 ? WalkLds<64, 2>::bytes : WalkLds<128, 2>::bytes;
-        auto walk = K == 64 ? (saved ? rwkv6_gated_delta_fwd_kernel<64, true> : rwkv6_gated_delta_fwd_kernel<64, false>)
-                            : (saved ? rwkv6_gated_delta_fwd_kernel<128, true> : rwkv6_gated_delta_fwd_kernel<128, false>);
-        hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / 64))), dim3(512), lds, s,
-                           qt, kt, vt, be, G, Tm, h0, (uint16_t*)o, hT, S, N, n, scale);
-    }
+    if (T > 0 || hT)
+        gd_walks(n, K, [&](auto k_, auto w_) {
+            constexpr int k = k_, w = w_;
+            auto walk = saved ? rwkv6_gated_delta_fwd_kernel<k, w, true> : rwkv6_gated_delta_fwd_kernel<k, w, false>;
+            const size_t lds = WalkLds<k, w, 2>::bytes;
+            hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / (16 * w)))), dim3(walk_threads<w>), lds, s, qt, kt, vt, be, G, Tm, h0,
+                               (uint16_t*)o, hT, S, N, n, scale);
+        });
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
 
@@ -1314,12 +1374,14 @@ int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const voi
     const float *be = reinterpret_cast<const float*>(base + at.B), *S = reinterpret_cast<const float*>(base + at.S),
                 *N = reinterpret_cast<const float*>(base + at.N);
     float *D = static_cast<float*>(workspace), *R = D + (at.N - at.S) / 4;
-    if (T > 0 || dh0) {
-        const size_t lds = K == 64 ? WalkLds<64, 3>::bytes : WalkLds<128, 3>::bytes;
-        auto walk = K == 64 ? rwkv6_gated_delta_bwd_kernel<64> : rwkv6_gated_delta_bwd_kernel<128>;
-        hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / 64))), dim3(512), lds, s,
-                           qt, kt, ot, be, G, Tm, dhT, (uint16_t*)dv, dh0, D, R, n, scale);
-    }
+    if (T > 0 || dh0)
+        gd_walks(n, K, [&](auto k_, auto w_) {
+            constexpr int k = k_, w = w_;
+            auto walk = rwkv6_gated_delta_bwd_kernel<k, w>;
+            const size_t lds = WalkLds<k, w, 3>::bytes;
+            hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / (16 * w)))), dim3(walk_threads<w>), lds, s, qt, kt, ot, be, G, Tm, dhT,
+                               (uint16_t*)dv, dh0, D, R, n, scale);
+        });
     if (T > 0) {
         auto grads = K == 64 ? rwkv6_gated_delta_grads_kernel<64> : rwkv6_gated_delta_grads_kernel<128>;
         hipLaunchKernelGGL(grads, dim3((unsigned)(B * H * n.NC)), dim3(512), K == 64 ? GradLds<64>::bytes : GradLds<128>::bytes, s,

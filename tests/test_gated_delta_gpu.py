@@ -108,8 +108,11 @@ SHAPES = [
     (2, 1, 3, 65, 64, 64), (1, 2, 2, 128, 128, 128), (3, 1, 2, 129, 128, 64), (1, 1, 1, 300, 64, 192), (2, 3, 3, 200, 64, 64),
 ]
 
+# more heads: a walk's block takes 16, 32 or 64 columns of the state by their number (up to 256, 512 and more tiles of 16)
+MANY = [(4, 17, 17, 70, 64, 64), (5, 30, 30, 66, 64, 64), (3, 6, 12, 70, 128, 128), (3, 24, 24, 66, 128, 128), (2, 33, 33, 5, 128, 192)]
 
-@pytest.mark.parametrize("shape", SHAPES, ids=str)
+
+@pytest.mark.parametrize("shape", SHAPES + MANY, ids=str)
 @pytest.mark.parametrize("strong", [False, True])
 def test_training(pkg, shape, strong):
     B, H, HV, T, K, V = shape
@@ -124,7 +127,7 @@ def test_training_with_states_on_both_ends(pkg, shape):
     run_train(pkg, d, scale=0.7, final=True, wo=torch.randn(B, HV, T, V).to(BF), wh=torch.randn(B, HV, K, V))
 
 
-@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES + MANY, ids=str)
 def test_prompt(pkg, shape):
     d = inputs(*shape, seed=2 + sum(shape), h0=True)
     with torch.no_grad():
