@@ -493,6 +493,8 @@ __device__ __forceinline__ void walk_help(const WalkIn& in, int NC, float scale,
 }
 // Everything before stays before, for the compiler: it would put each LDS read next to its use, and wait for it there.
 __device__ __forceinline__ void gd_issued() { __builtin_amdgcn_sched_barrier(0); }
+// x is there from here on: or the compiler computes it where the loop uses it, past the branches of the stores.
+__device__ __forceinline__ void gd_here(Three& x) { asm volatile("" : "+v"(x.h), "+v"(x.m), "+v"(x.l)); }
 // The order of the instructions since: N matrix instructions with V others after each, so that a wave has both pipes at
 // work.
 template <int N, int V> __device__ __forceinline__ void gd_weave() {
@@ -545,16 +547,30 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
 #pragma unroll
             for (int d = 0; d < ND; ++d) put_tiles(S_save + (at * ND + d) * 256, S[d], lane);
         __syncthreads();
-        bf16x8 f[NS][4], kc[ND];
-        f32x4 E[4], N[4], x[4], be[4], eg[4], el[4];
+        bf16x8 f[NS][4], k0[ND], k1[ND];
+        f32x4 E[4], N[4], O[4], x[4], be[4], eg[4], el[4];
         Three t0[4], t1[4];                                // T's columns 0 .. 31 and 32 .. 63
+        float qg[4];
+        // reads that 128 key channels leave no registers for yet come later there
+        const auto read_t0 = [&] {
+#pragma unroll
+            for (int I = 0; I < 4; ++I) t0[I] = t_rows(L.T, I, 0, lane);
+        };
+        const auto read_t1 = [&] {
+#pragma unroll
+            for (int I = 2; I < 4; ++I) t1[I] = t_rows(L.T, I, 1, lane);
+        };
+        const auto read_k1 = [&] {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) k1[d] = pcols(L.K, KS, 32, 16 * d, lane);
+        };
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int I = 0; I < 4; ++I) f[s][I] = prows(L.K, KS, 16 * I, 32 * s, lane);
         gd_issued();
 #pragma unroll
-        for (int I = 0; I < 4; ++I) E[I] = N[I] = zero;
+        for (int I = 0; I < 4; ++I) E[I] = N[I] = O[I] = zero;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             if (s == NS / 2) {                             // what comes next, once half of k's registers are free
@@ -564,8 +580,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
                     be[I] = at4(L.be, 16 * I + 4 * lq);
                     eg[I] = at4(L.eG, 16 * I + 4 * lq);
                 }
-#pragma unroll
-                for (int I = 0; I < 4; ++I) t0[I] = t_rows(L.T, I, 0, lane);
+                if constexpr (K == 64) read_t0();
                 gd_issued();
             }
 #pragma unroll
@@ -577,101 +592,117 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
         }
         gd_issued();
 #pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int I = 0; I < 4; ++I) f[s][I] = prows(L.Q, KS, 16 * I, 32 * s, lane);
+#pragma unroll
         for (int I = 0; I < 4; ++I) el[I] = at4(L.eL, 16 * I + 4 * lq);
         const float eC = L.eG[GD_C - 1];
-#pragma unroll
-        for (int d = 0; d < ND; ++d) kc[d] = pcols(L.K, KS, 0, 16 * d, lane);
         gd_issued();
+        // q S (transposed: a lane has four adjacent channels of a token) beside v - e^G k S and its parts
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+            for (int I = 0; I < 4; ++I) O[I] = mfma32(Sp[s].m, f[s][I], O[I]);
+#pragma unroll
+            for (int I = 0; I < 4; ++I) O[I] = mfma32(Sp[s].h, f[s][I], O[I]);
+        }
 #pragma unroll
         for (int I = 0; I < 4; ++I) E[I] = be[I] * (x[I] - eg[I] * E[I]);
         const Three e0 = three(E[0], E[1]);
+        gd_weave<8 * NS, K == 64 ? 5 : 3>();
+        gd_issued();
+        if constexpr (K == 64) read_t1();
+        else read_t0();
+#pragma unroll
+        for (int d = 0; d < ND; ++d) k0[d] = pcols(L.K, KS, 0, 16 * d, lane);
         gd_issued();
         // T (..): the first two tiles of n, then the other two beside taking the first ones apart
         mm_tiles<0, 2>(t0, e0, N);
         const Three e1 = three(E[2], E[3]);
         gd_weave<12, 4>();
         gd_issued();
-        for (int I = 2; I < 4; ++I) t1[I] = t_rows(L.T, I, 1, lane);
+        if constexpr (K == 128) read_t1();
         gd_issued();
         mm_tiles<2, 4>(t0, e0, N);
         const Three w0 = three(N[0] * el[0], N[1] * el[1]);
         gd_weave<12, 5>();
+        gd_issued();
+        if constexpr (K == 64) read_k1();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) qg[I] = L.eG[16 * I + lr];
         gd_issued();
         mm_tiles<2, 4>(t1, e1, N);
         const Two n0 = two(N[0], N[1]);
 #pragma unroll
         for (int d = 0; d < ND; ++d) S[d] *= eC;
         gd_weave<12, 4>();
-        gd_issued();
+        __syncthreads();                                   // P
+        Two pp[4][2];
+        const auto read_p = [&] {
 #pragma unroll
-        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w0.l, S[d]);
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w0.m, S[d]);
+                for (int I = 2 * s; I < 4; ++I)
+                    pp[I][s] = {prows(P, GD_TS, 16 * I, 32 * s, lane), prows(P + PS, GD_TS, 16 * I, 32 * s, lane)};
+            gd_issued();
+        };
+        if constexpr (K == 64) read_p();                   // (128: its registers are still taken)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w0.h, S[d]);
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k0[d], w0.l, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k0[d], w0.m, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k0[d], w0.h, S[d]);
         const Three w1 = three(N[2] * el[2], N[3] * el[3]);
         gd_weave<3 * ND, K == 64 ? 5 : 2>();
         gd_issued();
-#pragma unroll
-        for (int d = 0; d < ND; ++d) kc[d] = pcols(L.K, KS, 32, 16 * d, lane);
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int I = 0; I < 4; ++I) f[s][I] = prows(L.Q, KS, 16 * I, 32 * s, lane);
-        float qg[4];
-#pragma unroll
-        for (int I = 0; I < 4; ++I) qg[I] = L.eG[16 * I + lr];
-        gd_issued();
-#pragma unroll
-        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w1.l, S[d]);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w1.m, S[d]);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) S[d] = mfma32(kc[d], w1.h, S[d]);
-        // o transposed: a lane has four adjacent channels of a token
-#pragma unroll
-        for (int I = 0; I < 4; ++I) E[I] = zero;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-#pragma unroll
-            for (int I = 0; I < 4; ++I) E[I] = mfma32(Sp[s].m, f[s][I], E[I]);
-#pragma unroll
-            for (int I = 0; I < 4; ++I) E[I] = mfma32(Sp[s].h, f[s][I], E[I]);
+        if constexpr (K == 128) {
+            read_k1();
+            gd_issued();
         }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k1[d], w1.l, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k1[d], w1.m, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k1[d], w1.h, S[d]);
+        const Two n1 = two(N[2], N[3]);
+#pragma unroll
+        for (int I = 0; I < 4; ++I) O[I] *= scale * qg[I];
+        gd_weave<3 * ND, K == 64 ? 4 : 2>();
+        gd_issued();
         if constexpr (SAVE)
 #pragma unroll
             for (int I = 0; I < 4; ++I) put_tiles(n_save + (at * 4 + I) * 256, N[I], lane);
-        const Two n1 = two(N[2], N[3]);
-        __syncthreads();                                   // P
-        Two pp[4][2];
+        if constexpr (K == 128) read_p();
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int I = 0; I < 4; ++I) O[I] = mfma32(n0.l, pp[I][0].h, O[I]);
 #pragma unroll
-            for (int I = 2 * s; I < 4; ++I) pp[I][s] = {prows(P, GD_TS, 16 * I, 32 * s, lane), prows(P + PS, GD_TS, 16 * I, 32 * s, lane)};
-        gd_issued();
+        for (int I = 0; I < 4; ++I) O[I] = mfma32(n0.h, pp[I][0].l, O[I]);
 #pragma unroll
-        for (int I = 0; I < 4; ++I) E[I] *= scale * qg[I];
+        for (int I = 0; I < 4; ++I) O[I] = mfma32(n0.h, pp[I][0].h, O[I]);
 #pragma unroll
-        for (int I = 0; I < 4; ++I) E[I] = mfma32(n0.l, pp[I][0].h, E[I]);
+        for (int I = 2; I < 4; ++I) O[I] = mfma32(n1.l, pp[I][1].h, O[I]);
 #pragma unroll
-        for (int I = 0; I < 4; ++I) E[I] = mfma32(n0.h, pp[I][0].l, E[I]);
+        for (int I = 2; I < 4; ++I) O[I] = mfma32(n1.h, pp[I][1].l, O[I]);
 #pragma unroll
-        for (int I = 0; I < 4; ++I) E[I] = mfma32(n0.h, pp[I][0].h, E[I]);
-#pragma unroll
-        for (int I = 2; I < 4; ++I) E[I] = mfma32(n1.l, pp[I][1].h, E[I]);
-#pragma unroll
-        for (int I = 2; I < 4; ++I) E[I] = mfma32(n1.h, pp[I][1].l, E[I]);
-#pragma unroll
-        for (int I = 2; I < 4; ++I) E[I] = mfma32(n1.h, pp[I][1].h, E[I]);
+        for (int I = 2; I < 4; ++I) O[I] = mfma32(n1.h, pp[I][1].h, O[I]);
         // beside them the next chunk's state is taken apart
 #pragma unroll
-        for (int s = 0; s < NS; ++s) Sp[s] = three(S[2 * s], S[2 * s + 1]);
+        for (int s = 0; s < NS; ++s) {
+            Sp[s] = three(S[2 * s], S[2 * s + 1]);
+            gd_here(Sp[s]);
+        }
         gd_weave<18, K == 64 ? 5 : 10>();
         gd_issued();
+        uint2 ob[4];
+#pragma unroll
+        for (int I = 0; I < 4; ++I) ob[I] = make_uint2(pk2(O[I][0], O[I][1]), pk2(O[I][2], O[I][3]));
+        const bool full = (c + 1) * GD_C <= n.T;
 #pragma unroll
         for (int I = 0; I < 4; ++I)
-            if (c * GD_C + 16 * I + lr < n.T)
-                *reinterpret_cast<uint2*>(po + (int64_t)16 * I * n.V) = make_uint2(pk2(E[I][0], E[I][1]), pk2(E[I][2], E[I][3]));
+            if (full || c * GD_C + 16 * I + lr < n.T) *reinterpret_cast<uint2*>(po + (int64_t)16 * I * n.V) = ob[I];
     }
     if (hT)
 #pragma unroll
@@ -708,6 +739,7 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) D[d][r] = dhT ? dhT[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
+    const f32x4 zero = {0, 0, 0, 0};
     for (int c = n.NC - 1, u = 0; c >= 0; --c, u ^= 1) {
         const WalkBuf L = walk_buf<K, NW>(gd_lds + u * M::buf);
         const int64_t at = (w.bh * n.NC + c) * (n.V / 16) + ct;
@@ -718,29 +750,26 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
         for (int d = 0; d < ND; ++d) put_tiles(D_save + (at * ND + d) * 256, D[d], lane);
         __syncthreads();
         bf16x8 f[NS][4], fc[2][ND], dof[2];
-        f32x4 X[4], Y[4], el[4], eg[4], be[4];             // X: d_n; Y: scale e^G d_o
+        f32x4 X[4], Y[4], R[4], V[4], el[4], eg[4], be[4]; // X: d_n; Y: scale e^G d_o; V: d_v
+        Three t0[4], t1[4], pp[4][2];                      // T^T's columns 0 .. 31 and 32 .. 63; P^T's
+#pragma unroll
+        for (int I = 0; I < 4; ++I) {
+            Y[I] = as_acc(L.V, VS, 16 * I, 16 * wave, lane);
+            eg[I] = at4(L.eG, 16 * I + 4 * lq);
+        }
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int I = 0; I < 4; ++I) f[s][I] = prows(L.K, KS, 16 * I, 32 * s, lane);
 #pragma unroll
-        for (int I = 0; I < 4; ++I) {
-            Y[I] = as_acc(L.V, VS, 16 * I, 16 * wave, lane);
-            el[I] = at4(L.eL, 16 * I + 4 * lq);
-            eg[I] = at4(L.eG, 16 * I + 4 * lq);
-        }
+        for (int I = 0; I < 4; ++I) el[I] = at4(L.eL, 16 * I + 4 * lq);
+        const float eC = L.eG[GD_C - 1];
         gd_issued();
+        // k D beside scale e^G d_o and its parts
 #pragma unroll
-        for (int I = 0; I < 4; ++I) X[I] = f32x4{0, 0, 0, 0};
+        for (int I = 0; I < 4; ++I) X[I] = R[I] = zero;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            if (s == NS / 2) {
-#pragma unroll
-                for (int r = 0; r < 2; ++r)
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) fc[r][d] = pcols(L.Q, KS, 32 * r, 16 * d, lane);
-                gd_issued();
-            }
 #pragma unroll
             for (int I = 0; I < 4; ++I) X[I] = mfma32(f[s][I], Dp[s].l, X[I]);
 #pragma unroll
@@ -749,24 +778,45 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
             for (int I = 0; I < 4; ++I) X[I] = mfma32(f[s][I], Dp[s].h, X[I]);
         }
 #pragma unroll
-        for (int I = 0; I < 4; ++I) {
-            X[I] *= el[I];
-            Y[I] *= scale * eg[I];
-        }
+        for (int I = 0; I < 4; ++I) Y[I] *= scale * eg[I];
         const Three Yp[2] = {three(Y[0], Y[1]), three(Y[2], Y[3])};
-        const float eC = L.eG[GD_C - 1];
 #pragma unroll
         for (int d = 0; d < ND; ++d) D[d] *= eC;
+        gd_weave<12 * NS, K == 64 ? 6 : 3>();
+        gd_issued();
 #pragma unroll
         for (int s = 0; s < 2; ++s) dof[s] = cols(L.V, VS, 32 * s, 16 * wave, lane);
         __syncthreads();                                   // P
-        Three pp[4][2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 1; s >= 0; --s)
 #pragma unroll
-            for (int I = 0; I < 2 * s + 2; ++I)
+            for (int I = 2 * s + 1; I >= 0; --I)
                 pp[I][s] = {pcols(P, GD_TS, 32 * s, 16 * I, lane), pcols(P + PS, GD_TS, 32 * s, 16 * I, lane),
                             pcols(P + 2 * PS, GD_TS, 32 * s, 16 * I, lane)};
+#pragma unroll
+        for (int d = 0; d < ND; ++d) fc[0][d] = pcols(L.Q, KS, 0, 16 * d, lane);
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) X[I] *= el[I];
+        const auto p_do = [&](int I, int s) {
+            X[I] = mfma32(pp[I][s].l, dof[s], X[I]);
+            X[I] = mfma32(pp[I][s].m, dof[s], X[I]);
+            X[I] = mfma32(pp[I][s].h, dof[s], X[I]);
+        };
+        p_do(3, 1), p_do(2, 1);
+        gd_issued();
+#pragma unroll
+        for (int d = 0; d < ND; ++d) fc[1][d] = pcols(L.Q, KS, 32, 16 * d, lane);
+        gd_issued();
+        // the other tiles of P^T d_o, and q^T (..), beside the parts of d_n
+        p_do(1, 1), p_do(0, 1), p_do(1, 0), p_do(0, 0);
+        const Three x1 = three(X[2], X[3]);
+        gd_weave<12, 4>();
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) t1[I] = t_cols(L.T, I, 1, lane);
+#pragma unroll
+        for (int I = 0; I < 4; ++I) be[I] = at4(L.be, 16 * I + 4 * lq);
         gd_issued();
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -777,36 +827,17 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
 #pragma unroll
             for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[s][d], Yp[s].h, D[d]);
         }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-#pragma unroll
-            for (int I = 0; I < 2 * s + 2; ++I) X[I] = mfma32(pp[I][s].l, dof[s], X[I]);
-#pragma unroll
-            for (int I = 0; I < 2 * s + 2; ++I) X[I] = mfma32(pp[I][s].m, dof[s], X[I]);
-#pragma unroll
-            for (int I = 0; I < 2 * s + 2; ++I) X[I] = mfma32(pp[I][s].h, dof[s], X[I]);
-        }
-        Three t0[4], t1[4];                                // T^T's columns 0 .. 31 and 32 .. 63
-#pragma unroll
-        for (int I = 0; I < 4; ++I) t1[I] = t_cols(L.T, I, 1, lane);
-#pragma unroll
-        for (int I = 0; I < 4; ++I) be[I] = at4(L.be, 16 * I + 4 * lq);
-        const Three x1 = three(X[2], X[3]);
-        gd_issued();
-        f32x4 R[4];
-#pragma unroll
-        for (int I = 0; I < 4; ++I) R[I] = f32x4{0, 0, 0, 0};
-        mm_tiles<2, 4>(t1, x1, R);
         const Three x0 = three(X[0], X[1]);
-        gd_weave<12, 4>();
+        gd_weave<6 * ND, K == 64 ? 2 : 1>();
         gd_issued();
 #pragma unroll
         for (int I = 0; I < 2; ++I) t0[I] = t_cols(L.T, I, 0, lane);
 #pragma unroll
         for (int d = 0; d < ND; ++d) fc[0][d] = pcols(L.K, KS, 32, 16 * d, lane);
         gd_issued();
+        mm_tiles<2, 4>(t1, x1, R);
+        gd_issued();
         mm_tiles<0, 2>(t1, x1, R);
-        f32x4 V[4];
 #pragma unroll
         for (int I = 2; I < 4; ++I) {
             V[I] = be[I] * R[I];
@@ -815,23 +846,22 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
         const Three r1 = three(X[2], X[3]);
         gd_weave<12, 5>();
         gd_issued();
-        mm_tiles<0, 2>(t0, x0, R);
 #pragma unroll
         for (int d = 0; d < ND; ++d) fc[1][d] = pcols(L.K, KS, 0, 16 * d, lane);
         gd_issued();
-#pragma unroll
-        for (int I = 0; I < 4; ++I) put_tiles(r_save + (at * 4 + I) * 256, R[I], lane);
-#pragma unroll
-        for (int I = 0; I < 2; ++I) {
-            V[I] = be[I] * R[I];
-            X[I] = -eg[I] * V[I];
-        }
+        mm_tiles<0, 2>(t0, x0, R);
+        gd_issued();
 #pragma unroll
         for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[0][d], r1.l, D[d]);
 #pragma unroll
         for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[0][d], r1.m, D[d]);
 #pragma unroll
         for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[0][d], r1.h, D[d]);
+#pragma unroll
+        for (int I = 0; I < 2; ++I) {
+            V[I] = be[I] * R[I];
+            X[I] = -eg[I] * V[I];
+        }
         const Three r0 = three(X[0], X[1]);
         gd_weave<3 * ND, K == 64 ? 5 : 3>();
         gd_issued();
@@ -841,12 +871,22 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
         for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[1][d], r0.m, D[d]);
 #pragma unroll
         for (int d = 0; d < ND; ++d) D[d] = mfma32(fc[1][d], r0.h, D[d]);
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) put_tiles(r_save + (at * 4 + I) * 256, R[I], lane);
         uint16_t* pv = dv + (w.bh * n.T + c * GD_C + 4 * lq) * n.V + col;
+        if ((c + 1) * GD_C <= n.T) {
 #pragma unroll
-        for (int I = 0; I < 4; ++I)
+            for (int I = 0; I < 4; ++I)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (c * GD_C + 16 * I + 4 * lq + r < n.T) pv[(int64_t)(16 * I + r) * n.V] = f2bf(V[I][r]);
+                for (int r = 0; r < 4; ++r) pv[(16 * I + r) * n.V] = f2bf(V[I][r]);
+        } else {
+#pragma unroll
+            for (int I = 0; I < 4; ++I)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (c * GD_C + 16 * I + 4 * lq + r < n.T) pv[(16 * I + r) * n.V] = f2bf(V[I][r]);
+        }
     }
     if (dh0)
 #pragma unroll
