@@ -262,9 +262,9 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
     __shared__ float2 G[GD_C];
     __shared__ float be[GD_C];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q = lane >> 4;
-    const int64_t chunk = blockIdx.x, bh = chunk / n.NC;
-    const int c = (int)(chunk - bh * n.NC), hv = (int)(bh % n.HV), t0 = c * GD_C;
-    const uint16_t* kp = k.p + (bh / n.HV) * k.sb + (int64_t)(hv / (n.HV / n.H)) * k.sh;
+    const int64_t chunk = blockIdx.x, bh = blockIdx.x / (unsigned)n.NC;
+    const int c = (int)(blockIdx.x % (unsigned)n.NC), b = (int)bh / n.HV, hv = (int)bh % n.HV, t0 = c * GD_C;
+    const uint16_t* kp = k.p + b * k.sb + (hv / (n.HV / n.H)) * k.sh;
     bf16x8 f[4][K / 32];
 #pragma unroll
     for (int J = 0; J < 4; ++J)
@@ -442,11 +442,12 @@ struct WalkAt {
 };
 template <int NW> __device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
     WalkAt w;
-    w.bh = blockIdx.x % n.BH;
-    w.b = w.bh / n.HV;
-    w.hv = (int)(w.bh % n.HV);
+    const unsigned heads = (unsigned)n.BH, bh = blockIdx.x % heads;
+    w.bh = bh;
+    w.b = bh / (unsigned)n.HV;
+    w.hv = (int)(bh % (unsigned)n.HV);
     w.hk = w.hv / (n.HV / n.H);
-    w.v0 = 16 * NW * (int)(blockIdx.x / n.BH);
+    w.v0 = 16 * NW * (int)(blockIdx.x / heads);
     return w;
 }
 // A block's waves: NW walk (the first), four help.  Wave w runs on SIMD w % 4, so with fewer walking the helpers are
@@ -947,8 +948,8 @@ __device__ __forceinline__ bf16x8 plain_rows(const uint16_t* X, int stride, int 
 // d_q, d_k, d_g and d_beta of a chunk of a key head, its value heads one after the other.  Wave (I, half) has the
 // tokens 16 I .. 16 I + 15 against half of the key channels, and of the columns of p and m those of its parity; every
 // product is formed transposed, so that a lane has one token and four adjacent channels.
-template <int K>
-__global__ void __launch_bounds__(512, K == 64 ? 4 : 2)
+template <int K, bool GROUPED>
+__global__ void __launch_bounds__(512, K == 64 && !GROUPED ? 4 : 2)
 rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o, const float* __restrict__ beta, int beta_dt,
                                const float2* __restrict__ G_in, const float* __restrict__ S_save,
                                const float* __restrict__ n_save, const float* __restrict__ D_save,
@@ -975,13 +976,11 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
         lr = x & 15;
         lq = lane >> 4;
     };
-    const int group = n.HV / n.H;
-    const int64_t kc = blockIdx.x, bk = kc / n.NC, b = bk / n.H;
-    const int c = (int)(kc - bk * n.NC), hk = (int)(bk % n.H), t0 = c * GD_C;
-    if (half)
-        tile_store<K, false>(tile_load<K>(q.p + b * q.sb + hk * q.sh, q.st, t0, n.T, tid - 256), Qt, t0, n.T, tid - 256);
-    else
-        tile_store<K, false>(tile_load<K>(k.p + b * k.sb + hk * k.sh, k.st, t0, n.T, tid), Kt, t0, n.T, tid);
+    const int group = GROUPED ? n.HV / n.H : 1;
+    const int bk = (int)(blockIdx.x / (unsigned)n.NC), c = (int)(blockIdx.x % (unsigned)n.NC), hk = bk % n.H, t0 = c * GD_C;
+    const int64_t b = bk / n.H;
+    const auto tile = half ? tile_load<K>(q.p + b * q.sb + hk * q.sh, q.st, t0, n.T, tid - 256)
+                           : tile_load<K>(k.p + b * k.sb + hk * k.sh, k.st, t0, n.T, tid);
     const int d0 = ND * half;
     f32x4 aq[ND], ak[ND];
 #pragma unroll
@@ -1003,28 +1002,36 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
         P[0] = P[1] = R[0] = R[1] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < ND; ++d) Z[d] = Y[d] = W[d] = f32x4{0, 0, 0, 0};
-        for (int vb = 0; vb < n.V / 32; ++vb) {
+        f32x4 xn[1], xr[1], xs[K / 64], xd[K / 64];
+        uint4 ov, vv;
+        const auto load = [&](int vb) {
             const int64_t at = chunk * (n.V / 16) + 2 * vb;
-            f32x4 xn[1], xr[1], xs[K / 64], xd[K / 64];
             tiles_load<4>(n_save, at, tid, xn);
             tiles_load<4>(r_save, at, tid, xr);
             tiles_load<K / 16>(S_save, at, tid, xs);
             tiles_load<K / 16>(D_save, at, tid, xd);
-            const int row = t0 + 16 * I + lr, in = min(row, n.T - 1);
-            uint4 ov = *reinterpret_cast<const uint4*>(op + in * d_o.st + 32 * vb + 8 * lq);
-            uint4 vv = *reinterpret_cast<const uint4*>(vp + in * v.st + 32 * vb + 8 * lq);
-            if (row >= n.T) ov = vv = make_uint4(0, 0, 0, 0);
-            const bf16x8 fo = __builtin_bit_cast(bf16x8, ov), fv = __builtin_bit_cast(bf16x8, vv);
+            const int row = min(t0 + 16 * I + lr, n.T - 1);
+            ov = *reinterpret_cast<const uint4*>(op + row * d_o.st + 32 * vb + 8 * lq);
+            vv = *reinterpret_cast<const uint4*>(vp + row * v.st + 32 * vb + 8 * lq);
+        };
+        load(0);
+        if (e == 0) tile_store<K, false>(tile, half ? Qt : Kt, t0, n.T, tid & 255);
+        const int blocks = n.V / 32;
+        for (int vb = 0; vb < blocks; ++vb) {
 #pragma unroll
             for (int j = 0; j < K / 64; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sd += xs[j][r] * xd[j][r];
+            const bool live = t0 + 16 * I + lr < n.T;
+            const uint4 none = make_uint4(0, 0, 0, 0);
+            const bf16x8 fo = __builtin_bit_cast(bf16x8, live ? ov : none), fv = __builtin_bit_cast(bf16x8, live ? vv : none);
             __syncthreads();                               // the last block's operands, or p and m, are done with
             tiles_store<4>(xn, Nt, tid);
             tiles_store<4>(xr, Rt, tid);
             tiles_store<K / 16>(xs, St, tid);
             tiles_store<K / 16>(xd, Dt, tid);
             __syncthreads();
+            load(min(vb + 1, blocks - 1));                 // the next block's, under this one's products
             {
                 const Three fr = tr3(Rt, GD_TS, 16 * I, lane);
                 if (half) RV = mm(fr, fv, RV);
@@ -1169,7 +1176,7 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
             if (beta_dt == RWKV6_BF16) reinterpret_cast<uint16_t*>(dbeta)[at] = f2bf(x);
             else reinterpret_cast<float*>(dbeta)[at] = x;
         }
-        __syncthreads();                                   // the sums and G are written again
+        if (GROUPED) __syncthreads();                      // the sums and G are written again
     }
     anew();
     const int row = t0 + 16 * I + lr;
@@ -1316,8 +1323,10 @@ int gd_limits(hipStream_t stream) {
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<K, NW>), WalkLds<K, NW, 3>::bytes);
         GD_RAISE(64, 1) GD_RAISE(64, 2) GD_RAISE(64, 4) GD_RAISE(128, 1) GD_RAISE(128, 2) GD_RAISE(128, 4)
 #undef GD_RAISE
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<64>), GradLds<64>::bytes);
-        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<128>), GradLds<128>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<64, false>), GradLds<64>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<64, true>), GradLds<64>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<128, false>), GradLds<128>::bytes);
+        raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<128, true>), GradLds<128>::bytes);
         return e;
     });
 }
@@ -1423,7 +1432,8 @@ int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const voi
                                (uint16_t*)dv, dh0, D, R, n, scale);
         });
     if (T > 0) {
-        auto grads = K == 64 ? rwkv6_gated_delta_grads_kernel<64> : rwkv6_gated_delta_grads_kernel<128>;
+        auto grads = K == 64 ? (HV > H ? rwkv6_gated_delta_grads_kernel<64, true> : rwkv6_gated_delta_grads_kernel<64, false>)
+                             : (HV > H ? rwkv6_gated_delta_grads_kernel<128, true> : rwkv6_gated_delta_grads_kernel<128, false>);
         hipLaunchKernelGGL(grads, dim3((unsigned)(B * H * n.NC)), dim3(512), K == 64 ? GradLds<64>::bytes : GradLds<128>::bytes, s,
                            qt, kt, vt, ot, be, beta_dtype, G, S, N, D, R, (uint16_t*)dq, (uint16_t*)dk, dg, dbeta, n, scale);
     }
