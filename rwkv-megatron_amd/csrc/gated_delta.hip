@@ -994,7 +994,7 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
     };
     const int group = GROUPED ? n.HV / n.H : 1;
     const int bk = (int)(blockIdx.x / (unsigned)n.NC), c = (int)(blockIdx.x % (unsigned)n.NC), hk = bk % n.H, t0 = c * GD_C;
-    const int64_t b = bk / n.H;
+    const int64_t b = bk / n.H, head = bk;
     const auto tile = half ? tile_load<K>(q.p + b * q.sb + hk * q.sh, q.st, t0, n.T, tid - 256)
                            : tile_load<K>(k.p + b * k.sb + hk * k.sh, k.st, t0, n.T, tid);
     const int d0 = ND * half;
@@ -1199,7 +1199,7 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
     if (row < n.T)
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const int64_t at = (bk * n.T + row) * K + 16 * (d0 + d) + 4 * lq;
+            const int64_t at = (head * n.T + row) * K + 16 * (d0 + d) + 4 * lq;
             *reinterpret_cast<uint2*>(dq + at) = make_uint2(pk2(aq[d][0], aq[d][1]), pk2(aq[d][2], aq[d][3]));
             *reinterpret_cast<uint2*>(dk + at) = make_uint2(pk2(ak[d][0], ak[d][1]), pk2(ak[d][2], ak[d][3]));
         }
@@ -1273,11 +1273,11 @@ inline bool gd_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15
 int gd_shape(int64_t B, int64_t H, int64_t HV, int64_t T, int64_t K, int64_t V, GdShape* n) {
     if (B < 0 || H < 1 || HV < 1 || T < 0 || K < 1 || V < 1 || HV % H) return RWKV6_ERR_INVALID_ARG;
     if ((K != 64 && K != 128) || V % 64 || V > 512) return RWKV6_ERR_UNSUPPORTED;
-    // a launch holds fewer than 2^32 threads, 512 a chunk and head, and 64 a wave of a step
+    // a launch holds fewer than 2^32 threads: 512 a chunk and head, or a head and 64 value channels
     const int64_t most = ((int64_t)1 << 23) - 1;
     if (HV > most || B > most / HV || T > ((int64_t)1 << 30)) return RWKV6_ERR_UNSUPPORTED;
     const int64_t NC = (T + GD_C - 1) / GD_C;
-    if (B * HV * (NC > V / 8 ? NC : V / 8) > most) return RWKV6_ERR_UNSUPPORTED;
+    if (B * HV * (NC > V / 64 ? NC : V / 64) > most) return RWKV6_ERR_UNSUPPORTED;
     *n = {(int)H, (int)HV, (int)T, (int)NC, (int)V, B * HV};
     return RWKV6_OK;
 }
