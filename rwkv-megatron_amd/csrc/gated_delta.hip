@@ -44,7 +44,7 @@
 #define GD_C 64                 // tokens of a chunk
 #define GD_PAD 8                // elements behind a row of an LDS tile
 #define GD_TS (GD_C + GD_PAD)   // row of a bf16 tile of 64 columns
-#define GD_TF (GD_C + 4)        // row of T in 32 bits
+#define GD_BF 20                // row of a 16 x 16 block in 32 bits
 #define GD_TB 7680              // T in memory: the ten 16 x 16 blocks of its triangle in three parts
 #define GD_TP 3584              // a part of T in LDS: 32 rows of 32 columns, 32 of 64
 #define GD_TROW(i) ((i) < 32 ? (i) * 40 : 1280 + ((i) - 32) * GD_TS)
@@ -131,9 +131,9 @@ __device__ __forceinline__ f32x4 as_acc(const uint16_t* X, int stride, int r0, i
     return f32x4{f[0], f[1], f[2], f[3]};
 }
 __device__ __forceinline__ f32x4 at4(const float* p, int i) { return *reinterpret_cast<const f32x4*>(p + i); }
-// Block (I, l) of a 32-bit tile times an accumulator tile, in 32 bits.  Step r contracts over rows 4q + r.
-__device__ __forceinline__ f32x4 mul_f32(const float* T, int I, int l, const f32x4& x, f32x4 c, int lane) {
-    const f32x4 t = at4(T, (16 * I + (lane & 15)) * GD_TF + 16 * l + 4 * (lane >> 4));
+// A 16 x 16 block times an accumulator tile, in 32 bits.  Step r contracts over rows 4q + r.
+__device__ __forceinline__ f32x4 mul_f32(const float* B, const f32x4& x, f32x4 c, int lane) {
+    const f32x4 t = at4(B, (lane & 15) * GD_BF + 4 * (lane >> 4));
 #pragma unroll
     for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(t[r], x[r], c, 0, 0, 0);
     return c;
@@ -258,7 +258,9 @@ template <int K>
 __global__ void __launch_bounds__(256)
 rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const void* __restrict__ beta, int beta_dt,
                               float2* __restrict__ G_out, float* __restrict__ b_out, uint16_t* __restrict__ T_out, GdShape n) {
-    __shared__ __attribute__((aligned(16))) float As[GD_C][GD_TF], Ts[GD_C][GD_TF];
+    // the blocks of the triangles, row by row: 26 KB of LDS leave room for six blocks a CU (126 to 101 us for 16384 chunks,
+    // whole squares for four)
+    __shared__ __attribute__((aligned(16))) float As[10][16 * GD_BF], Ts[10][16 * GD_BF];
     __shared__ float2 G[GD_C];
     __shared__ float be[GD_C];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q = lane >> 4;
@@ -305,26 +307,27 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
             f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = i > j + r ? be[i] * ex2(gd_gap(gi, G[j + r])) * a[r] : 0.f;
-            *reinterpret_cast<f32x4*>(&As[i][j]) = x;
+            *reinterpret_cast<f32x4*>(&As[I * (I + 1) / 2 + J][lr * GD_BF + 4 * q]) = x;
         }
     }
     __syncthreads();
     {
         float x[16];
-        const int b = 16 * wave;
+        const float* A = As[wave * (wave + 3) / 2];
+        float* D = Ts[wave * (wave + 3) / 2];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float a[16], s0 = r == lr ? 1.f : 0.f, s1 = 0.f;
 #pragma unroll
             for (int s = 0; s < r; s += 4) {
-                const f32x4 v = at4(&As[b + r][b + s], 0);
+                const f32x4 v = at4(A, r * GD_BF + s);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) a[s + j] = v[j];
             }
 #pragma unroll
             for (int s = 0; s < r; ++s) (s & 1 ? s1 : s0) -= a[s] * x[s];
             x[r] = s0 + s1;
-            if ((r >> 2) == q) Ts[b + r][b + lr] = x[r];
+            if ((r >> 2) == q) D[r * GD_BF + lr] = x[r];
         }
     }
     __syncthreads();
@@ -333,22 +336,22 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
         if (J != wave) continue;
         f32x4 t[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[J][r] = Ts[16 * J + 4 * q + r][16 * J + lr];
+        for (int r = 0; r < 4; ++r) t[J][r] = Ts[J * (J + 3) / 2][(4 * q + r) * GD_BF + lr];
 #pragma unroll
         for (int I = J + 1; I < 4; ++I) {
             f32x4 a = {0, 0, 0, 0}, d = {0, 0, 0, 0};
 #pragma unroll
-            for (int l = J; l < I; ++l) a = mul_f32(&As[0][0], I, l, t[l], a, lane);
-            d = mul_f32(&Ts[0][0], I, I, a, d, lane);
+            for (int l = J; l < I; ++l) a = mul_f32(As[I * (I + 1) / 2 + l], t[l], a, lane);
+            d = mul_f32(Ts[I * (I + 3) / 2], a, d, lane);
             t[I] = -d;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) Ts[16 * I + 4 * q + r][16 * J + lr] = t[I][r];
+            for (int r = 0; r < 4; ++r) Ts[I * (I + 1) / 2 + J][(4 * q + r) * GD_BF + lr] = t[I][r];
         }
     }
     __syncthreads();
     for (int i = tid; i < 320; i += 256) {
-        const int t = i >> 5, row = (i >> 1) & 15, half = i & 1, I = gd_block_row(t), J = t - I * (I + 1) / 2;
-        const float* p = &Ts[16 * I + row][16 * J + 8 * half];
+        const int t = i >> 5, row = (i >> 1) & 15, half = i & 1;
+        const float* p = &Ts[t][row * GD_BF + 8 * half];
         const Three x = three(at4(p, 0), at4(p, 4));
         uint4* out = reinterpret_cast<uint4*>(T_out + chunk * GD_TB) + 96 * t + 2 * row + half;
         out[0] = __builtin_bit_cast(uint4, x.h);
