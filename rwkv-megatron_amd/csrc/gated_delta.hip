@@ -45,7 +45,7 @@
 #define GD_PAD 8                // elements behind a row of an LDS tile
 #define GD_TS (GD_C + GD_PAD)   // row of a bf16 tile of 64 columns
 #define GD_BF 20                // row of a 16 x 16 block in 32 bits
-#define GD_TB 7680              // T in memory: the ten 16 x 16 blocks of its triangle in three parts
+#define GD_TB 2560              // T in memory: the ten 16 x 16 blocks of its triangle
 #define GD_TP 3584              // a part of T in LDS: 32 rows of 32 columns, 32 of 64
 #define GD_TROW(i) ((i) < 32 ? (i) * 40 : 1280 + ((i) - 32) * GD_TS)
 #define GD_FLOOR (-1024.f)      // log decays below are this one: e^-1024 is 0 in 32 bits
@@ -253,11 +253,11 @@ template <int N> __device__ __forceinline__ void gd_zero_p(uint16_t* P, int tid)
 // G and T of a chunk.  Wave w forms the rows of its 16-token block of A = beta L k k^T, inverts the block
 // on the diagonal by substitution, and then column w of the blocks below it, in the 32-bit matrix instructions:
 // T_IJ = -T_II sum_{J<=l<I} A_Il T_lJ.  Out: G [chunk][64] as pairs of floats in base-2 units, beta
-// in 32 bits, T [chunk][10 blocks][3 parts][16][16].
+// in 32 bits, T [chunk][10 blocks][16][16].
 template <int K>
 __global__ void __launch_bounds__(256)
 rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const void* __restrict__ beta, int beta_dt,
-                              float2* __restrict__ G_out, float* __restrict__ b_out, uint16_t* __restrict__ T_out, GdShape n) {
+                              float2* __restrict__ G_out, float* __restrict__ b_out, float* __restrict__ T_out, GdShape n) {
     // the blocks of the triangles, row by row: 26 KB of LDS leave room for six blocks a CU (126 to 101 us for 16384 chunks,
     // whole squares for four)
     __shared__ __attribute__((aligned(16))) float As[10][16 * GD_BF], Ts[10][16 * GD_BF];
@@ -349,15 +349,8 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
         }
     }
     __syncthreads();
-    for (int i = tid; i < 320; i += 256) {
-        const int t = i >> 5, row = (i >> 1) & 15, half = i & 1;
-        const float* p = &Ts[t][row * GD_BF + 8 * half];
-        const Three x = three(at4(p, 0), at4(p, 4));
-        uint4* out = reinterpret_cast<uint4*>(T_out + chunk * GD_TB) + 96 * t + 2 * row + half;
-        out[0] = __builtin_bit_cast(uint4, x.h);
-        out[32] = __builtin_bit_cast(uint4, x.m);
-        out[64] = __builtin_bit_cast(uint4, x.l);
-    }
+    for (int i = tid; i < GD_TB / 4; i += 256)
+        *reinterpret_cast<f32x4*>(T_out + chunk * GD_TB + 4 * i) = at4(Ts[i >> 6], ((i >> 2) & 15) * GD_BF + 4 * (i & 3));
 }
 
 namespace {
@@ -389,14 +382,14 @@ template <int K, int NW> __device__ __forceinline__ WalkBuf walk_buf(uint16_t* p
 template <int K, int NW> struct WalkRegs {
     TileRegs<K> q, k;
     TileRegs<16 * NW> v;
-    uint4 t[4];
+    f32x4 t[3];
     float2 G, GC;
     float be;
 };
 struct WalkIn {
     const uint16_t *q, *k, *v;
     int64_t qs, ks, vs;
-    const uint16_t* T;          // of the head's first chunk
+    const float* T;             // of the head's first chunk
     const float* beta;
     const float2* G;
     int tokens;
@@ -408,9 +401,9 @@ __device__ __forceinline__ WalkRegs<K, NW> walk_load(const WalkIn& w, int c, int
     r.k = tile_load<K>(w.k, w.ks, t0, w.tokens, tid);
     r.q = tile_load<K>(w.q, w.qs, t0, w.tokens, tid);
     r.v = tile_load<16 * NW>(w.v, w.vs, t0, w.tokens, tid);
-    const uint4* T = reinterpret_cast<const uint4*>(w.T + (int64_t)c * GD_TB);
+    const f32x4* T = reinterpret_cast<const f32x4*>(w.T + (int64_t)c * GD_TB);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.t[i] = T[min(tid + 256 * i, GD_TB / 8 - 1)];
+    for (int i = 0; i < 3; ++i) r.t[i] = T[min(tid + 256 * i, GD_TB / 4 - 1)];
     r.G = w.G[t0 + (tid & 63)];
     r.GC = w.G[t0 + GD_C - 1];
     r.be = w.beta[t0 + (tid & 63)];
@@ -423,12 +416,17 @@ __device__ __forceinline__ void walk_store(const WalkRegs<K, NW>& r, const WalkI
     tile_store<K, true>(r.q, L.Q, t0, w.tokens, tid);
     tile_store<16 * NW, false>(r.v, L.V, t0, w.tokens, tid);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (i == 3 && tid >= GD_TB / 8 - 768) break;
-        const int p = tid + 256 * i, t = p / 96, part = (p >> 5) % 3, I = gd_block_row(t), J = t - I * (I + 1) / 2;
-        uint16_t* x = L.T + part * GD_TP + GD_TROW(16 * I + ((p >> 1) & 15)) + GD_POS(16 * J + 8 * (p & 1));
-        *reinterpret_cast<uint2*>(x) = make_uint2(r.t[i].x, r.t[i].y);
-        *reinterpret_cast<uint2*>(x + 8) = make_uint2(r.t[i].z, r.t[i].w);
+    for (int i = 0; i < 3; ++i) {
+        if (i == 2 && tid >= GD_TB / 4 - 512) break;
+        const int t = (tid >> 6) + 4 * i, I = gd_block_row(t), J = t - I * (I + 1) / 2;
+        uint16_t* p = L.T + GD_TROW(16 * I + ((tid >> 2) & 15)) + GD_POS(16 * J + 4 * (tid & 3));
+        float x[4] = {r.t[i][0], r.t[i][1], r.t[i][2], r.t[i][3]};
+        uint2 part = make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
+#pragma unroll
+        for (int m = 0; m < 3; ++m) {
+            *reinterpret_cast<uint2*>(p + m * GD_TP) = part;
+            if (m < 2) part = rest4(x, part);
+        }
     }
     if (tid < GD_C) {
         L.G[tid] = r.G;
@@ -515,7 +513,7 @@ template <int N, int V> __device__ __forceinline__ void gd_weave() {
 template <int K, int NW, bool SAVE>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
-                             const float2* __restrict__ G, const uint16_t* __restrict__ T, const float* __restrict__ h0,
+                             const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ h0,
                              uint16_t* __restrict__ o, float* __restrict__ hT, float* __restrict__ S_save,
                              float* __restrict__ n_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
@@ -703,10 +701,14 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
         uint2 ob[4];
 #pragma unroll
         for (int I = 0; I < 4; ++I) ob[I] = make_uint2(pk2(O[I][0], O[I][1]), pk2(O[I][2], O[I][3]));
-        const bool full = (c + 1) * GD_C <= n.T;
+        if ((c + 1) * GD_C <= n.T) {                       // one branch, not four
 #pragma unroll
-        for (int I = 0; I < 4; ++I)
-            if (full || c * GD_C + 16 * I + lr < n.T) *reinterpret_cast<uint2*>(po + (int64_t)16 * I * n.V) = ob[I];
+            for (int I = 0; I < 4; ++I) *reinterpret_cast<uint2*>(po + (int64_t)16 * I * n.V) = ob[I];
+        } else {
+#pragma unroll
+            for (int I = 0; I < 4; ++I)
+                if (c * GD_C + 16 * I + lr < n.T) *reinterpret_cast<uint2*>(po + (int64_t)16 * I * n.V) = ob[I];
+        }
     }
     if (hT)
 #pragma unroll
@@ -719,7 +721,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
 template <int K, int NW>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* __restrict__ beta,
-                             const float2* __restrict__ G, const uint16_t* __restrict__ T, const float* __restrict__ dhT,
+                             const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ dhT,
                              uint16_t* __restrict__ dv, float* __restrict__ dh0, float* __restrict__ D_save,
                              float* __restrict__ r_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
@@ -1302,7 +1304,7 @@ struct GdSaved {
     GdSaved(const GdShape& n, int64_t K) {
         const size_t chunks = (size_t)n.BH * n.NC;
         T = 0;
-        G = T + chunks * 2 * GD_TB;
+        G = T + chunks * 4 * GD_TB;
         B = G + chunks * 8 * GD_C;
         S = B + chunks * 4 * GD_C;
         N = S + chunks * 4 * K * n.V;
@@ -1394,7 +1396,7 @@ int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int
     if ((st = gd_limits(s))) return st;
     char* base = static_cast<char*>(saved ? saved : workspace);
     float2* G = reinterpret_cast<float2*>(base + at.G);
-    uint16_t* Tm = reinterpret_cast<uint16_t*>(base);
+    float* Tm = reinterpret_cast<float*>(base);
     float *be = reinterpret_cast<float*>(base + at.B), *S = saved ? reinterpret_cast<float*>(base + at.S) : nullptr,
           *N = saved ? reinterpret_cast<float*>(base + at.N) : nullptr;
     if (T > 0) {
@@ -1440,7 +1442,7 @@ int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const voi
     if ((st = gd_limits(s))) return st;
     const char* base = static_cast<const char*>(saved);
     const float2* G = reinterpret_cast<const float2*>(base + at.G);
-    const uint16_t* Tm = reinterpret_cast<const uint16_t*>(base);
+    const float* Tm = reinterpret_cast<const float*>(base);
     const float *be = reinterpret_cast<const float*>(base + at.B), *S = reinterpret_cast<const float*>(base + at.S),
                 *N = reinterpret_cast<const float*>(base + at.N);
     float *D = static_cast<float*>(workspace), *R = D + (at.N - at.S) / 4;

@@ -89,11 +89,11 @@ def test_sizes(pkg):
     L = pkg._lib.load()
     B, HV, T = 8, 32, 4096
     chunks = B * HV * T // 64
-    # 64 tokens of a head: T 15 KB, G and beta, states and written values of 16 KB
-    assert L.rwkv6_gated_delta_saved_bytes(B, HV, T, 64, 64) == chunks * (15360 + 512 + 256 + 16384 + 16384)
-    assert L.rwkv6_gated_delta_workspace_bytes(B, HV, T, 64, 64, 0) == chunks * (15360 + 512 + 256)
+    # 64 tokens of a head: T 10 KB, G and beta, states and written values of 16 KB
+    assert L.rwkv6_gated_delta_saved_bytes(B, HV, T, 64, 64) == chunks * (10240 + 512 + 256 + 16384 + 16384)
+    assert L.rwkv6_gated_delta_workspace_bytes(B, HV, T, 64, 64, 0) == chunks * (10240 + 512 + 256)
     assert L.rwkv6_gated_delta_workspace_bytes(B, HV, T, 64, 64, 1) == chunks * (16384 + 16384)
-    assert L.rwkv6_gated_delta_saved_bytes(1, 1, 1, 128, 64) == 15360 + 512 + 256 + 32768 + 16384
+    assert L.rwkv6_gated_delta_saved_bytes(1, 1, 1, 128, 64) == 10240 + 512 + 256 + 32768 + 16384
     assert L.rwkv6_gated_delta_saved_bytes(B, HV, 0, 64, 64) == 0 == L.rwkv6_gated_delta_saved_bytes(B, HV, T, 32, 64)
 
 
