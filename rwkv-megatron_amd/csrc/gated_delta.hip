@@ -60,6 +60,7 @@ struct GdTensor {               // [B, heads, T, channels], channels adjacent
 struct GdShape {
     int H, HV, T, NC, V;        // key heads, value heads, tokens, chunks, value channels
     int64_t BH;                 // sequences times value heads
+    int per, segs;              // the forward's chunks of a segment, segments
 };
 struct Two {                    // a computed operand: h + l, 2^-16 off at most
     bf16x8 h, l;
@@ -394,12 +395,12 @@ struct WalkIn {
     const float2* G;
     int tokens;
 };
-template <int K, int NW>
+template <int K, int NW, bool Q>
 __device__ __forceinline__ WalkRegs<K, NW> walk_load(const WalkIn& w, int c, int tid) {
     WalkRegs<K, NW> r;
     const int t0 = c * GD_C;
     r.k = tile_load<K>(w.k, w.ks, t0, w.tokens, tid);
-    r.q = tile_load<K>(w.q, w.qs, t0, w.tokens, tid);
+    if constexpr (Q) r.q = tile_load<K>(w.q, w.qs, t0, w.tokens, tid);
     r.v = tile_load<16 * NW>(w.v, w.vs, t0, w.tokens, tid);
     const f32x4* T = reinterpret_cast<const f32x4*>(w.T + (int64_t)c * GD_TB);
 #pragma unroll
@@ -409,11 +410,11 @@ __device__ __forceinline__ WalkRegs<K, NW> walk_load(const WalkIn& w, int c, int
     r.be = w.beta[t0 + (tid & 63)];
     return r;
 }
-template <int K, int NW>
+template <int K, int NW, bool Q>
 __device__ __forceinline__ void walk_store(const WalkRegs<K, NW>& r, const WalkIn& w, int c, const WalkBuf& L, int tid) {
     const int t0 = c * GD_C;
     tile_store<K, true>(r.k, L.K, t0, w.tokens, tid);
-    tile_store<K, true>(r.q, L.Q, t0, w.tokens, tid);
+    if constexpr (Q) tile_store<K, true>(r.q, L.Q, t0, w.tokens, tid);
     tile_store<16 * NW, false>(r.v, L.V, t0, w.tokens, tid);
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -439,7 +440,7 @@ __device__ __forceinline__ void walk_store(const WalkRegs<K, NW>& r, const WalkI
 // heads are one, on the same XCD, and find its q, k and T in that L2.
 struct WalkAt {
     int64_t bh, b;
-    int hv, hk, v0;
+    int hv, hk, v0, seg;
 };
 template <int NW> __device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
     WalkAt w;
@@ -448,8 +449,26 @@ template <int NW> __device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
     w.b = bh / (unsigned)n.HV;
     w.hv = (int)(bh % (unsigned)n.HV);
     w.hk = w.hv / (n.HV / n.H);
-    w.v0 = 16 * NW * (int)(blockIdx.x / heads);
+    const int col = (int)(blockIdx.x / heads), cols = n.V / (16 * NW);
+    w.v0 = 16 * NW * (col % cols);
+    w.seg = col / cols;
     return w;
+}
+// The inputs of a head from chunk c0 on.
+__device__ __forceinline__ WalkIn walk_in(const WalkAt& w, const GdShape& n, int c0, const GdTensor& q, const GdTensor& k,
+                                          const GdTensor& v, const float* T, const float* beta, const float2* G) {
+    const int64_t at = w.bh * n.NC + c0, t = (int64_t)c0 * GD_C;
+    return {q.p + w.b * q.sb + w.hk * q.sh + t * q.st, k.p + w.b * k.sb + w.hk * k.sh + t * k.st,
+            v.p + w.b * v.sb + w.hv * v.sh + t * v.st + w.v0, q.st, k.st, v.st, T + at * GD_TB, beta + at * GD_C, G + at * GD_C,
+            n.T - c0 * GD_C};
+}
+// What a segment but the last leaves: its map M [K][K] of the state that enters it, and the state it leaves for an empty
+// one (the first: for h0), in tiles; `join` makes that the state which the next one starts from.
+template <int K> __device__ __forceinline__ float* seg_map(float* E, const GdShape& n, int64_t bh, int seg) {
+    return E + (bh * (n.segs - 1) + seg) * K * (K + n.V);
+}
+template <int K> __device__ __forceinline__ float* seg_state(float* E, const GdShape& n, int64_t bh, int seg, int ct) {
+    return seg_map<K>(E, n, bh, seg) + K * K + ct * (K * 16);
 }
 // A block's waves: NW walk (the first), four help.  Wave w runs on SIMD w % 4, so with fewer walking the helpers are
 // placed on the other SIMDs and the waves between, which have nothing to do, end at once.
@@ -464,12 +483,13 @@ template <int NW> __device__ __forceinline__ int walk_role(int wave) {       // 
 
 namespace {
 // What the four helper waves of a walk do: chunk c is in LDS before the first barrier of its step and P of it before
-// the second; the loads of the chunk after the next are in flight meanwhile.
+// the second; the loads of the chunk after the next are in flight meanwhile.  NP = 0: no q, no P, no second barrier.
 template <int K, int NW, int NP, bool BACK>
 __device__ __forceinline__ void walk_help(const WalkIn& in, int NC, float scale, uint16_t* lds, int tid) {
     using M = WalkLds<K, NW, NP>;
     uint16_t* const P = lds + 2 * M::buf;
     const int lane = tid & 63, wave = tid >> 6;
+    constexpr bool Q = NP > 0;
     const auto at = [&](int x) { return BACK ? NC - 1 - min(x, NC - 1) : min(x, NC - 1); };
     gd_zero_p<NP>(P, tid);
     if (tid < 128)                                         // the blocks of T right of the diagonal that a step of 32 takes in
@@ -480,16 +500,18 @@ __device__ __forceinline__ void walk_help(const WalkIn& in, int NC, float scale,
             *reinterpret_cast<uint2*>(T + GD_TROW(32 * b + ((tid >> 2) & 15)) + GD_POS(32 * b + 16 + 4 * (tid & 3))) = make_uint2(0, 0);
         }
     if (!NC) return;
-    walk_store<K, NW>(walk_load<K, NW>(in, at(0), tid), in, at(0), walk_buf<K, NW>(lds), tid);
-    WalkRegs<K, NW> next = walk_load<K, NW>(in, at(1), tid);
+    walk_store<K, NW, Q>(walk_load<K, NW, Q>(in, at(0), tid), in, at(0), walk_buf<K, NW>(lds), tid);
+    WalkRegs<K, NW> next = walk_load<K, NW, Q>(in, at(1), tid);
     for (int x = 0; x < NC; ++x) {
         const int u = x & 1;
         const WalkBuf L = walk_buf<K, NW>(lds + u * M::buf);
         __syncthreads();
-        const WalkRegs<K, NW> later = walk_load<K, NW>(in, at(x + 2), tid);
-        gd_p<K, NP>(L.Q, L.K, L.G, scale, P, wave, lane);
-        __syncthreads();
-        if (x + 1 < NC) walk_store<K, NW>(next, in, at(x + 1), walk_buf<K, NW>(lds + (u ^ 1) * M::buf), tid);
+        const WalkRegs<K, NW> later = walk_load<K, NW, Q>(in, at(x + 2), tid);
+        if constexpr (Q) {
+            gd_p<K, NP>(L.Q, L.K, L.G, scale, P, wave, lane);
+            __syncthreads();
+        }
+        if (x + 1 < NC) walk_store<K, NW, Q>(next, in, at(x + 1), walk_buf<K, NW>(lds + (u ^ 1) * M::buf), tid);
         next = later;
     }
 }
@@ -508,43 +530,51 @@ template <int N, int V> __device__ __forceinline__ void gd_weave() {
 }
 }  // namespace
 
-// A block walks one head's chunks with 16 NW columns of the state.  SAVE: S_save and n_save get the state entering each
-// chunk and the values it writes, for the backward.
+// A block walks a segment of one head's chunks with 16 NW columns of the state.  SAVE: S_save and n_save get the state
+// entering each chunk and the values it writes, for the backward.
 template <int K, int NW, bool SAVE>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
                              const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ h0,
-                             uint16_t* __restrict__ o, float* __restrict__ hT, float* __restrict__ S_save,
-                             float* __restrict__ n_save, GdShape n, float scale) {
+                             float* __restrict__ E_in, uint16_t* __restrict__ o, float* __restrict__ hT,
+                             float* __restrict__ S_save, float* __restrict__ n_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
     using M = WalkLds<K, NW, 2>;
     uint16_t* const P = gd_lds + 2 * M::buf;
     constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS, VS = 16 * NW + GD_PAD;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+    const int wave = threadIdx.x >> 6;
+    int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
     const WalkAt w = walk_at<NW>(n);
     const int role = walk_role<NW>(__builtin_amdgcn_readfirstlane(wave));
     if (role == -2) return;
+    const int c0 = w.seg * n.per, c1 = min(n.NC, c0 + n.per);
     if (role >= 0) {
-        const int64_t first = w.bh * n.NC;
-        const WalkIn in = {q.p + w.b * q.sb + w.hk * q.sh, k.p + w.b * k.sb + w.hk * k.sh, v.p + w.b * v.sb + w.hv * v.sh + w.v0,
-                           q.st, k.st, v.st, T + first * GD_TB, beta + first * GD_C, G + first * GD_C, n.T};
-        walk_help<K, NW, 2, false>(in, n.NC, scale, gd_lds, 64 * role + lane);
+        walk_help<K, NW, 2, false>(walk_in(w, n, c0, q, k, v, T, beta, G), c1 - c0, scale, gd_lds, 64 * role + lane);
         return;
     }
     const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
     f32x4 S[ND];
+    if (w.seg == 0)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[d][r] = h0 ? h0[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
+            for (int r = 0; r < 4; ++r) S[d][r] = h0 ? h0[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
+    else
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = at4(seg_state<K>(E_in, n, w.bh, w.seg - 1, ct), 256 * d + 4 * lane);
     Three Sp[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) Sp[s] = three(S[2 * s], S[2 * s + 1]);
-    uint16_t* po = o + (w.bh * n.T + lr) * n.V + w.v0 + 16 * wave + 4 * lq;
+    uint16_t* po = o + (w.bh * n.T + c0 * GD_C + lr) * n.V + w.v0 + 16 * wave + 4 * lq;
     const f32x4 zero = {0, 0, 0, 0};
-    for (int c = 0; c < n.NC; ++c, po += (int64_t)GD_C * n.V) {
-        const WalkBuf L = walk_buf<K, NW>(gd_lds + (c & 1) * M::buf);
+    for (int c = c0; c < c1; ++c, po += (int64_t)GD_C * n.V) {
+        const WalkBuf L = walk_buf<K, NW>(gd_lds + ((c - c0) & 1) * M::buf);
         const int64_t at = (w.bh * n.NC + c) * (n.V / 16) + ct;
+        if constexpr (K == 128) {                          // taken anew: no registers for a lane's addresses over the loop
+            asm volatile("" : "+v"(lane));
+            lr = lane & 15;
+            lq = lane >> 4;
+        }
         if constexpr (SAVE)
 #pragma unroll
             for (int d = 0; d < ND; ++d) put_tiles(S_save + (at * ND + d) * 256, S[d], lane);
@@ -710,11 +740,223 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
                 if (c * GD_C + 16 * I + lr < n.T) *reinterpret_cast<uint2*>(po + (int64_t)16 * I * n.V) = ob[I];
         }
     }
-    if (hT)
+    if (hT && c1 == n.NC)
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int r = 0; r < 4; ++r) hT[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] = S[d][r];
+}
+
+// What a segment does to a state, before the segments' walks: S alone is carried through, without q and o.  The map of
+// the state that enters it is one more walk, of K columns that begin as the identity and to which nothing is written.
+// Blocks: the V columns of segment 0 (from h0), then the V + K of each other one but the last.
+template <int K, int NW>
+__global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
+rwkv6_gated_delta_segment_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
+                                 const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ h0,
+                                 float* __restrict__ E_out, GdShape n) {
+    extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
+    using M = WalkLds<K, NW, 0>;
+    constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, VS = 16 * NW + GD_PAD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+    WalkAt w = walk_at<NW>(n);
+    const int vcols = n.V / (16 * NW), cols = vcols + K / (16 * NW);
+    int x0 = (int)(blockIdx.x / (unsigned)n.BH), i0 = -1;                 // i0: the first column of the map
+    w.seg = 0;
+    if (x0 >= vcols) {
+        x0 -= vcols;
+        w.seg = 1 + x0 / cols;
+        x0 %= cols;
+        if (x0 >= vcols) {
+            i0 = 16 * NW * (x0 - vcols);
+            x0 = 0;
+        }
+    }
+    w.v0 = 16 * NW * x0;
+    const int role = walk_role<NW>(__builtin_amdgcn_readfirstlane(wave));
+    if (role == -2) return;
+    const int c0 = w.seg * n.per;
+    if (role >= 0) {
+        walk_help<K, NW, 0, false>(walk_in(w, n, c0, q, k, v, T, beta, G), n.per, 0.f, gd_lds, 64 * role + lane);
+        return;
+    }
+    const int col = (i0 < 0 ? w.v0 : i0) + 16 * wave + lr;
+    f32x4 S[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * d + 4 * lq + r;
+            if (i0 >= 0) S[d][r] = row == col ? 1.f : 0.f;
+            else S[d][r] = w.seg == 0 && h0 ? h0[(w.bh * K + row) * n.V + col] : 0.f;
+        }
+    Three Sp[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) Sp[s] = three(S[2 * s], S[2 * s + 1]);
+    const f32x4 zero = {0, 0, 0, 0};
+    for (int c = 0; c < n.per; ++c) {
+        const WalkBuf L = walk_buf<K, NW>(gd_lds + (c & 1) * M::buf);
+        __syncthreads();
+        bf16x8 f[NS][4], k0[ND], k1[ND];
+        f32x4 E[4], N[4], x[4], be[4], eg[4], el[4];
+        Three t0[4], t1[4];
+        const auto read_t0 = [&] {
+#pragma unroll
+            for (int I = 0; I < 4; ++I) t0[I] = t_rows(L.T, I, 0, lane);
+        };
+        const auto read_k1 = [&] {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) k1[d] = pcols(L.K, KS, 32, 16 * d, lane);
+        };
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int I = 0; I < 4; ++I) f[s][I] = prows(L.K, KS, 16 * I, 32 * s, lane);
+        gd_issued();
+        // half the chunk at a time: e0 beside the other half's products
+#pragma unroll
+        for (int I = 0; I < 4; ++I) E[I] = N[I] = zero;
+        const auto read_s = [&](int I0) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+#pragma unroll
+                for (int I = I0; I < I0 + 2; ++I) E[I] = mfma32(f[s][I], Sp[s].l, E[I]);
+#pragma unroll
+                for (int I = I0; I < I0 + 2; ++I) E[I] = mfma32(f[s][I], Sp[s].m, E[I]);
+#pragma unroll
+                for (int I = I0; I < I0 + 2; ++I) E[I] = mfma32(f[s][I], Sp[s].h, E[I]);
+            }
+        };
+        const auto written = [&](int I0) {
+#pragma unroll
+            for (int I = I0; I < I0 + 2; ++I) E[I] = be[I] * (x[I] - eg[I] * E[I]);
+            return three(E[I0], E[I0 + 1]);
+        };
+        read_s(0);
+        gd_issued();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) {
+            be[I] = at4(L.be, 16 * I + 4 * lq);
+            eg[I] = at4(L.eG, 16 * I + 4 * lq);
+            x[I] = as_acc(L.V, VS, 16 * I, 16 * wave, lane);
+            if (i0 >= 0) x[I] = zero;
+        }
+        if constexpr (K == 64) read_t0();
+        gd_issued();
+        read_s(2);
+        const Three e0 = written(0);
+        gd_weave<6 * NS, 4>();
+        gd_issued();
+        if constexpr (K == 128) read_t0();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) el[I] = at4(L.eL, 16 * I + 4 * lq);
+        const float eC = L.eG[GD_C - 1];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) k0[d] = pcols(L.K, KS, 0, 16 * d, lane);
+        gd_issued();
+        mm_tiles<0, 2>(t0, e0, N);
+        const Three e1 = written(2);
+        gd_weave<12, 4>();
+        gd_issued();
+#pragma unroll
+        for (int I = 2; I < 4; ++I) t1[I] = t_rows(L.T, I, 1, lane);
+        gd_issued();
+        mm_tiles<2, 4>(t0, e0, N);
+        const Three w0 = three(N[0] * el[0], N[1] * el[1]);
+        gd_weave<12, 4>();
+        gd_issued();
+        if constexpr (K == 64) read_k1();
+        gd_issued();
+        mm_tiles<2, 4>(t1, e1, N);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] *= eC;
+        gd_weave<12, K / 32>();
+        gd_issued();
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k0[d], w0.l, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k0[d], w0.m, S[d]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) S[d] = mfma32(k0[d], w0.h, S[d]);
+        const Three w1 = three(N[2] * el[2], N[3] * el[3]);
+        gd_weave<3 * ND, K == 64 ? 4 : 2>();
+        gd_issued();
+        if constexpr (K == 128) read_k1();
+        gd_issued();
+        // two tiles at a time, taken apart for the next chunk beside the next two
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+            for (int d = 2 * s; d < 2 * s + 2; ++d) S[d] = mfma32(k1[d], w1.l, S[d]);
+#pragma unroll
+            for (int d = 2 * s; d < 2 * s + 2; ++d) S[d] = mfma32(k1[d], w1.m, S[d]);
+#pragma unroll
+            for (int d = 2 * s; d < 2 * s + 2; ++d) S[d] = mfma32(k1[d], w1.h, S[d]);
+            Sp[s] = three(S[2 * s], S[2 * s + 1]);
+            gd_here(Sp[s]);
+        }
+        gd_weave<6, 1>();
+        gd_weave<6 * (NS - 1), 6>();
+        gd_issued();
+    }
+    if (i0 >= 0) {
+        float* p = seg_map<K>(E_out, n, w.bh, w.seg) + col;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[(16 * d + 4 * lq + r) * K] = S[d][r];
+    } else {
+        float* p = seg_state<K>(E_out, n, w.bh, w.seg, w.v0 / 16 + wave);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) put_tiles(p + 256 * d, S[d], lane);
+    }
+}
+
+// The states that the segments start from, one after the other: a block has 16 columns, a wave a quarter of the rows;
+// S_s+1 = M_s S_s + what segment s left for an empty state, in the 32-bit matrix instructions, the next map on its way
+// meanwhile.
+template <int K>
+__global__ void __launch_bounds__(256) rwkv6_gated_delta_join_kernel(float* __restrict__ E, GdShape n) {
+    constexpr int ND = K / 16, NR = ND / 4;
+    __shared__ f32x4 S[2][ND][64];
+    const int lane = threadIdx.x & 63, d0 = NR * (int)(threadIdx.x >> 6), ct = (int)(blockIdx.x / (unsigned)n.BH);
+    const int64_t bh = blockIdx.x % (unsigned)n.BH;
+    const auto own = [&](int s, int d) { return seg_state<K>(E, n, bh, s, ct) + 256 * (d0 + d) + 4 * lane; };
+    f32x4 m[NR][ND], x[NR];
+    const auto load = [&](int s) {
+        const float* p = seg_map<K>(E, n, bh, s) + (16 * d0 + (lane & 15)) * K + 4 * (lane >> 4);
+#pragma unroll
+        for (int d = 0; d < NR; ++d) {
+            x[d] = at4(own(s, d), 0);
+#pragma unroll
+            for (int j = 0; j < ND; ++j) m[d][j] = at4(p, 16 * d * K + 16 * j);
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < NR; ++d) S[0][d0 + d][lane] = at4(own(0, d), 0);
+    const int last = n.segs - 2;
+    load(1);
+    for (int s = 1; s <= last; ++s) {
+        __syncthreads();
+        f32x4 y[NR], a[NR][ND];
+#pragma unroll
+        for (int d = 0; d < NR; ++d) {
+            y[d] = x[d];
+#pragma unroll
+            for (int j = 0; j < ND; ++j) a[d][j] = m[d][j];
+        }
+        load(min(s + 1, last));
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+            const f32x4 t = S[(s - 1) & 1][j][lane];
+#pragma unroll
+            for (int d = 0; d < NR; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[d][j][r], t[r], y[d], 0, 0, 0);
+        }
+#pragma unroll
+        for (int d = 0; d < NR; ++d) *reinterpret_cast<f32x4*>(own(s, d)) = S[s & 1][d0 + d][lane] = y[d];
+    }
 }
 
 // The walk back: d_v, and for the other gradients r and the gradient D of the state that each chunk leaves.
@@ -733,10 +975,7 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
     const int role = walk_role<NW>(__builtin_amdgcn_readfirstlane(wave));
     if (role == -2) return;
     if (role >= 0) {
-        const int64_t first = w.bh * n.NC;
-        const WalkIn in = {q.p + w.b * q.sb + w.hk * q.sh, k.p + w.b * k.sb + w.hk * k.sh, d_o.p + w.b * d_o.sb + w.hv * d_o.sh + w.v0,
-                           q.st, k.st, d_o.st, T + first * GD_TB, beta + first * GD_C, G + first * GD_C, n.T};
-        walk_help<K, NW, 3, true>(in, n.NC, scale, gd_lds, 64 * role + lane);
+        walk_help<K, NW, 3, true>(walk_in(w, n, 0, q, k, d_o, T, beta, G), n.NC, scale, gd_lds, 64 * role + lane);
         return;
     }
     const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
@@ -1275,6 +1514,38 @@ rwkv6_gated_delta_step_kernel(GdTensor q, GdTensor k, GdTensor v, const float* _
 
 namespace {
 inline bool gd_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// How a head's columns are dealt to blocks: a block of 4 waves of 16 columns, or of fewer where all blocks still find a
+// CU of their own (256 and 512 tiles).  A wave then has its SIMD and the CU's LDS to itself: 0.99 ms against 1.47 with 4
+// for 32 heads of 512 chunks, 47 us against 61 for both walks of 16 heads of 8.
+inline int gd_waves(int64_t tiles) { return tiles <= 256 ? 1 : tiles <= 512 ? 2 : 4; }
+// Microseconds that `chunks` chunks of that many 16-column tiles take, before the segments' walks and in them: a block's
+// start, and a chunk as measured for each way to deal the tiles; 1024 have the chip at once.
+inline double gd_time(int64_t tiles, int64_t K, bool before, int chunks) {
+    const double pace[2][2][3] = {{{1.75, 2.0, 3.2}, {1.4, 1.55, 1.9}}, {{2.65, 2.9, 4.1}, {2.0, 2.2, 2.6}}};
+    const double* p = pace[K == 128][before];
+    return tiles <= 512 ? 4 + chunks * p[tiles > 256] : (double)((tiles + 1023) / 1024) * (4 + chunks * p[2]);
+}
+// Segments of the forward.  Few heads leave most of the chip idle and a walk as long as the sequence: p segments walk
+// side by side from states that a cheaper walk over all but the last has found (with the K columns of its map beside the
+// V of its state) and `join` has put together.  The number with the least time by the paces above is taken, 1 where none
+// beats it.  4, 8 and 32 heads of 64 x 64 of 65536, 32768 and 32768 tokens: 1760 to 256 us, 900 to 176, 980 to 567;
+// 256 heads of 4096 tokens fill the chip as they are.
+void gd_segments(GdShape* n, int64_t K) {
+    n->segs = 1;
+    n->per = n->NC;
+    const int64_t vt = n->BH * (n->V / 16), kt = n->BH * (K / 16);
+    double best = gd_time(vt, K, false, n->NC);
+    for (int p = 2; p <= 16; ++p) {
+        const int per = (n->NC + p - 1) / p, segs = per ? (n->NC + per - 1) / per : 0;
+        if (segs != p) continue;
+        const double t = 4 + 1.5 * (p - 2) + gd_time(vt + (p - 2) * (vt + kt), K, true, per) + gd_time(vt * p, K, false, per);
+        if (t < best) {
+            best = t;
+            n->segs = p;
+            n->per = per;
+        }
+    }
+}
 int gd_shape(int64_t B, int64_t H, int64_t HV, int64_t T, int64_t K, int64_t V, GdShape* n) {
     if (B < 0 || H < 1 || HV < 1 || T < 0 || K < 1 || V < 1 || HV % H) return RWKV6_ERR_INVALID_ARG;
     if ((K != 64 && K != 128) || V % 64 || V > 512) return RWKV6_ERR_UNSUPPORTED;
@@ -1283,7 +1554,8 @@ int gd_shape(int64_t B, int64_t H, int64_t HV, int64_t T, int64_t K, int64_t V, 
     if (HV > most || B > most / HV || T > ((int64_t)1 << 30)) return RWKV6_ERR_UNSUPPORTED;
     const int64_t NC = (T + GD_C - 1) / GD_C;
     if (B * HV * (NC > V / 64 ? NC : V / 64) > most) return RWKV6_ERR_UNSUPPORTED;
-    *n = {(int)H, (int)HV, (int)T, (int)NC, (int)V, B * HV};
+    *n = {(int)H, (int)HV, (int)T, (int)NC, (int)V, B * HV, 0, 0};
+    gd_segments(n, K);
     return RWKV6_OK;
 }
 // A strided [B, heads, T, C] tensor: its strides, and the bytes from its first to its last element.
@@ -1298,29 +1570,25 @@ int gd_tensor(const void* p, const int64_t* s, int64_t B, int64_t heads, int64_t
     span->n = (size_t)((B - 1) * s[0] + (heads - 1) * s[1] + (T - 1) * s[2] + C) * 2;
     return RWKV6_OK;
 }
-// What the forward leaves for the backward (or uses itself): T, G, beta, and the states and written values.
+// What the forward uses itself (T, G, beta, the segments' maps and states) and leaves for the backward (and the states and
+// written values).
 struct GdSaved {
-    size_t T, G, B, S, N, end;
+    size_t T, G, B, E, S, N, end;
     GdSaved(const GdShape& n, int64_t K) {
         const size_t chunks = (size_t)n.BH * n.NC;
         T = 0;
         G = T + chunks * 4 * GD_TB;
         B = G + chunks * 8 * GD_C;
-        S = B + chunks * 4 * GD_C;
+        E = B + chunks * 4 * GD_C;
+        S = E + (size_t)n.BH * (n.segs - 1) * 4 * K * (K + n.V);
         N = S + chunks * 4 * K * n.V;
         end = N + chunks * 4 * GD_C * n.V;
     }
 };
-// How a head's columns are dealt to blocks: a block of 4 waves of 16 columns, or of fewer where all blocks still find a
-// CU of their own.  A wave then has its SIMD and the CU's LDS to itself.
-inline int gd_waves(const GdShape& n) {
-    const int64_t tiles = n.BH * (n.V / 16);
-    return tiles <= 256 ? 1 : tiles <= 512 ? 2 : 4;
-}
 // f(integral constants of the key channels and of gd_waves)
-template <class F> void gd_walks(const GdShape& n, int64_t K, F&& f) {
+template <class F> void gd_walks(int64_t tiles, int64_t K, F&& f) {
     const auto by_waves = [&](auto k) {
-        switch (gd_waves(n)) {
+        switch (gd_waves(tiles)) {
         case 1: f(k, std::integral_constant<int, 1>()); break;
         case 2: f(k, std::integral_constant<int, 2>()); break;
         default: f(k, std::integral_constant<int, 4>());
@@ -1343,6 +1611,7 @@ int gd_limits(hipStream_t stream) {
 #define GD_RAISE(K, NW)                                                                                              \
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, false>), WalkLds<K, NW, 2>::bytes);       \
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, true>), WalkLds<K, NW, 2>::bytes);        \
+    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_segment_kernel<K, NW>), WalkLds<K, NW, 0>::bytes);          \
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<K, NW>), WalkLds<K, NW, 3>::bytes);
         GD_RAISE(64, 1) GD_RAISE(64, 2) GD_RAISE(64, 4) GD_RAISE(128, 1) GD_RAISE(128, 2) GD_RAISE(128, 4)
 #undef GD_RAISE
@@ -1398,18 +1667,32 @@ int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int
     float2* G = reinterpret_cast<float2*>(base + at.G);
     float* Tm = reinterpret_cast<float*>(base);
     float *be = reinterpret_cast<float*>(base + at.B), *S = saved ? reinterpret_cast<float*>(base + at.S) : nullptr,
-          *N = saved ? reinterpret_cast<float*>(base + at.N) : nullptr;
+          *N = saved ? reinterpret_cast<float*>(base + at.N) : nullptr, *E = reinterpret_cast<float*>(base + at.E);
     if (T > 0) {
         auto prep = K == 64 ? rwkv6_gated_delta_prep_kernel<64> : rwkv6_gated_delta_prep_kernel<128>;
         hipLaunchKernelGGL(prep, dim3((unsigned)(n.BH * n.NC)), dim3(256), 0, s, kt, g, beta, beta_dtype, G, be, Tm, n);
     }
+    if (n.segs > 1) {
+        const int64_t cols = V + (n.segs - 2) * (V + K);               // of the segments but the last
+        gd_walks(n.BH * (cols / 16), K, [&](auto k_, auto w_) {
+            constexpr int k = k_, w = w_;
+            auto segment = rwkv6_gated_delta_segment_kernel<k, w>;
+            const size_t lds = WalkLds<k, w, 0>::bytes;
+            hipLaunchKernelGGL(segment, dim3((unsigned)(n.BH * (cols / (16 * w)))), dim3(walk_threads<w>), lds, s, qt, kt, vt, be, G,
+                               Tm, h0, E, n);
+        });
+    }
+    if (n.segs > 2) {
+        auto join = K == 64 ? rwkv6_gated_delta_join_kernel<64> : rwkv6_gated_delta_join_kernel<128>;
+        hipLaunchKernelGGL(join, dim3((unsigned)(n.BH * (V / 16))), dim3(256), 0, s, E, n);
+    }
     if (T > 0 || hT)
-        gd_walks(n, K, [&](auto k_, auto w_) {
+        gd_walks(n.BH * (V / 16) * n.segs, K, [&](auto k_, auto w_) {
             constexpr int k = k_, w = w_;
             auto walk = saved ? rwkv6_gated_delta_fwd_kernel<k, w, true> : rwkv6_gated_delta_fwd_kernel<k, w, false>;
             const size_t lds = WalkLds<k, w, 2>::bytes;
-            hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / (16 * w)))), dim3(walk_threads<w>), lds, s, qt, kt, vt, be, G, Tm, h0,
-                               (uint16_t*)o, hT, S, N, n, scale);
+            hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / (16 * w)) * n.segs)), dim3(walk_threads<w>), lds, s, qt, kt, vt, be, G,
+                               Tm, h0, E, (uint16_t*)o, hT, S, N, n, scale);
         });
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
@@ -1447,7 +1730,7 @@ int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const voi
                 *N = reinterpret_cast<const float*>(base + at.N);
     float *D = static_cast<float*>(workspace), *R = D + (at.N - at.S) / 4;
     if (T > 0 || dh0)
-        gd_walks(n, K, [&](auto k_, auto w_) {
+        gd_walks(n.BH * (V / 16), K, [&](auto k_, auto w_) {
             constexpr int k = k_, w = w_;
             auto walk = rwkv6_gated_delta_bwd_kernel<k, w>;
             const size_t lds = WalkLds<k, w, 3>::bytes;

@@ -164,6 +164,62 @@ def test_a_long_sequence(pkg, T):
     run_train(pkg, d, final=True, wo=torch.randn(1, 2, T, 64).to(BF), wh=torch.randn(1, 2, 64, 64))
 
 
+# few heads: the chunks are walked in segments side by side (7 to 13 of them here), the last of them shorter
+SEGMENTED = [(1, 1, 1, 1500, 64, 64), (1, 1, 2, 2049, 64, 128), (2, 1, 1, 1300, 128, 64), (1, 2, 2, 1999, 128, 128), (1, 1, 3, 1500, 128, 192)]
+
+
+@pytest.mark.parametrize("shape", SEGMENTED, ids=str)
+@pytest.mark.parametrize("states", [False, True])
+def test_segments(pkg, shape, states):
+    """A decay that leaves half of a state after 300 tokens: what a segment gets from the one before it counts."""
+    B, H, HV, T, K, V = shape
+    L = pkg._lib.load()
+    chunks = B * HV * ((T + 63) // 64)                    # T of 10 KB, G and beta, then a map and a state a segment but the last
+    n = L.rwkv6_gated_delta_workspace_bytes(B, HV, T, K, V, 0) - chunks * (10240 + 512 + 256)
+    assert n % (B * HV * K * (K + V) * 4) == 0 and n >= 2 * B * HV * K * (K + V) * 4
+    d = inputs(*shape, seed=sum(shape), h0=states)
+    d["g"] = d["g"].clamp(min=-0.0023)
+    d["g"][:, :, 700] = -float("inf") if not states else -0.1
+    with torch.no_grad():                                 # without what a backward needs
+        o, S = pkg.gated_delta.gated_delta_rule(*[d[n].cuda() for n in NAMES], initial_state=d["h0"].cuda() if states else None,
+                                                output_final_state=True)
+    ro, rS = recurrence(*[d[n].double() for n in NAMES], K ** -0.5, d["h0"].double() if states else None)
+    check("o", o, ro)
+    check("state", S, rS)
+    if states:
+        run_train(pkg, d, final=True, wo=torch.randn(B, HV, T, V).to(BF), wh=torch.randn(B, HV, K, V))
+
+
+def test_segments_captured_and_on_other_streams(pkg):
+    d = on_gpu(inputs(2, 2, 2, 2000, 64, 64, seed=15, h0=True))
+
+    def prompt():
+        with torch.no_grad():
+            return pkg.gated_delta.gated_delta_rule(*[d[n] for n in NAMES], initial_state=d["h0"], output_final_state=True)
+
+    want = prompt()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for s in streams * 2:
+        with torch.cuda.stream(s):
+            got.append(prompt())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(prompt())
+    for rep in range(3):
+        d["h0"].mul_(2)
+        for g in graphs:
+            g.replay()
+        want = prompt()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want)), rep
+
+
 def test_slow_decay_keeps_an_old_state(pkg):
     d = inputs(1, 1, 1, 2000, 64, 64, seed=4, h0=True)
     d["g"].fill_(-1e-6)
