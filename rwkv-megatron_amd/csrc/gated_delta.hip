@@ -440,7 +440,7 @@ __device__ __forceinline__ void walk_store(const WalkRegs<K, NW>& r, const WalkI
 // heads are one, on the same XCD, and find its q, k and T in that L2.
 struct WalkAt {
     int64_t bh, b;
-    int hv, hk, v0, seg;
+    int hv, hk, v0, seg, i0;    // i0: the map's first column, or -1
 };
 template <int NW> __device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
     WalkAt w;
@@ -452,6 +452,25 @@ template <int NW> __device__ __forceinline__ WalkAt walk_at(const GdShape& n) {
     const int col = (int)(blockIdx.x / heads), cols = n.V / (16 * NW);
     w.v0 = 16 * NW * (col % cols);
     w.seg = col / cols;
+    w.i0 = -1;
+    return w;
+}
+// The same of the blocks that go before: the V columns of the first segment, then the V + K of each other one but the last.
+template <int K, int NW> __device__ __forceinline__ WalkAt segment_at(const GdShape& n) {
+    WalkAt w = walk_at<NW>(n);
+    const int vcols = n.V / (16 * NW), cols = vcols + K / (16 * NW);
+    int x = (int)(blockIdx.x / (unsigned)n.BH);
+    w.seg = 0;
+    if (x >= vcols) {
+        x -= vcols;
+        w.seg = 1 + x / cols;
+        x %= cols;
+        if (x >= vcols) {
+            w.i0 = 16 * NW * (x - vcols);
+            x = 0;
+        }
+    }
+    w.v0 = 16 * NW * x;
     return w;
 }
 // The inputs of a head from chunk c0 on.
@@ -469,6 +488,19 @@ template <int K> __device__ __forceinline__ float* seg_map(float* E, const GdSha
 }
 template <int K> __device__ __forceinline__ float* seg_state(float* E, const GdShape& n, int64_t bh, int seg, int ct) {
     return seg_map<K>(E, n, bh, seg) + K * K + ct * (K * 16);
+}
+template <int K> __device__ __forceinline__ void put_segment(float* E, const GdShape& n, const WalkAt& w, const f32x4* S, int wave, int lane) {
+    if (w.i0 >= 0) {
+        float* p = seg_map<K>(E, n, w.bh, w.seg) + w.i0 + 16 * wave + (lane & 15);
+#pragma unroll
+        for (int d = 0; d < K / 16; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[(16 * d + 4 * (lane >> 4) + r) * K] = S[d][r];
+    } else {
+        float* p = seg_state<K>(E, n, w.bh, w.seg, w.v0 / 16 + wave);
+#pragma unroll
+        for (int d = 0; d < K / 16; ++d) put_tiles(p + 256 * d, S[d], lane);
+    }
 }
 // A block's waves: NW walk (the first), four help.  Wave w runs on SIMD w % 4, so with fewer walking the helpers are
 // placed on the other SIMDs and the waves between, which have nothing to do, end at once.
@@ -749,7 +781,6 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
 
 // What a segment does to a state, before the segments' walks: S alone is carried through, without q and o.  The map of
 // the state that enters it is one more walk, of K columns that begin as the identity and to which nothing is written.
-// Blocks: the V columns of segment 0 (from h0), then the V + K of each other one but the last.
 template <int K, int NW>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_segment_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
@@ -759,20 +790,7 @@ rwkv6_gated_delta_segment_kernel(GdTensor q, GdTensor k, GdTensor v, const float
     using M = WalkLds<K, NW, 0>;
     constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, VS = 16 * NW + GD_PAD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
-    WalkAt w = walk_at<NW>(n);
-    const int vcols = n.V / (16 * NW), cols = vcols + K / (16 * NW);
-    int x0 = (int)(blockIdx.x / (unsigned)n.BH), i0 = -1;                 // i0: the first column of the map
-    w.seg = 0;
-    if (x0 >= vcols) {
-        x0 -= vcols;
-        w.seg = 1 + x0 / cols;
-        x0 %= cols;
-        if (x0 >= vcols) {
-            i0 = 16 * NW * (x0 - vcols);
-            x0 = 0;
-        }
-    }
-    w.v0 = 16 * NW * x0;
+    const WalkAt w = segment_at<K, NW>(n);
     const int role = walk_role<NW>(__builtin_amdgcn_readfirstlane(wave));
     if (role == -2) return;
     const int c0 = w.seg * n.per;
@@ -780,14 +798,14 @@ rwkv6_gated_delta_segment_kernel(GdTensor q, GdTensor k, GdTensor v, const float
         walk_help<K, NW, 0, false>(walk_in(w, n, c0, q, k, v, T, beta, G), n.per, 0.f, gd_lds, 64 * role + lane);
         return;
     }
-    const int col = (i0 < 0 ? w.v0 : i0) + 16 * wave + lr;
+    const int col = (w.i0 < 0 ? w.v0 : w.i0) + 16 * wave + lr;
     f32x4 S[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 16 * d + 4 * lq + r;
-            if (i0 >= 0) S[d][r] = row == col ? 1.f : 0.f;
+            if (w.i0 >= 0) S[d][r] = row == col ? 1.f : 0.f;
             else S[d][r] = w.seg == 0 && h0 ? h0[(w.bh * K + row) * n.V + col] : 0.f;
         }
     Three Sp[NS];
@@ -839,7 +857,7 @@ rwkv6_gated_delta_segment_kernel(GdTensor q, GdTensor k, GdTensor v, const float
             be[I] = at4(L.be, 16 * I + 4 * lq);
             eg[I] = at4(L.eG, 16 * I + 4 * lq);
             x[I] = as_acc(L.V, VS, 16 * I, 16 * wave, lane);
-            if (i0 >= 0) x[I] = zero;
+            if (w.i0 >= 0) x[I] = zero;
         }
         if constexpr (K == 64) read_t0();
         gd_issued();
@@ -899,17 +917,7 @@ rwkv6_gated_delta_segment_kernel(GdTensor q, GdTensor k, GdTensor v, const float
         gd_weave<6 * (NS - 1), 6>();
         gd_issued();
     }
-    if (i0 >= 0) {
-        float* p = seg_map<K>(E_out, n, w.bh, w.seg) + col;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) p[(16 * d + 4 * lq + r) * K] = S[d][r];
-    } else {
-        float* p = seg_state<K>(E_out, n, w.bh, w.seg, w.v0 / 16 + wave);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) put_tiles(p + 256 * d, S[d], lane);
-    }
+    put_segment<K>(E_out, n, w, S, wave, lane);
 }
 
 // The states that the segments start from, one after the other: a block has 16 columns, a wave a quarter of the rows;
@@ -960,39 +968,51 @@ __global__ void __launch_bounds__(256) rwkv6_gated_delta_join_kernel(float* __re
 }
 
 // The walk back: d_v, and for the other gradients r and the gradient D of the state that each chunk leaves.
-template <int K, int NW>
+// BEFORE: what the segments but the first do to D, as in `segment`, the last segment being the first to be walked.
+template <int K, int NW, bool BEFORE>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* __restrict__ beta,
                              const float2* __restrict__ G, const float* __restrict__ T, const float* __restrict__ dhT,
-                             uint16_t* __restrict__ dv, float* __restrict__ dh0, float* __restrict__ D_save,
+                             float* __restrict__ E, uint16_t* __restrict__ dv, float* __restrict__ dh0, float* __restrict__ D_save,
                              float* __restrict__ r_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
     using M = WalkLds<K, NW, 3>;
     uint16_t* const P = gd_lds + 2 * M::buf;
     constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS, VS = 16 * NW + GD_PAD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
-    const WalkAt w = walk_at<NW>(n);
+    const WalkAt w = BEFORE ? segment_at<K, NW>(n) : walk_at<NW>(n);       // w.seg: from the back
+    const int c0 = (n.segs - 1 - w.seg) * n.per, c1 = min(n.NC, c0 + n.per);
     const int role = walk_role<NW>(__builtin_amdgcn_readfirstlane(wave));
     if (role == -2) return;
     if (role >= 0) {
-        walk_help<K, NW, 3, true>(walk_in(w, n, 0, q, k, d_o, T, beta, G), n.NC, scale, gd_lds, 64 * role + lane);
+        walk_help<K, NW, 3, true>(walk_in(w, n, c0, q, k, d_o, T, beta, G), c1 - c0, scale, gd_lds, 64 * role + lane);
         return;
     }
     const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
     f32x4 D[ND];
+    if (!BEFORE && w.seg)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d) D[d] = at4(seg_state<K>(E, n, w.bh, w.seg - 1, ct), 256 * d + 4 * lane);
+    else if (BEFORE && w.i0 >= 0)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) D[d][r] = dhT ? dhT[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) D[d][r] = 16 * d + 4 * lq + r == w.i0 + 16 * wave + lr ? 1.f : 0.f;
+    else
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) D[d][r] = w.seg == 0 && dhT ? dhT[(w.bh * K + 16 * d + 4 * lq + r) * n.V + col] : 0.f;
     Three Dp[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) Dp[s] = three(D[2 * s], D[2 * s + 1]);
     const f32x4 zero = {0, 0, 0, 0};
-    for (int c = n.NC - 1, u = 0; c >= 0; --c, u ^= 1) {
+    for (int c = c1 - 1, u = 0; c >= c0; --c, u ^= 1) {
         const WalkBuf L = walk_buf<K, NW>(gd_lds + u * M::buf);
         const int64_t at = (w.bh * n.NC + c) * (n.V / 16) + ct;
+        if constexpr (!BEFORE)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) put_tiles(D_save + (at * ND + d) * 256, D[d], lane);
+            for (int d = 0; d < ND; ++d) put_tiles(D_save + (at * ND + d) * 256, D[d], lane);
         __syncthreads();
         bf16x8 f[NS][4], fc[2][ND], dof[2];
         f32x4 X[4], Y[4], R[4], V[4], el[4], eg[4], be[4]; // X: d_n; Y: scale e^G d_o; V: d_v
@@ -1000,6 +1020,7 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
 #pragma unroll
         for (int I = 0; I < 4; ++I) {
             Y[I] = as_acc(L.V, VS, 16 * I, 16 * wave, lane);
+            if (BEFORE && w.i0 >= 0) Y[I] = zero;
             eg[I] = at4(L.eG, 16 * I + 4 * lq);
         }
 #pragma unroll
@@ -1030,7 +1051,10 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
         gd_weave<12 * NS, K == 64 ? 6 : 3>();
         gd_issued();
 #pragma unroll
-        for (int s = 0; s < 2; ++s) dof[s] = cols(L.V, VS, 32 * s, 16 * wave, lane);
+        for (int s = 0; s < 2; ++s) {
+            dof[s] = cols(L.V, VS, 32 * s, 16 * wave, lane);
+            if (BEFORE && w.i0 >= 0) dof[s] = bf16x8{};
+        }
         __syncthreads();                                   // P
 #pragma unroll
         for (int s = 1; s >= 0; --s)
@@ -1133,6 +1157,7 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
         gd_weave<6, 1>();
         gd_weave<6 * (NS - 1), 6>();
         gd_issued();
+        if constexpr (BEFORE) continue;
 #pragma unroll
         for (int I = 0; I < 4; ++I) put_tiles(r_save + (at * 4 + I) * 256, R[I], lane);
         uint16_t* pv = dv + (w.bh * n.T + c * GD_C + 4 * lq) * n.V + col;
@@ -1149,7 +1174,8 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
                     if (c * GD_C + 16 * I + 4 * lq + r < n.T) pv[(16 * I + r) * n.V] = f2bf(V[I][r]);
         }
     }
-    if (dh0)
+    if constexpr (BEFORE) put_segment<K>(E, n, w, D, wave, lane);
+    else if (dh0 && c0 == 0)
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -1520,25 +1546,27 @@ inline bool gd_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15
 inline int gd_waves(int64_t tiles) { return tiles <= 256 ? 1 : tiles <= 512 ? 2 : 4; }
 // Microseconds that `chunks` chunks of that many 16-column tiles take, before the segments' walks and in them: a block's
 // start, and a chunk as measured for each way to deal the tiles; 1024 have the chip at once.
-inline double gd_time(int64_t tiles, int64_t K, bool before, int chunks) {
-    const double pace[2][2][3] = {{{1.75, 2.0, 3.2}, {1.4, 1.55, 1.9}}, {{2.65, 2.9, 4.1}, {2.0, 2.2, 2.6}}};
-    const double* p = pace[K == 128][before];
-    return tiles <= 512 ? 4 + chunks * p[tiles > 256] : (double)((tiles + 1023) / 1024) * (4 + chunks * p[2]);
+inline double gd_time(int tiles, int64_t K, bool back, bool before, int chunks) {
+    const double pace[2][2][2][3] = {{{{1.75, 2.0, 3.2}, {1.4, 1.55, 1.9}}, {{2.65, 2.9, 4.1}, {2.0, 2.2, 2.6}}},
+                                     {{{2.8, 3.1, 4.4}, {2.45, 2.85, 3.8}}, {{3.8, 4.3, 6.2}, {3.4, 3.8, 5.1}}}};
+    const double* p = pace[back][K == 128][before];
+    return tiles <= 512 ? 4 + chunks * p[tiles > 256] : ((tiles + 1023) >> 10) * (4 + chunks * p[2]);
 }
-// Segments of the forward.  Few heads leave most of the chip idle and a walk as long as the sequence: p segments walk
-// side by side from states that a cheaper walk over all but the last has found (with the K columns of its map beside the
-// V of its state) and `join` has put together.  The number with the least time by the paces above is taken, 1 where none
-// beats it.  4, 8 and 32 heads of 64 x 64 of 65536, 32768 and 32768 tokens: 1760 to 256 us, 900 to 176, 980 to 567;
-// 256 heads of 4096 tokens fill the chip as they are.
-void gd_segments(GdShape* n, int64_t K) {
+// Segments of a walk.  Few heads leave most of the chip idle and a walk as long as the sequence: p segments walk
+// side by side from states that a walk over all but the last has found (with the K columns of its map beside the
+// V of its state) and `join` has put together.  The number with the least time by the paces above and what
+// two more launches cost is taken, 1 where none beats it.  Forward of 4, 8 and 32 heads of 64 x 64 of 65536, 32768 and 32768 tokens: 1760 to 256 us, 900 to 176, 980 to
+// 567; backward of 8 and 32 of 16384 tokens: 722 to 189, 952 to 600; 256 heads of 4096 tokens fill the chip as they are.
+void gd_segments(GdShape* n, int64_t K, bool back) {
     n->segs = 1;
     n->per = n->NC;
-    const int64_t vt = n->BH * (n->V / 16), kt = n->BH * (K / 16);
-    double best = gd_time(vt, K, false, n->NC);
+    if (n->NC < 8 || n->BH * (n->V / 16) > 512) return;   // nothing to win with fewer chunks, a seventh at most with more tiles
+    const int vt = (int)n->BH * (n->V / 16), kt = (int)n->BH * ((int)K / 16);
+    double best = gd_time(vt, K, back, false, n->NC);
     for (int p = 2; p <= 16; ++p) {
-        const int per = (n->NC + p - 1) / p, segs = per ? (n->NC + per - 1) / per : 0;
-        if (segs != p) continue;
-        const double t = 4 + 1.5 * (p - 2) + gd_time(vt + (p - 2) * (vt + kt), K, true, per) + gd_time(vt * p, K, false, per);
+        const int per = (n->NC + p - 1) / p;
+        if ((n->NC + per - 1) / per != p) continue;
+        const double t = 12 + (p - 2) + gd_time(vt + (p - 2) * (vt + kt), K, back, true, per) + gd_time(vt * p, K, back, false, per);
         if (t < best) {
             best = t;
             n->segs = p;
@@ -1555,7 +1583,7 @@ int gd_shape(int64_t B, int64_t H, int64_t HV, int64_t T, int64_t K, int64_t V, 
     const int64_t NC = (T + GD_C - 1) / GD_C;
     if (B * HV * (NC > V / 64 ? NC : V / 64) > most) return RWKV6_ERR_UNSUPPORTED;
     *n = {(int)H, (int)HV, (int)T, (int)NC, (int)V, B * HV, 0, 0};
-    gd_segments(n, K);
+    gd_segments(n, K, false);
     return RWKV6_OK;
 }
 // A strided [B, heads, T, C] tensor: its strides, and the bytes from its first to its last element.
@@ -1585,6 +1613,11 @@ struct GdSaved {
         end = N + chunks * 4 * GD_C * n.V;
     }
 };
+// The backward's workspace: gradients like the states and values, and its own segments' maps and states.
+size_t gd_work(const GdSaved& s, GdShape n, int64_t K) {
+    gd_segments(&n, K, true);
+    return s.end - s.S + (size_t)n.BH * (n.segs - 1) * 4 * K * (K + n.V);
+}
 // f(integral constants of the key channels and of gd_waves)
 template <class F> void gd_walks(int64_t tiles, int64_t K, F&& f) {
     const auto by_waves = [&](auto k) {
@@ -1596,6 +1629,13 @@ template <class F> void gd_walks(int64_t tiles, int64_t K, F&& f) {
     };
     if (K == 64) by_waves(std::integral_constant<int, 64>());
     else by_waves(std::integral_constant<int, 128>());
+}
+// Columns that are walked before the segments.
+inline int64_t gd_before(const GdShape& n, int64_t K) { return n.V + (n.segs - 2) * (n.V + K); }
+void gd_join(const GdShape& n, int64_t K, float* E, hipStream_t s) {
+    if (n.segs == 2) return;
+    auto join = K == 64 ? rwkv6_gated_delta_join_kernel<64> : rwkv6_gated_delta_join_kernel<128>;
+    hipLaunchKernelGGL(join, dim3((unsigned)(n.BH * (n.V / 16))), dim3(256), 0, s, E, n);
 }
 // The walks' and gradients' LDS is past what a launch gets by itself: raised once on each device.
 int gd_limits(hipStream_t stream) {
@@ -1612,7 +1652,8 @@ int gd_limits(hipStream_t stream) {
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, false>), WalkLds<K, NW, 2>::bytes);       \
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, true>), WalkLds<K, NW, 2>::bytes);        \
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_segment_kernel<K, NW>), WalkLds<K, NW, 0>::bytes);          \
-    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<K, NW>), WalkLds<K, NW, 3>::bytes);
+    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<K, NW, false>), WalkLds<K, NW, 3>::bytes);       \
+    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<K, NW, true>), WalkLds<K, NW, 3>::bytes);
         GD_RAISE(64, 1) GD_RAISE(64, 2) GD_RAISE(64, 4) GD_RAISE(128, 1) GD_RAISE(128, 2) GD_RAISE(128, 4)
 #undef GD_RAISE
         raise(reinterpret_cast<const void*>(rwkv6_gated_delta_grads_kernel<64, false>), GradLds<64>::bytes);
@@ -1636,7 +1677,7 @@ size_t rwkv6_gated_delta_workspace_bytes(int64_t B, int64_t HV, int64_t T, int64
     GdShape n;
     if (gd_shape(B, 1, HV, T, K, V, &n)) return 0;
     const GdSaved s(n, K);
-    return for_bwd ? s.end - s.S : s.S;                   // D and r have the sizes of S and N; T, G, beta
+    return for_bwd ? gd_work(s, n, K) : s.S;
 }
 
 int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const float* g,
@@ -1673,7 +1714,7 @@ int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int
         hipLaunchKernelGGL(prep, dim3((unsigned)(n.BH * n.NC)), dim3(256), 0, s, kt, g, beta, beta_dtype, G, be, Tm, n);
     }
     if (n.segs > 1) {
-        const int64_t cols = V + (n.segs - 2) * (V + K);               // of the segments but the last
+        const int64_t cols = gd_before(n, K);
         gd_walks(n.BH * (cols / 16), K, [&](auto k_, auto w_) {
             constexpr int k = k_, w = w_;
             auto segment = rwkv6_gated_delta_segment_kernel<k, w>;
@@ -1681,10 +1722,7 @@ int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int
             hipLaunchKernelGGL(segment, dim3((unsigned)(n.BH * (cols / (16 * w)))), dim3(walk_threads<w>), lds, s, qt, kt, vt, be, G,
                                Tm, h0, E, n);
         });
-    }
-    if (n.segs > 2) {
-        auto join = K == 64 ? rwkv6_gated_delta_join_kernel<64> : rwkv6_gated_delta_join_kernel<128>;
-        hipLaunchKernelGGL(join, dim3((unsigned)(n.BH * (V / 16))), dim3(256), 0, s, E, n);
+        gd_join(n, K, E, s);
     }
     if (T > 0 || hT)
         gd_walks(n.BH * (V / 16) * n.segs, K, [&](auto k_, auto w_) {
@@ -1718,7 +1756,7 @@ int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const voi
     const GdSaved at(n, K);
     const size_t tok = (size_t)n.BH * T, states = (size_t)n.BH * K * V * 4, qk = (size_t)(B * H) * T * K * 2;
     if (any_alias({{dq, qk}, {dk, qk}, {dv, tok * V * 2}, {dg, tok * 4}, {dbeta, tok * param_bytes(beta_dtype)}, {dh0, states},
-                   {workspace, at.end - at.S}},
+                   {workspace, gd_work(at, n, K)}},
                   {qs, ks, vs, os, {beta, tok * param_bytes(beta_dtype)}, {dhT, states}, {saved, at.end}}))
         return RWKV6_ERR_INVALID_ARG;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -1728,15 +1766,22 @@ int rwkv6_gated_delta_bwd(const void* q, const void* k, const void* v, const voi
     const float* Tm = reinterpret_cast<const float*>(base);
     const float *be = reinterpret_cast<const float*>(base + at.B), *S = reinterpret_cast<const float*>(base + at.S),
                 *N = reinterpret_cast<const float*>(base + at.N);
-    float *D = static_cast<float*>(workspace), *R = D + (at.N - at.S) / 4;
-    if (T > 0 || dh0)
-        gd_walks(n.BH * (V / 16), K, [&](auto k_, auto w_) {
+    float *D = static_cast<float*>(workspace), *R = D + (at.N - at.S) / 4, *E = D + (at.end - at.S) / 4;
+    gd_segments(&n, K, true);
+    const auto walks = [&](int64_t cols, auto before) {
+        gd_walks(n.BH * (cols / 16), K, [&](auto k_, auto w_) {
             constexpr int k = k_, w = w_;
-            auto walk = rwkv6_gated_delta_bwd_kernel<k, w>;
+            auto walk = rwkv6_gated_delta_bwd_kernel<k, w, decltype(before)::value>;
             const size_t lds = WalkLds<k, w, 3>::bytes;
-            hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / (16 * w)))), dim3(walk_threads<w>), lds, s, qt, kt, ot, be, G, Tm, dhT,
-                               (uint16_t*)dv, dh0, D, R, n, scale);
+            hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (cols / (16 * w)))), dim3(walk_threads<w>), lds, s, qt, kt, ot, be, G, Tm,
+                               dhT, E, (uint16_t*)dv, dh0, D, R, n, scale);
         });
+    };
+    if (n.segs > 1) {
+        walks(gd_before(n, K), std::true_type());
+        gd_join(n, K, E, s);
+    }
+    if (T > 0 || dh0) walks(V * n.segs, std::false_type());
     if (T > 0) {
         auto grads = K == 64 ? (HV > H ? rwkv6_gated_delta_grads_kernel<64, true> : rwkv6_gated_delta_grads_kernel<64, false>)
                              : (HV > H ? rwkv6_gated_delta_grads_kernel<128, true> : rwkv6_gated_delta_grads_kernel<128, false>);

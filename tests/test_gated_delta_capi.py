@@ -97,7 +97,7 @@ def test_sizes(pkg):
     maps = L.rwkv6_gated_delta_workspace_bytes(1, 4, 65536, 64, 64, 0) - 4096 * (10240 + 512 + 256)
     assert maps == 4 * 15 * 64 * 128 * 4
     assert L.rwkv6_gated_delta_saved_bytes(1, 4, 65536, 64, 64) == 4096 * (10240 + 512 + 256 + 16384 + 16384) + maps
-    assert L.rwkv6_gated_delta_workspace_bytes(1, 4, 65536, 64, 64, 1) == 4096 * (16384 + 16384)
+    assert L.rwkv6_gated_delta_workspace_bytes(1, 4, 65536, 64, 64, 1) == 4096 * (16384 + 16384) + maps
     assert L.rwkv6_gated_delta_saved_bytes(1, 1, 1, 128, 64) == 10240 + 512 + 256 + 32768 + 16384
     assert L.rwkv6_gated_delta_saved_bytes(B, HV, 0, 64, 64) == 0 == L.rwkv6_gated_delta_saved_bytes(B, HV, T, 32, 64)
 
@@ -160,8 +160,8 @@ def test_launches_of_large_calls(tmp_path):
     out = subprocess.run([sys.executable, str(tmp_path / "child.py"), str(tmp_path / "runtime.so"), LIB, json.dumps(calls)], check=True,
                          capture_output=True, text=True)
     for c, (status, *launches) in zip(calls, json.loads(out.stdout.splitlines()[-1])):
-        long = c[4] >= 1 << 24                                   # the forward's segments, and what joins them
-        assert status == OK and len(launches) == {"fwd": 4 if long else 2, "bwd": 2, "step": 1}[c[0]], (c, status, launches)
+        long = c[4] >= 1 << 24                                   # the walks' segments, and what joins them
+        assert status == OK and len(launches) == {"fwd": 4 if long else 2, "bwd": 4 if long else 2, "step": 1}[c[0]], (c, status, launches)
         for blocks, threads, lds in launches:
             assert 0 < blocks * threads < 1 << 32 and threads <= 1024 and lds <= 163840, (c, launches)
 

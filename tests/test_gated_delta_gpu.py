@@ -164,7 +164,7 @@ def test_a_long_sequence(pkg, T):
     run_train(pkg, d, final=True, wo=torch.randn(1, 2, T, 64).to(BF), wh=torch.randn(1, 2, 64, 64))
 
 
-# few heads: the chunks are walked in segments side by side (7 to 13 of them here), the last of them shorter
+# few heads: the chunks are walked in segments side by side (7 to 16 of them here), the last of them shorter
 SEGMENTED = [(1, 1, 1, 1500, 64, 64), (1, 1, 2, 2049, 64, 128), (2, 1, 1, 1300, 128, 64), (1, 2, 2, 1999, 128, 128), (1, 1, 3, 1500, 128, 192)]
 
 
@@ -174,9 +174,10 @@ def test_segments(pkg, shape, states):
     """A decay that leaves half of a state after 300 tokens: what a segment gets from the one before it counts."""
     B, H, HV, T, K, V = shape
     L = pkg._lib.load()
-    chunks = B * HV * ((T + 63) // 64)                    # T of 10 KB, G and beta, then a map and a state a segment but the last
-    n = L.rwkv6_gated_delta_workspace_bytes(B, HV, T, K, V, 0) - chunks * (10240 + 512 + 256)
-    assert n % (B * HV * K * (K + V) * 4) == 0 and n >= 2 * B * HV * K * (K + V) * 4
+    chunks, one = B * HV * ((T + 63) // 64), B * HV * K * (K + V) * 4       # a map and a state for each segment but the last
+    for back, rest in ((0, 10240 + 512 + 256), (1, 4 * K * V + 256 * V)):
+        n = L.rwkv6_gated_delta_workspace_bytes(B, HV, T, K, V, back) - chunks * rest
+        assert n % one == 0 and n >= 2 * one
     d = inputs(*shape, seed=sum(shape), h0=states)
     d["g"] = d["g"].clamp(min=-0.0023)
     d["g"][:, :, 700] = -float("inf") if not states else -0.1
@@ -193,31 +194,39 @@ def test_segments(pkg, shape, states):
 def test_segments_captured_and_on_other_streams(pkg):
     d = on_gpu(inputs(2, 2, 2, 2000, 64, 64, seed=15, h0=True))
 
+    w = torch.randn(2, 2, 2000, 64, device="cuda").to(BF)
+    leaves = [d[n].clone().requires_grad_(True) for n in NAMES]
+
     def prompt():
         with torch.no_grad():
             return pkg.gated_delta.gated_delta_rule(*[d[n] for n in NAMES], initial_state=d["h0"], output_final_state=True)
 
-    want = prompt()
+    def train():
+        o, S = pkg.gated_delta.gated_delta_rule(*leaves, initial_state=d["h0"], output_final_state=True)
+        return torch.autograd.grad((o, S), leaves, (w, d["h0"]))
+
+    want = [prompt(), train()]
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
     got = []
     for s in streams * 2:
         with torch.cuda.stream(s):
-            got.append(prompt())
+            got.append([prompt(), train()])
     torch.cuda.synchronize()
-    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
-    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
-    outs = []
-    for g in graphs:
-        with torch.cuda.graph(g):
-            outs.append(prompt())
+    assert all(torch.equal(a, b) for g in got for x, y in zip(g, want) for a, b in zip(x, y))
+    graphs, outs = [], []
+    for f in (prompt, prompt, train):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(f())
     for rep in range(3):
         d["h0"].mul_(2)
         for g in graphs:
             g.replay()
-        want = prompt()
         torch.cuda.synchronize()
-        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want)), rep
+        got = [[t.clone() for t in o] for o in outs]
+        want = [prompt(), prompt(), train()]
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y)), rep
 
 
 def test_slow_decay_keeps_an_old_state(pkg):
