@@ -445,7 +445,8 @@ int rwkv6_residual_norm_dropout_bwd(const void* x, int x_dtype, const void* bran
  * `workspace` (rwkv6_gated_delta_workspace_bytes, for_bwd 0) is used.  bwd: gradients of losses on o (d_o) and on
  * the final state (dhT, nullable); dq, dk [B,H,T,K] (the sums over the value heads of a key head), dv [B,HV,T,V]
  * bf16, dg f32, dbeta in beta_dtype [B,HV,T], dh0 f32 nullable.
- * hT, dh0, dg and dbeta have the precision of 32-bit arithmetic.
+ * hT, dh0, dg and dbeta have the precision of 32-bit arithmetic.  A NaN or an infinity in a token may reach every
+ * token of its chunk of 64, also those before it.
  * step: the same for a few tokens, `state` [B,HV,K,V] f32 updated where it lies: state_strides are a sequence's
  * and a head's (multiples of 4); states that overlap each other are refused.
  * A caller that captures a call into a graph makes one eager call of fwd on the device first.

@@ -17,7 +17,8 @@
 //   d_g = the suffix sums of d_G in the chunk.
 //
 // Kernels: `prep` (G and T, a block a chunk), `fwd` (a walk over the chunks), `bwd` (the walk back,
-// for d_v and D), `grads` (the rest, a block a chunk), `step` (a few tokens).
+// for d_v and D), `segment` and `join` (where the walks of long sequences of few heads start in the middle),
+// `grads` (the rest, a block a chunk), `step` (a few tokens).
 //
 // A walk.  Only k S, T (..) and k^T (..) follow one another from chunk to chunk, and their columns are
 // independent of each other: a wave keeps 16 columns of S in its accumulators, and since an accumulator's rows are
@@ -253,7 +254,8 @@ template <int N> __device__ __forceinline__ void gd_zero_p(uint16_t* P, int tid)
 
 // G and T of a chunk.  Wave w forms the rows of its 16-token block of A = beta L k k^T, inverts the block
 // on the diagonal by substitution, and then column w of the blocks below it, in the 32-bit matrix instructions:
-// T_IJ = -T_II sum_{J<=l<I} A_Il T_lJ.  Out: G [chunk][64] as pairs of floats in base-2 units, beta
+// T_IJ = -T_II sum_{J<=l<I} A_Il T_lJ.  Bound by the latency of that chain of products and of the substitution, blocks
+// side by side filling it: 16384 chunks 93 us, 308 MB at 3.3 TB/s (K = 64).  Out: G [chunk][64] as pairs of floats in base-2 units, beta
 // in 32 bits, T [chunk][10 blocks][16][16].
 template <int K>
 __global__ void __launch_bounds__(256)
@@ -489,7 +491,8 @@ template <int K> __device__ __forceinline__ float* seg_map(float* E, const GdSha
 template <int K> __device__ __forceinline__ float* seg_state(float* E, const GdShape& n, int64_t bh, int seg, int ct) {
     return seg_map<K>(E, n, bh, seg) + K * K + ct * (K * 16);
 }
-template <int K> __device__ __forceinline__ void put_segment(float* E, const GdShape& n, const WalkAt& w, const f32x4* S, int wave, int lane) {
+template <int K>
+__device__ __forceinline__ void put_segment(float* E, const GdShape& n, const WalkAt& w, const f32x4* S, int wave, int lane) {
     if (w.i0 >= 0) {
         float* p = seg_map<K>(E, n, w.bh, w.seg) + w.i0 + 16 * wave + (lane & 15);
 #pragma unroll
@@ -563,7 +566,9 @@ template <int N, int V> __device__ __forceinline__ void gd_weave() {
 }  // namespace
 
 // A block walks a segment of one head's chunks with 16 NW columns of the state.  SAVE: S_save and n_save get the state
-// entering each chunk and the values it writes, for the backward.
+// entering each chunk and the values it writes, for the backward.  256 heads of 64 chunks, 64 x 64, with them: 230 us, 1.25
+// GB at 5.4 TB/s, the memory's rate; fewer heads are bound by the chain's instructions, 1.75 us a chunk (118 matrix
+// instructions and some 400 others of one wave, about one in 5.5 cycles), 2.65 with 128 key channels.
 template <int K, int NW, bool SAVE>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
@@ -781,6 +786,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
 
 // What a segment does to a state, before the segments' walks: S alone is carried through, without q and o.  The map of
 // the state that enters it is one more walk, of K columns that begin as the identity and to which nothing is written.
+// 1.4 us a chunk, where the whole walk takes 1.75; 32 heads of 512 chunks in eight segments 252 us, `join` 9.
 template <int K, int NW>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_segment_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
@@ -969,6 +975,8 @@ __global__ void __launch_bounds__(256) rwkv6_gated_delta_join_kernel(float* __re
 
 // The walk back: d_v, and for the other gradients r and the gradient D of the state that each chunk leaves.
 // BEFORE: what the segments but the first do to D, as in `segment`, the last segment being the first to be walked.
+// 256 heads of 64 chunks, 64 x 64: 280 us, 1.25 GB at 4.5 TB/s: the memory would allow 230, the chain is longer than
+// the forward's (P in three parts, scale e^G d_o taken apart too); 2.8 us a chunk where heads are few.
 template <int K, int NW, bool BEFORE>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* __restrict__ beta,
@@ -1233,7 +1241,10 @@ __device__ __forceinline__ bf16x8 plain_rows(const uint16_t* X, int stride, int 
 
 // d_q, d_k, d_g and d_beta of a chunk of a key head, its value heads one after the other.  Wave (I, half) has the
 // tokens 16 I .. 16 I + 15 against half of the key channels, and of the columns of p and m those of its parity; every
-// product is formed transposed, so that a lane has one token and four adjacent channels.
+// product is formed transposed, so that a lane has one token and four adjacent channels.  Bound by its other
+// instructions (55 % of the cycles: parts of S, D, n, r), LDS (45 %) and the waits between barriers of two blocks a CU:
+// 16384 chunks of 64 x 64 484 us, 1.90 GB at 3.9 TB/s.  Two value heads a key head and more hold d_q and d_k over
+// them, which takes more registers (GROUPED).
 template <int K, bool GROUPED>
 __global__ void __launch_bounds__(512, K == 64 && !GROUPED ? 4 : 2)
 rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o, const float* __restrict__ beta, int beta_dt,
@@ -1555,8 +1566,9 @@ inline double gd_time(int tiles, int64_t K, bool back, bool before, int chunks) 
 // Segments of a walk.  Few heads leave most of the chip idle and a walk as long as the sequence: p segments walk
 // side by side from states that a walk over all but the last has found (with the K columns of its map beside the
 // V of its state) and `join` has put together.  The number with the least time by the paces above and what
-// two more launches cost is taken, 1 where none beats it.  Forward of 4, 8 and 32 heads of 64 x 64 of 65536, 32768 and 32768 tokens: 1760 to 256 us, 900 to 176, 980 to
-// 567; backward of 8 and 32 of 16384 tokens: 722 to 189, 952 to 600; 256 heads of 4096 tokens fill the chip as they are.
+// two more launches cost is taken, 1 where none beats it.  Forward of 4 heads (64 x 64) of 65536 tokens 1760 to 256 us,
+// of 8 and of 32 heads of 32768 900 to 176 and 980 to 567; backward of 8 and of 32 heads of 16384 722 to 189 and 952 to
+// 600; 256 heads of 4096 tokens fill the chip as they are.
 void gd_segments(GdShape* n, int64_t K, bool back) {
     n->segs = 1;
     n->per = n->NC;

@@ -32,7 +32,11 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, output_fi
     q, k, v are used as bf16 (fp32 and fp16 are rounded on entry), o [B,HV,T,V] has v's type.  g and the states
     are fp32, beta bf16 or fp32; final_state and the gradients of g, beta and initial_state are computed in 32
     bits.  q, k, v may be strided (a projection's output seen as [B,H,T,K] is read where it lies).  Gradients for
-    all inputs, also from final_state; the backward itself cannot be differentiated.  The same bits every time."""
+    all inputs, also from final_state; the backward itself cannot be differentiated.  The same bits every time.
+
+    Kept for the backward: about 680 bytes a token and value head at K = V = 64 (of each chunk of 64 tokens its
+    triangle, the state that enters it and the values it writes, in 32 bits).  A chunk is one system of equations: a NaN
+    or an infinity in a token may reach every token of its chunk, those before it too, so padding holds finite numbers."""
     scale = q.shape[-1] ** -0.5 if scale is None and isinstance(q, torch.Tensor) and q.dim() else scale
     try:
         out = _lib.native().gated_delta_rule(q, k, v, g, beta, initial_state, float(scale), bool(output_final_state))
