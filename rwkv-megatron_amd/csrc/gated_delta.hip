@@ -45,7 +45,7 @@
 #define GD_C 64                 // tokens of a chunk
 #define GD_PAD 8                // elements behind a row of an LDS tile
 #define GD_TS (GD_C + GD_PAD)   // row of a bf16 tile of 64 columns
-#define GD_BF 20                // row of a 16 x 16 block in 32 bits
+#define GD_BF 16                // row of a 16 x 16 block in 32 bits: what a wave reads of one is adjacent
 #define GD_TB 2560              // T in memory: the ten 16 x 16 blocks of its triangle
 #define GD_TP 3584              // a part of T in LDS: 32 rows of 32 columns, 32 of 64
 #define GD_TROW(i) ((i) < 32 ? (i) * 40 : 1280 + ((i) - 32) * GD_TS)
@@ -252,21 +252,25 @@ template <int N> __device__ __forceinline__ void gd_zero_p(uint16_t* P, int tid)
 
 }  // namespace
 
-// G and T of a chunk.  Wave w forms the rows of its 16-token block of A = beta L k k^T, inverts the block
-// on the diagonal by substitution, and then column w of the blocks below it, in the 32-bit matrix instructions:
+// G and T of a chunk.  Wave w forms the rows of its 16-token block of A = beta L k k^T, one wave inverts the blocks
+// on the diagonal by substitution, and wave w then forms column w of the blocks below it, in the 32-bit matrix instructions:
 // T_IJ = -T_II sum_{J<=l<I} A_Il T_lJ.  Bound by the latency of that chain of products and of the substitution, blocks
-// side by side filling it: 16384 chunks 93 us, 308 MB at 3.3 TB/s (K = 64).  Out: G [chunk][64] as pairs of floats in base-2 units, beta
+// side by side filling it: 16384 chunks 86 us, 323 MB at 3.8 TB/s (K = 64).  Out: G [chunk][64] as pairs of floats in base-2 units, beta
 // in 32 bits, T [chunk][10 blocks][16][16].
 template <int K>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, K == 64 ? 8 : 4)
 rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const void* __restrict__ beta, int beta_dt,
                               float2* __restrict__ G_out, float* __restrict__ b_out, float* __restrict__ T_out, GdShape n) {
-    // the blocks of the triangles, row by row: 26 KB of LDS leave room for six blocks a CU (126 to 101 us for 16384 chunks,
-    // whole squares for four)
-    __shared__ __attribute__((aligned(16))) float As[10][16 * GD_BF], Ts[10][16 * GD_BF];
+    // the blocks of the triangles, row by row: A's ten, whose diagonal T's replaces, and T's six below it.  17 KB of LDS leave
+    // room for eight blocks a CU (126 us for 16384 chunks with whole squares, four blocks a CU; 101 with padded rows, six)
+    __shared__ __attribute__((aligned(16))) float X[16][16 * GD_BF];
+    const auto at_A = [](int I, int J) { return X[I * (I + 1) / 2 + J]; };
+    const auto at_T = [](int I, int J) { return I == J ? X[I * (I + 3) / 2] : X[10 + I * (I - 1) / 2 + J]; };
     __shared__ float2 G[GD_C];
     __shared__ float be[GD_C];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, q = lane >> 4;
+    // the waves' shares differ: from block to block they move on by a SIMD
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(((tid >> 6) + blockIdx.x) & 3);
     const int64_t chunk = blockIdx.x, bh = blockIdx.x / (unsigned)n.NC;
     const int c = (int)(blockIdx.x % (unsigned)n.NC), b = (int)bh / n.HV, hv = (int)bh % n.HV, t0 = c * GD_C;
     const uint16_t* kp = k.p + b * k.sb + (hv / (n.HV / n.H)) * k.sh;
@@ -310,14 +314,13 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
             f32x4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = i > j + r ? be[i] * ex2(gd_gap(gi, G[j + r])) * a[r] : 0.f;
-            *reinterpret_cast<f32x4*>(&As[I * (I + 1) / 2 + J][lr * GD_BF + 4 * q]) = x;
+            *reinterpret_cast<f32x4*>(at_A(I, J) + lr * GD_BF + 4 * q) = x;
         }
     }
     __syncthreads();
-    {
+    if (wave == 3) {                                       // the four blocks on the diagonal, 16 lanes each
         float x[16];
-        const float* A = As[wave * (wave + 3) / 2];
-        float* D = Ts[wave * (wave + 3) / 2];
+        float* A = at_A(q, q);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float a[16], s0 = r == lr ? 1.f : 0.f, s1 = 0.f;
@@ -330,7 +333,7 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
 #pragma unroll
             for (int s = 0; s < r; ++s) (s & 1 ? s1 : s0) -= a[s] * x[s];
             x[r] = s0 + s1;
-            if ((r >> 2) == q) D[r * GD_BF + lr] = x[r];
+            A[r * GD_BF + lr] = x[r];
         }
     }
     __syncthreads();
@@ -339,21 +342,23 @@ rwkv6_gated_delta_prep_kernel(GdTensor k, const float* __restrict__ g, const voi
         if (J != wave) continue;
         f32x4 t[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[J][r] = Ts[J * (J + 3) / 2][(4 * q + r) * GD_BF + lr];
+        for (int r = 0; r < 4; ++r) t[J][r] = at_T(J, J)[(4 * q + r) * GD_BF + lr];
 #pragma unroll
         for (int I = J + 1; I < 4; ++I) {
             f32x4 a = {0, 0, 0, 0}, d = {0, 0, 0, 0};
 #pragma unroll
-            for (int l = J; l < I; ++l) a = mul_f32(As[I * (I + 1) / 2 + l], t[l], a, lane);
-            d = mul_f32(Ts[I * (I + 3) / 2], a, d, lane);
+            for (int l = J; l < I; ++l) a = mul_f32(at_A(I, l), t[l], a, lane);
+            d = mul_f32(at_T(I, I), a, d, lane);
             t[I] = -d;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) Ts[I * (I + 1) / 2 + J][(4 * q + r) * GD_BF + lr] = t[I][r];
+            for (int r = 0; r < 4; ++r) at_T(I, J)[(4 * q + r) * GD_BF + lr] = t[I][r];
         }
     }
     __syncthreads();
-    for (int i = tid; i < GD_TB / 4; i += 256)
-        *reinterpret_cast<f32x4*>(T_out + chunk * GD_TB + 4 * i) = at4(Ts[i >> 6], ((i >> 2) & 15) * GD_BF + 4 * (i & 3));
+    for (int i = tid; i < GD_TB / 4; i += 256) {
+        const int t = i >> 6, I = gd_block_row(t);
+        *reinterpret_cast<f32x4*>(T_out + chunk * GD_TB + 4 * i) = at4(at_T(I, t - I * (I + 1) / 2), 4 * (i & 63));
+    }
 }
 
 namespace {
