@@ -1494,20 +1494,21 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
 // A few tokens.  A wave has 32 columns of a head's state in registers: lane group lane / 8 has K / 8 adjacent
 // rows, a lane four columns of them, so a row is read in 128 bytes and the sums over rows cross the groups only.
 // The state is read and written once, whatever the number of tokens, past the caches (a layer's state is next read
-// after every other layer's), and that is all that bounds it: 256 x 32 heads of 128 x 128 195 us, 5.5 TB/s, where a
-// copy of 1 GiB reaches 5.2; 215 through the caches.
+// after every other layer's), and that is all that bounds it: 256 x 32 heads of 128 x 128 190 us, 5.7 TB/s, where a
+// copy of 1 GiB reaches 5.2; through the caches it takes 20 us more.  The next token's inputs come under this one's
+// arithmetic.
 template <int K>
 __global__ void __launch_bounds__(64 * GD_STEP_WAVES)
 rwkv6_gated_delta_step_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ g, const void* __restrict__ beta,
                               int beta_dt, float* __restrict__ state, int64_t ssb, int64_t ssh, uint16_t* __restrict__ o,
-                              GdShape n, float scale, int64_t waves) {
+                              GdShape n, float scale, unsigned waves) {
     constexpr int R = K / 8;
     const int lane = threadIdx.x & 63, grp = lane >> 3;
-    const int64_t w = (int64_t)blockIdx.x * GD_STEP_WAVES + (threadIdx.x >> 6);
+    const unsigned w = blockIdx.x * GD_STEP_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (w >= waves) return;
-    const int nb = n.V / 32;
-    const int64_t bh = w / nb, b = bh / n.HV;
-    const int hv = (int)(bh % n.HV), hk = hv / (n.HV / n.H), c0 = 32 * (int)(w % nb) + 4 * (lane & 7);
+    const unsigned nb = n.V / 32, head = w / nb;           // fewer than 2^27 waves
+    const int64_t bh = head, b = head / (unsigned)n.HV;
+    const int hv = (int)(head % (unsigned)n.HV), hk = hv / (n.HV / n.H), c0 = 32 * (int)(w % nb) + 4 * (lane & 7);
     const uint16_t *qp = q.p + b * q.sb + hk * q.sh + R * grp, *kp = k.p + b * k.sb + hk * k.sh + R * grp;
     const uint16_t* vp = v.p + b * v.sb + hv * v.sh + c0;
     float* sp = state + b * ssb + hv * ssh + (int64_t)(R * grp) * n.V + c0;
@@ -1523,15 +1524,34 @@ rwkv6_gated_delta_step_kernel(GdTensor q, GdTensor k, GdTensor v, const float* _
         }
         return x;
     };
+    uint4 kr[R / 8], qr[R / 8];
+    uint2 vr;
+    float gr;
+    uint16_t bh_, bl_;                                     // beta's halves: a branch on its type would wait for all loads
+    const uint16_t* bp = reinterpret_cast<const uint16_t*>(beta);
+    const int wide = beta_dt == RWKV6_F32;
+    const auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < R / 8; ++i) {
+            kr[i] = *reinterpret_cast<const uint4*>(kp + t * k.st + 8 * i);
+            qr[i] = *reinterpret_cast<const uint4*>(qp + t * q.st + 8 * i);
+        }
+        vr = *reinterpret_cast<const uint2*>(vp + t * v.st);
+        gr = g[bh * n.T + t];
+        bl_ = bp[(bh * n.T + t) << wide];
+        bh_ = bp[((bh * n.T + t) << wide) + wide];
+    };
+    load(0);
     for (int t = 0; t < n.T; ++t) {
         float kf[R], qf[R], x[4];
 #pragma unroll
-        for (int i = 0; i < R; i += 8) {
-            load8(kp + t * k.st + i, kf + i);
-            load8(qp + t * q.st + i, qf + i);
+        for (int i = 0; i < R / 8; ++i) {
+            unpack8(kr[i], kf + 8 * i);
+            unpack8(qr[i], qf + 8 * i);
         }
-        unpack4(*reinterpret_cast<const uint2*>(vp + t * v.st), x);
-        const float a = expf(g[bh * n.T + t]), be = gd_beta(beta, beta_dt, bh * n.T + t);
+        unpack4(vr, x);
+        const float a = expf(gr), be = __builtin_bit_cast(float, (uint32_t)bh_ << 16 | (wide ? (uint32_t)bl_ : 0u));
+        load(min(t + 1, n.T - 1));                         // under this token's arithmetic
         f32x4 e = {0, 0, 0, 0}, y = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -1838,7 +1858,7 @@ int rwkv6_gated_delta_step(const void* q, const void* k, const void* v, const in
     auto step = K == 64 ? rwkv6_gated_delta_step_kernel<64> : rwkv6_gated_delta_step_kernel<128>;
     hipLaunchKernelGGL(step, dim3((unsigned)((waves + GD_STEP_WAVES - 1) / GD_STEP_WAVES)), dim3(64 * GD_STEP_WAVES), 0,
                        reinterpret_cast<hipStream_t>(stream), qt, kt, vt, g, beta, beta_dtype, state, sb, sh, (uint16_t*)o, n, scale,
-                       waves);
+                       (unsigned)waves);
     return hipGetLastError() == hipSuccess ? RWKV6_OK : RWKV6_ERR_LAUNCH;
 }
 
