@@ -1404,7 +1404,8 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
                     const float l = ex2(gd_gap(g, G[j + r])), w = i > j + r ? -l * R[u][r] : 0.f;
                     p[r] = i >= j + r ? scale * l * P[u][r] : 0.f;
                     m[r] = bi * w;
-                    cs[r] = p[r] * qk[r] + m[r] * kk[r];
+                    // without the diagonal, which no decay enters: its share of row and column would only round
+                    cs[r] = i > j + r ? p[r] * qk[r] + m[r] * kk[r] : 0.f;
                     own += cs[r];
                     db += w * kk[r];
                 }

@@ -265,6 +265,15 @@ def test_edges_of_decay_and_beta(pkg, case):
         run_train(pkg, d, wo=torch.randn(1, 2, 150, 64).to(BF))
 
 
+@pytest.mark.parametrize("T, h0", [(2, False), (5, False), (40, True), (130, True)])
+def test_the_decay_s_gradient_where_little_is_kept(pkg, T, h0):
+    """e^-18 = 1.5e-8 of a state is left after a token: what a token reads of itself, which no decay enters, is 10^8 times
+    the gradient of g, and rounds none of it.  Bounds as everywhere, of the gradient's own norm."""
+    d = inputs(2, 2, 2, T, 64, 64, seed=T, h0=h0)
+    d["g"] = d["g"] * 0.01 - 18
+    run_train(pkg, d, wo=torch.randn(2, 2, T, 64, generator=torch.Generator().manual_seed(T)).to(BF))
+
+
 @pytest.mark.parametrize("scale", [1e-12, 1e12])
 def test_gradients_of_any_size(pkg, scale):
     """d_o is taken as it is: its size goes through to all gradients."""
