@@ -274,6 +274,18 @@ def test_the_decay_s_gradient_where_little_is_kept(pkg, T, h0):
     run_train(pkg, d, wo=torch.randn(2, 2, T, 64, generator=torch.Generator().manual_seed(T)).to(BF))
 
 
+@pytest.mark.parametrize("K", [64, 128])
+@pytest.mark.parametrize("period", [1, 3])
+def test_the_same_keys_again(pkg, K, period):
+    """Every correction taken whole and nothing forgotten: the chunk's triangle is as full as it gets."""
+    d = inputs(1, 1, 1, 200, K, 64, seed=K + period, h0=True)
+    d["k"] = d["k"][:, :, torch.arange(200) % period].contiguous()
+    d["beta"].fill_(1)
+    d["g"].zero_()
+    G = torch.Generator().manual_seed(period)
+    run_train(pkg, d, final=True, wo=torch.randn(1, 1, 200, 64, generator=G).to(BF), wh=torch.randn(1, 1, K, 64, generator=G))
+
+
 @pytest.mark.parametrize("scale", [1e-12, 1e12])
 def test_gradients_of_any_size(pkg, scale):
     """d_o is taken as it is: its size goes through to all gradients."""
