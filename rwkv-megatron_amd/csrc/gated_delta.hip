@@ -32,9 +32,10 @@
 // 32 bits becomes three of bf16 (bf16 times computed) or six (computed times computed, without the halves that
 // lie below 2^-24), 5 and 2.5 times the rate of the matrix instructions in 32 bits, which also keep a wave's other
 // instructions from running beside them (33 cycles each and 6 for each of five multiply-adds between two of them
-// took 61; the bf16 ones, of 17 cycles, hide theirs).  What ends in a bf16 output alone (o; p and m of d_q and d_k) is
-// taken as two numbers, 2^-16 off at most.  Final states and the gradients of g and beta so have the precision of
-// 32-bit arithmetic, not of bf16.
+// took 61; the bf16 ones, of 17 cycles, hide theirs).  Where
+// a write takes the place of what was read, o is the small difference of q S and P n, so these come of three numbers too;
+// p and m of d_q and d_k are taken as two, 2^-16 off at most.  o, final states and the gradients of g and beta so have the
+// precision of 32-bit arithmetic, not of bf16.
 // G is summed in 64 bits and kept as a pair of floats: decays between neighbours late in a chunk are
 // differences of large sums.
 #include <type_traits>
@@ -81,11 +82,6 @@ __device__ __forceinline__ Three three(f32x4 a, f32x4 b) {
     float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     const uint4 h = pack8(x), m = rest8(x, h), l = rest8(x, m);
     return {__builtin_bit_cast(bf16x8, h), __builtin_bit_cast(bf16x8, m), __builtin_bit_cast(bf16x8, l)};
-}
-__device__ __forceinline__ Two two(f32x4 a, f32x4 b) {
-    float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    const uint4 h = pack8(x);
-    return {__builtin_bit_cast(bf16x8, h), __builtin_bit_cast(bf16x8, rest8(x, h))};
 }
 // four values in parts of bf16, 8 bytes each
 __device__ __forceinline__ uint2 rest4(float* x, uint2 h) {
@@ -581,7 +577,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
                              float* __restrict__ E_in, uint16_t* __restrict__ o, float* __restrict__ hT,
                              float* __restrict__ S_save, float* __restrict__ n_save, GdShape n, float scale) {
     extern __shared__ __attribute__((aligned(16))) uint16_t gd_lds[];
-    using M = WalkLds<K, NW, 2>;
+    using M = WalkLds<K, NW, 3>;
     uint16_t* const P = gd_lds + 2 * M::buf;
     constexpr int KS = K + GD_PAD, ND = K / 16, NS = K / 32, PS = GD_C * GD_TS, VS = 16 * NW + GD_PAD;
     const int wave = threadIdx.x >> 6;
@@ -591,7 +587,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
     if (role == -2) return;
     const int c0 = w.seg * n.per, c1 = min(n.NC, c0 + n.per);
     if (role >= 0) {
-        walk_help<K, NW, 2, false>(walk_in(w, n, c0, q, k, v, T, beta, G), c1 - c0, scale, gd_lds, 64 * role + lane);
+        walk_help<K, NW, 3, false>(walk_in(w, n, c0, q, k, v, T, beta, G), c1 - c0, scale, gd_lds, 64 * role + lane);
         return;
     }
     const int ct = w.v0 / 16 + wave, col = w.v0 + 16 * wave + lr;
@@ -665,29 +661,43 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
             for (int I = 0; I < 4; ++I) E[I] = mfma32(f[s][I], Sp[s].h, E[I]);
         }
         gd_issued();
+        const auto read_q = [&](int s0) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+            for (int s = s0; s < s0 + 2; ++s)
 #pragma unroll
-            for (int I = 0; I < 4; ++I) f[s][I] = prows(L.Q, KS, 16 * I, 32 * s, lane);
-#pragma unroll
-        for (int I = 0; I < 4; ++I) el[I] = at4(L.eL, 16 * I + 4 * lq);
-        const float eC = L.eG[GD_C - 1];
-        gd_issued();
+                for (int I = 0; I < 4; ++I) f[s][I] = prows(L.Q, KS, 16 * I, 32 * s, lane);
+        };
         // q S (transposed: a lane has four adjacent channels of a token) beside v - e^G k S and its parts
+        const auto q_s = [&](int s0) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
+            for (int s = s0; s < s0 + 2; ++s) {
 #pragma unroll
-            for (int I = 0; I < 4; ++I) O[I] = mfma32(Sp[s].m, f[s][I], O[I]);
+                for (int I = 0; I < 4; ++I) O[I] = mfma32(Sp[s].l, f[s][I], O[I]);
 #pragma unroll
-            for (int I = 0; I < 4; ++I) O[I] = mfma32(Sp[s].h, f[s][I], O[I]);
-        }
+                for (int I = 0; I < 4; ++I) O[I] = mfma32(Sp[s].m, f[s][I], O[I]);
+#pragma unroll
+                for (int I = 0; I < 4; ++I) O[I] = mfma32(Sp[s].h, f[s][I], O[I]);
+            }
+        };
+        read_q(0);
+        gd_issued();
+        q_s(0);
 #pragma unroll
         for (int I = 0; I < 4; ++I) E[I] = be[I] * (x[I] - eg[I] * E[I]);
         const Three e0 = three(E[0], E[1]);
-        gd_weave<8 * NS, K == 64 ? 5 : 3>();
+        gd_weave<24, 4>();
         gd_issued();
+        if constexpr (K == 128) {
+            read_q(2);
+            gd_issued();
+            q_s(2);
+            gd_issued();
+        }
         if constexpr (K == 64) read_t1();
         else read_t0();
+#pragma unroll
+        for (int I = 0; I < 4; ++I) el[I] = at4(L.eL, 16 * I + 4 * lq);
+        const float eC = L.eG[GD_C - 1];
 #pragma unroll
         for (int d = 0; d < ND; ++d) k0[d] = pcols(L.K, KS, 0, 16 * d, lane);
         gd_issued();
@@ -707,21 +717,20 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
         for (int I = 0; I < 4; ++I) qg[I] = L.eG[16 * I + lr];
         gd_issued();
         mm_tiles<2, 4>(t1, e1, N);
-        const Two n0 = two(N[0], N[1]);
+        const Three n0 = three(N[0], N[1]);
 #pragma unroll
         for (int d = 0; d < ND; ++d) S[d] *= eC;
         gd_weave<12, 4>();
         __syncthreads();                                   // P
-        Two pp[4][2];
-        const auto read_p = [&] {
+        Three pp[4][2];
+        const auto read_p = [&](int s) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int I = 2 * s; I < 4; ++I)
-                    pp[I][s] = {prows(P, GD_TS, 16 * I, 32 * s, lane), prows(P + PS, GD_TS, 16 * I, 32 * s, lane)};
+            for (int I = 2 * s; I < 4; ++I)
+                pp[I][s] = {prows(P, GD_TS, 16 * I, 32 * s, lane), prows(P + PS, GD_TS, 16 * I, 32 * s, lane),
+                            prows(P + 2 * PS, GD_TS, 16 * I, 32 * s, lane)};
             gd_issued();
         };
-        if constexpr (K == 64) read_p();                   // (128: its registers are still taken)
+        if constexpr (K == 64) read_p(0);                  // (128: its registers are still taken)
 #pragma unroll
         for (int d = 0; d < ND; ++d) S[d] = mfma32(k0[d], w0.l, S[d]);
 #pragma unroll
@@ -741,7 +750,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
         for (int d = 0; d < ND; ++d) S[d] = mfma32(k1[d], w1.m, S[d]);
 #pragma unroll
         for (int d = 0; d < ND; ++d) S[d] = mfma32(k1[d], w1.h, S[d]);
-        const Two n1 = two(N[2], N[3]);
+        const Three n1 = three(N[2], N[3]);
 #pragma unroll
         for (int I = 0; I < 4; ++I) O[I] *= scale * qg[I];
         gd_weave<3 * ND, K == 64 ? 4 : 2>();
@@ -749,26 +758,37 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
         if constexpr (SAVE)
 #pragma unroll
             for (int I = 0; I < 4; ++I) put_tiles(n_save + (at * 4 + I) * 256, N[I], lane);
-        if constexpr (K == 128) read_p();
+        // beside P n the next chunk's state is taken apart
+        const auto p_n = [&](const Three& x, int s) {
 #pragma unroll
-        for (int I = 0; I < 4; ++I) O[I] = mfma32(n0.l, pp[I][0].h, O[I]);
+            for (int I = 2 * s; I < 4; ++I) O[I] = mfma32(x.l, pp[I][s].h, O[I]);
 #pragma unroll
-        for (int I = 0; I < 4; ++I) O[I] = mfma32(n0.h, pp[I][0].l, O[I]);
+            for (int I = 2 * s; I < 4; ++I) O[I] = mfma32(x.h, pp[I][s].l, O[I]);
 #pragma unroll
-        for (int I = 0; I < 4; ++I) O[I] = mfma32(n0.h, pp[I][0].h, O[I]);
+            for (int I = 2 * s; I < 4; ++I) O[I] = mfma32(x.m, pp[I][s].m, O[I]);
 #pragma unroll
-        for (int I = 2; I < 4; ++I) O[I] = mfma32(n1.l, pp[I][1].h, O[I]);
+            for (int I = 2 * s; I < 4; ++I) O[I] = mfma32(x.m, pp[I][s].h, O[I]);
 #pragma unroll
-        for (int I = 2; I < 4; ++I) O[I] = mfma32(n1.h, pp[I][1].l, O[I]);
+            for (int I = 2 * s; I < 4; ++I) O[I] = mfma32(x.h, pp[I][s].m, O[I]);
 #pragma unroll
-        for (int I = 2; I < 4; ++I) O[I] = mfma32(n1.h, pp[I][1].h, O[I]);
-        // beside them the next chunk's state is taken apart
+            for (int I = 2 * s; I < 4; ++I) O[I] = mfma32(x.h, pp[I][s].h, O[I]);
+        };
+        const auto part = [&](int s0) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            Sp[s] = three(S[2 * s], S[2 * s + 1]);
-            gd_here(Sp[s]);
-        }
-        gd_weave<18, K == 64 ? 5 : 10>();
+            for (int s = s0; s < s0 + NS / 2; ++s) {
+                Sp[s] = three(S[2 * s], S[2 * s + 1]);
+                gd_here(Sp[s]);
+            }
+        };
+        if constexpr (K == 128) read_p(0);
+        read_p(1);
+        p_n(n0, 0);
+        part(0);
+        gd_weave<24, K == 64 ? 3 : 5>();
+        gd_issued();
+        p_n(n1, 1);
+        part(NS / 2);
+        gd_weave<12, K == 64 ? 5 : 9>();
         gd_issued();
         uint2 ob[4];
 #pragma unroll
@@ -1687,8 +1707,8 @@ int gd_limits(hipStream_t stream) {
             if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         };
 #define GD_RAISE(K, NW)                                                                                              \
-    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, false>), WalkLds<K, NW, 2>::bytes);       \
-    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, true>), WalkLds<K, NW, 2>::bytes);        \
+    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, false>), WalkLds<K, NW, 3>::bytes);       \
+    raise(reinterpret_cast<const void*>(rwkv6_gated_delta_fwd_kernel<K, NW, true>), WalkLds<K, NW, 3>::bytes);        \
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_segment_kernel<K, NW>), WalkLds<K, NW, 0>::bytes);          \
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<K, NW, false>), WalkLds<K, NW, 3>::bytes);       \
     raise(reinterpret_cast<const void*>(rwkv6_gated_delta_bwd_kernel<K, NW, true>), WalkLds<K, NW, 3>::bytes);
@@ -1766,7 +1786,7 @@ int rwkv6_gated_delta_fwd(const void* q, const void* k, const void* v, const int
         gd_walks(n.BH * (V / 16) * n.segs, K, [&](auto k_, auto w_) {
             constexpr int k = k_, w = w_;
             auto walk = saved ? rwkv6_gated_delta_fwd_kernel<k, w, true> : rwkv6_gated_delta_fwd_kernel<k, w, false>;
-            const size_t lds = WalkLds<k, w, 2>::bytes;
+            const size_t lds = WalkLds<k, w, 3>::bytes;
             hipLaunchKernelGGL(walk, dim3((unsigned)(n.BH * (V / (16 * w)) * n.segs)), dim3(walk_threads<w>), lds, s, qt, kt, vt, be, G,
                                Tm, h0, E, (uint16_t*)o, hT, S, N, n, scale);
         });
