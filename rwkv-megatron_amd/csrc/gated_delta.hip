@@ -32,10 +32,9 @@
 // 32 bits becomes three of bf16 (bf16 times computed) or six (computed times computed, without the halves that
 // lie below 2^-24), 5 and 2.5 times the rate of the matrix instructions in 32 bits, which also keep a wave's other
 // instructions from running beside them (33 cycles each and 6 for each of five multiply-adds between two of them
-// took 61; the bf16 ones, of 17 cycles, hide theirs).  Where
-// a write takes the place of what was read, o is the small difference of q S and P n, so these come of three numbers too;
-// p and m of d_q and d_k are taken as two, 2^-16 off at most.  o, final states and the gradients of g and beta so have the
-// precision of 32-bit arithmetic, not of bf16.
+// took 61; the bf16 ones, of 17 cycles, hide theirs).  What ends in a
+// bf16 output alone is no exception: where a write takes the place of what is read, o is the small difference of q S and
+// P n, and d_q and d_k are such differences too.  All outputs so have the precision of 32-bit arithmetic, rounded once.
 // G is summed in 64 bits and kept as a pair of floats: decays between neighbours late in a chunk are
 // differences of large sums.
 #include <type_traits>
@@ -64,10 +63,7 @@ struct GdShape {
     int64_t BH;                 // sequences times value heads
     int per, segs;              // the forward's chunks of a segment, segments
 };
-struct Two {                    // a computed operand: h + l, 2^-16 off at most
-    bf16x8 h, l;
-};
-struct Three {                  // h + m + l, exact
+struct Three {                  // a computed operand: h + m + l, exact
     bf16x8 h, m, l;
 };
 
@@ -91,7 +87,9 @@ __device__ __forceinline__ uint2 rest4(float* x, uint2 h) {
     for (int j = 0; j < 4; ++j) x[j] -= f[j];
     return make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
 }
-__device__ __forceinline__ f32x4 mm(bf16x8 a, const Two& b, f32x4 c) { return mfma32(a, b.h, mfma32(a, b.l, c)); }
+__device__ __forceinline__ f32x4 mm(bf16x8 a, const Three& b, f32x4 c) {
+    return mfma32(a, b.h, mfma32(a, b.m, mfma32(a, b.l, c)));
+}
 __device__ __forceinline__ f32x4 mm(const Three& a, bf16x8 b, f32x4 c) {
     return mfma32(a.h, b, mfma32(a.m, b, mfma32(a.l, b, c)));
 }
@@ -1217,10 +1215,10 @@ rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* 
 
 namespace {
 // LDS of the gradients: q and k; 32 value channels of n, r [32][64 tokens] and S, D [32][K] in three parts, in
-// whose place p and m [64][64] in two parts come afterwards; sums.
+// whose place p and m [64][64] in three parts come afterwards; sums.
 template <int K> struct GradLds {
     static constexpr int qk = GD_C * (K + GD_PAD), nv = 32 * GD_TS, sv = 32 * (K + GD_PAD), pm = GD_C * GD_TS;
-    static constexpr int shared_ = 6 * nv + 6 * sv > 4 * pm ? 6 * nv + 6 * sv : 4 * pm;
+    static constexpr int shared_ = 6 * nv + 6 * sv > 6 * pm ? 6 * nv + 6 * sv : 6 * pm;
     static constexpr int sums = 3 + 4 + 2 * 3 + 1;         // of 64: e^G, e^{G_C - G}, beta; columns; rows' three by half; rest
     static constexpr size_t bytes = (size_t)(2 * qk + shared_) * 2 + GD_C * 8 + sums * GD_C * 4;
 };
@@ -1282,7 +1280,7 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
     constexpr int KS = K + GD_PAD, ND = K / 32, NS = K / 32;              // ND: a half's channel tiles
     uint16_t *Qt = gd_lds, *Kt = Qt + M::qk, *X = Kt + M::qk;
     uint16_t *Nt = X, *Rt = Nt + 3 * M::nv, *St = Rt + 3 * M::nv, *Dt = St + 3 * M::sv;
-    uint16_t *pt = X, *mt = pt + 2 * M::pm;
+    uint16_t *pt = X, *mt = pt + 3 * M::pm;
     float2* G = reinterpret_cast<float2*>(X + M::shared_);
     float *eG = reinterpret_cast<float*>(G + GD_C), *eL = eG + GD_C, *be = eL + GD_C, *colsum = be + GD_C;
     float *own_ = colsum + 4 * GD_C, *kept_ = own_ + 2 * GD_C, *db_ = kept_ + 2 * GD_C, *part = db_ + 2 * GD_C;
@@ -1290,6 +1288,14 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
     // of all of them at once would not fit the registers
     int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), I = wave & 3, half = wave >> 2;
+    const auto put_parts = [](uint16_t* to, float* x) {
+        uint2 part = make_uint2(pk2(x[0], x[1]), pk2(x[2], x[3]));
+#pragma unroll
+        for (int l = 0; l < 3; ++l) {
+            *reinterpret_cast<uint2*>(to + l * M::pm) = part;
+            if (l < 2) part = rest4(x, part);
+        }
+    };
     const auto anew = [&] {
         int x = threadIdx.x;
         asm volatile("" : "+v"(x));
@@ -1430,11 +1436,8 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
                     db += w * kk[r];
                 }
             }
-            uint2 hp = make_uint2(pk2(p[0], p[1]), pk2(p[2], p[3])), hm = make_uint2(pk2(m[0], m[1]), pk2(m[2], m[3]));
-            *reinterpret_cast<uint2*>(pt + i * GD_TS + j) = hp;
-            *reinterpret_cast<uint2*>(mt + i * GD_TS + j) = hm;
-            *reinterpret_cast<uint2*>(pt + M::pm + i * GD_TS + j) = rest4(p, hp);
-            *reinterpret_cast<uint2*>(mt + M::pm + i * GD_TS + j) = rest4(m, hm);
+            put_parts(pt + i * GD_TS + j, p);
+            put_parts(mt + i * GD_TS + j, m);
 #pragma unroll
             for (int r = 0; r < 4; ++r) cs[r] = sum16(cs[r]);
             if (lr == 0) *reinterpret_cast<float4*>(colsum + I * GD_C + j) = make_float4(cs[0], cs[1], cs[2], cs[3]);
@@ -1456,15 +1459,17 @@ rwkv6_gated_delta_grads_kernel(GdTensor q, GdTensor k, GdTensor v, GdTensor d_o,
         for (int s = 0; s < 2; ++s) {
             // own rows: columns up to the diagonal; transposed: rows from it
             const bool left = 2 * s <= I, right = 2 * s + 1 >= I;
-            Two p0, m0, p1, m1;
-            if (left) {
-                p0 = {plain_rows(pt, GD_TS, 16 * I, 32 * s, lane), plain_rows(pt + M::pm, GD_TS, 16 * I, 32 * s, lane)};
-                m0 = {plain_rows(mt, GD_TS, 16 * I, 32 * s, lane), plain_rows(mt + M::pm, GD_TS, 16 * I, 32 * s, lane)};
-            }
-            if (right) {
-                p1 = {lds_tr8(pt, GD_TS, 32 * s, 16 * I, lane), lds_tr8(pt + M::pm, GD_TS, 32 * s, 16 * I, lane)};
-                m1 = {lds_tr8(mt, GD_TS, 32 * s, 16 * I, lane), lds_tr8(mt + M::pm, GD_TS, 32 * s, 16 * I, lane)};
-            }
+            const auto rows = [&](const uint16_t* x) {
+                return Three{plain_rows(x, GD_TS, 16 * I, 32 * s, lane), plain_rows(x + M::pm, GD_TS, 16 * I, 32 * s, lane),
+                             plain_rows(x + 2 * M::pm, GD_TS, 16 * I, 32 * s, lane)};
+            };
+            const auto turned = [&](const uint16_t* x) {
+                return Three{lds_tr8(x, GD_TS, 32 * s, 16 * I, lane), lds_tr8(x + M::pm, GD_TS, 32 * s, 16 * I, lane),
+                             lds_tr8(x + 2 * M::pm, GD_TS, 32 * s, 16 * I, lane)};
+            };
+            Three p0, m0, p1, m1;
+            if (left) p0 = rows(pt), m0 = rows(mt);
+            if (right) p1 = turned(pt), m1 = turned(mt);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 const bf16x8 fk = lds_tr8(Kt, KS, 32 * s, 16 * (d0 + d), lane);

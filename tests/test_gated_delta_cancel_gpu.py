@@ -105,3 +105,14 @@ SIZES = [(64, 64), (128, 64), (64, 192), (128, 128)]
 @pytest.mark.parametrize("name", ["other keys", "one key"])
 def test_a_read_of_what_was_just_written(pkg, name, K, V):
     held("o", *run(pkg, name, K, V), least=300)
+
+
+@pytest.mark.parametrize("K,V", SIZES)
+def test_the_queries_gradient_of_such_reads(pkg, K, V):
+    held("q", *run(pkg, "one key", K, V), least=300)
+
+
+@pytest.mark.parametrize("K,V", SIZES)
+def test_the_keys_gradient_where_a_write_doubles_what_was_kept(pkg, K, V):
+    """d_k = D n - S' (D^T k) and both are k's direction times u d_o."""
+    held("k", *run(pkg, "twice", K, V), least=300)
