@@ -320,6 +320,9 @@ py::object gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v, c
         recorded({&q, &k, &v, &g, &beta}, OptTensor()))
         return py::none();
     no_transforms();
+    for (const Tensor* t : {&q, &k, &v, &g, &beta, &state})
+        if (t->_fw_grad(0).defined())
+            C10_THROW_ERROR(NotImplementedError, "gated_delta_step has no forward-mode derivative (a dual tensor's tangent would be lost)");
     const c10::DeviceGuard on(q.device());
     return py::cast(unlocked([&] {
         const Strided qs = strided(q), ks = strided(k), vs = strided(v);

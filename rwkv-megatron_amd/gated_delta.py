@@ -56,7 +56,7 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None):
 
     Shapes and types as gated_delta_rule's; state is fp32, each [K,V] of it dense, sequences and heads at any
     strides that are multiples of 4 (a slice of a larger pool is updated where it lies).  Arithmetic in 32 bits.  There is no backward: nothing
-    that requires a gradient is taken while gradients are recorded."""
+    that requires a gradient is taken while gradients are recorded, and no dual tensor of forward-mode derivatives."""
     scale = q.shape[-1] ** -0.5 if scale is None and isinstance(q, torch.Tensor) and q.dim() else scale
     try:
         out = _lib.native().gated_delta_step(q, k, v, g, beta, state, float(scale))
