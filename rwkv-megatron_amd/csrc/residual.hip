@@ -292,12 +292,19 @@ rwkv6_residual_norm_bwd_kernel(RnIn in, const void* __restrict__ gamma, int pdt,
                     if (in.stepwise) round8(f[i]);
                 }
                 if constexpr (GATE) sigmoid8(sg[i], in.stepwise);
+                if constexpr (DROP) {                      // an infinity or a NaN that is dropped reaches no gradient either
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        f[i][j] = dr[i][j] != 0.f ? f[i][j] : 0.f;
+                        if constexpr (GATE) sg[i][j] = dr[i][j] != 0.f ? sg[i][j] : 0.f;
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) t[j] = GATE ? f[i][j] * sg[i][j] : f[i][j];
                 if constexpr (DROP) {
                     if (GATE && in.stepwise) round8(t);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) t[j] = dr[i][j] != 0.f ? t[j] * dr[i][j] : 0.f;
+                    for (int j = 0; j < 8; ++j) t[j] *= dr[i][j];
                     if (in.stepwise) round8(t);
                 }
 #pragma unroll

@@ -41,7 +41,8 @@ def residual_norm(x, branch, weight, bias, eps, gate=None, branch_bias=None, sca
     the same mask for a tensor of the same sizes, so every call wants one of its own (torch.randint's, say, which a
     captured graph draws anew on each replay); what the backward uses is the value that the forward read.
     Element e of f is kept where the 16-bit number e % 8 of Philox4x32-10(counter e // 8, key seed) is at
-    least 65536 p.  stepwise rounds the dropped-out product too.
+    least 65536 p.  An infinity or a NaN in a dropped place of branch or gate is dropped with it, from the gradients
+    too.  stepwise rounds the dropped-out product too.
 
     Gradients for x, branch, gate, weight, bias and branch_bias; sums over the rows run in a fixed
     order.  A backward that is differentiated again runs through torch's operators."""
