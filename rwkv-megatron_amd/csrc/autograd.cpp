@@ -657,7 +657,12 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         Tensor s = x.to(at::kFloat), f, sg;
         if (branch.defined()) {
             f = cbias.defined() ? branch.to(at::kFloat) + cbias.to(at::kFloat) : branch.to(at::kFloat);
-            if (gate.defined()) sg = at::sigmoid(gate.to(at::kFloat));
+            Tensor gf = gate.defined() ? gate.to(at::kFloat) : Tensor();
+            if (drop.defined()) {                         // what is dropped is gone, an infinity or a NaN too
+                f = at::where(drop > 0, f, 0.);
+                if (gf.defined()) gf = at::where(drop > 0, gf, 0.);
+            }
+            if (gf.defined()) sg = at::sigmoid(gf);
             const Tensor fg = gate.defined() ? f * sg : f;
             s = s + (drop.defined() ? fg * drop : fg) * scale;
         }

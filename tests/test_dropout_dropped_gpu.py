@@ -1,5 +1,5 @@
-"""What is dropped is gone: an infinity or a NaN in a dropped place of the branch or of its gate leaves every output
-and gradient as a zero there does, bit for bit."""
+"""What is dropped is gone: an infinity or a NaN in a dropped place of the branch or of its gate leaves every output,
+gradient and second derivative as a zero there does, bit for bit."""
 import pytest
 import torch
 
@@ -43,3 +43,16 @@ def test_gradients(pkg, N, C, gate, cbias, xt, pt, stepwise):
     assert all(t.isfinite().all() for t in got[0])
     for name, a, b in zip(["s", "y", *zeros], *got):
         assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("gate,cbias", [(True, True), (False, False)])
+def test_second_derivatives(pkg, gate, cbias):
+    zeros, wild, ds, dy = both(7, 64, gate, cbias, F32, F32)
+    got = []
+    for d in (zeros, wild):
+        u, s, y = call(pkg, d, False)
+        first = torch.autograd.grad((s, y), list(u.values()), (ds, dy), create_graph=True)
+        got.append([*first, *torch.autograd.grad(sum(t.float().square().sum() for t in first), [t for n, t in u.items() if n != "bias"])])
+    assert all(t.isfinite().all() for t in got[0])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
