@@ -358,6 +358,8 @@ class RWKV6Layer(nn.Module):
     LN -> time mix -> residual -> LN -> channel mix -> residual, with the config's hidden_dropout on what the
     residuals add, in training."""
 
+    hidden_dropout = 0.0                         # of layers saved whole before they had one
+
     def __init__(self, config, layer_number=1, device=None):
         super().__init__()
         C = config.hidden_size
