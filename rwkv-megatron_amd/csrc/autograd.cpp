@@ -23,6 +23,7 @@
 
 #include <array>
 #include <cstring>
+#include <limits>
 #include <optional>
 #include <vector>
 
@@ -685,7 +686,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         return run(zero, one, gamma.detach(), gamma.detach(), Tensor(), Tensor(), 1., 1., false, false, p, seed, Tensor())[0];
     }
 };
-// None when the kernels do not take the call (layers: nor one that a mode or transform wants to see);
+// None when the kernels do not take the call (layers: nor one that a mode or transform wants to see; without a seed one is
+// drawn from the device's generator);
 // the callers check and raise, or run torch's operators.
 py::object residual_norm_dropout(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta, double eps,
                                  const OptTensor& gate, const OptTensor& cbias, double scale, bool stepwise, bool layers, double p,
@@ -702,12 +704,15 @@ py::object residual_norm_dropout(const Tensor& x, const Tensor& branch, const Te
         if (t->device() != x.device() || t->sizes() != at::IntArrayRef({C}) ||
             (t->scalar_type() != at::kBFloat16 && t->scalar_type() != at::kFloat && t->scalar_type() != at::kHalf))
             return py::none();
-    if (p != 0. && (!seed_in || seed_in->device() != x.device() || seed_in->scalar_type() != at::kLong || seed_in->numel() != 1))
+    const bool draws = p != 0. && layers && !seed_in;
+    if (p != 0. && !draws && (!seed_in || seed_in->device() != x.device() || seed_in->scalar_type() != at::kLong || seed_in->numel() != 1))
         return py::none();
-    const Tensor seed = p != 0. ? *seed_in : Tensor();
     if (layers && !plain({&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})) return py::none();
     no_transforms();
     const c10::DeviceGuard on(x.device());           // the default stream is the current device's
+    // drawn here, where the call is taken: the operators that stand for a call that is not draw numbers of their own
+    const Tensor seed = draws ? unlocked([&] { return at::randint(std::numeric_limits<int64_t>::max(), {1}, x.options().dtype(at::kLong)); })
+                        : p != 0. ? *seed_in : Tensor();
     bool grad = recorded({&x, &branch, &gamma, &beta, gate ? &*gate : &x}, cbias);
     for (const Tensor* t : {&x, &branch, &gamma, &beta, gate ? &*gate : &x, cbias ? &*cbias : &x})
         grad = grad || t->_fw_grad(0).defined();          // forward-mode derivatives are refused there
@@ -718,7 +723,7 @@ py::object residual_norm_dropout(const Tensor& x, const Tensor& branch, const Te
         });
         return py::make_tuple(o[0], o[1]);
     }
-    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, stepwise, layers, p, p != 0. ? seed_in : OptTensor()); });
+    const variable_list o = unlocked([&] { return ResidualNorm::apply(x, branch, gamma, beta, gate, cbias, eps, scale, stepwise, layers, p, seed.defined() ? OptTensor(seed) : OptTensor()); });
     return py::make_tuple(o[0], o[1]);
 }
 py::object residual_norm(const Tensor& x, const Tensor& branch, const Tensor& gamma, const Tensor& beta, double eps,

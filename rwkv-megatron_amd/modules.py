@@ -326,11 +326,11 @@ def _add_norm(norm, x, branch, bias=None, gate=None, dropout=0.0):
     """(s, LayerNorm(s)) for s = x + dropout((branch + bias) sigmoid(gate)): in one kernel
     (residual.residual_norm, stepwise: rounded where the separate operators round) where it takes the call,
     else by the operators it stands for.  A norm that is not this package's own class, or that has hooks, is
-    called as a module.  Dropout's seed is drawn from torch's generator of the device, once a call."""
+    called as a module.  Dropout's seed is one number of torch's generator of the device, drawn where the kernel takes
+    the call; the operators draw their own."""
     if _plain_module(norm, LayerNorm) and norm.weight is not None and norm.bias is not None and x.is_cuda:
-        seed = torch.randint(2 ** 63 - 1, (1,), device=x.device) if dropout else None
         out = _lib.native().residual_norm_dropout(x, branch, norm.weight, norm.bias, norm.eps, gate, bias, 1.0, True, True,
-                                                  dropout, seed)
+                                                  dropout, None)
         if out is not None:
             return out
     if bias is not None:
