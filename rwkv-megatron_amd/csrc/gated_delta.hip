@@ -1609,7 +1609,7 @@ inline int gd_waves(int64_t tiles) { return tiles <= 256 ? 1 : tiles <= 512 ? 2 
 // Microseconds that `chunks` chunks of that many 16-column tiles take, before the segments' walks and in them: a block's
 // start, and a chunk as measured for each way to deal the tiles; 1024 have the chip at once.
 inline double gd_time(int tiles, int64_t K, bool back, bool before, int chunks) {
-    const double pace[2][2][2][3] = {{{{1.75, 2.0, 3.2}, {1.4, 1.55, 1.9}}, {{2.65, 2.9, 4.1}, {2.0, 2.2, 2.6}}},
+    const double pace[2][2][2][3] = {{{{1.95, 2.25, 3.5}, {1.4, 1.55, 1.9}}, {{2.9, 3.3, 4.3}, {2.0, 2.2, 2.6}}},
                                      {{{2.8, 3.1, 4.4}, {2.45, 2.85, 3.8}}, {{3.8, 4.3, 6.2}, {3.4, 3.8, 5.1}}}};
     const double* p = pace[back][K == 128][before];
     return tiles <= 512 ? 4 + chunks * p[tiles > 256] : ((tiles + 1023) >> 10) * (4 + chunks * p[2]);
@@ -1617,16 +1617,16 @@ inline double gd_time(int tiles, int64_t K, bool back, bool before, int chunks) 
 // Segments of a walk.  Few heads leave most of the chip idle and a walk as long as the sequence: p segments walk
 // side by side from states that a walk over all but the last has found (with the K columns of its map beside the
 // V of its state) and `join` has put together.  The number with the least time by the paces above and what
-// two more launches cost is taken, 1 where none beats it.  Forward of 4 heads (64 x 64) of 65536 tokens 1760 to 256 us,
-// of 8 and of 32 heads of 32768 900 to 176 and 980 to 567; backward of 8 and of 32 heads of 16384 722 to 189 and 952 to
-// 600; 256 heads of 4096 tokens fill the chip as they are.
+// two more launches cost is taken, 1 where none beats it (two segments never do by two hundredths).  Forward of 4 heads
+// (64 x 64) of 65536 tokens 1980 to 290 us, of 8 and of 32 heads of 32768 1010 to 190 and 1080 to 550; backward of 8 and of 32
+// heads of 16384 730 to 203 and 940 to 640; 256 heads of 4096 tokens fill the chip as they are.
 void gd_segments(GdShape* n, int64_t K, bool back) {
     n->segs = 1;
     n->per = n->NC;
     if (n->NC < 8 || n->BH * (n->V / 16) > 512) return;   // nothing to win with fewer chunks, a seventh at most with more tiles
     const int vt = (int)n->BH * (n->V / 16), kt = (int)n->BH * ((int)K / 16);
     double best = gd_time(vt, K, back, false, n->NC);
-    for (int p = 2; p <= 16; ++p) {
+    for (int p = 3; p <= 16; ++p) {
         const int per = (n->NC + p - 1) / p;
         if ((n->NC + per - 1) / per != p) continue;
         const double t = 12 + (p - 2) + gd_time(vt + (p - 2) * (vt + kt), K, back, true, per) + gd_time(vt * p, K, back, false, per);
@@ -1696,7 +1696,6 @@ template <class F> void gd_walks(int64_t tiles, int64_t K, F&& f) {
 // Columns that are walked before the segments.
 inline int64_t gd_before(const GdShape& n, int64_t K) { return n.V + (n.segs - 2) * (n.V + K); }
 void gd_join(const GdShape& n, int64_t K, float* E, hipStream_t s) {
-    if (n.segs == 2) return;
     auto join = K == 64 ? rwkv6_gated_delta_join_kernel<64> : rwkv6_gated_delta_join_kernel<128>;
     hipLaunchKernelGGL(join, dim3((unsigned)(n.BH * (n.V / 16))), dim3(256), 0, s, E, n);
 }
