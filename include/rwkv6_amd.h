@@ -415,7 +415,8 @@ int rwkv6_wkv_bwd_ex(const void* r, const void* k, const void* v, const void* w,
 /* residual_norm with dropout of probability p on f (the reference's bias-dropout-add, rwkv6_layer_specs.py:545,
  * :548): element e of f [N,C] is kept and scaled by 1 / (1 - p) where the 16-bit number e % 8 of Philox4x32-10
  * with counter e / 8 and key *seed (a device pointer; low halves of the four words first) is at least 65536 p,
- * which is rounded to a whole number below 65536.  seed_used (nullable) gets the seed's value for a backward after
+ * which is rounded to a whole number below 65536; what is dropped, an infinity or a NaN too, reaches no output and no
+ * gradient.  seed_used (nullable) gets the seed's value for a backward after
  * the seed has changed; the backward draws the same numbers, no mask is stored.  p = 0 is the call without. */
 int rwkv6_residual_norm_dropout_fwd(const void* x, int x_dtype, const void* branch,
                                     const void* branch_bias, int bias_dtype, const void* gate,
@@ -445,7 +446,7 @@ int rwkv6_residual_norm_dropout_bwd(const void* x, int x_dtype, const void* bran
  * `workspace` (rwkv6_gated_delta_workspace_bytes, for_bwd 0) is used.  bwd: gradients of losses on o (d_o) and on
  * the final state (dhT, nullable); dq, dk [B,H,T,K] (the sums over the value heads of a key head), dv [B,HV,T,V]
  * bf16, dg f32, dbeta in beta_dtype [B,HV,T], dh0 f32 nullable.
- * hT, dh0, dg and dbeta have the precision of 32-bit arithmetic.  A NaN or an infinity in a token may reach every
+ * All outputs have the precision of 32-bit arithmetic, bf16 ones rounded once.  A NaN or an infinity in a token may reach every
  * token of its chunk of 64, also those before it.
  * step: the same for a few tokens, `state` [B,HV,K,V] f32 updated where it lies: state_strides are a sequence's
  * and a head's (multiples of 4); states that overlap each other are refused.

@@ -32,9 +32,9 @@
 // 32 bits becomes three of bf16 (bf16 times computed) or six (computed times computed, without the halves that
 // lie below 2^-24), 5 and 2.5 times the rate of the matrix instructions in 32 bits, which also keep a wave's other
 // instructions from running beside them (33 cycles each and 6 for each of five multiply-adds between two of them
-// took 61; the bf16 ones, of 17 cycles, hide theirs).  What ends in a
-// bf16 output alone is no exception: where a write takes the place of what is read, o is the small difference of q S and
-// P n, and d_q and d_k are such differences too.  All outputs so have the precision of 32-bit arithmetic, rounded once.
+// took 61; independent bf16 ones, of 16 cycles, hide theirs).  What ends in a bf16 output alone is no exception: where a
+// write takes the place of what is read, o is the small difference of q S and P n, and d_q and d_k are such differences
+// too.  All outputs so have the precision of 32-bit arithmetic, rounded once.
 // G is summed in 64 bits and kept as a pair of floats: decays between neighbours late in a chunk are
 // differences of large sums.
 #include <type_traits>
@@ -249,7 +249,7 @@ template <int N> __device__ __forceinline__ void gd_zero_p(uint16_t* P, int tid)
 // G and T of a chunk.  Wave w forms the rows of its 16-token block of A = beta L k k^T, one wave inverts the blocks
 // on the diagonal by substitution, and wave w then forms column w of the blocks below it, in the 32-bit matrix instructions:
 // T_IJ = -T_II sum_{J<=l<I} A_Il T_lJ.  Bound by the latency of that chain of products and of the substitution, blocks
-// side by side filling it: 16384 chunks 86 us, 323 MB at 3.8 TB/s (K = 64).  Out: G [chunk][64] as pairs of floats in base-2 units, beta
+// side by side filling it: 16384 chunks 82 to 88 us, 323 MB at 3.8 TB/s (K = 64).  Out: G [chunk][64] as pairs of floats in base-2 units, beta
 // in 32 bits, T [chunk][10 blocks][16][16].
 template <int K>
 __global__ void __launch_bounds__(256, K == 64 ? 8 : 4)
@@ -565,9 +565,12 @@ template <int N, int V> __device__ __forceinline__ void gd_weave() {
 }  // namespace
 
 // A block walks a segment of one head's chunks with 16 NW columns of the state.  SAVE: S_save and n_save get the state
-// entering each chunk and the values it writes, for the backward.  256 heads of 64 chunks, 64 x 64, with them: 230 us, 1.25
-// GB at 5.4 TB/s, the memory's rate; fewer heads are bound by the chain's instructions, 1.75 us a chunk (118 matrix
-// instructions and some 400 others of one wave, about one in 5.5 cycles), 2.65 with 128 key channels.
+// entering each chunk and the values it writes, for the backward.  Bound by the chain's instructions: at 64 channels 144
+// matrix instructions of 16 cycles a chunk and some 500 others of 4, 4300 of the 4600 cycles (1.95 us) of a wave with a
+// SIMD to itself: what runs under the matrix instructions, waits for LDS, barriers and products cost again (2.9 us at 128 key
+// channels).  With four chain waves a block each shares its SIMD with a helper: 6900 cycles, 3.5 us at the 2.0 GHz that a
+// full chip runs at; with S_save and n_save 8150, near the memory's rate: 256 heads of 64 chunks, 64 x 64, 237 to 255 us, 1.25
+// GB at 4.9 to 5.3 TB/s.
 template <int K, int NW, bool SAVE>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
@@ -809,7 +812,7 @@ rwkv6_gated_delta_fwd_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __
 
 // What a segment does to a state, before the segments' walks: S alone is carried through, without q and o.  The map of
 // the state that enters it is one more walk, of K columns that begin as the identity and to which nothing is written.
-// 1.4 us a chunk, where the whole walk takes 1.75; 32 heads of 512 chunks in eight segments 252 us, `join` 9.
+// 1.4 us a chunk, where the whole walk takes 1.95; 32 heads of 512 chunks in eight segments 237 to 254 us, `join` 9.
 template <int K, int NW>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_segment_kernel(GdTensor q, GdTensor k, GdTensor v, const float* __restrict__ beta,
@@ -998,8 +1001,9 @@ __global__ void __launch_bounds__(256) rwkv6_gated_delta_join_kernel(float* __re
 
 // The walk back: d_v, and for the other gradients r and the gradient D of the state that each chunk leaves.
 // BEFORE: what the segments but the first do to D, as in `segment`, the last segment being the first to be walked.
-// 256 heads of 64 chunks, 64 x 64: 280 us, 1.25 GB at 4.5 TB/s: the memory would allow 230, the chain is longer than
-// the forward's (P in three parts, scale e^G d_o taken apart too); 2.8 us a chunk where heads are few.
+// 256 heads of 64 chunks, 64 x 64: 268 to 289 us, 1.25 GB at 4.3 to 4.7 TB/s; 2.8 us a chunk where heads are few: 126 matrix
+// instructions and some 530 others are 64 % of its 6470 cycles, waits for LDS and for P, which the chain wants first, the
+// rest (8650 cycles on a full chip).
 template <int K, int NW, bool BEFORE>
 __global__ void __launch_bounds__(walk_threads<NW>) __attribute__((amdgpu_waves_per_eu(2, 2)))
 rwkv6_gated_delta_bwd_kernel(GdTensor q, GdTensor k, GdTensor d_o, const float* __restrict__ beta,
@@ -1265,8 +1269,9 @@ __device__ __forceinline__ bf16x8 plain_rows(const uint16_t* X, int stride, int 
 // d_q, d_k, d_g and d_beta of a chunk of a key head, its value heads one after the other.  Wave (I, half) has the
 // tokens 16 I .. 16 I + 15 against half of the key channels, and of the columns of p and m those of its parity; every
 // product is formed transposed, so that a lane has one token and four adjacent channels.  Bound by its other
-// instructions (55 % of the cycles: parts of S, D, n, r), LDS (45 %) and the waits between barriers of two blocks a CU:
-// 16384 chunks of 64 x 64 484 us, 1.90 GB at 3.9 TB/s.  Two value heads a key head and more hold d_q and d_k over
+// instructions (50 % of the cycles: parts of S, D, n, r), LDS (55 %, 25 in bank conflicts), matrix instructions (28 %) and the
+// waits between barriers of two blocks a CU: 16384 chunks of 64 x 64 473 to 503 us, 1.90 GB at 3.8 to 4.0 TB/s.  At 128 key
+// channels one block a CU leaves each of them below 40 %.  Two value heads a key head and more hold d_q and d_k over
 // them, which takes more registers (GROUPED).
 template <int K, bool GROUPED>
 __global__ void __launch_bounds__(512, K == 64 && !GROUPED ? 4 : 2)
@@ -1603,8 +1608,8 @@ rwkv6_gated_delta_step_kernel(GdTensor q, GdTensor k, GdTensor v, const float* _
 namespace {
 inline bool gd_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 // How a head's columns are dealt to blocks: a block of 4 waves of 16 columns, or of fewer where all blocks still find a
-// CU of their own (256 and 512 tiles).  A wave then has its SIMD and the CU's LDS to itself: 0.99 ms against 1.47 with 4
-// for 32 heads of 512 chunks, 47 us against 61 for both walks of 16 heads of 8.
+// CU of their own (256 and 512 tiles).  A wave then has its SIMD and the CU's LDS to itself: 1.08 ms against 1.55 with 4
+// for 32 heads of 512 chunks, 32 us against 40 forward and 44 against 50 backward for 16 heads of 8.
 inline int gd_waves(int64_t tiles) { return tiles <= 256 ? 1 : tiles <= 512 ? 2 : 4; }
 // Microseconds that `chunks` chunks of that many 16-column tiles take, before the segments' walks and in them: a block's
 // start, and a chunk as measured for each way to deal the tiles; 1024 have the chip at once.

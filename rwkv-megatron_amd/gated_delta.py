@@ -30,8 +30,8 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, output_fi
     here.  scale None means K**-0.5.  initial_state [B,HV,K,V]; final_state is fp32.
 
     q, k, v are used as bf16 (fp32 and fp16 are rounded on entry), o [B,HV,T,V] has v's type.  g and the states
-    are fp32, beta bf16 or fp32; final_state and the gradients of g, beta and initial_state are computed in 32
-    bits.  q, k, v may be strided (a projection's output seen as [B,H,T,K] is read where it lies).  Gradients for
+    are fp32, beta bf16 or fp32.  Inside, 32 bits: o and the gradients of q, k and v are rounded to bf16 once (then to
+    their tensor's type), final_state and the gradients of g and initial_state not at all.  q, k, v may be strided (a projection's output seen as [B,H,T,K] is read where it lies).  Gradients for
     all inputs, also from final_state; the backward itself cannot be differentiated.  The same bits every time.
 
     Kept for the backward: about 680 bytes a token and value head at K = V = 64 (of each chunk of 64 tokens its

@@ -356,7 +356,8 @@ def _plain_module(m, cls):
 class RWKV6Layer(nn.Module):
     """The TransformerLayer that get_rwkv6_layer_spec() builds (:539-550):
     LN -> time mix -> residual -> LN -> channel mix -> residual, with the config's hidden_dropout on what the
-    residuals add, in training."""
+    residuals add, in training.  Called by itself it has no norm to fuse the last add with and takes torch's dropout
+    there; in a model the kernels draw that mask too (other numbers of the same generator)."""
 
     hidden_dropout = 0.0                         # of layers saved whole before they had one
 
